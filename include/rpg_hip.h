@@ -222,6 +222,114 @@ RPG_HIP_API int32_t rpg_hip_bench_matmul(uint32_t type, const uint8_t* w, int64_
                                          const int32_t* ns, int32_t n_count, int32_t copies, int32_t iters,
                                          double* out);
 
+/* ---- serving operators on device buffers: a paged key-value cache that many
+ * sequences share, the attention that reads it, and a sampler of many rows. No
+ * counterpart in the reference, whose cache belongs to one session
+ * (src/kv_cache.h:19-34) and whose sampler draws its own numbers; for hosts
+ * that schedule sessions themselves.
+ *
+ * Every pointer is a device pointer of the current GPU. The work is enqueued
+ * on `stream` (a hipStream_t; NULL = the null stream), without allocation or
+ * synchronisation, so calls may be captured into a graph; it is complete when
+ * the stream is. Lengths, pages, starts and sampling parameters are read on
+ * the device, so a replayed graph takes the values of that moment. Return 0
+ * when enqueued, -1 with a message in rpg_hip_last_error() and nothing
+ * enqueued when the arguments are refused.
+ *
+ * Element types are ggml ids: 0 = f32, 1 = f16, 30 = bf16. Rows of head_dim
+ * elements are contiguous; pointers and strides are multiples of 16 bytes,
+ * strides are counted in elements. */
+
+/* A pool of n_pages pages, each of page_size positions (a power of two, 16 or
+ * more) of n_kv heads of head_dim (64 or 128) elements: position r of head h of
+ * page p at p * page_stride + h * head_stride + r * row_stride, alike in k and v. */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride;
+  int32_t n_pages, page_size, n_kv, head_dim, type;
+} rpg_hip_paged_cache;
+
+/* n_seqs sequences. Sequence s holds lens[s] positions (at most pages *
+ * page_size, 0 and less: none), the new tokens among them; position p lies in
+ * page table[s * table_stride + p / page_size]. A page number outside [0,
+ * n_pages) is never followed: its positions take no part. The new tokens of
+ * sequence s are the packed rows starts[s] .. starts[s + 1] (starts[n_seqs + 1],
+ * not decreasing), at its last positions; rows of no sequence are left as they
+ * are. starts is not read by rpg_hip_paged_decode (one token each). */
+typedef struct {
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* starts;
+  int32_t pages, n_seqs, n_tokens;
+} rpg_hip_sequences;
+
+/* [token][head] rows of head_dim elements of the cache's type */
+typedef struct {
+  void* data;
+  int64_t token_stride, head_stride;
+} rpg_hip_rows;
+
+/* Stores the new tokens' keys and values in their pages. Keys, and queries
+ * from q into q_out (which may be q; q->data NULL: no queries), are RMS-normed
+ * per head with the gains k_norm and q_norm (f32 [head_dim]; NULL: not normed)
+ * and rotated by row `position` of rope (f32 [rope_rows][head_dim], cos |
+ * sin, as rpg_hip_model_rope_row; NULL: not rotated), as the engine's own
+ * QK-norm and RoPE (reference src/qwen3.cc:139-167), computed in f32 and
+ * rounded once. A token whose position is below 0 (more new tokens than
+ * positions) or at or past rope_rows is left out: no key, value or query of
+ * it is written. */
+RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                         const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
+                                         const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm,
+                                         const float* k_norm, float eps, const float* rope, int64_t rope_rows,
+                                         void* stream);
+
+/* Attention of one token per sequence, row s of q, over all of the sequence's
+ * positions: out = softmax(scale q . k) v per head, heads kv * (n_heads / n_kv)
+ * .. sharing key head kv (reference src/qwen3.cc:79-117). scale > 0. Sums and
+ * softmax in f32; for 16-bit types the weights are rounded to that type before
+ * they multiply the values. A sequence without positions gives zeros. out may
+ * be q. work: rpg_hip_paged_work bytes, read and written by this call alone
+ * until it is complete (any contents; may be NULL when that is 0). */
+RPG_HIP_API int32_t rpg_hip_paged_decode(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                         const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
+                                         void* work, int64_t work_bytes, void* stream);
+
+/* Causal attention of the packed new tokens: as rpg_hip_paged_decode, the token
+ * at position p over positions 0 .. p. */
+RPG_HIP_API int32_t rpg_hip_paged_prompt(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                         const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
+                                         void* work, int64_t work_bytes, void* stream);
+
+/* Bytes of work memory that rpg_hip_paged_decode (prompt = 0) or
+ * rpg_hip_paged_prompt (prompt = 1) takes for these sizes; -1 when they are
+ * refused. Host only; reads the sizes of *cache and *seqs, no pointers. */
+RPG_HIP_API int64_t rpg_hip_paged_work(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                       int32_t n_heads, int32_t prompt);
+
+/* One token per row of logits ([rows][vocab], row_stride elements apart, any
+ * alignment of the type): weights exp((x - max) / temperature), tokens ranked
+ * by value, equal ones by index; kept are the first top_k of them, of those
+ * the shortest head that holds top_p of their weight, and of those the ones
+ * whose weight is at least min_p times the largest. The token is the first, by
+ * index, at which the kept weights' running sum passes u times their sum
+ * (u in [0, 1), brought there from outside); logprobs (may be NULL) receives
+ * the log of its weight over the kept ones' sum. temperature <= 0: the first
+ * largest value, log 1. top_k <= 0 or >= vocab, top_p outside (0, 1) and min_p
+ * <= 0 set no limit; each of the four [rows] arrays may be NULL: temperature
+ * 1, no limit. NaN counts as -inf; a row with nothing above -inf gives token
+ * -1 and log 0 = -inf. Other than rpg_hip_sample, top_k keeps exactly that many,
+ * top_k = 1 keeps one, and the weights are exact to 2^-45 of the largest, in
+ * any order of summation. vocab <= 262144, rows <= 65535. work:
+ * rpg_hip_sample_rows_work bytes. */
+RPG_HIP_API int32_t rpg_hip_sample_rows(int32_t type, const void* logits, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, const float* temperature, const int32_t* top_k,
+                                        const float* top_p, const float* min_p, const float* u, int32_t* tokens,
+                                        float* logprobs, void* work, int64_t work_bytes, void* stream);
+RPG_HIP_API int64_t rpg_hip_sample_rows_work(int64_t rows, int64_t vocab);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,372 @@
+// Attention of one new token per sequence over its cache pages
+// (rpg_hip_paged_decode, include/rpg_hip.h):
+//   out[h] = sum_j p_j v_j,  p = softmax over j < len of scale q[h] . k_j.
+//
+// One pass over the keys with a running maximum, sum and output. Workgroup
+// (sequence, key head, 16 query heads of its group, key range); its four waves
+// take the range's key tiles in turn and join their states in LDS at the end.
+// Scores and outputs are formed transposed on the matrix cores, S^T = K Q^T
+// and O^T = V^T P^T (16 x 16 tiles, columns = query heads), so that a lane
+// keeps to one query head: its scores are the B operand of the second product
+// as they stand, and maximum, sum and rescaling are per lane. The key index of
+// a product is free, so V is taken in the order the scores come in: a lane
+// reads 16 bytes of each of its keys' rows (whole rows per load instruction)
+// and for the 16-bit types pairs up its keys' values with one v_perm_b32 per
+// operand register. K and V go from HBM to registers, LDS is not used on the
+// way.
+//
+// Bound: the K and V bytes, each read once (16 columns are computed for any
+// group size: at 8 heads f32 the products would take 1/2 of the time the bytes
+// do, the 16-bit types' 1/10). Ranges: see DecodeSplits.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "lanes.h"
+#include "paged.h"
+#include "paged_dev.h"
+
+namespace rpg {
+namespace paged {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kCols = 16;  // query heads of a workgroup
+constexpr int kRangeUnit = 128;  // a key range's positions are a multiple of this: the workgroup's step (64 in f32)
+
+// Positions of one key range of a sequence of len positions.
+__device__ __forceinline__ int RangeOf(int len, int splits) {
+  return ((len - 1) / splits / kRangeUnit + 1) * kRangeUnit;
+}
+
+// x - y of maxima that may both be -inf (no key yet): then 0.
+__device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
+
+// A wave's keys of one step, as 16-key halves (two, in f32 one): K as A operands
+// (lane: 16 bytes of key l % 16 per 64 bytes of a row), V as the lane's
+// dimensions of keys 4 (l / 16) + r.
+template <typename T, int kDim>
+struct Tile {
+  static constexpr int kHalves = 4 / kBytes<T>;
+  static constexpr int kKeys = 16 * kHalves;
+  static constexpr int kChunks = kDim * kBytes<T> / 64;  // K: 16-byte pieces; V: dwords per key
+  U4 k[kHalves][kChunks];
+  uint32_t v[kHalves][4][kChunks];
+  bool ok[kHalves];  // its page is there
+
+  // Rows of positions pos .. of the sequence whose last one is `last`; those
+  // past it and those of unnamed pages are read from rows that are there.
+  __device__ __forceinline__ void Load(const Cache& c, const int32_t* table, int64_t head_off, int pos, int last,
+                                       int lane) {
+    const int in_page = (1 << c.page_log2) - 1, l16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const int p0 = min(pos + 16 * h, last & ~15);
+      const int page = PageAt(c, table, p0);
+      ok[h] = page >= 0;
+      const int64_t at = max(page, 0) * c.page_bytes + head_off + (p0 & in_page) * static_cast<int64_t>(c.row_bytes);
+      const char* kb = c.k + at;
+      const char* vb = c.v + at;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) k[h][i] = Load16(kb + static_cast<uint32_t>(l16 * c.row_bytes + 64 * i + 16 * g));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const char* row = vb + static_cast<uint32_t>((4 * g + r) * c.row_bytes);
+        if constexpr (kChunks == 2) {
+          const U2 x = *(const __attribute__((address_space(1))) U2*)(row + 8 * l16);
+          v[h][r][0] = x[0], v[h][r][1] = x[1];
+        } else {
+#pragma unroll
+          for (int w = 0; w < kChunks; w += 4) {
+            const U4 x = Load16(row + 64 * w + 16 * l16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[h][r][w + e] = x[e];
+          }
+        }
+      }
+    }
+  }
+};
+
+// The dimension of row m of output block w.
+template <typename T, int kDim>
+__device__ __forceinline__ int DimOf(int w, int m) {
+  if constexpr (kBytes<T> == 4) return 64 * (w / 4) + 4 * m + w % 4;
+  return (kDim / 16) * m + w;
+}
+
+// A query head's running state in a lane: maximum (of scale log2(e) q.k) and
+// the output of its column, alike over the lanes of a column; the sum of the
+// lane's own keys.
+template <typename T, int kDim>
+struct State {
+  float m = kNegInf, l = 0.0f;
+  F4 o[kDim / 16] = {};
+
+  // Adds a tile whose first position is pos.
+  __device__ __forceinline__ void Add(Tile<T, kDim>& t, const U4 (&q)[Tile<T, kDim>::kChunks], float c, int pos,
+                                      int last, int lane) {
+    using Tl = Tile<T, kDim>;
+    const int g = lane >> 4;
+    F4 s[Tl::kHalves];
+#pragma unroll
+    for (int h = 0; h < Tl::kHalves; ++h) {
+      F4 x = {};
+#pragma unroll
+      for (int i = 0; i < Tl::kChunks; ++i) {
+        if constexpr (kBytes<T> == 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = Mfma16F32(__uint_as_float(t.k[h][i][e]), __uint_as_float(q[i][e]), x);
+        } else {
+          x = Mfma16<T>(t.k[h][i], q[i], x);
+        }
+      }
+      s[h] = x * c;
+    }
+    bool whole = pos + Tl::kKeys - 1 <= last;
+#pragma unroll
+    for (int h = 0; h < Tl::kHalves; ++h) whole = whole && t.ok[h];
+    if (!whole) {
+      // Masked keys: no weight, and nothing of what their rows hold (which may
+      // be anything, NaN among it) reaches the second product.
+#pragma unroll
+      for (int h = 0; h < Tl::kHalves; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool in = t.ok[h] && pos + 16 * h + 4 * g + r <= last;
+          s[h][r] = in ? s[h][r] : kNegInf;
+#pragma unroll
+          for (int w = 0; w < Tl::kChunks; ++w) t.v[h][r][w] = in ? t.v[h][r][w] : 0u;
+        }
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int h = 0; h < Tl::kHalves; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[h][r]);
+    top = lanes::MaxXor32(lanes::MaxXor16(top));
+    if (__any(top > m)) {
+      const float now = fmaxf(m, top), f = __builtin_amdgcn_exp2f(MaxDiff(m, now));
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int w = 0; w < kDim / 16; ++w) o[w] *= f;
+    }
+    const float base = m == kNegInf ? 0.0f : m;
+#pragma unroll
+    for (int h = 0; h < Tl::kHalves; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[h][r] = __builtin_amdgcn_exp2f(s[h][r] - base);
+        l += s[h][r];
+      }
+    if constexpr (kBytes<T> == 4) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int w = 0; w < kDim / 16; ++w) o[w] = Mfma16F32(__uint_as_float(t.v[0][r][w]), s[0][r], o[w]);
+    } else {
+      // The weights are rounded to the cache's 16 bits for the product (each by
+      // at most half a step, as V itself was); the sum takes them unrounded.
+      const U4 p = {Pack2<T>(s[0][0], s[0][1]), Pack2<T>(s[0][2], s[0][3]), Pack2<T>(s[1][0], s[1][1]),
+                    Pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int w = 0; w < kDim / 16; ++w) {
+        const uint32_t sel = w % 2 ? 0x07060302u : 0x05040100u;
+        U4 a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          a[j] = __builtin_amdgcn_perm(t.v[j / 2][2 * (j % 2) + 1][w / 2], t.v[j / 2][2 * (j % 2)][w / 2], sel);
+        o[w] = Mfma16<T>(a, p, o[w]);
+      }
+    }
+  }
+};
+
+// Work: [row][splits] (maximum, sum), then [row][splits][kDim] outputs that are
+// not yet divided by the sum; row = sequence x query head.
+__device__ __forceinline__ F2* PartStats(const AttentionArgs& a, int64_t row) {
+  return reinterpret_cast<F2*>(a.work) + row * a.splits;
+}
+template <int kDim>
+__device__ __forceinline__ float* PartOut(const AttentionArgs& a, int64_t rows, int64_t row) {
+  return a.work + 2 * rows * a.splits + row * a.splits * kDim;
+}
+
+template <typename T>
+__device__ __forceinline__ void Store4(char* p, F4 x) {
+  if constexpr (kBytes<T> == 4)
+    *reinterpret_cast<F4*>(p) = x;
+  else
+    *reinterpret_cast<U2*>(p) = U2{Pack2<T>(x[0], x[1]), Pack2<T>(x[2], x[3])};
+}
+
+// grid (sequence x key head x block of 16 query heads, key range)
+template <typename T, int kDim>
+__global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
+  using Tl = Tile<T, kDim>;
+  __shared__ float sm[kWaves][kCols], sl[kWaves][kCols];
+  __shared__ __align__(16) float so[kWaves][kCols][kDim + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = a.n_heads / a.c.n_kv, blocks = (group + kCols - 1) / kCols;
+  const int hb = blockIdx.x % blocks, kh = blockIdx.x / blocks % a.c.n_kv, seq = blockIdx.x / blocks / a.c.n_kv;
+  const int h0 = kh * group + hb * kCols, n_cols = min(kCols, group - hb * kCols);
+  const int len = Length(a.s, seq);
+  const int range = RangeOf(max(len, 1), a.splits), start = blockIdx.y * range, end = min(len, start + range);
+  if (start >= end && blockIdx.y > 0) return;
+  State<T, kDim> st;
+  if (start < end) {
+    const int32_t* table = a.s.table + seq * a.s.table_stride;
+    const int64_t head_off = kh * a.c.head_bytes;
+    const int col = min(lane & 15, n_cols - 1);
+    const char* qp = a.q.p + seq * a.q.token_bytes + (h0 + col) * a.q.head_bytes + 16 * (lane >> 4);
+    U4 q[Tl::kChunks];
+#pragma unroll
+    for (int i = 0; i < Tl::kChunks; ++i) q[i] = Load16(qp + 64 * i);
+    const float c = a.scale * 1.44269504088896341f;
+    int pos = start + wave * Tl::kKeys;
+    Tl now, next;
+    if (pos < end) now.Load(a.c, table, head_off, pos, end - 1, lane);
+    for (; pos < end; pos += kWaves * Tl::kKeys) {
+      next.Load(a.c, table, head_off, pos + kWaves * Tl::kKeys, end - 1, lane);
+      st.Add(now, q, c, pos, end - 1, lane);
+      now = next;
+    }
+  }
+  st.l = lanes::AddXor32(lanes::AddXor16(st.l));
+  const int col = lane & 15, g = lane >> 4;
+  if (lane < kCols) sm[wave][lane] = st.m, sl[wave][lane] = st.l;
+  __syncthreads();
+  float top = sm[0][col];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][col]);
+  const float f = __builtin_amdgcn_exp2f(MaxDiff(st.m, top));
+  if (col < n_cols) {
+#pragma unroll
+    for (int w = 0; w < kDim / 16; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) so[wave][col][DimOf<T, kDim>(w, 4 * g + e)] = st.o[w][e] * f;
+  }
+  __syncthreads();
+  const bool alone = range >= len;
+  const int64_t rows = static_cast<int64_t>(a.s.n_seqs) * a.n_heads;
+  for (int i = tid; i < n_cols * (kDim / 4); i += 64 * kWaves) {
+    const int h = i / (kDim / 4), d = i % (kDim / 4) * 4;
+    float m = sm[0][h], l = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sm[w][h]);
+    F4 o = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      l += sl[w][h] * __builtin_amdgcn_exp2f(MaxDiff(sm[w][h], m));
+      o += *reinterpret_cast<const F4*>(&so[w][h][d]);
+    }
+    if (alone) {
+      // No key left (an empty sequence, pages that are not there): zeros.
+      o *= l > 0.0f ? 1.0f / l : (m == kNegInf ? 0.0f : 1.0f / l);
+      Store4<T>(a.out.p + seq * a.out.token_bytes + (h0 + h) * a.out.head_bytes + d * kBytes<T>, o);
+    } else {
+      const int64_t row = static_cast<int64_t>(seq) * a.n_heads + h0 + h;
+      if (d == 0) PartStats(a, row)[blockIdx.y] = F2{m, l};
+      *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, row) + static_cast<int64_t>(blockIdx.y) * kDim + d) = o;
+    }
+  }
+}
+
+// Joins the ranges of one row: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+// Workgroup = row; its 256 threads are kDim / 4 columns of four dimensions times
+// the parts that take the ranges in turn.
+constexpr int kMaxSplits = 512;
+template <typename T, int kDim>
+__global__ __launch_bounds__(256) void JoinKernel(AttentionArgs a) {
+  constexpr int kThreadsD = kDim / 4, kParts = 256 / kThreadsD;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float sm[4], sl[4];
+  __shared__ __align__(16) float so[kParts][kDim];
+  const int64_t row = blockIdx.x, rows = static_cast<int64_t>(a.s.n_seqs) * a.n_heads;
+  const int seq = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
+  const int len = Length(a.s, seq), range = RangeOf(max(len, 1), a.splits);
+  if (range >= len) return;  // written by its one range
+  const int n = (len + range - 1) / range, tid = threadIdx.x;
+  const F2* stats = PartStats(a, row);
+  F2 mine[kMaxSplits / 256];
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    mine[i] = tid + 256 * i < n ? stats[tid + 256 * i] : F2{kNegInf, 0.0f};
+    top = fmaxf(top, mine[i][0]);
+  }
+  top = lanes::WaveMaxF(top);
+  if ((tid & 63) == 0) sm[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    const float f = __builtin_amdgcn_exp2f(MaxDiff(mine[i][0], top));
+    if (tid + 256 * i < n) weight[tid + 256 * i] = f;
+    l += mine[i][1] * f;
+  }
+  l = lanes::WaveSumF(l);
+  if ((tid & 63) == 0) sl[tid >> 6] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const int d = tid % kThreadsD * 4, part = tid / kThreadsD;
+  const float* po = PartOut<kDim>(a, rows, row) + d;
+  F4 o = {};
+#pragma unroll 4
+  for (int s = part; s < n; s += kParts) o += *reinterpret_cast<const F4*>(po + static_cast<int64_t>(s) * kDim) * weight[s];
+  *reinterpret_cast<F4*>(&so[part][d]) = o;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int p = 1; p < kParts; ++p) o += *reinterpret_cast<const F4*>(&so[p][d]);
+  o *= l > 0.0f ? 1.0f / l : (top == kNegInf ? 0.0f : 1.0f / l);
+  Store4<T>(a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes + d * kBytes<T>, o);
+}
+
+template <typename T, int kDim>
+void Launch(const AttentionArgs& a, hipStream_t s) {
+  const int group = a.n_heads / a.c.n_kv;
+  const int64_t x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(group, kCols);
+  DecodeKernel<T, kDim><<<dim3(static_cast<uint32_t>(x), a.splits), 64 * kWaves, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
+  if (a.splits == 1) return;
+  JoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_seqs) * a.n_heads, 256, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
+}
+
+template <typename T>
+void LaunchDim(const AttentionArgs& a, hipStream_t s) {
+  if (a.c.head_dim == 128)
+    Launch<T, 128>(a, s);
+  else
+    Launch<T, 64>(a, s);
+}
+
+}  // namespace
+
+int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
+  const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));
+  const int64_t want = std::max(CeilDiv(1024, base), CeilDiv(capacity, 2048));
+  return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, kRangeUnit), int64_t{kMaxSplits}})));
+}
+
+int64_t WorkBytes(int64_t rows, int head_dim, int splits) {
+  return splits == 1 ? 0 : rows * splits * (2 + head_dim) * 4;
+}
+
+void Decode(const AttentionArgs& a, hipStream_t s) {
+  if (a.s.n_seqs == 0) return;
+  if (a.c.type == kF32)
+    LaunchDim<F32>(a, s);
+  else if (a.c.type == kF16)
+    LaunchDim<F16>(a, s);
+  else
+    LaunchDim<BF16>(a, s);
+}
+
+}  // namespace paged
+}  // namespace rpg
