@@ -16,15 +16,15 @@
 // Four launches over (row, slice of the vocabulary), without a sort:
 //   Max    largest value (and its first index) and least finite one per slice
 //   Count  histogram of 2048 equal steps of x below the row's maximum: count
-//          and weight, slices added by atomics
-//   Split  the step that holds the cut, from the histogram: weight of the
-//          steps above it per slice, and its own tokens as a list
-//   Draw   one workgroup a row: the cut inside the list, the slice that the
-//          draw falls into, the token inside that slice
-// A list of more than kList tokens (thousands of equal values, a temperature
-// that flattens everything) or a cut whose step the histogram cannot tell
-// (top_k inside one step deciding top_p's) is found by Draw over the whole
-// row, digit by digit.
+//          and weight, slices added by atomics; the row's last slice looks up
+//          the step that holds the cut
+//   Split  a list of the tokens down to that step; where those are more than kList, the list of its
+//          own tokens and the weight above it per 4096 tokens
+//   Draw   one workgroup a row: the list sorted and cut, then the draw, among
+//          the list's tokens by index or in the unit that it falls into
+// A step of more than kList tokens (thousands of equal values) and a cut whose
+// step the histogram cannot tell (a large top_k whose last step decides
+// top_p's) are found by Draw over the whole row, digit by digit.
 //
 // Bound: the logits' bytes, read once from HBM (later launches find them in
 // the memory-side cache); a single row is bound by its four launches.
@@ -52,18 +52,15 @@ constexpr int kThreads = 256;
 constexpr int kBins = 2048;
 constexpr int kDrawThreads = 1024;
 constexpr int kList = 1024;      // tokens of the cut's step that Draw ranks in LDS
-constexpr int kMaxSlices = 64;
-constexpr int kUnit = 4096;      // a slice's tokens are a multiple of this
+constexpr int kUnit = 4096;      // Draw looks for the token in a run of this many; slices are multiples of it
+constexpr int kMaxUnits = 64;    // of a row: 262144 tokens
 constexpr float kNone = -__builtin_inff();
 
 struct Bin {
   uint64_t weight;
   uint32_t count, pad;
 };
-struct Item {
-  float x;
-  int32_t index;
-};
+struct Cut;
 struct SliceMax {
   float max, min;
   int32_t index, pad;
@@ -71,7 +68,7 @@ struct SliceMax {
 
 struct Layout {
   int slices, length;  // tokens per slice
-  int64_t max_at, bins_at, weights_at, lists_at, counts_at, bytes;
+  int64_t max_at, bins_at, weights_at, lists_at, counts_at, cuts_at, bytes;
 };
 
 __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
@@ -81,15 +78,16 @@ __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   const int64_t most = (vocab + kUnit - 1) / kUnit;
   int64_t want = rows < 1 ? 1 : (1536 + rows - 1) / rows;
   want = want < 1 ? 1 : want > most ? most : want;
-  want = want > kMaxSlices ? kMaxSlices : want;
+  want = want > kMaxUnits ? kMaxUnits : want;
   l.length = static_cast<int>(((vocab + want - 1) / want + kUnit - 1) / kUnit * kUnit);
   l.slices = static_cast<int>((vocab + l.length - 1) / l.length);
   l.bins_at = 0;
   l.max_at = l.bins_at + rows * kBins * static_cast<int64_t>(sizeof(Bin));
   l.weights_at = l.max_at + rows * l.slices * static_cast<int64_t>(sizeof(SliceMax));
-  l.lists_at = l.weights_at + rows * l.slices * 8;
-  l.counts_at = l.lists_at + rows * kList * static_cast<int64_t>(sizeof(Item));
-  l.bytes = (l.counts_at + rows * 4 + 255) / 256 * 256;
+  l.lists_at = l.weights_at + rows * kMaxUnits * 8;
+  l.counts_at = l.lists_at + rows * kList * 8;
+  l.cuts_at = (l.counts_at + rows * 8 + 63) / 64 * 64;
+  l.bytes = l.cuts_at + rows * 64;
   return l;
 }
 
@@ -97,15 +95,17 @@ __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
 struct Work {
   Bin* bins;
   SliceMax* max;
-  uint64_t* weights;
-  Item* list;
-  uint32_t* count;
+  uint64_t* weights;  // per unit
+  uint64_t* list;  // rank keys
+  uint32_t* count;  // tokens listed; slices counted
+  Cut* cut;
   __device__ Work(const SampleArgs& a, const Layout& l, int row)
       : bins(reinterpret_cast<Bin*>(a.work + l.bins_at) + static_cast<int64_t>(row) * kBins),
         max(reinterpret_cast<SliceMax*>(a.work + l.max_at) + static_cast<int64_t>(row) * l.slices),
-        weights(reinterpret_cast<uint64_t*>(a.work + l.weights_at) + static_cast<int64_t>(row) * l.slices),
-        list(reinterpret_cast<Item*>(a.work + l.lists_at) + static_cast<int64_t>(row) * kList),
-        count(reinterpret_cast<uint32_t*>(a.work + l.counts_at) + row) {}
+        weights(reinterpret_cast<uint64_t*>(a.work + l.weights_at) + static_cast<int64_t>(row) * kMaxUnits),
+        list(reinterpret_cast<uint64_t*>(a.work + l.lists_at) + static_cast<int64_t>(row) * kList),
+        count(reinterpret_cast<uint32_t*>(a.work + l.counts_at) + 2 * row),
+        cut(reinterpret_cast<Cut*>(a.work + l.cuts_at + static_cast<int64_t>(row) * 64)) {}
 };
 
 template <typename T>
@@ -125,27 +125,24 @@ __device__ __forceinline__ float One(const char* row, int i) {
   }
 }
 
-// Values i .. i + kPer - 1 of a row (-inf past its end); wide: the row lies at
-// a multiple of 16 bytes.
+// Two neighbouring values of a run: those of its first dword (16-bit types) or
+// dwords (f32). Next moves on to the two behind them.
 template <typename T>
-__device__ __forceinline__ void Values(const char* row, int i, int vocab, bool wide, float (&x)[kPer<T>]) {
-  if (wide && i + kPer<T> <= vocab) {
-    const U4 v = paged::Load16(row + static_cast<int64_t>(i) * paged::kBytes<T>);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (paged::kBytes<T> == 4) {
-        x[e] = Clean(__uint_as_float(v[e]));
-      } else {
-        Unpack2<T>(v[e], &x[2 * e], &x[2 * e + 1]);
-        x[2 * e] = Clean(x[2 * e]);
-        x[2 * e + 1] = Clean(x[2 * e + 1]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kPer<T>; ++e) x[e] = i + e < vocab ? One<T>(row, i + e) : kNone;
-  }
+__device__ __forceinline__ void Two(U4 v, float* a, float* b) {
+  if constexpr (paged::kBytes<T> == 4)
+    *a = __uint_as_float(v[0]), *b = __uint_as_float(v[1]);
+  else
+    Unpack2<T>(v[0], a, b);
+  *a = Clean(*a);
+  *b = Clean(*b);
 }
+template <typename T>
+__device__ __forceinline__ U4 Next(U4 v) {
+  if constexpr (paged::kBytes<T> == 4) return U4{v[2], v[3], 0u, 0u};
+  return U4{v[1], v[2], v[3], 0u};
+}
+template <typename T>
+constexpr uint32_t kNoneBits = paged::kBytes<T> == 4 ? 0xFF800000u : __is_same(T, BF16) ? 0xFF80FF80u : 0xFC00FC00u;
 
 // 2^(-j / 32)
 __device__ const double kPow2[32] = {
@@ -169,13 +166,20 @@ struct Row {
   bool greedy;
   int32_t k;      // 0: no limit
   double p, floor;  // 0: no limit; min_p in weight units
+  float reach;      // how far below max a weight can reach the floor
+  bool weightless_end;  // the histogram's last step holds only what has no weight
+
+  // top_k so small that the tokens up to the k-th are listed whole: only their
+  // number is needed of the histogram
+  __device__ __forceinline__ bool Lean() const { return k > 0 && k <= kList / 2; }
 
   // w 2^44, at most half a unit off when rounded; 0 where it would be less
   // than half of one.
   __device__ __forceinline__ double Weight(float x, const double* pow2) const {
     const double d = x == max ? 0.0 : static_cast<double>(max) - static_cast<double>(x);
-    const double y = d == 0.0 ? 0.0 : d * c;
-    if (!(y < 45.5)) return 0.0;
+    const double far = d == 0.0 ? 0.0 : d * c;
+    const bool in = far < 45.5;
+    const double y = in ? far : 0.0;  // (no branch: a run's weights are computed side by side)
     const int n = static_cast<int>(y * 32.0);
     const double z = (static_cast<double>(n) * 0.03125 - y) * 0.69314718055994530942;  // (-ln 2 / 32, 0]
     double e = __builtin_fma(z, 1.0 / 120.0, 1.0 / 24.0);
@@ -184,12 +188,21 @@ struct Row {
     e = __builtin_fma(z, e, 1.0);
     e = __builtin_fma(z, e, 1.0);
     const uint64_t t = __builtin_bit_cast(uint64_t, pow2[n & 31]) + (static_cast<uint64_t>(44 - (n >> 5)) << 52);
-    return e * __builtin_bit_cast(double, t);
+    return in ? e * __builtin_bit_cast(double, t) : 0.0;
   }
   // rounded to an integer (weights are below 2^52)
   static __device__ __forceinline__ uint64_t Units(double w) {
     return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
   }
+  // Tokens without weight are not counted where that is plain: those of -inf, and
+  // the last step of a histogram that ends where weights do (which may be most
+  // of a row, on one counter). Where fewer than k are counted, top_k sets no limit.
+  __device__ __forceinline__ bool Counted(float x, int bin) const {
+    return x > kNone && !(weightless_end && bin == kBins - 1);
+  }
+  // false only where the weight is below the floor (the margin covers the
+  // rounding of the difference and of reach)
+  __device__ __forceinline__ bool MayReach(float x) const { return max - x <= reach || x == max; }
   // monotone: never less for a smaller x
   __device__ __forceinline__ int Bin(float x) const {
     return static_cast<int>(fminf((x == max ? 0.0f : max - x) * scale, static_cast<float>(kBins - 1)));
@@ -211,6 +224,7 @@ __device__ __forceinline__ Row RowOf(const SampleArgs& a, const Layout& l, const
   r.greedy = !(t > 0.0f);
   r.c = 1.4426950408889634074 / static_cast<double>(t);
   const float span = fminf(31.6f * t, max - min);
+  r.weightless_end = 31.6f * t <= max - min;
   r.scale = span > 0.0f ? static_cast<float>(kBins) / span : 0.0f;
   const int32_t k = a.top_k != nullptr ? a.top_k[row] : 0;
   r.k = k > 0 && k < a.vocab ? k : 0;
@@ -218,12 +232,81 @@ __device__ __forceinline__ Row RowOf(const SampleArgs& a, const Layout& l, const
   r.p = p > 0.0f && p < 1.0f ? static_cast<double>(p) : 0.0;
   const float f = a.min_p != nullptr ? a.min_p[row] : 0.0f;
   r.floor = f > 0.0f ? static_cast<double>(fminf(f, 1.0f)) * kOne : 0.0;
+  r.reach = t * (f > 0.0f ? -__logf(fminf(f, 1.0f)) * 1.0001f + 1e-3f : 31.6f);
   return r;
 }
 
+// f(run, i, lo) for the runs of 16 bytes of `length` tokens from `start` on, a
+// run to a lane, kAhead of a lane's runs in flight. Tokens i .. i + kPer - 1 lie
+// in the run; it stands for those from lo on (the row's last run reaches back
+// into the one before it, and a lane behind the row has none: lo past its
+// tokens). The length is a multiple of a workgroup's runs; whole waves go round
+// together, so f may use their lanes. The loads take any alignment, depend on no
+// branch (a join would wait for them) and never reach past the row. One copy of
+// f: a launch starts on a cold instruction cache.
+constexpr int kAhead = 4;
+typedef U4 U4Any __attribute__((aligned(2)));
+template <typename T, typename F>
+__device__ __forceinline__ void ForRuns(const SampleArgs& a, const char* row, int start, int length, F&& f) {
+  const int end = min(a.vocab, start + length), step = kThreads * kPer<T>;
+  if (a.vocab < kPer<T>) {  // less than a run
+    if (start > 0 || threadIdx.x >= 64) return;
+    U4 v = {kNoneBits<T>, kNoneBits<T>, kNoneBits<T>, kNoneBits<T>};
+    for (int e = 0; e < a.vocab; ++e) {
+      const float x = One<T>(row, e);
+      const uint32_t u = paged::kBytes<T> == 4 ? __float_as_uint(x) : reinterpret_cast<const uint16_t*>(row)[e];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (paged::kBytes<T> == 4 && k == e) v[k] = u;
+        if (paged::kBytes<T> == 2 && k == e / 2) v[k] = e % 2 ? (v[k] & 0xFFFFu) | u << 16 : (v[k] & 0xFFFF0000u) | u;
+      }
+    }
+    // (values past the row are -inf; the lane past kPer - vocab has none to stand for)
+    f(v, 0, threadIdx.x == 0 ? 0 : kPer<T>);
+    return;
+  }
+  const int wave_first = start + static_cast<int>(threadIdx.x / 64) * 64 * kPer<T>;
+  const int n = wave_first < end ? (end - wave_first - 1) / step + 1 : 0;
+  const int mine = start + threadIdx.x * kPer<T>, last = a.vocab - kPer<T>;
+  auto load = [&](int r) {
+    return *(const __attribute__((address_space(1))) U4Any*)(row + static_cast<int64_t>(min(mine + r * step, last)) * paged::kBytes<T>);
+  };
+  U4 ring[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) ring[k] = load(k);
+#pragma unroll 1
+  for (int r = 0; r < n; ++r) {
+    const U4 run = ring[0];
+#pragma unroll
+    for (int k = 0; k + 1 < kAhead; ++k) ring[k] = ring[k + 1];
+    ring[kAhead - 1] = load(r + kAhead);
+    const int at = mine + r * step;
+    f(run, min(at, last), at);
+  }
+}
+
+// f(x, y, i) for neighbouring values of a run.
+template <typename T, typename F>
+__device__ __forceinline__ void ForTwo(U4 run, int i, F&& f) {
+#pragma unroll 1
+  for (int e = 0; e < kPer<T>; e += 2) {
+    float x, y;
+    Two<T>(run, &x, &y);
+    f(x, y, i + e);
+    run = Next<T>(run);
+  }
+}
 template <typename T>
-__device__ __forceinline__ bool Wide(const SampleArgs& a) {
-  return ((reinterpret_cast<uintptr_t>(a.logits) | static_cast<uint64_t>(a.row_bytes)) & 15) == 0;
+__device__ __forceinline__ float Top(U4 run) {
+  float top = kNone;
+#pragma unroll
+  for (int e = 0; e < kPer<T>; e += 2) {
+    float x, y;
+    Two<T>(run, &x, &y);
+    top = fmaxf(top, fmaxf(x, y));
+    run = Next<T>(run);
+  }
+  return top;
 }
 
 // grid (slice, row)
@@ -232,22 +315,21 @@ __global__ __launch_bounds__(kThreads) void MaxKernel(SampleArgs a, Layout l) {
   const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
   const Work w(a, l, row);
   const char* x = a.logits + row * a.row_bytes;
-  const bool wide = Wide<T>(a);
   for (int i = slice * kThreads + tid; i < kBins; i += l.slices * kThreads) w.bins[i] = Bin{0, 0, 0};
-  if (slice == 0 && tid == 0) *w.count = 0;
+  if (slice == 0 && tid == 0) w.count[0] = w.count[1] = 0;
   float most = kNone, least = -kNone;
   int at = INT32_MAX;
-  const int end = min(a.vocab, (slice + 1) * l.length);
-#pragma unroll 4
-  for (int i = slice * l.length + tid * kPer<T>; i < end; i += kThreads * kPer<T>) {
-    float v[kPer<T>];
-    Values<T>(x, i, a.vocab, wide, v);
+  ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int) {  // (a token met twice changes nothing)
 #pragma unroll
-    for (int e = 0; e < kPer<T>; ++e) {
-      if (v[e] > most) most = v[e], at = i + e;
-      if (v[e] > kNone) least = fminf(least, v[e]);
+    for (int e = 0; e < kPer<T>; e += 2) {
+      float y, z;
+      Two<T>(run, &y, &z);
+      if (y > most) most = y, at = i + e;
+      if (z > most) most = z, at = i + e + 1;
+      least = fminf(least, fminf(y > kNone ? y : -kNone, z > kNone ? z : -kNone));
+      run = Next<T>(run);
     }
-  }
+  });
   __shared__ SliceMax s[kThreads / 64];
   const float top = lanes::WaveMaxF(most);
   const float low = -lanes::WaveMaxF(-least);
@@ -269,6 +351,150 @@ __device__ __forceinline__ void LoadPow2(double* pow2) {
   if (threadIdx.x < 32) pow2[threadIdx.x] = kPow2[threadIdx.x];
 }
 
+// Order of the ranking: x descending, index ascending. The key of x grows with it.
+__device__ __forceinline__ uint32_t KeyOf(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t RankKey(float x, int index) {
+  return static_cast<uint64_t>(KeyOf(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ float ValueOf(uint64_t rank_key) {
+  const uint32_t k = static_cast<uint32_t>(rank_key >> 32);
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ int IndexOf(uint64_t rank_key) {
+  return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(rank_key));
+}
+
+// Sums over the threads before this one, in a workgroup of kN (every thread
+// calls it), of weights and of counts.
+template <int kN>
+__device__ __forceinline__ uint64_t Before(uint64_t q, uint64_t* total, uint32_t n = 0, uint32_t* before_n = nullptr) {
+  constexpr int kParts = kN / 64;
+  __shared__ unsigned long long part[kParts];
+  __shared__ uint32_t part_n[kParts];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long x = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(q));
+  const uint32_t c = before_n != nullptr ? lanes::WaveInclusiveAdd(n) : 0;
+  __syncthreads();
+  if (lane == 63) {
+    part[wave] = x;
+    if (before_n != nullptr) part_n[wave] = c;
+  }
+  __syncthreads();
+  // every wave sums the parts again, a lane for each
+  const unsigned long long p = lanes::WaveInclusiveAdd(lane < kParts ? part[lane] : 0ull);
+  *total = lanes::ReadLaneT(p, kParts - 1);
+  const int up_lane = __builtin_amdgcn_readfirstlane(wave > 0 ? wave - 1 : 0);
+  const unsigned long long up = lanes::ReadLaneT(p, up_lane);
+  if (before_n != nullptr) {
+    const uint32_t pn = lanes::WaveInclusiveAdd(lane < kParts ? part_n[lane] : 0u);
+    const uint32_t un = lanes::ReadLaneT(pn, up_lane);
+    *before_n = c - n + (wave > 0 ? un : 0);
+  }
+  return x - q + (wave > 0 ? up : 0);
+}
+
+// Where the cut lies, from the row's histogram.
+struct Cut {
+  int k_bin, p_bin;             // the steps that hold the k-th token and top_p's last one; kBins: none
+  uint32_t k_left;              // tokens to keep of k_bin
+  uint32_t unused;
+  uint64_t k_before, p_before;  // weight of the steps above
+  uint64_t all;                 // the row's weight
+  // (words: a copy of a struct with padding would go through private memory,
+  // which the compiler puts into LDS by reading the dispatch packet, 14 us away)
+  uint32_t whole;  // all tokens down to the cut's step are listed (there are at most kList)
+  uint32_t slow;   // the histogram does not tell
+  __device__ __forceinline__ int End() const { return min(k_bin, p_bin); }
+};
+static_assert(sizeof(Cut) <= 64, "a row's place for its cut");
+
+template <int kN>
+__device__ __forceinline__ Cut FindCut(const Row& r, const Bin* bins) {
+  __shared__ Cut s;
+  __shared__ int bins_of[2];
+  __shared__ uint64_t s_through[2];
+  __shared__ uint32_t s_ranked;
+  constexpr int kEach = kBins / kN;
+  const int tid = threadIdx.x;
+  uint64_t q[kEach], sum = 0, all;
+  uint32_t n[kEach], count = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    q[i] = __hip_atomic_load(&bins[tid * kEach + i].weight, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    n[i] = __hip_atomic_load(&bins[tid * kEach + i].count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sum += q[i];
+    count += n[i];
+  }
+  uint32_t ranked;
+  const uint64_t before = Before<kN>(sum, &all, count, &ranked);
+  if (tid == 0) s = Cut{kBins, kBins, 0, 0, 0, 0, all, 0, 0}, bins_of[0] = bins_of[1] = kBins;
+  if (tid == 0) s_through[0] = s_through[1] = all;
+  __syncthreads();
+  if (r.k != 0) {
+    const uint32_t k = static_cast<uint32_t>(r.k);
+    if (ranked < k && ranked + count >= k) {  // one thread's
+      uint64_t b = before, q_bin = 0;
+      uint32_t c = ranked, n_bin = 0;
+      int bin = -1;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (bin < 0 && c + n[i] >= k) bin = tid * kEach + i, q_bin = q[i], n_bin = n[i];
+        if (bin < 0) b += q[i], c += n[i];
+      }
+      if (r.Lean()) {
+        s.k_bin = bin;
+        s.whole = c + n_bin <= kList;
+        s.slow = !s.whole;
+      } else if (q_bin != 0) {
+        s.k_bin = bin;
+        s.k_left = k - c;
+        s.k_before = b;
+        s.whole = c + n_bin <= kList;
+        s_through[0] = b;
+        s_through[1] = b + q_bin;
+      }  // (else the k-th token has no weight: no limit)
+    } else if (tid == kN - 1 && ranked + count < k && r.Lean()) {
+      s.k_bin = r.weightless_end ? kBins - 2 : kBins - 1;  // all that are counted
+      s.whole = 1;
+    }
+    __syncthreads();
+    if (s.whole || s.slow) return s;
+  }
+  if (r.p != 0.0) {
+    // the first step at which the weight so far reaches p x the weight of the
+    // first k tokens, which lies between that above k_bin and that with it
+    const double t[2] = {r.p * static_cast<double>(s_through[0]), r.p * static_cast<double>(s_through[1])};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool from = tid == 0 || static_cast<double>(before) < t[j];
+      if (from && static_cast<double>(before + sum) >= t[j]) {  // one thread's
+        uint64_t b = before;
+        uint32_t c = ranked;
+        int bin = -1;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          if (bin < 0) c += n[i];
+          if (bin < 0 && static_cast<double>(b + q[i]) >= t[j]) bin = tid * kEach + i;
+          if (bin < 0) b += q[i];
+        }
+        bins_of[j] = bin;
+        if (j == 1) s.p_before = b, s_ranked = c;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      s.p_bin = bins_of[1];
+      s.slow = bins_of[0] != bins_of[1];
+      s.whole = r.k == 0 && s_ranked <= kList;
+    }
+    __syncthreads();
+  }
+  return s;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) {
   const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
@@ -283,125 +509,54 @@ __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) 
   for (int i = tid; i < kBins; i += kThreads) weight[i] = 0, count[i] = 0;
   __syncthreads();
   const char* x = a.logits + row * a.row_bytes;
-  const bool wide = Wide<T>(a);
-  const int end = min(a.vocab, (slice + 1) * l.length);
-  for (int i = slice * l.length + tid * kPer<T>; i < end; i += kThreads * kPer<T>) {
-    float v[kPer<T>];
-    Values<T>(x, i, a.vocab, wide, v);
-#pragma unroll
-    for (int e = 0; e < kPer<T>; ++e) {
-      if (i + e >= a.vocab) continue;
-      const int b = r.Bin(v[e]);
-      const uint64_t q = Row::Units(r.Weight(v[e], pow2));
-      if (q != 0) atomicAdd(&weight[b], static_cast<unsigned long long>(q));
-      if (r.k != 0) atomicAdd(&count[b], 1u);
-    }
-  }
+  const bool lean = r.Lean();
+  ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
+    ForTwo<T>(run, i, [&](float y, float z, int at) {
+      const int by = r.Bin(y), bz = r.Bin(z);
+      const bool cy = at >= lo && r.Counted(y, by), cz = at + 1 >= lo && r.Counted(z, bz);
+      if (!__any(cy || cz)) return;
+      if (!lean) {
+        const uint64_t qy = cy ? Row::Units(r.Weight(y, pow2)) : 0, qz = cz ? Row::Units(r.Weight(z, pow2)) : 0;
+        if (qy != 0) atomicAdd(&weight[by], static_cast<unsigned long long>(qy));
+        if (qz != 0) atomicAdd(&weight[bz], static_cast<unsigned long long>(qz));
+      }
+      if (cy) atomicAdd(&count[by], 1u);
+      if (cz) atomicAdd(&count[bz], 1u);
+    });
+  });
   __syncthreads();
-  for (int i = tid; i < kBins; i += kThreads) {
+  // For a small top_k the steps down to the slice's own k-th token: the row's
+  // lies no further down, and those steps get every slice's counts.
+  int last = kBins - 1;
+  if (lean) {
+    __shared__ int s_last;
+    if (tid == 0) s_last = last;
+    constexpr int kEach = kBins / kThreads;
+    uint32_t n = 0, before;
+    uint64_t unused;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) n += count[tid * kEach + i];
+    Before<kThreads>(0, &unused, n, &before);
+    const uint32_t k = static_cast<uint32_t>(r.k);
+    if (before < k && before + n >= k) s_last = tid * kEach + kEach - 1;
+    __syncthreads();
+    last = s_last;
+  }
+  for (int i = tid; i <= last; i += kThreads) {
     if (weight[i] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&w.bins[i].weight), weight[i]);
     if (count[i] != 0) atomicAdd(&w.bins[i].count, count[i]);
   }
-}
-
-// Sums over the threads before this one, in a workgroup of kN (every thread
-// calls it).
-template <int kN, typename V>
-__device__ __forceinline__ V Before(V v, V* total) {
-  __shared__ V part[kN / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  V x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  // The row's last slice to get here finds the cut: every slice's atomics have
+  // been carried out, at the device's point of coherence, before it counts
+  // itself, and that is where FindCut reads them.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (lane == 63) part[wave] = x;
+  __shared__ uint32_t s_before;
+  if (tid == 0) s_before = atomicAdd(&w.count[1], 1u);
   __syncthreads();
-  V before = x - v, sum = 0;
-  for (int i = 0; i < kN / 64; ++i) {
-    if (i < wave) before += part[i];
-    sum += part[i];
-  }
-  *total = sum;
-  return before;
-}
-
-// Where the cut lies, from the row's histogram.
-struct Cut {
-  int k_bin, p_bin;        // the steps that hold the k-th token and top_p's last one; kBins: no limit
-  uint32_t k_left;         // tokens to keep of k_bin
-  uint64_t k_before, p_before;  // weight of the steps above
-  uint64_t all;            // the row's weight
-  bool unclear;            // p_bin hangs on which tokens of k_bin are kept
-  __device__ __forceinline__ int End() const { return min(k_bin, p_bin); }
-};
-
-template <int kN>
-__device__ __forceinline__ Cut FindCut(const Row& r, const Bin* bins) {
-  __shared__ Cut s;
-  __shared__ int bins_of[2];
-  constexpr int kEach = kBins / kN;
-  const int tid = threadIdx.x;
-  uint64_t q[kEach], sum = 0, all;
-  uint32_t n[kEach], count = 0, unused;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    q[i] = bins[tid * kEach + i].weight;
-    n[i] = bins[tid * kEach + i].count;
-    sum += q[i];
-    count += n[i];
-  }
-  uint64_t before = Before<kN>(sum, &all);
-  uint32_t ranked = Before<kN>(count, &unused);
-  __syncthreads();
-  if (tid == 0) s = Cut{kBins, kBins, 0, 0, 0, all, false}, bins_of[0] = bins_of[1] = kBins;
-  __syncthreads();
-  uint64_t lo = all, hi = all;
-  if (r.k != 0) {
-    uint64_t b = before;
-    uint32_t c = ranked;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (c < static_cast<uint32_t>(r.k) && c + n[i] >= static_cast<uint32_t>(r.k)) {
-        s.k_bin = tid * kEach + i;
-        s.k_left = r.k - c;
-        s.k_before = b;
-        s.p_before = b + q[i];  // for the others, until they have read it
-      }
-      b += q[i];
-      c += n[i];
-    }
-    __syncthreads();
-    lo = s.k_before, hi = s.p_before;
-    __syncthreads();
-  }
-  if (r.p != 0.0) {
-    // the first step with its weight and that above it >= p x the weight
-    const double t[2] = {r.p * static_cast<double>(lo), r.p * static_cast<double>(hi)};
-    uint64_t b = before;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bool first = tid * kEach + i == 0;
-        if ((first || static_cast<double>(b) < t[j]) && static_cast<double>(b + q[i]) >= t[j]) {
-          if (j == 0) {
-            bins_of[0] = tid * kEach + i;
-          } else {
-            bins_of[1] = tid * kEach + i;
-            s.p_before = b;
-          }
-        }
-      }
-      b += q[i];
-    }
-    __syncthreads();
-    if (tid == 0) s.p_bin = bins_of[1], s.unclear = bins_of[0] != bins_of[1];
-  }
-  __syncthreads();
-  return s;
+  if (s_before != static_cast<uint32_t>(l.slices - 1)) return;
+  const Cut cut = FindCut<kThreads>(r, w.bins);
+  if (tid == 0) *w.cut = cut;
 }
 
 template <typename T>
@@ -412,44 +567,66 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
   if (r.greedy || r.max == kNone) return;
   __shared__ double pow2[32];
   LoadPow2(pow2);
-  Cut cut{kBins, kBins, 0, 0, 0, 0, false};
-  if (r.k != 0 || r.p != 0.0) cut = FindCut<kThreads>(r, w.bins);
+  Cut cut{kBins, kBins, 0, 0, 0, 0, 0, 0, 0};
+  if (r.k != 0 || r.p != 0.0) cut = *w.cut;
   __syncthreads();
-  if (cut.unclear) return;
+  if (cut.slow) return;
   const int end_bin = cut.End();
   const char* x = a.logits + row * a.row_bytes;
-  const bool wide = Wide<T>(a);
-  const int end = min(a.vocab, (slice + 1) * l.length);
-  uint64_t sum = 0;
-  for (int i = slice * l.length + tid * kPer<T>; i < end; i += kThreads * kPer<T>) {
-    float v[kPer<T>];
-    Values<T>(x, i, a.vocab, wide, v);
-#pragma unroll
-    for (int e = 0; e < kPer<T>; ++e) {
-      if (i + e >= a.vocab) continue;
-      const int b = r.Bin(v[e]);
-      if (b < end_bin) {
-        const double f = r.Weight(v[e], pow2);
-        if (f >= r.floor) sum += Row::Units(f);
-      }
-      if (b == cut.k_bin || b == cut.p_bin) {
-        const uint32_t at = atomicAdd(w.count, 1u);
-        if (at < kList) w.list[at] = Item{v[e], i + e};
-      }
-    }
+  // Listed tokens gather in LDS and go to the row's list together: a place in it
+  // for each would be a round trip to memory.
+  __shared__ uint64_t found[kList];
+  __shared__ uint32_t n_found, s_at;
+  if (tid == 0) n_found = 0;
+  __syncthreads();
+  auto list = [&](float v, int i) {
+    const uint32_t at = atomicAdd(&n_found, 1u);
+    if (at < kList) found[at] = RankKey(v, i);
+  };
+  auto flush = [&] {
+    __syncthreads();
+    const uint32_t n = n_found;
+    if (n == 0) return;
+    if (tid == 0) s_at = atomicAdd(w.count, n);
+    __syncthreads();
+    for (uint32_t i = tid; i < min(n, static_cast<uint32_t>(kList)); i += kThreads)
+      if (s_at + i < kList) w.list[s_at + i] = found[i];
+  };
+  if (cut.whole) {
+    ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
+      if (!__any(r.Bin(Top<T>(run)) <= end_bin)) return;  // few runs hold a listed token
+      ForTwo<T>(run, i, [&](float y, float z, int at) {
+        if (at >= lo && y > kNone && r.Bin(y) <= end_bin) list(y, at);
+        if (at + 1 >= lo && z > kNone && r.Bin(z) <= end_bin) list(z, at + 1);
+      });
+    });
+    flush();
+    return;
   }
-  uint64_t all;
-  Before<kThreads>(sum, &all);
-  if (tid == 0) w.weights[slice] = all;
-}
-
-// Order of the ranking: x descending, index ascending. The key of x grows with it.
-__device__ __forceinline__ uint32_t KeyOf(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ uint64_t RankKey(float x, int index) {
-  return static_cast<uint64_t>(KeyOf(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+  const int listed_last = max(cut.k_bin < kBins ? cut.k_bin : -1, cut.p_bin < kBins ? cut.p_bin : -1);
+  __shared__ uint64_t part[kThreads / 64];
+  for (int start = slice * l.length; start < min(a.vocab, (slice + 1) * l.length); start += kUnit) {
+    uint64_t sum = 0;
+    ForRuns<T>(a, x, start, kUnit, [&](U4 run, int i, int lo) {
+      const float top = Top<T>(run);
+      if (!__any(r.MayReach(top) || r.Bin(top) <= listed_last)) return;
+      ForTwo<T>(run, i, [&](float y, float z, int at) {
+        const int by = at >= lo && y > kNone ? r.Bin(y) : kBins;
+        const int bz = at + 1 >= lo && z > kNone ? r.Bin(z) : kBins;
+        const double fy = r.Weight(y, pow2), fz = r.Weight(z, pow2);
+        sum += by < end_bin && fy >= r.floor ? Row::Units(fy) : 0;
+        sum += bz < end_bin && fz >= r.floor ? Row::Units(fz) : 0;
+        if (by < kBins && (by == cut.k_bin || by == cut.p_bin)) list(y, at);
+        if (bz < kBins && (bz == cut.k_bin || bz == cut.p_bin)) list(z, at + 1);
+      });
+    });
+    sum = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(sum));
+    __syncthreads();
+    if ((tid & 63) == 63) part[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) w.weights[start / kUnit] = part[0] + part[1] + part[2] + part[3];
+  }
+  flush();
 }
 
 // The rank key of the last token kept when tokens are taken from the best on
@@ -501,11 +678,79 @@ __device__ uint64_t CutByDigits(const SampleArgs& a, const Row& r, const char* x
   return prefix;
 }
 
+// The value of the lane whose number differs in bit kBit.
+template <int kBit>
+__device__ __forceinline__ uint32_t Across(uint32_t v) {
+  if constexpr (kBit == 1) return lanes::Dpp<lanes::kQuadXor1>(v);
+  if constexpr (kBit == 2) return lanes::Dpp<lanes::kQuadXor2>(v);
+  if constexpr (kBit == 4) return lanes::Dpp<0x1B>(lanes::Dpp<lanes::kRowHalfMirror>(v));  // 7 - i, then 3 - i of a quad
+  if constexpr (kBit == 8) return lanes::Dpp<lanes::kRowRor8>(v);
+  if constexpr (kBit == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return threadIdx.x & 32 ? r[0] : r[1];
+}
+template <int kBit>
+__device__ __forceinline__ uint64_t Across64(uint64_t v) {
+  return Across<kBit>(static_cast<uint32_t>(v)) |
+         static_cast<uint64_t>(Across<kBit>(static_cast<uint32_t>(v >> 32))) << 32;
+}
+
+// Sorts the first n (a power of two from 64 to kDrawThreads) threads' keys,
+// largest first; every thread of the workgroup calls it.
+__device__ __forceinline__ uint64_t SortDown(uint64_t key, int n, uint64_t* lds) {
+  const int tid = threadIdx.x;
+#pragma unroll 1
+  for (int size = 2; size <= n; size <<= 1) {
+    const bool up = (tid & size) != 0 && size < n;
+#pragma unroll 1
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      uint64_t other = 0;
+      if (stride >= 64) {
+        __syncthreads();
+        if (tid < n) lds[tid] = key;
+        __syncthreads();
+        if (tid < n) other = lds[tid ^ stride];
+      } else if (tid < n) {  // (whole waves)
+        switch (stride) {
+          case 1: other = Across64<1>(key); break;
+          case 2: other = Across64<2>(key); break;
+          case 4: other = Across64<4>(key); break;
+          case 8: other = Across64<8>(key); break;
+          case 16: other = Across64<16>(key); break;
+          default: other = Across64<32>(key);
+        }
+      }
+      const bool lower = (tid & stride) == 0;
+      if (tid < n) key = (lower == up) == (key < other) ? key : other;
+    }
+  }
+  return key;
+}
+__device__ __forceinline__ int PowerFor(int n) {
+  int p = 64;
+  while (p < n) p <<= 1;
+  return p;
+}
+
+__device__ __forceinline__ void Write(const SampleArgs& a, int row, int token, double weight, uint64_t total) {
+  a.tokens[row] = token;
+  if (a.logprobs != nullptr) a.logprobs[row] = static_cast<float>(log(weight / static_cast<double>(total)));
+}
+
 // One workgroup per row.
 template <typename T>
 __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout l) {
   const int row = blockIdx.x, tid = threadIdx.x;
   const Work w(a, l, row);
+  // All that may be needed, in one round trip (what was not written is not used).
+  const int units = (a.vocab + kUnit - 1) / kUnit;
+  const uint64_t item = w.list[tid], unit_item = w.weights[tid & (kMaxUnits - 1)];
+  const uint32_t listed = w.count[0];
+  const Cut stored = *w.cut;
+  const float u_given = a.u[row];
   const Row r = RowOf(a, l, w, row);
   if (r.greedy || r.max == kNone) {
     if (tid == 0) {
@@ -515,22 +760,61 @@ __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout 
     return;
   }
   __shared__ double pow2[32];
-  __shared__ float lx[kList];
-  __shared__ int li[kList];
-  __shared__ uint64_t lq[kList];
-  __shared__ unsigned long long slice_weight[kMaxSlices];
-  __shared__ uint64_t s_kept;
+  __shared__ uint64_t keys[kDrawThreads];
+  __shared__ unsigned long long unit_weight[kMaxUnits];
+  __shared__ double weights[kDrawThreads];
+  __shared__ uint64_t s_taken, s_last;
   LoadPow2(pow2);
   const char* x = a.logits + row * a.row_bytes;
-  Cut cut{kBins, kBins, 0, 0, 0, 0, false};
-  if (r.k != 0 || r.p != 0.0) cut = FindCut<kDrawThreads>(r, w.bins);
+  Cut cut{kBins, kBins, 0, 0, 0, 0, 0, 0, 0};
+  if (r.k != 0 || r.p != 0.0) cut = stored;
   const int end_bin = cut.End();
-  const uint32_t n = end_bin < kBins && !cut.unclear ? *w.count : 0;
-  const bool slow = cut.unclear || n > kList;
-  if (tid < l.slices) slice_weight[tid] = slow ? 0 : w.weights[tid];
-  if (tid == 0) s_kept = 0;
+  const double u = fmax(0.0, fmin(static_cast<double>(u_given), 1.0));
+  const uint32_t n = end_bin < kBins && !cut.slow ? listed : 0;
+  const bool slow = cut.slow || n > kList;
   __syncthreads();
-  uint64_t last = 0;  // rank key of the last token before the limits of weight; 0: every token
+
+  // The list, best first: this thread's token and the weight before it. Where
+  // the list holds all that can be kept, those that are, by index: a second
+  // round of the same code.
+  uint64_t key = 0, q = 0, before = 0, sum = 0;
+  double f = 0.0;
+  if (n > 0 && !slow) {
+    key = tid < static_cast<int>(n) ? item : 0;
+    int here = static_cast<int>(n);
+#pragma unroll 1
+    for (int round = 0;; ++round) {
+      key = SortDown(key, PowerFor(here), keys);
+      f = round == 0 ? (tid < here ? r.Weight(ValueOf(key), pow2) : 0.0)
+                     : (tid < here ? weights[key & 0xFFFFFFFFu] : 0.0);
+      q = Row::Units(f);
+      before = Before<kDrawThreads>(q, &sum);
+      if (!cut.whole || round == 1) break;
+      uint64_t taken = cut.all;
+      if (r.k != 0) {
+        if (tid == min(here, r.k) - 1) s_taken = before + q;
+        __syncthreads();
+        taken = s_taken;
+      }
+      const bool in = tid < here && (r.k == 0 || tid < r.k) && q != 0 && f >= r.floor &&
+                      (r.p == 0.0 || static_cast<double>(before) < r.p * static_cast<double>(taken));
+      weights[tid] = f;
+      here = __syncthreads_count(in);  // kept are the first threads
+      key = in ? key << 32 | tid : 0;
+    }
+    if (cut.whole) {
+      const double mark = u * static_cast<double>(sum);
+      const bool past = static_cast<double>(before + q) > mark || tid == here - 1;
+      if (tid < here && past && (tid == 0 || !(static_cast<double>(before) > mark)))
+        Write(a, row, static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key >> 32)), f, sum);
+      return;
+    }
+  }
+
+  if (tid < units) unit_weight[tid] = slow ? 0 : unit_item;
+  if (tid == 0) s_last = 0, s_taken = cut.k_before;
+  __syncthreads();
+  uint64_t last = 0;  // rank key of the last token that top_k and top_p keep; 0: every token
   if (slow) {
     uint64_t taken = cut.all;
     if (r.k != 0) last = CutByDigits<T>(a, r, x, pow2, r.k, -1.0, &taken);
@@ -538,111 +822,80 @@ __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout 
       const uint64_t by_p = CutByDigits<T>(a, r, x, pow2, 0, r.p * static_cast<double>(taken), &taken);
       last = max(last, by_p);
     }
-    for (int s = 0; s < l.slices; ++s) {
-      uint64_t sum = 0, all;
-      for (int i = s * l.length + tid; i < min(a.vocab, (s + 1) * l.length); i += kDrawThreads) {
+    for (int s = 0; s < units; ++s) {
+      uint64_t part = 0, all;
+      for (int i = s * kUnit + tid; i < min(a.vocab, (s + 1) * kUnit); i += kDrawThreads) {
         const float v = One<T>(x, i);
-        const double f = r.Weight(v, pow2);
-        if (RankKey(v, i) >= last && f >= r.floor) sum += Row::Units(f);
+        const double g = r.Weight(v, pow2);
+        if (RankKey(v, i) >= last && g >= r.floor) part += Row::Units(g);
       }
-      Before<kDrawThreads>(sum, &all);
-      if (tid == 0) slice_weight[s] = all;
+      Before<kDrawThreads>(part, &all);
+      if (tid == 0) unit_weight[s] = all;
     }
   } else if (n > 0) {
-    float v = 0.0f;
-    int index = 0, bin = -1;
-    uint64_t q = 0;
-    double f = 0.0;
-    if (tid < static_cast<int>(n)) {
-      v = w.list[tid].x, index = w.list[tid].index;
-      f = r.Weight(v, pow2);
-      q = Row::Units(f);
-      bin = r.Bin(v);
-      lx[tid] = v, li[tid] = index, lq[tid] = q;
-    }
+    // One step's tokens, or top_p's step's and then k_bin's.
+    const int bin = tid < static_cast<int>(n) ? r.Bin(ValueOf(key)) : -1;
+    const bool both = cut.k_bin < kBins && cut.p_bin < cut.k_bin;
+    const int p_tokens = both ? __syncthreads_count(bin == cut.p_bin) : 0;
+    if (tid == p_tokens) s_last = before;  // (weight of top_p's step, where k_bin's follow)
     __syncthreads();
-    // rank and weight above within the step
-    uint32_t rank = 0;
-    uint64_t above = 0;
-    if (tid < static_cast<int>(n)) {
-      const int other = bin == cut.k_bin ? cut.p_bin : cut.k_bin;
-      for (int j = 0; j < static_cast<int>(n); ++j) {
-        const float y = lx[j];
-        const bool better = y > v || (y == v && li[j] < index);
-        if (better && (cut.k_bin == cut.p_bin || other == kBins || r.Bin(y) == bin)) ++rank, above += lq[j];
-      }
-    }
-    bool in = bin >= 0 && bin == end_bin;
+    const uint64_t in_step = before - (bin == cut.k_bin ? s_last : 0);
     uint64_t taken = cut.all;
+    bool in = bin >= 0 && bin == end_bin;
     if (cut.k_bin < kBins) {
-      const bool in_k = bin == cut.k_bin && rank < cut.k_left;
-      if (in_k) atomicAdd(reinterpret_cast<unsigned long long*>(&s_kept), static_cast<unsigned long long>(q));
+      const uint32_t rank = tid - p_tokens;
+      if (bin == cut.k_bin && rank == cut.k_left - 1) s_taken = cut.k_before + in_step + q;
       __syncthreads();
-      taken = cut.k_before + s_kept;
-      if (bin == cut.k_bin) in = in && in_k;
+      taken = s_taken;
+      if (bin == cut.k_bin) in = in && rank < cut.k_left;
     }
-    if (cut.p_bin < kBins && bin == cut.p_bin)
-      in = in && static_cast<double>(cut.p_before + above) < r.p * static_cast<double>(taken);
-    if (in && f >= r.floor) atomicAdd(&slice_weight[index / l.length], static_cast<unsigned long long>(q));
-    // the kept token with the smallest key
-    uint64_t key = in ? RankKey(v, index) : ~0ull;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) key = min(key, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(key), o, 64)));
-    __shared__ uint64_t keys[kDrawThreads / 64];
-    if ((tid & 63) == 0) keys[tid >> 6] = key;
+    if (bin == cut.p_bin) in = in && static_cast<double>(cut.p_before + in_step) < r.p * static_cast<double>(taken);
+    if (in && f >= r.floor) atomicAdd(&unit_weight[IndexOf(key) / kUnit], static_cast<unsigned long long>(q));
+    // the kept ones are the first threads of the step
+    const int kept = __syncthreads_count(in);
+    if (tid == kept - 1) s_last = key;
     __syncthreads();
-    last = keys[0];
-    for (int i = 1; i < kDrawThreads / 64; ++i) last = min(last, keys[i]);
+    last = s_last;
   }
   __syncthreads();
-  // The slice, then the token in it.
-  __shared__ int s_slice;
+  // The unit, then the token in it.
+  __shared__ int s_unit;
   __shared__ uint64_t s_before, s_total;
-  const double u = fmax(0.0, fmin(static_cast<double>(a.u[row]), 1.0));
   if (tid < 64) {
-    const uint64_t mine = tid < l.slices ? slice_weight[tid] : 0;
-    uint64_t up_to = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t y = __shfl_up(static_cast<unsigned long long>(up_to), o, 64);
-      if (tid >= o) up_to += y;
-    }
-    const uint64_t total = __shfl(static_cast<unsigned long long>(up_to), 63, 64);
+    const uint64_t mine = tid < units ? unit_weight[tid] : 0;
+    const uint64_t up_to = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(mine));
+    const uint64_t total = lanes::ReadLaneT(up_to, 63);
     uint64_t hit = __ballot(mine != 0 && static_cast<double>(up_to) > u * static_cast<double>(total));
     if (hit == 0) hit = 1ull << (63 - __clzll(static_cast<long long>(__ballot(mine != 0))));  // u = 1: the last one
-    const int s = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-    if (tid == s) s_slice = s, s_before = up_to - mine, s_total = total;
+    if (tid == __ffsll(static_cast<unsigned long long>(hit)) - 1) s_unit = tid, s_before = up_to - mine, s_total = total;
   }
   __syncthreads();
-  const int slice = s_slice;
-  const uint64_t total = s_total;
-  const int each = l.length / kDrawThreads;
-  const int from = slice * l.length + tid * each, to = min(from + each, a.vocab);
-  auto kept = [&](int i, double* f) {
-    const float v = One<T>(x, i);
-    *f = r.Weight(v, pow2);
-    return RankKey(v, i) >= last && *f >= r.floor ? Row::Units(*f) : 0;
-  };
-  uint64_t sum = 0, all;
-  double f;
-  for (int i = from; i < to; ++i) sum += kept(i, &f);
-  uint64_t before = s_before + Before<kDrawThreads>(sum, &all);
-  const double mark = u * static_cast<double>(total);
+  constexpr int kEach = kUnit / kDrawThreads;
+  const int from = s_unit * kUnit + tid * kEach;
+  double weight[kEach];
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const float v = from + e < a.vocab ? One<T>(x, from + e) : kNone;
+    weight[e] = r.Weight(v, pow2);
+    if (RankKey(v, from + e) < last || !(weight[e] >= r.floor)) weight[e] = 0.0;
+    sum += Row::Units(weight[e]);
+  }
+  uint64_t all;
+  before = s_before + Before<kDrawThreads>(sum, &all);
+  const double mark = u * static_cast<double>(s_total);
   // the first thread whose sum passes the mark (or the last with a weight)
   const bool past = sum != 0 && (static_cast<double>(before + sum) > mark || before + sum == s_before + all);
-  const bool first = past && !(static_cast<double>(before) > mark);
-  if (first) {
+  if (past && !(static_cast<double>(before) > mark)) {
     int token = -1;
     double at = 0.0;
-    for (int i = from; i < to; ++i) {
-      const uint64_t q = kept(i, &f);
-      if (q == 0) continue;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const uint64_t q = Row::Units(weight[e]);
+      if (q != 0 && !(static_cast<double>(before) > mark)) token = from + e, at = weight[e];
       before += q;
-      token = i, at = f;
-      if (static_cast<double>(before) > mark) break;
     }
-    a.tokens[row] = token;
-    if (a.logprobs != nullptr) a.logprobs[row] = static_cast<float>(log(at / static_cast<double>(total)));
+    Write(a, row, token, at, s_total);
   }
 }
 
