@@ -146,14 +146,14 @@ constexpr uint32_t kNoneBits = paged::kBytes<T> == 4 ? 0xFF800000u : __is_same(T
 
 // 2^(-j / 32)
 __device__ const double kPow2[32] = {
-    1.0, 0.9785720620877001, 0.9576032806985737, 0.93708381705515,
-    0.9170040432046712, 0.8973545375015536, 0.8781260801866497, 0.859309649061239,
-    0.8408964152537145, 0.8228777390769825, 0.8052451659746271, 0.7879904225539432,
-    0.7711054127039704, 0.7545822137967114, 0.7384130729697497, 0.7225904034885233,
-    0.7071067811865476, 0.691954940981916, 0.6771277734684463, 0.6626183215798707,
-    0.6484197773255048, 0.6345254785958666, 0.620928906036742, 0.6076236799902345,
-    0.5946035575013605, 0.5818624293887887, 0.5693943173783458, 0.5571933712979462,
-    0.5452538663326288, 0.5335702003384118, 0.5221368912137069, 0.5109485743270583};
+    0x1.0000000000000p+0, 0x1.f50765b6e4540p-1, 0x1.ea4afa2a490dap-1, 0x1.dfc97337b9b5fp-1,
+    0x1.d5818dcfba487p-1, 0x1.cb720dcef9069p-1, 0x1.c199bdd85529cp-1, 0x1.b7f76f2fb5e47p-1,
+    0x1.ae89f995ad3adp-1, 0x1.a5503b23e255dp-1, 0x1.9c49182a3f090p-1, 0x1.93737b0cdc5e5p-1,
+    0x1.8ace5422aa0dbp-1, 0x1.82589994cce13p-1, 0x1.7a11473eb0187p-1, 0x1.71f75e8ec5f74p-1,
+    0x1.6a09e667f3bcdp-1, 0x1.6247eb03a5585p-1, 0x1.5ab07dd485429p-1, 0x1.5342b569d4f82p-1,
+    0x1.4bfdad5362a27p-1, 0x1.44e086061892dp-1, 0x1.3dea64c123422p-1, 0x1.371a7373aa9cbp-1,
+    0x1.306fe0a31b715p-1, 0x1.29e9df51fdee1p-1, 0x1.2387a6e756238p-1, 0x1.1d4873168b9aap-1,
+    0x1.172b83c7d517bp-1, 0x1.11301d0125b51p-1, 0x1.0b5586cf9890fp-1, 0x1.059b0d3158574p-1};
 
 constexpr double kOne = 17592186044416.0;  // 2^44: the largest weight
 

@@ -23,6 +23,8 @@ gradients are refused while gradients are recorded.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 
 import torch
 
@@ -30,21 +32,8 @@ from . import EngineError, lib
 
 _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml ids
-
-
-class _Cache(ctypes.Structure):
-    _fields_ = [("k", _P), ("v", _P), ("page_stride", _I64), ("head_stride", _I64), ("row_stride", _I64),
-                ("n_pages", _I32), ("page_size", _I32), ("n_kv", _I32), ("head_dim", _I32), ("type", _I32)]
-
-
-class _Seqs(ctypes.Structure):
-    _fields_ = [("table", _P), ("table_stride", _I64), ("lens", _P), ("starts", _P), ("pages", _I32),
-                ("n_seqs", _I32), ("n_tokens", _I32)]
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
-
+# rpg_hip_paged_cache, rpg_hip_sequences, rpg_hip_rows, packed as C lays them out
+_CACHE, _SEQS, _ROWS = struct.Struct("PPqqqiiiii"), struct.Struct("PqPPiii"), struct.Struct("Pqq")
 
 _SIGS = {
     "rpg_hip_paged_append": ([_P, _P, _P, _P, _P, _P, _I32, _P, _P, _F, _P, _I64, _P], _I32),
@@ -74,7 +63,7 @@ def _ok(rc):
     return rc
 
 
-def _check(cond, what):
+def _need(cond, what):
     if not cond:
         raise EngineError(what)
 
@@ -84,18 +73,16 @@ class PagedCache:
     (f32, f16 or bf16; views of a larger pool are fine)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        _check(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
-        _check(k.dtype in _TYPES and v.dtype == k.dtype, "k and v are both float32, float16 or bfloat16")
-        _check(k.is_cuda and v.device == k.device, "k and v lie on one GPU")
-        _check(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
+        _need(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
+        _need(k.dtype in _TYPES and v.dtype == k.dtype, "k and v are both float32, float16 or bfloat16")
+        _need(k.is_cuda and v.device == k.device, "k and v lie on one GPU")
+        _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
         self.k, self.v = k, v
         self.device, self.dtype = k.device, k.dtype
         n_pages, n_kv, page, dim = k.shape
         self.n_kv, self.head_dim, self.page_size = n_kv, dim, page
         strides = [s if n > 1 else page * dim * 16 for n, s in zip(k.shape, k.stride())]
-        self._c = _Cache(k.data_ptr(), v.data_ptr(), strides[0], strides[1], strides[2], n_pages, page, n_kv, dim,
-                         _TYPES[k.dtype])
-        self._p = ctypes.byref(self._c)
+        self._c = _CACHE.pack(k.data_ptr(), v.data_ptr(), *strides[:3], n_pages, page, n_kv, dim, _TYPES[k.dtype])
 
     @classmethod
     def zeros(cls, n_pages: int, page_size: int, n_kv: int, head_dim: int, dtype=torch.float32,
@@ -105,51 +92,62 @@ class PagedCache:
 
 
 def _ints(x, name, dims, device):
-    _check(x.dtype == torch.int32 and x.dim() == dims and x.device == device and (x.shape[-1] <= 1 or x.stride(-1) == 1),
-           f"{name} is int32, of {dims} dimension(s), contiguous in the last, on the cache's GPU")
-    return x.data_ptr()
+    shape = x.shape
+    if x.dtype is not torch.int32 or len(shape) != dims or x.device != device or (shape[-1] > 1 and x.stride(-1) != 1):
+        raise EngineError(f"{name} is int32, of {dims} dimension(s), contiguous in the last, on the cache's GPU")
+    return shape
 
 
 def _seqs(cache, table, lens, starts, n_tokens):
     dev = cache.device
-    n, pages = table.shape if table.dim() == 2 else (-1, 0)
-    t, le = _ints(table, "table", 2, dev), _ints(lens, "lens", 1, dev)
-    _check(lens.shape[0] == n, "lens and table are of one number of sequences")
-    st = None
+    n, pages = _ints(table, "table", 2, dev)
+    if _ints(lens, "lens", 1, dev)[0] != n:
+        raise EngineError("lens and table are of one number of sequences")
+    at = 0
     if starts is not None:
-        st = _ints(starts, "starts", 1, dev)
-        _check(starts.shape[0] == n + 1, "starts has one value more than there are sequences")
-    return _Seqs(t, table.stride(0), le, st, pages, n, n_tokens)
+        if _ints(starts, "starts", 1, dev)[0] != n + 1:
+            raise EngineError("starts has one value more than there are sequences")
+        at = starts.data_ptr()
+    return _SEQS.pack(table.data_ptr(), table.stride(0), lens.data_ptr(), at, pages, n, n_tokens), n, pages
 
 
-def _rows(x, name, cache, heads=None):
-    _check(x.dim() == 3 and x.dtype == cache.dtype and x.device == cache.device and x.shape[2] == cache.head_dim
-           and x.stride(2) == 1 and (heads is None or x.shape[1] == heads),
-           f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension")
-    _check(not (x.requires_grad and torch.is_grad_enabled()), f"{name} requires gradients: there is no backward pass")
-    t, h = x.stride(0), x.stride(1)
-    if x.shape[0] == 1:
-        t = x.shape[1] * x.shape[2]
-    if x.shape[1] == 1:
-        h = x.shape[2]
-    return _Rows(x.data_ptr(), t, h)
+def _rows(x, name, cache):
+    shape, strides = x.shape, x.stride()
+    if (len(shape) != 3 or x.dtype is not cache.dtype or x.device != cache.device or shape[2] != cache.head_dim
+            or strides[2] != 1):
+        raise EngineError(f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise EngineError(f"{name} requires gradients: there is no backward pass")
+    n, heads, dim = shape
+    return _ROWS.pack(x.data_ptr(), strides[0] if n > 1 else heads * dim, strides[1] if heads > 1 else dim)
 
 
 def _vector(x, name, n, dtype, device):
     """The address of a contiguous vector; None stays None."""
     if x is None:
         return None
-    _check(x.dtype == dtype and x.shape == (n,) and x.device == device and (n <= 1 or x.stride(0) == 1),
-           f"{name} is {dtype} [{n}], contiguous, on the same GPU")
+    if x.dtype is not dtype or x.shape != (n,) or x.device != device or (n > 1 and x.stride(0) != 1):
+        raise EngineError(f"{name} is {dtype} [{n}], contiguous, on the same GPU")
     return x.data_ptr()
 
 
-def _enqueue(device, call):
-    """call(stream) with the tensors' GPU current."""
+def _enqueue(device, f, *args):
+    """f(*args, stream) on the current stream of the tensors' GPU, that GPU current."""
     if torch.cuda.current_device() == device.index:
-        return _ok(call(torch.cuda.current_stream().cuda_stream))
-    with torch.cuda.device(device):
-        return _ok(call(torch.cuda.current_stream().cuda_stream))
+        rc = f(*args, _stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = f(*args, _stream(device.index))
+    if rc < 0:
+        _ok(rc)
+
+
+def _stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same without a Stream object for each call
+    _stream = torch._C._cuda_getCurrentRawStream
 
 
 def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_norm=None, k_norm=None,
@@ -159,46 +157,51 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
     given; may be q). Keys and queries are RMS-normed per head with the gains
     k_norm and q_norm (float32 [dim]) and rotated by rope (float32 [positions,
     dim]: cos | sin) where those are given. Returns q_out."""
-    L = _lib()
-    seqs = _seqs(cache, table, lens, starts, k.shape[0])
-    kr, vr = _rows(k, "k", cache, cache.n_kv), _rows(v, "v", cache, cache.n_kv)
-    _check(v.shape == k.shape, "k and v are of one number of tokens")
+    n = k.shape[0]
+    seqs = _seqs(cache, table, lens, starts, n)[0]
+    kr, vr = _rows(k, "k", cache), _rows(v, "v", cache)
+    if v.shape != k.shape or k.shape[1] != cache.n_kv:
+        raise EngineError("k and v are [tokens, key heads of the cache, head dim]")
     heads, qr, qo = 0, None, None
     if q is not None:
         heads = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _check(q.shape[0] == k.shape[0] and q_out.shape == q.shape, "q, q_out and k are of one number of tokens")
-        qr, qo = ctypes.byref(_rows(q, "q", cache)), ctypes.byref(_rows(q_out, "q_out", cache))
+        if q.shape[0] != n or q_out.shape != q.shape:
+            raise EngineError("q, q_out and k are of one number of tokens")
+        qr, qo = _rows(q, "q", cache), _rows(q_out, "q_out", cache)
     dev, dim = cache.device, cache.head_dim
-    qn, kn = _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev)
     rp, rope_rows = None, 0
     if rope is not None:
-        _check(rope.dtype == torch.float32 and rope.dim() == 2 and rope.shape[1] == dim and rope.is_contiguous()
-               and rope.device == dev, "rope is float32 [positions, head dim], contiguous, on the same GPU")
+        if (rope.dtype is not torch.float32 or rope.dim() != 2 or rope.shape[1] != dim or not rope.is_contiguous()
+                or rope.device != dev):
+            raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
-    _enqueue(dev, lambda s: L.rpg_hip_paged_append(cache._p, ctypes.byref(seqs), ctypes.byref(kr), ctypes.byref(vr), qr,
-                                                   qo, heads, qn, kn, eps, rp, rope_rows, s))
+    _enqueue(dev, _lib().rpg_hip_paged_append, cache._c, seqs, kr, vr, qr, qo, heads,
+             _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
+             rp, rope_rows)
     return q_out
 
 
-def _attention(q, cache, seqs, scale, out, prompt):
-    L = _lib()
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(n_kv, page_size, head_dim, kind, pages, n_seqs, n_tokens, heads, prompt):
+    """rpg_hip_paged_work of these sizes."""
+    wide = page_size * head_dim
+    c = _CACHE.pack(0, 0, n_kv * wide, wide, head_dim, 1, page_size, n_kv, head_dim, kind)
+    return _ok(_lib().rpg_hip_paged_work(c, _SEQS.pack(0, pages, 0, 0, pages, n_seqs, n_tokens), heads, prompt))
+
+
+def _attention(f, q, cache, seqs, n_seqs, pages, n_tokens, scale, out, prompt):
     qr = _rows(q, "q", cache)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        _check(out.shape == q.shape, "out has the shape of q")
-    o = _rows(out, "out", cache)
-    heads = q.shape[1]
-    if scale is None:
-        scale = cache.head_dim ** -0.5
-    sp = ctypes.byref(seqs)
-    size = _ok(L.rpg_hip_paged_work(cache._p, sp, heads, prompt))
+    elif out.shape != q.shape:
+        raise EngineError("out has the shape of q")
+    heads, dim = q.shape[1], cache.head_dim
+    size = _work_bytes(cache.n_kv, cache.page_size, dim, _TYPES[cache.dtype], pages, n_seqs, n_tokens, heads, prompt)
     work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
-    f = L.rpg_hip_paged_prompt if prompt else L.rpg_hip_paged_decode
-    _enqueue(cache.device, lambda s: f(cache._p, sp, ctypes.byref(qr), ctypes.byref(o), heads, scale,
-                                       work.data_ptr() if size else None, size, s))
+    _enqueue(cache.device, f, cache._c, seqs, qr, _rows(out, "out", cache), heads, dim ** -0.5 if scale is None else scale,
+             work.data_ptr() if size else None, size)
     return out
 
 
@@ -206,16 +209,24 @@ def decode_attention(q, cache: PagedCache, table, lens, scale=None, out=None):
     """Attention of one token per sequence, q [sequences, heads, dim], over all of
     its sequence's positions. scale: 1 / sqrt(dim) when not given. out (may be q)
     is made when not given."""
-    _check(q.dim() == 3 and q.shape[0] == lens.shape[0], "q has a row for each sequence")
-    return _attention(q, cache, _seqs(cache, table, lens, None, 0), scale, out, 0)
+    seqs, n, pages = _seqs(cache, table, lens, None, 0)
+    if q.shape[0] != n:
+        raise EngineError("q has a row for each sequence")
+    return _attention(_lib().rpg_hip_paged_decode, q, cache, seqs, n, pages, 0, scale, out, 0)
 
 
 def prompt_attention(q, cache: PagedCache, table, lens, starts, scale=None, out=None):
     """Causal attention of the packed new tokens, q [tokens, heads, dim]: the token
     at position p of its sequence over positions 0 .. p, whose keys and values
     lie in the cache (the new tokens' own too)."""
-    _check(q.dim() == 3, "q is [tokens, heads, head dim]")
-    return _attention(q, cache, _seqs(cache, table, lens, starts, q.shape[0]), scale, out, 1)
+    tokens = q.shape[0]
+    seqs, n, pages = _seqs(cache, table, lens, starts, tokens)
+    return _attention(_lib().rpg_hip_paged_prompt, q, cache, seqs, n, pages, tokens, scale, out, 1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _sample_bytes(rows, vocab):
+    return _ok(_lib().rpg_hip_sample_rows_work(rows, vocab))
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
@@ -223,22 +234,21 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     temperature, top_p and min_p (float32), top_k (int32) and u are [rows] on the
     logits' GPU; None sets no limit (temperature 1). Returns (tokens int32, log
     of each token's probability among those kept, float32)."""
-    L = _lib()
-    _check(logits.dim() == 2 and logits.dtype in _TYPES and logits.is_cuda
-           and (logits.shape[1] <= 1 or logits.stride(1) == 1),
-           "logits are [rows, vocab] float32, float16 or bfloat16 on a GPU, contiguous in the last dimension")
-    _check(not (logits.requires_grad and torch.is_grad_enabled()), "logits require gradients: there is no backward pass")
+    if (logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise EngineError("logits are [rows, vocab] float32, float16 or bfloat16 on a GPU, contiguous in the last dimension")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise EngineError("logits require gradients: there is no backward pass")
+    if u is None:
+        raise EngineError("u is needed")
     rows, vocab = logits.shape
     dev, f32 = logits.device, torch.float32
-    _check(u is not None, "u is needed")
-    up, t, p = _vector(u, "u", rows, f32, dev), _vector(temperature, "temperature", rows, f32, dev), _vector(
-        top_p, "top_p", rows, f32, dev)
-    m, k = _vector(min_p, "min_p", rows, f32, dev), _vector(top_k, "top_k", rows, torch.int32, dev)
-    size = _ok(L.rpg_hip_sample_rows_work(rows, vocab))
+    size = _sample_bytes(rows, vocab)
     tokens = torch.empty(rows, dtype=torch.int32, device=dev)
     logprobs = torch.empty(rows, dtype=f32, device=dev)
     work = torch.empty(size, dtype=torch.uint8, device=dev)
-    _enqueue(dev, lambda s: L.rpg_hip_sample_rows(_TYPES[logits.dtype], logits.data_ptr(), rows, vocab, logits.stride(0),
-                                                  t, k, p, m, up, tokens.data_ptr(), logprobs.data_ptr(),
-                                                  work.data_ptr(), size, s))
+    _enqueue(dev, _lib().rpg_hip_sample_rows, _TYPES[logits.dtype], logits.data_ptr(), rows, vocab, logits.stride(0),
+             _vector(temperature, "temperature", rows, f32, dev), _vector(top_k, "top_k", rows, torch.int32, dev),
+             _vector(top_p, "top_p", rows, f32, dev), _vector(min_p, "min_p", rows, f32, dev), _vector(u, "u", rows, f32, dev),
+             tokens.data_ptr(), logprobs.data_ptr(), work.data_ptr(), size)
     return tokens, logprobs

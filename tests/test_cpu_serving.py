@@ -13,25 +13,40 @@ import serving_plain as plain
 from rpgbarengine_amd import serving
 
 A = 0x10000  # an address: refused calls follow none
+P, I32, I64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+class Cache(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("page_stride", I64), ("head_stride", I64), ("row_stride", I64), ("n_pages", I32),
+                ("page_size", I32), ("n_kv", I32), ("head_dim", I32), ("type", I32)]
+
+
+class Seqs(ctypes.Structure):
+    _fields_ = [("table", P), ("table_stride", I64), ("lens", P), ("starts", P), ("pages", I32), ("n_seqs", I32),
+                ("n_tokens", I32)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", P), ("token_stride", I64), ("head_stride", I64)]
 
 
 def cache(**over):
     f = dict(k=A, v=A, page_stride=4 * 16 * 128, head_stride=16 * 128, row_stride=128, n_pages=9, page_size=16, n_kv=4,
              head_dim=128, type=1)
     f.update(over)
-    return serving._Cache(**f)
+    return Cache(**f)
 
 
 def seqs(**over):
     f = dict(table=A, table_stride=8, lens=A, starts=A, pages=8, n_seqs=3, n_tokens=7)
     f.update(over)
-    return serving._Seqs(**f)
+    return Seqs(**f)
 
 
 def rows(**over):
     f = dict(data=A, token_stride=1024, head_stride=128)
     f.update(over)
-    return serving._Rows(**f)
+    return Rows(**f)
 
 
 def refused(rc, word):
@@ -145,6 +160,14 @@ def test_work_sizes():
     refused(L.rpg_hip_sample_rows_work(1, 262145), "logits")
     refused(L.rpg_hip_sample_rows_work(70000, 10), "rows")
     assert L.rpg_hip_sample_rows_work(300, 151936) > L.rpg_hip_sample_rows_work(1, 151936)
+
+
+def test_packed_structs_are_laid_out_as_c_does():
+    c = Cache(1, 2, 3, 4, 5, 6, 7, 8, 9, 10)
+    assert bytes(c)[:serving._CACHE.size] == serving._CACHE.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10)
+    s = Seqs(1, 2, 3, 4, 5, 6, 7)
+    assert bytes(s)[:serving._SEQS.size] == serving._SEQS.pack(1, 2, 3, 4, 5, 6, 7)
+    assert bytes(Rows(1, -2, 3)) == serving._ROWS.pack(1, -2, 3)
 
 
 def test_tensors_without_a_gpu_are_refused():
