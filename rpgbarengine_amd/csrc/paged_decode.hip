@@ -34,16 +34,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kCols = 16;  // query heads of a workgroup
-constexpr int kRangeUnit = 128;  // a key range's positions are a multiple of this: the workgroup's step (64 in f32)
-
-// Positions of one key range of a sequence of len positions.
-__device__ __forceinline__ int RangeOf(int len, int splits) {
-  return ((len - 1) / splits / kRangeUnit + 1) * kRangeUnit;
-}
-
-// x - y of maxima that may both be -inf (no key yet): then 0.
-__device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
-
 // A wave's keys of one step, as 16-key halves (two, in f32 one): K as A operands
 // (lane: 16 bytes of key l % 16 per 64 bytes of a row), V as the lane's
 // dimensions of keys 4 (l / 16) + r.
@@ -185,24 +175,6 @@ struct State {
   }
 };
 
-// Work: [row][splits] (maximum, sum), then [row][splits][kDim] outputs that are
-// not yet divided by the sum; row = sequence x query head.
-__device__ __forceinline__ F2* PartStats(const AttentionArgs& a, int64_t row) {
-  return reinterpret_cast<F2*>(a.work) + row * a.splits;
-}
-template <int kDim>
-__device__ __forceinline__ float* PartOut(const AttentionArgs& a, int64_t rows, int64_t row) {
-  return a.work + 2 * rows * a.splits + row * a.splits * kDim;
-}
-
-template <typename T>
-__device__ __forceinline__ void Store4(char* p, F4 x) {
-  if constexpr (kBytes<T> == 4)
-    *reinterpret_cast<F4*>(p) = x;
-  else
-    *reinterpret_cast<U2*>(p) = U2{Pack2<T>(x[0], x[1]), Pack2<T>(x[2], x[3])};
-}
-
 // grid (sequence x key head x block of 16 query heads, key range)
 template <typename T, int kDim>
 __global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
@@ -264,8 +236,7 @@ __global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
       o += *reinterpret_cast<const F4*>(&so[w][h][d]);
     }
     if (alone) {
-      // No key left (an empty sequence, pages that are not there): zeros.
-      o *= l > 0.0f ? 1.0f / l : (m == kNegInf ? 0.0f : 1.0f / l);
+      o *= Inverse(m, l);
       Store4<T>(a.out.p + seq * a.out.token_bytes + (h0 + h) * a.out.head_bytes + d * kBytes<T>, o);
     } else {
       const int64_t row = static_cast<int64_t>(seq) * a.n_heads + h0 + h;
@@ -275,56 +246,14 @@ __global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
   }
 }
 
-// Joins the ranges of one row: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
-// Workgroup = row; its 256 threads are kDim / 4 columns of four dimensions times
-// the parts that take the ranges in turn.
-constexpr int kMaxSplits = 512;
 template <typename T, int kDim>
-__global__ __launch_bounds__(256) void JoinKernel(AttentionArgs a) {
-  constexpr int kThreadsD = kDim / 4, kParts = 256 / kThreadsD;
-  __shared__ float weight[kMaxSplits];
-  __shared__ float sm[4], sl[4];
-  __shared__ __align__(16) float so[kParts][kDim];
-  const int64_t row = blockIdx.x, rows = static_cast<int64_t>(a.s.n_seqs) * a.n_heads;
+__global__ __launch_bounds__(256) void DecodeJoinKernel(AttentionArgs a) {
+  const int64_t row = blockIdx.x;
   const int seq = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
   const int len = Length(a.s, seq), range = RangeOf(max(len, 1), a.splits);
   if (range >= len) return;  // written by its one range
-  const int n = (len + range - 1) / range, tid = threadIdx.x;
-  const F2* stats = PartStats(a, row);
-  F2 mine[kMaxSplits / 256];
-  float top = kNegInf;
-#pragma unroll
-  for (int i = 0; i < kMaxSplits / 256; ++i) {
-    mine[i] = tid + 256 * i < n ? stats[tid + 256 * i] : F2{kNegInf, 0.0f};
-    top = fmaxf(top, mine[i][0]);
-  }
-  top = lanes::WaveMaxF(top);
-  if ((tid & 63) == 0) sm[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kMaxSplits / 256; ++i) {
-    const float f = __builtin_amdgcn_exp2f(MaxDiff(mine[i][0], top));
-    if (tid + 256 * i < n) weight[tid + 256 * i] = f;
-    l += mine[i][1] * f;
-  }
-  l = lanes::WaveSumF(l);
-  if ((tid & 63) == 0) sl[tid >> 6] = l;
-  __syncthreads();
-  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const int d = tid % kThreadsD * 4, part = tid / kThreadsD;
-  const float* po = PartOut<kDim>(a, rows, row) + d;
-  F4 o = {};
-#pragma unroll 4
-  for (int s = part; s < n; s += kParts) o += *reinterpret_cast<const F4*>(po + static_cast<int64_t>(s) * kDim) * weight[s];
-  *reinterpret_cast<F4*>(&so[part][d]) = o;
-  __syncthreads();
-  if (part != 0) return;
-#pragma unroll
-  for (int p = 1; p < kParts; ++p) o += *reinterpret_cast<const F4*>(&so[p][d]);
-  o *= l > 0.0f ? 1.0f / l : (top == kNegInf ? 0.0f : 1.0f / l);
-  Store4<T>(a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes + d * kBytes<T>, o);
+  JoinRow<T, kDim>(a, static_cast<int64_t>(a.s.n_seqs) * a.n_heads, row, (len + range - 1) / range,
+                   a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes);
 }
 
 template <typename T, int kDim>
@@ -334,7 +263,7 @@ void Launch(const AttentionArgs& a, hipStream_t s) {
   DecodeKernel<T, kDim><<<dim3(static_cast<uint32_t>(x), a.splits), 64 * kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
   if (a.splits == 1) return;
-  JoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_seqs) * a.n_heads, 256, 0, s>>>(a);
+  DecodeJoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_seqs) * a.n_heads, 256, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
 }
 

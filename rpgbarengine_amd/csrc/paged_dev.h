@@ -5,6 +5,7 @@
 
 #include <cstdint>
 
+#include "lanes.h"
 #include "paged.h"
 
 namespace rpg {
@@ -35,8 +36,9 @@ __device__ __forceinline__ int Length(const Seqs& s, int seq) { return max(0, mi
 // The page of the 16 positions from pos on (a page holds a multiple of 16), or
 // -1 where the table names none: such a page is never read or written, and its
 // positions take no part.
+// (Read by a scalar load: nothing writes the table while a kernel runs.)
 __device__ __forceinline__ int PageAt(const Cache& c, const int32_t* row, int pos) {
-  const int page = row[pos >> c.page_log2];
+  const int page = *(const __attribute__((address_space(4))) int32_t*)(row + (pos >> c.page_log2));
   return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.n_pages) ? page : -1;
 }
 
@@ -68,9 +70,11 @@ __device__ __forceinline__ void Unpack2(uint32_t u, float* a, float* b) {
   }
 }
 
-// The empty asm behind a product keeps its sources live past it, so that the
-// result is never allocated over them (an MFMA whose destination aliases its
-// A or B registers gives wrong sums on gfx950).
+// An MFMA whose destination aliases its A or B registers gives wrong sums on
+// gfx950, and the compiler allows it where the sum starts or moves to other
+// registers. The empty asm behind such a product holds the sources past it. It
+// also holds back the loads behind it, so running sums that stay where they are
+// go without; a test reads the built kernels for overlaps.
 // D[4 (l / 16) + e][l % 16] += sum_k A[l % 16][k] B[k][l % 16]; a lane holds the
 // eight k of its l / 16 (16-bit types), the one k = l / 16 (f32).
 template <typename T>
@@ -89,21 +93,138 @@ __device__ __forceinline__ F4 Mfma16F32(float a, float b, F4 c) {
   return r;
 }
 // D[8 (e / 4) + 4 (l / 32) + e % 4][l % 32] += sum_k A[l % 32][k] B[k][l % 32]; a
-// lane holds the eight k of its l / 32 (16-bit types), the one k = l / 32 (f32).
+// lane holds the eight k of its l / 32.
 template <typename T>
 __device__ __forceinline__ F16v Mfma32(U4 a, U4 b, F16v c) {
-  F16v r;
   if constexpr (__is_same(T, BF16))
-    r = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(B8, a), __builtin_bit_cast(B8, b), c, 0, 0, 0);
   else
-    r = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(H8, a), __builtin_bit_cast(H8, b), c, 0, 0, 0);
+}
+// the first product of a sum
+template <typename T>
+__device__ __forceinline__ F16v Mfma32First(U4 a, U4 b) {
+  const F16v r = Mfma32<T>(a, b, F16v{});
   asm volatile("" ::"v"(a), "v"(b), "v"(r));
   return r;
 }
-__device__ __forceinline__ F16v Mfma32F32(float a, float b, F16v c) {
-  const F16v r = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
-  asm volatile("" ::"v"(a), "v"(b), "v"(r));
-  return r;
+
+// x = hi + mid + lo exactly, three bf16 parts of a pair of floats: hi truncated
+// (so that no finite value becomes infinite), mid to nearest, lo what is left
+// (8 bits). Not for values that are not finite (inf - inf).
+struct Parts {
+  uint32_t hi, mid, lo;
+};
+__device__ __forceinline__ Parts Split3(float a, float b) {
+  Parts p;
+  p.hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  const float a1 = a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+  const float b1 = b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+  p.mid = Pack2<BF16>(a1, b1);
+  float am, bm;
+  Unpack2<BF16>(p.mid, &am, &bm);
+  p.lo = Pack2<BF16>(a1 - am, b1 - bm);
+  return p;
+}
+struct Parts8 {
+  U4 hi, mid, lo;
+  __device__ __forceinline__ void Set(int i, Parts p) { hi[i] = p.hi, mid[i] = p.mid, lo[i] = p.lo; }
+};
+// f32 products on the bf16 matrix units: the six products of parts down to
+// 2^-16 of the whole (the dropped ones, mid lo, lo mid and lo lo, are below 2^-22
+// of it and of either sign, as fp32's own roundings), 192 cycles for 16 keys or
+// dimensions where the f32 instruction takes 512. Smallest first.
+__device__ __forceinline__ F16v Mfma32x5(const Parts8& a, const Parts8& b, F16v c) {
+  c = Mfma32<BF16>(a.hi, b.lo, c);
+  c = Mfma32<BF16>(a.mid, b.mid, c);
+  c = Mfma32<BF16>(a.mid, b.hi, c);
+  c = Mfma32<BF16>(a.hi, b.mid, c);
+  return Mfma32<BF16>(a.hi, b.hi, c);
+}
+__device__ __forceinline__ F16v Mfma32x6(const Parts8& a, const Parts8& b, F16v c) {
+  return Mfma32x5(a, b, Mfma32<BF16>(a.lo, b.hi, c));
+}
+__device__ __forceinline__ F16v Mfma32x6First(const Parts8& a, const Parts8& b) {
+  return Mfma32x5(a, b, Mfma32First<BF16>(a.lo, b.hi));
+}
+
+constexpr int kRangeUnit = 128;  // a key range's positions are a multiple of this, a workgroup's step
+
+// Positions of one key range of a sequence of len positions.
+__device__ __forceinline__ int RangeOf(int len, int splits) {
+  return ((len - 1) / splits / kRangeUnit + 1) * kRangeUnit;
+}
+
+// x - y of maxima that may both be -inf (no key yet): then 0.
+__device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
+
+// Work: [row][splits] (maximum, sum), then [row][splits][kDim] outputs that are
+// not yet divided by the sum; row = query
+// token x head.
+__device__ __forceinline__ F2* PartStats(const AttentionArgs& a, int64_t row) {
+  return reinterpret_cast<F2*>(a.work) + row * a.splits;
+}
+template <int kDim>
+__device__ __forceinline__ float* PartOut(const AttentionArgs& a, int64_t rows, int64_t row) {
+  return a.work + 2 * rows * a.splits + row * a.splits * kDim;
+}
+
+template <typename T>
+__device__ __forceinline__ void Store4(char* p, F4 x) {
+  if constexpr (kBytes<T> == 4)
+    *reinterpret_cast<F4*>(p) = x;
+  else
+    *reinterpret_cast<U2*>(p) = U2{Pack2<T>(x[0], x[1]), Pack2<T>(x[2], x[3])};
+}
+
+// 1 / l; no key at all (an empty sequence, pages that are not there): 0.
+__device__ __forceinline__ float Inverse(float m, float l) { return m == kNegInf && l == 0.0f ? 0.0f : 1.0f / l; }
+
+// Joins the n ranges of one row: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).
+// A workgroup's 256 threads are kDim / 4 columns of four dimensions times the
+// parts that take the ranges in turn.
+constexpr int kMaxSplits = 512;
+template <typename T, int kDim>
+__device__ __forceinline__ void JoinRow(const AttentionArgs& a, int64_t rows, int64_t row, int n, char* out) {
+  constexpr int kThreadsD = kDim / 4, kParts = 256 / kThreadsD;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float sm[4], sl[4];
+  __shared__ __align__(16) float so[kParts][kDim];
+  const int tid = threadIdx.x;
+  const F2* stats = PartStats(a, row);
+  F2 mine[kMaxSplits / 256];
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    mine[i] = tid + 256 * i < n ? stats[tid + 256 * i] : F2{kNegInf, 0.0f};
+    top = fmaxf(top, mine[i][0]);
+  }
+  top = lanes::WaveMaxF(top);
+  if ((tid & 63) == 0) sm[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / 256; ++i) {
+    const float f = __builtin_amdgcn_exp2f(MaxDiff(mine[i][0], top));
+    if (tid + 256 * i < n) weight[tid + 256 * i] = f;
+    l += mine[i][1] * f;
+  }
+  l = lanes::WaveSumF(l);
+  if ((tid & 63) == 0) sl[tid >> 6] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const int d = tid % kThreadsD * 4, part = tid / kThreadsD;
+  const float* po = PartOut<kDim>(a, rows, row) + d;
+  F4 o = {};
+#pragma unroll 4
+  for (int s = part; s < n; s += kParts) o += *reinterpret_cast<const F4*>(po + static_cast<int64_t>(s) * kDim) * weight[s];
+  *reinterpret_cast<F4*>(&so[part][d]) = o;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int p = 1; p < kParts; ++p) o += *reinterpret_cast<const F4*>(&so[p][d]);
+  Store4<T>(out + d * kBytes<T>, o * Inverse(top, l));
 }
 
 }  // namespace paged

@@ -29,18 +29,22 @@ namespace paged {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kRows = 32 * kWaves;  // rows of a workgroup's tile
 
-template <typename T, int kDim>
+template <typename T, int kDim, int kGroups>
 struct Shape {
-  static constexpr int kKeys = kBytes<T> == 4 ? 32 : 64;      // keys of a step
+  static constexpr int kGroupWaves = kWaves / kGroups;
+  static constexpr int kRows = 32 * kGroupWaves;              // rows of a workgroup's tile
+  static constexpr int kKeys = kBytes<T> == 4 || kGroups > 1 ? 32 : 64;  // keys of a group's step
   static constexpr int kBlocks = kKeys / 32;                  // 32-key score blocks
   static constexpr int kRowBytes = kDim * kBytes<T>;          // a cache row
   static constexpr int kChunks = kRowBytes / 16;              // its 16-byte chunks
-  static constexpr int kPerThread = kKeys * kChunks / (64 * kWaves);
+  static constexpr int kPerThread = kKeys * kChunks / (64 * kGroupWaves);
   static constexpr int kRowsPerLoad = 64 / kChunks;           // rows of a wave's load instruction
+  static constexpr int kWaveRows = kKeys / kGroupWaves;       // rows that a wave stages
+  static constexpr int kUnit = kWaveRows < 16 ? kWaveRows : 16;  // rows looked up in the page table together
+  static constexpr int kUnits = kKeys / kUnit;
   static constexpr int kTileBytes = kKeys * kRowBytes;
-  static constexpr int kQ = kDim * kBytes<T> / 32;            // 16-byte pieces of a query row per lane
+  static constexpr int kQ = kDim / 16;                        // products over a query row
 };
 
 // Chunk c of row r lies at chunk c ^ KSwizzle(r) or VSwizzle(r) of its LDS row.
@@ -49,22 +53,42 @@ struct Shape {
 // is one lane's base, xored with a constant.
 template <typename T, int kDim>
 __device__ __forceinline__ constexpr int KSwizzle(int r) {
-  return r & (Shape<T, kDim>::kChunks - 1);
+  return r & (kDim * kBytes<T> / 16 - 1);
 }
 template <typename T, int kDim>
 __device__ __forceinline__ constexpr int VSwizzle(int r) {
   if constexpr (kBytes<T> == 4) return 0;  // read a row at a time
-  return (((r & 3) << 2) | ((r >> 2) & 3)) & (Shape<T, kDim>::kChunks - 1);
+  return (((r & 3) << 2) | ((r >> 2) & 3)) & (kDim * kBytes<T> / 16 - 1);
+}
+
+// A product's operand: eight values, in f32 as three bf16 parts.
+template <typename T>
+struct OperandOf {
+  typedef U4 type;
+};
+template <>
+struct OperandOf<F32> {
+  typedef Parts8 type;
+};
+template <typename T>
+using Operand = typename OperandOf<T>::type;
+__device__ __forceinline__ Parts8 Split8(U4 x, U4 y) {
+  Parts8 p;
+  p.Set(0, Split3(__uint_as_float(x[0]), __uint_as_float(x[1])));
+  p.Set(1, Split3(__uint_as_float(x[2]), __uint_as_float(x[3])));
+  p.Set(2, Split3(__uint_as_float(y[0]), __uint_as_float(y[1])));
+  p.Set(3, Split3(__uint_as_float(y[2]), __uint_as_float(y[3])));
+  return p;
 }
 
 // The sequence that row tile b belongs to, -1 for none: tiles of sequence s
-// start at floor(starts[s] G / kRows) + s, which leaves each its
-// ceil(n_new G / kRows) tiles wherever the starts lie.
-__device__ __forceinline__ int SequenceOfTile(const Seqs& s, int group, int b) {
+// start at floor(starts[s] G / rows) + s, which leaves each its ceil(n_new G /
+// rows) tiles wherever the starts lie.
+__device__ __forceinline__ int SequenceOfTile(const Seqs& s, int group, int rows, int b) {
   const int lane = threadIdx.x & 63;
   int n = 0;
   for (int j = 0; j < s.n_seqs; j += 64) {
-    const bool le = j + lane < s.n_seqs && s.starts[j + lane] * group / kRows + j + lane <= b;
+    const bool le = j + lane < s.n_seqs && s.starts[j + lane] * group / rows + j + lane <= b;
     n += __popcll(__ballot(le));
   }
   return n - 1;
@@ -89,99 +113,176 @@ __device__ __forceinline__ int OddKind(uint32_t u) {
   return (u & (kSign - 1)) != kInf ? 2 : u & kSign ? 1 : 0;
 }
 
-typedef __amdgpu_buffer_rsrc_t Rsrc;
-// 16 bytes per lane from the resource to LDS, a wave's lanes side by side
-__device__ __forceinline__ void LdsDma(Rsrc src, char* to, int voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, voff, soff, 0, 0);
+// What a row whose last key is `limit` has added in dimension d.
+template <int kDim>
+__device__ __forceinline__ float OddSum(const int (&first_odd)[kOddKinds][kDim], int d, int limit) {
+  const bool plus = first_odd[0][d] <= limit, minus = first_odd[1][d] <= limit, nan = first_odd[2][d] <= limit;
+  const float inf = -kNegInf;
+  return nan || (plus && minus) ? __builtin_nanf("") : plus ? inf : minus ? -inf : 0.0f;
 }
 
-// grid (row tile x key head): key heads next to each other, the tiles with
-// the most keys first.
+// The dimension of row m of output block w.
 template <typename T, int kDim>
-__global__ __launch_bounds__(64 * kWaves, 2) void PromptKernel(AttentionArgs a) {
-  using Sh = Shape<T, kDim>;
-  __shared__ __align__(256) char lds[4 * Sh::kTileBytes];  // [2][K tile, V tile]
-  __shared__ uint32_t page_ok[2];              // per buffer: a byte for each wave's rows
+__device__ __forceinline__ int DimOf(int w, int m) {
+  return kBytes<T> == 4 ? (kDim / 32) * m + w : 32 * w + m;
+}
+
+// A buffer resource (wave-uniform) over `bytes` bytes from p.
+__device__ __forceinline__ U4 Resource(const char* p, uint32_t bytes) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  return U4{static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(u))),
+            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(u >> 32))) & 0xFFFFu, bytes, 0x00020000u};
+}
+// 16 bytes per lane from the resource to LDS, a wave's lanes side by side. In
+// assembly, since the compiler holds every LDS read after the builtin until the
+// load is done, though the reads are of another buffer: the waits are those of
+// `landed`, before the tile's first read. It writes no register.
+__device__ __forceinline__ void LdsDma(U4 src, char* to, int voff, int soff) {
+  const uint32_t at = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(at), "v"(voff), "s"(src), "s"(soff));
+}
+
+// A row tile: its sequence and rows, and the positions it stands for.
+struct RowTile {
+  int first, row0, n_rows, len, pos0;  // first: the sequence's first token; row0: of the sequence's n_rows
+  __device__ __forceinline__ int Position(int row, int group) const { return pos0 + min(row, n_rows - 1) / group; }
+};
+// false: there is no such tile
+__device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int tile, int* seq, RowTile* t) {
+  *seq = SequenceOfTile(s, group, rows, tile);
+  if (*seq < 0) return false;
+  t->first = s.starts[*seq];
+  const int n_new = s.starts[*seq + 1] - t->first;
+  if (t->first < 0 || n_new <= 0 || t->first > s.n_tokens - n_new) return false;
+  t->n_rows = n_new * group;
+  t->row0 = (tile - (t->first * group / rows + *seq)) * rows;
+  t->len = Length(s, *seq);
+  t->pos0 = t->len - n_new;
+  return t->row0 >= 0 && t->row0 < t->n_rows;
+}
+
+// grid (row tile x key head, key range): key heads next to each other, the tiles
+// with the most keys first.
+template <typename T, int kDim, int kGroups>
+__global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKernel(AttentionArgs a) {
+  using Sh = Shape<T, kDim, kGroups>;
+  __shared__ __align__(256) char lds[kGroups * 4 * Sh::kTileBytes];  // per group [2][K tile, V tile]
+  __shared__ uint32_t page_ok[kGroups][2];     // per buffer: a byte for each unit of rows
   __shared__ int any_odd, first_odd[kOddKinds][kDim];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / Sh::kGroupWaves, gw = wave % Sh::kGroupWaves;  // the wave's group, its place there
   const int group = a.n_heads / a.c.n_kv;
   const int kh = blockIdx.x % a.c.n_kv;
-  const int tile = static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.c.n_kv);
-  const int seq = SequenceOfTile(a.s, group, tile);
-  if (seq < 0) return;
-  const int first = a.s.starts[seq], n_new = a.s.starts[seq + 1] - first;
-  if (first < 0 || n_new <= 0 || first > a.s.n_tokens - n_new) return;
-  const int row0 = (tile - (first * group / kRows + seq)) * kRows, n_rows = n_new * group;
-  if (row0 < 0 || row0 >= n_rows) return;
-  const int len = Length(a.s, seq), pos0 = len - n_new;
+  int seq;
+  RowTile t;
+  if (!TileOf(a.s, group, Sh::kRows, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.c.n_kv), &seq, &t)) return;
+  const int first = t.first, n_rows = t.n_rows, row0 = t.row0, len = t.len, pos0 = t.pos0;
 
   // this lane's row: a query token and head, and the last key it sees
   const int h = lane >> 5;
-  const int row = min(row0 + 32 * wave + (lane & 31), n_rows - 1);
+  const int row = min(row0 + 32 * gw + (lane & 31), n_rows - 1);
   const int token = row / group, head = kh * group + row % group;
   const int limit = pos0 + token;  // (< len)
-  const int wave_first = pos0 + min(row0 + 32 * wave, n_rows - 1) / group;
-  const int wave_last = pos0 + min(row0 + 32 * wave + 31, n_rows - 1) / group;
-  const int tile_first = pos0 + row0 / group, tile_last = pos0 + min(row0 + kRows - 1, n_rows - 1) / group;
-  const int steps = tile_last < 0 ? 0 : tile_last / Sh::kKeys + 1;
+  const int wave_first = t.Position(row0 + 32 * gw, group), wave_last = t.Position(row0 + 32 * gw + 31, group);
+  const int tile_first = t.Position(row0, group), keys = t.Position(row0 + Sh::kRows - 1, group) + 1;
+  int key_begin = 0, key_end = max(keys, 0);
+  if constexpr (kGroups == 4) {
+    const int range = RangeOf(max(keys, 1), a.splits);
+    key_begin = blockIdx.y * range;
+    key_end = min(key_end, key_begin + range);
+    if (key_begin >= key_end && blockIdx.y > 0) return;
+  }
+  // steps of the workgroup: a step of every group each
+  const int steps = key_end <= key_begin ? 0 : (key_end - key_begin - 1) / (Sh::kKeys * kGroups) + 1;
 
-  U4 q[Sh::kQ];
+  // The query row as B operands: dimensions 16 i + 8 h .. + 7 (f32: in parts).
+  Operand<T> q[Sh::kQ];
   {
-    const char* qp = a.q.p + (first + token) * a.q.token_bytes + head * a.q.head_bytes + 16 * h;
+    const char* qp = a.q.p + (first + token) * a.q.token_bytes + head * a.q.head_bytes + 8 * h * kBytes<T>;
 #pragma unroll
-    for (int i = 0; i < Sh::kQ; ++i) q[i] = Load16(qp + 32 * i);
+    for (int i = 0; i < Sh::kQ; ++i) {
+      if constexpr (kBytes<T> == 4)
+        q[i] = Split8(Load16(qp + 64 * i), Load16(qp + 64 * i + 16));
+      else
+        q[i] = Load16(qp + 32 * i);
+    }
   }
   const int32_t* table = a.s.table + seq * a.s.table_stride;
   const int64_t head_off = kh * a.c.head_bytes;
   const int in_page = (1 << a.c.page_log2) - 1;
   if (tid == 0) any_odd = 0;
+  if (tid < 2 * kGroups) page_ok[tid / 2][tid % 2] = 0x01010101u;
   for (int i = tid; i < kOddKinds * kDim; i += 64 * kWaves) first_odd[i / kDim][i % kDim] = INT32_MAX;
   __syncthreads();
 
-  // Staging by LDS DMA: a wave brings kKeys / 4 rows (of one page), a lane
-  // kPerThread chunks of K and of V, in LDS the wave's lanes side by side.
-  constexpr int kWaveRows = Sh::kKeys / kWaves;
+  // Staging by LDS DMA: a wave brings kWaveRows rows, a lane kPerThread chunks
+  // of K and of V, in LDS the wave's lanes side by side.
+  constexpr int kWaveRows = Sh::kWaveRows, kWaveUnits = kWaveRows / Sh::kUnit;
   const int srow = lane / Sh::kChunks, sc = lane % Sh::kChunks;
   const int row_from = srow * a.c.row_bytes;
-  const int k_from = 16 * (sc ^ KSwizzle<T, kDim>(wave * kWaveRows + srow));
-  const int v_from = 16 * (sc ^ VSwizzle<T, kDim>(wave * kWaveRows + srow));
-  const int to = wave * kWaveRows * Sh::kRowBytes;
-  bool ok = false;
-  auto fetch = [&](int step) {
-    const int p0 = step * Sh::kKeys + wave * kWaveRows;
-    const int p = min(p0, (len - 1) & ~(kWaveRows - 1));  // rows that are there
-    const int page = PageAt(a.c, table, p);
-    ok = page >= 0 && p0 < len;
-    const int64_t at = max(page, 0) * a.c.page_bytes + head_off + (p & in_page & ~(kWaveRows - 1)) * static_cast<int64_t>(a.c.row_bytes);
-    const int bytes = (kWaveRows - 1) * a.c.row_bytes + Sh::kRowBytes;
-    const Rsrc kb = __builtin_amdgcn_make_buffer_rsrc(a.c.k + at, 0, bytes, 0x00020000);
-    const Rsrc vb = __builtin_amdgcn_make_buffer_rsrc(a.c.v + at, 0, bytes, 0x00020000);
-    char* kt = lds + (step & 1) * 2 * Sh::kTileBytes + to;
+  const int k_from = 16 * (sc ^ KSwizzle<T, kDim>(gw * kWaveRows + srow));
+  const int v_from = 16 * (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + srow));
+  const int to = gw * kWaveRows * Sh::kRowBytes;
+  bool ok[kWaveUnits] = {};
+  // the first key of the group's part of a step
+  auto first_key = [&](int step) { return key_begin + (step * kGroups + grp) * Sh::kKeys; };
+  // Page numbers a step ahead of the loads that follow them.
+  int ahead[kWaveUnits];
+  auto look_up = [&](int step) {
 #pragma unroll
-    for (int i = 0; i < Sh::kPerThread; ++i) {
-      const int up = i * Sh::kRowsPerLoad;
-      LdsDma(kb, kt + 1024 * i, row_from + (k_from ^ 16 * KSwizzle<T, kDim>(up)), up * a.c.row_bytes);
-      LdsDma(vb, kt + Sh::kTileBytes + 1024 * i, row_from + (v_from ^ 16 * VSwizzle<T, kDim>(up)), up * a.c.row_bytes);
+    for (int u = 0; u < kWaveUnits; ++u) {
+      const int p0 = first_key(step) + gw * kWaveRows + u * Sh::kUnit;
+      ahead[u] = PageAt(a.c, table, max(min(p0, len - 1), 0));
     }
   };
-  // The wave's rows have landed; what they need before the others read them.
+  char* tiles = lds + grp * 4 * Sh::kTileBytes;
+  auto fetch = [&](int step) {
+    char* kt = tiles + (step & 1) * 2 * Sh::kTileBytes + to;
+#pragma unroll
+    for (int u = 0; u < kWaveUnits; ++u) {
+      const int p0 = first_key(step) + gw * kWaveRows + u * Sh::kUnit;
+      const int p = min(p0, (len - 1) & ~(Sh::kUnit - 1));  // rows that are there
+      const int page = __builtin_amdgcn_readfirstlane(ahead[u]);
+      ok[u] = page >= 0 && p0 < len;
+      const int64_t at = max(page, 0) * a.c.page_bytes + head_off + (p & in_page) * static_cast<int64_t>(a.c.row_bytes);
+      const uint32_t bytes = (Sh::kUnit - 1) * a.c.row_bytes + Sh::kRowBytes;
+      const U4 kb = Resource(a.c.k + at, bytes), vb = Resource(a.c.v + at, bytes);
+      constexpr int kLoads = Sh::kPerThread / kWaveUnits;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int up = i * Sh::kRowsPerLoad, in_wave = u * Sh::kUnit + up;
+        char* to_k = kt + 1024 * (u * kLoads + i);
+        LdsDma(kb, to_k, row_from + (k_from ^ 16 * KSwizzle<T, kDim>(in_wave)), up * a.c.row_bytes);
+        LdsDma(vb, to_k + Sh::kTileBytes, row_from + (v_from ^ 16 * VSwizzle<T, kDim>(in_wave)), up * a.c.row_bytes);
+      }
+    }
+  };
+  // The wave's rows have landed; what they need before they are read.
   auto landed = [&](int step) {
-    const int buf = step & 1, p0 = step * Sh::kKeys + wave * kWaveRows;
+    const int buf = step & 1, p0 = first_key(step) + gw * kWaveRows;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if ((step + 1) * Sh::kKeys > tile_first || !ok) {  // some row does not see all keys
-      char* vt = lds + buf * 2 * Sh::kTileBytes + Sh::kTileBytes + to + 16 * lane;
+    bool all = true;
+#pragma unroll
+    for (int u = 0; u < kWaveUnits; ++u) all = all && ok[u];
+    // A step that some row does not see all keys of; in f32 every step, since
+    // the parts of an infinity are not one.
+    if (kBytes<T> == 4 || first_key(step) + Sh::kKeys > tile_first || !all) {
+      char* vt = tiles + (2 * buf + 1) * Sh::kTileBytes + to + 16 * lane;
 #pragma unroll
       for (int i = 0; i < Sh::kPerThread; ++i) {
         // Rows past the sequence and of unnamed pages may hold anything, NaN
         // among it: zeros in place of their values (their scores are masked).
         const int r = i * Sh::kRowsPerLoad + srow;
         U4 v = *reinterpret_cast<const U4*>(vt + 1024 * i);
-        const bool in = ok && p0 + r < len;
+        const bool in = ok[i * Sh::kRowsPerLoad / Sh::kUnit] && p0 + r < len;
         bool odd = !in;
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd = odd || NotFinite<T>(v[e]);
         if (odd) {
-          const int d0 = (sc ^ VSwizzle<T, kDim>(wave * kWaveRows + r)) * (16 / kBytes<T>);
+          const int d0 = (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + r)) * (16 / kBytes<T>);
 #pragma unroll 1
           for (int e = 0; e < 16 / kBytes<T>; ++e) {
             const int word = e * kBytes<T> / 4, shift = kBytes<T> == 4 ? 0 : 16 * (e & 1);
@@ -196,13 +297,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PromptKernel(AttentionArgs a) 
         }
       }
     }
-    if (lane == 0) reinterpret_cast<volatile uint8_t*>(&page_ok[buf])[wave] = ok ? 1 : 0;
-    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int u = 0; u < kWaveUnits; ++u)
+        reinterpret_cast<volatile uint8_t*>(&page_ok[grp][buf])[gw * kWaveUnits + u] = ok[u] ? 1 : 0;
+    }
+    if constexpr (Sh::kGroupWaves > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_wave_barrier();
   };
 
   // where this lane reads: K row l % 32, chunks 2 i + h; V rows 4 h + 8 u + (0 .. 3),
   // chunk pairs of its 16 lanes' dimensions
-  const int k_at = (lane & 31) * Sh::kRowBytes + 16 * (h ^ KSwizzle<T, kDim>(lane & 31));
+  const int k_at = (lane & 31) * Sh::kRowBytes + 16 * (h * (kBytes<T> / 2) ^ KSwizzle<T, kDim>(lane & 31));
   int v_at[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -213,38 +321,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PromptKernel(AttentionArgs a) 
   float m = kNegInf, l = 0.0f;
   F16v o[kDim / 32] = {};
   if (steps > 0) {
+    look_up(0);
     fetch(0);
+    look_up(1);
     landed(0);
   }
   for (int step = 0; step < steps; ++step) {
-    if (step + 1 < steps) fetch(step + 1);
-    const int key0 = step * Sh::kKeys;
-    if (key0 <= wave_last) {
+    if (step + 1 < steps) {
+      fetch(step + 1);
+      look_up(step + 2);
+    }
+    const int key0 = first_key(step);
+    if (key0 <= wave_last && key0 < key_end) {
       const int buf = step & 1;
-      const char* kt = lds + buf * 2 * Sh::kTileBytes;
+      const char* kt = tiles + 2 * buf * Sh::kTileBytes;
       const char* vt = kt + Sh::kTileBytes;
-      F16v s[Sh::kBlocks] = {};
+      F16v s[Sh::kBlocks];
 #pragma unroll
       for (int b = 0; b < Sh::kBlocks; ++b) {
 #pragma unroll
         for (int i = 0; i < Sh::kQ; ++i) {
-          const U4 k = *reinterpret_cast<const U4*>(kt + (k_at ^ 32 * i) + 32 * b * Sh::kRowBytes);
+          const char* at = kt + 32 * b * Sh::kRowBytes;
           if constexpr (kBytes<T> == 4) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[b] = Mfma32F32(__uint_as_float(k[e]), __uint_as_float(q[i][e]), s[b]);
+            const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 64 * i));
+            const U4 y = *reinterpret_cast<const U4*>(at + (k_at ^ (64 * i + 16)));
+            s[b] = i == 0 ? Mfma32x6First(Split8(x, y), q[i]) : Mfma32x6(Split8(x, y), q[i], s[b]);
           } else {
-            s[b] = Mfma32<T>(k, q[i], s[b]);
+            const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 32 * i));
+            s[b] = i == 0 ? Mfma32First<T>(x, q[i]) : Mfma32<T>(x, q[i], s[b]);
           }
         }
       }
-      const uint32_t pages = page_ok[buf];
+      const uint32_t pages = page_ok[grp][buf];
       if (key0 + Sh::kKeys - 1 > wave_first || pages != 0x01010101u) {
 #pragma unroll
         for (int b = 0; b < Sh::kBlocks; ++b)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int key = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
-            const bool in = key0 + key <= limit && ((pages >> (8 * (key / kWaveRows))) & 1);
+            const bool in = key0 + key <= limit && ((pages >> (8 * (key / Sh::kUnit))) & 1);
             s[b][e] = in ? s[b][e] : kNegInf;
           }
       }
@@ -273,13 +388,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PromptKernel(AttentionArgs a) 
         // dimension (kDim / 32) m + w in row m of output block w
         const char* vl = vt + 4 * h * Sh::kRowBytes + (kDim / 8) * (lane & 31);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float* v = reinterpret_cast<const float*>(vl + (8 * (e / 4) + e % 4) * Sh::kRowBytes);
-          float x[kDim / 32];
+        for (int j = 0; j < 2; ++j) {
+          // keys 16 j + 4 h + {0 .. 3, 8 .. 11}, as the scores come
+          Parts8 p, v[kDim / 32];
 #pragma unroll
-          for (int w = 0; w < kDim / 32; ++w) x[w] = v[w];
+          for (int e = 0; e < 4; ++e) {
+            p.Set(e, Split3(s[0][8 * j + 2 * e], s[0][8 * j + 2 * e + 1]));
+            const int key = 16 * j + 8 * (e / 2) + 2 * (e % 2);
+            const float* x = reinterpret_cast<const float*>(vl + key * Sh::kRowBytes);
+            const float* y = reinterpret_cast<const float*>(vl + (key + 1) * Sh::kRowBytes);
 #pragma unroll
-          for (int w = 0; w < kDim / 32; ++w) o[w] = Mfma32F32(x[w], s[0][e], o[w]);
+            for (int w = 0; w < kDim / 32; ++w) v[w].Set(e, Split3(x[w], y[w]));
+          }
+#pragma unroll
+          for (int w = 0; w < kDim / 32; ++w) o[w] = Mfma32x6(v[w], p, o[w]);
         }
       } else {
         // The weights are rounded to the cache's 16 bits for the product (each
@@ -312,49 +434,143 @@ __global__ __launch_bounds__(64 * kWaves, 2) void PromptKernel(AttentionArgs a) 
   }
 
   l = lanes::AddXor32(l);
-  if (any_odd) {
+  if constexpr (kGroups == 1) {
+    if (any_odd) {  // (all of it was found before the last step's barrier)
 #pragma unroll
-    for (int w = 0; w < kDim / 32; ++w)
+      for (int w = 0; w < kDim / 32; ++w)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int mm = 8 * (e / 4) + 4 * h + e % 4, d = kBytes<T> == 4 ? (kDim / 32) * mm + w : 32 * w + mm;
-        const float inf = -kNegInf;
-        if (first_odd[0][d] <= limit) o[w][e] += inf;
-        if (first_odd[1][d] <= limit) o[w][e] -= inf;
-        if (first_odd[2][d] <= limit) o[w][e] += __builtin_nanf("");
+        for (int e = 0; e < 16; ++e) o[w][e] += OddSum(first_odd, DimOf<T, kDim>(w, 8 * (e / 4) + 4 * h + e % 4), limit);
+    }
+    const float inv = Inverse(m, l);
+    if (row0 + 32 * gw + (lane & 31) < n_rows) {
+      char* out = a.out.p + (first + token) * a.out.token_bytes + head * a.out.head_bytes;
+      if constexpr (kBytes<T> == 4) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float* to = reinterpret_cast<float*>(out) + (kDim / 32) * (8 * (e / 4) + 4 * h + e % 4);
+          if constexpr (kDim == 128)
+            *reinterpret_cast<F4*>(to) = F4{o[0][e], o[1][e], o[2][e], o[3][e]} * inv;
+          else
+            *reinterpret_cast<F2*>(to) = F2{o[0][e], o[1][e]} * inv;
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < kDim / 32; ++w)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            Store4<T>(out + 2 * (32 * w + 2 * e + 4 * h), F4{o[w][e], o[w][e + 1], o[w][e + 2], o[w][e + 3]} * inv);
       }
-  }
-  // No key (positions before the cache's first, pages that are not there): zeros.
-  const float inv = m == kNegInf && l == 0.0f ? 0.0f : 1.0f / l;
-  if (row0 + 32 * wave + (lane & 31) < n_rows) {
-    char* out = a.out.p + (first + token) * a.out.token_bytes + head * a.out.head_bytes;
-    if constexpr (kBytes<T> == 4) {
+    }
+  } else {
+    // The groups' states, joined in LDS where the tiles were.
+    __shared__ float sm[kGroups][Sh::kRows], sl[kGroups][Sh::kRows];
+    static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= 4 * Sh::kTileBytes, "a group's state fits its tiles");
+    // chunk c (four dimensions) of row r of group g
+    auto at = [&](int g, int r, int c) {
+      return reinterpret_cast<F4*>(lds + g * 4 * Sh::kTileBytes + r * kDim * 4 + (c ^ (r & 15)) * 16);
+    };
+    const int r = 32 * gw + (lane & 31);
+    if (h == 0) sm[grp][r] = m, sl[grp][r] = l;
+    __syncthreads();
+    float top = sm[0][r];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float* to = reinterpret_cast<float*>(out) + (kDim / 32) * (8 * (e / 4) + 4 * h + e % 4);
-        if constexpr (kDim == 128)
-          *reinterpret_cast<F4*>(to) = F4{o[0][e], o[1][e], o[2][e], o[3][e]} * inv;
-        else
-          *reinterpret_cast<F2*>(to) = F2{o[0][e], o[1][e]} * inv;
-      }
+    for (int i = 1; i < kGroups; ++i) top = fmaxf(top, sm[i][r]);
+    const float f = __builtin_amdgcn_exp2f(MaxDiff(m, top));
+    if constexpr (kBytes<T> == 4 && kDim == 128) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) *at(grp, r, 8 * (e / 4) + 4 * h + e % 4) = F4{o[0][e], o[1][e], o[2][e], o[3][e]} * f;
+    } else if constexpr (kBytes<T> == 4) {
+#pragma unroll
+      for (int e = 0; e < 16; e += 2)
+        *at(grp, r, (8 * (e / 4) + 4 * h + e % 4) / 2) = F4{o[0][e], o[1][e], o[0][e + 1], o[1][e + 1]} * f;
     } else {
 #pragma unroll
       for (int w = 0; w < kDim / 32; ++w)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<U2*>(out + 2 * (32 * w + 2 * e + 4 * h)) =
-              U2{Pack2<T>(o[w][e] * inv, o[w][e + 1] * inv), Pack2<T>(o[w][e + 2] * inv, o[w][e + 3] * inv)};
+          *at(grp, r, (32 * w + 2 * e + 4 * h) / 4) = F4{o[w][e], o[w][e + 1], o[w][e + 2], o[w][e + 3]} * f;
     }
+    __syncthreads();
+    const bool odd = any_odd != 0;
+    const bool alone = a.splits == 1 || RangeOf(max(keys, 1), a.splits) >= keys;
+    for (int i = tid; i < Sh::kRows * (kDim / 4); i += 64 * kWaves) {
+      const int ri = i / (kDim / 4), d = i % (kDim / 4) * 4, row_i = row0 + ri;
+      if (row_i >= n_rows) break;
+      float mi = sm[0][ri], li = 0.0f;
+#pragma unroll
+      for (int k = 1; k < kGroups; ++k) mi = fmaxf(mi, sm[k][ri]);
+      F4 x = {};
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        li += sl[k][ri] * __builtin_amdgcn_exp2f(MaxDiff(sm[k][ri], mi));
+        x += *at(k, ri, d / 4);
+      }
+      const int token_i = row_i / group, head_i = kh * group + row_i % group;
+      if (odd) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += OddSum(first_odd, d + e, pos0 + token_i);
+      }
+      if (alone) {
+        Store4<T>(a.out.p + (first + token_i) * a.out.token_bytes + head_i * a.out.head_bytes + d * kBytes<T>,
+                  x * Inverse(mi, li));
+      } else {
+        const int64_t rows = static_cast<int64_t>(a.s.n_tokens) * a.n_heads;
+        const int64_t out_row = static_cast<int64_t>(first + token_i) * a.n_heads + head_i;
+        if (d == 0) PartStats(a, out_row)[blockIdx.y] = F2{mi, li};
+        *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(blockIdx.y) * kDim + d) = x;
+      }
+    }
+  }
+}
+
+// Joins the key ranges of a tile's rows (four groups, 32 rows): workgroup = row.
+template <typename T, int kDim>
+__global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
+  const int64_t row = blockIdx.x;
+  const int token = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
+  const int group = a.n_heads / a.c.n_kv;
+  // the sequence, and the row's tile there
+  const int lane = threadIdx.x & 63;
+  int seq = 0;
+  for (int j = 0; j < a.s.n_seqs; j += 64)
+    seq += __popcll(__ballot(j + lane < a.s.n_seqs && a.s.starts[j + lane + 1] <= token));
+  if (seq >= a.s.n_seqs) return;
+  const int first = a.s.starts[seq], n_new = a.s.starts[seq + 1] - first;
+  if (token < first || first < 0 || first > a.s.n_tokens - n_new) return;
+  const int len = Length(a.s, seq), pos0 = len - n_new;
+  const int tile = ((token - first) * group + head % group) / 32;
+  const int keys = pos0 + min(32 * tile + 31, n_new * group - 1) / group + 1;
+  const int range = RangeOf(max(keys, 1), a.splits);
+  if (range >= keys) return;  // written by its one range
+  JoinRow<T, kDim>(a, static_cast<int64_t>(a.s.n_tokens) * a.n_heads, row, (keys + range - 1) / range,
+                   a.out.p + token * a.out.token_bytes + head * a.out.head_bytes);
+}
+
+int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups);
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes);
+
+template <typename T, int kDim, int kGroups>
+void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
+  const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, kGroups);
+  RPG_CHECK(tiles * a.c.n_kv < (int64_t{1} << 31), "paged_prompt: too many rows for one launch");
+  PromptKernel<T, kDim, kGroups>
+      <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * kWaves, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
+  if constexpr (kGroups == 4) {
+    if (a.splits == 1) return;
+    PromptJoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_tokens) * a.n_heads, 256, 0, s>>>(a);
+    HIP_CHECK(hipGetLastError());
   }
 }
 
 template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
-  const int64_t rows = static_cast<int64_t>(a.s.n_tokens) * (a.n_heads / a.c.n_kv);
-  const int64_t tiles = rows / kRows + a.s.n_seqs;
-  RPG_CHECK(tiles * a.c.n_kv < (int64_t{1} << 31), "paged_prompt: too many rows for one launch");
-  PromptKernel<T, kDim><<<static_cast<uint32_t>(tiles * a.c.n_kv), 64 * kWaves, 0, s>>>(a);
-  HIP_CHECK(hipGetLastError());
+  const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv, kBytes<T>);
+  if constexpr (kBytes<T> == 2) {
+    if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
+  }
+  if (groups == 2) return LaunchGroups<T, kDim, 2>(a, s);
+  LaunchGroups<T, kDim, 1>(a, s);
 }
 
 template <typename T>
@@ -365,7 +581,26 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
     Launch<T, 64>(a, s);
 }
 
+int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
+  return n_tokens * group / (128 / groups) + n_seqs;
+}
+
+// Groups of a workgroup (its rows: 128 / groups).
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes) {
+  const int group = n_heads / n_kv;
+  if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 512) return 1;
+  if (bytes == 4 || TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 512) return 2;
+  return 4;
+}
+
 }  // namespace
+
+int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
+  if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv, bytes) != 4) return 1;
+  const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv;
+  const int64_t want = wgs >= 256 ? 1 : CeilDiv(512, wgs);
+  return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
+}
 
 void Prompt(const AttentionArgs& a, hipStream_t s) {
   if (a.s.n_tokens == 0 || a.s.n_seqs == 0) return;
