@@ -42,7 +42,6 @@ struct Shape {
   static constexpr int kRowsPerLoad = 64 / kChunks;           // rows of a wave's load instruction
   static constexpr int kWaveRows = kKeys / kGroupWaves;       // rows that a wave stages
   static constexpr int kUnit = kWaveRows < 16 ? kWaveRows : 16;  // rows looked up in the page table together
-  static constexpr int kUnits = kKeys / kUnit;
   static constexpr int kTileBytes = kKeys * kRowBytes;
   static constexpr int kQ = kDim / 16;                        // products over a query row
 };
@@ -135,8 +134,8 @@ __device__ __forceinline__ U4 Resource(const char* p, uint32_t bytes) {
 }
 // 16 bytes per lane from the resource to LDS, a wave's lanes side by side. In
 // assembly, since the compiler holds every LDS read after the builtin until the
-// load is done, though the reads are of another buffer: the waits are those of
-// `landed`, before the tile's first read. It writes no register.
+// load is done, though the reads are of another buffer: the waits are
+// written out, before the tile's first read. It writes no register.
 __device__ __forceinline__ void LdsDma(U4 src, char* to, int voff, int soff) {
   const uint32_t at = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to));
@@ -167,9 +166,15 @@ __device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int t
 // grid (row tile x key head, key range): key heads next to each other, the tiles
 // with the most keys first.
 template <typename T, int kDim, int kGroups>
-__global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kGroups == 2 ? 1 : 2) void PromptKernel(AttentionArgs a) {
   using Sh = Shape<T, kDim, kGroups>;
-  __shared__ __align__(256) char lds[kGroups * 4 * Sh::kTileBytes];  // per group [2][K tile, V tile]
+  // A group of one wave needs no barriers: it takes the next K tile in as soon as
+  // the scores are done and the next V tile after the second product, each in the
+  // place of the last (half the LDS: two workgroups per compute unit). Groups of
+  // several waves have two of each in turn.
+  constexpr bool kSolo = Sh::kGroupWaves == 1;
+  constexpr int kBuffers = kSolo ? 1 : 2;
+  __shared__ __align__(256) char lds[kGroups * 2 * kBuffers * Sh::kTileBytes];  // per group [buffer][K tile, V tile]
   __shared__ uint32_t page_ok[kGroups][2];     // per buffer: a byte for each unit of rows
   __shared__ int any_odd, first_odd[kOddKinds][kDim];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -226,10 +231,14 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKerne
   const int k_from = 16 * (sc ^ KSwizzle<T, kDim>(gw * kWaveRows + srow));
   const int v_from = 16 * (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + srow));
   const int to = gw * kWaveRows * Sh::kRowBytes;
-  bool ok[kWaveUnits] = {};
+  char* tiles = lds + grp * 2 * kBuffers * Sh::kTileBytes;
   // the first key of the group's part of a step
   auto first_key = [&](int step) { return key_begin + (step * kGroups + grp) * Sh::kKeys; };
-  // Page numbers a step ahead of the loads that follow them.
+  // Where a step's rows of this wave lie. Page numbers are looked up a step ahead.
+  struct Place {
+    int64_t at[kWaveUnits];
+    bool ok[kWaveUnits];
+  };
   int ahead[kWaveUnits];
   auto look_up = [&](int step) {
 #pragma unroll
@@ -238,74 +247,72 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKerne
       ahead[u] = PageAt(a.c, table, max(min(p0, len - 1), 0));
     }
   };
-  char* tiles = lds + grp * 4 * Sh::kTileBytes;
-  auto fetch = [&](int step) {
-    char* kt = tiles + (step & 1) * 2 * Sh::kTileBytes + to;
+  auto place_of = [&](int step) {
+    Place x;
 #pragma unroll
     for (int u = 0; u < kWaveUnits; ++u) {
       const int p0 = first_key(step) + gw * kWaveRows + u * Sh::kUnit;
       const int p = min(p0, (len - 1) & ~(Sh::kUnit - 1));  // rows that are there
       const int page = __builtin_amdgcn_readfirstlane(ahead[u]);
-      ok[u] = page >= 0 && p0 < len;
-      const int64_t at = max(page, 0) * a.c.page_bytes + head_off + (p & in_page) * static_cast<int64_t>(a.c.row_bytes);
-      const uint32_t bytes = (Sh::kUnit - 1) * a.c.row_bytes + Sh::kRowBytes;
-      const U4 kb = Resource(a.c.k + at, bytes), vb = Resource(a.c.v + at, bytes);
+      x.ok[u] = page >= 0 && p0 < len;
+      x.at[u] = max(page, 0) * a.c.page_bytes + head_off + (p & in_page) * static_cast<int64_t>(a.c.row_bytes);
+    }
+    return x;
+  };
+  // The wave's rows of a K or V tile: kPerThread loads.
+  auto fetch = [&](const char* pool, const Place& x, char* tile, int from, auto swizzle) {
+#pragma unroll
+    for (int u = 0; u < kWaveUnits; ++u) {
+      const U4 src = Resource(pool + x.at[u], (Sh::kUnit - 1) * a.c.row_bytes + Sh::kRowBytes);
       constexpr int kLoads = Sh::kPerThread / kWaveUnits;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int up = i * Sh::kRowsPerLoad, in_wave = u * Sh::kUnit + up;
-        char* to_k = kt + 1024 * (u * kLoads + i);
-        LdsDma(kb, to_k, row_from + (k_from ^ 16 * KSwizzle<T, kDim>(in_wave)), up * a.c.row_bytes);
-        LdsDma(vb, to_k + Sh::kTileBytes, row_from + (v_from ^ 16 * VSwizzle<T, kDim>(in_wave)), up * a.c.row_bytes);
+        const int up = i * Sh::kRowsPerLoad;
+        LdsDma(src, tile + to + 1024 * (u * kLoads + i), row_from + (from ^ 16 * swizzle(u * Sh::kUnit + up)),
+               up * a.c.row_bytes);
       }
     }
   };
-  // The wave's rows have landed; what they need before they are read.
-  auto landed = [&](int step) {
-    const int buf = step & 1, p0 = first_key(step) + gw * kWaveRows;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  auto fetch_k = [&](const Place& x, char* tile) { fetch(a.c.k, x, tile, k_from, [](int r) { return KSwizzle<T, kDim>(r); }); };
+  auto fetch_v = [&](const Place& x, char* tile) { fetch(a.c.v, x, tile, v_from, [](int r) { return VSwizzle<T, kDim>(r); }); };
+  // What the wave's rows of a V tile need before they are read: rows past the
+  // sequence and of unnamed pages may hold anything, NaN among it, and become
+  // zeros (their scores are masked); values that are not finite go to first_odd
+  // where some row does not see all of the step's keys (in f32 always, since the
+  // parts of an infinity are not one).
+  auto settle_v = [&](int step, const Place& x, char* tile) {
+    const int p0 = first_key(step) + gw * kWaveRows;
     bool all = true;
 #pragma unroll
-    for (int u = 0; u < kWaveUnits; ++u) all = all && ok[u];
-    // A step that some row does not see all keys of; in f32 every step, since
-    // the parts of an infinity are not one.
-    if (kBytes<T> == 4 || first_key(step) + Sh::kKeys > tile_first || !all) {
-      char* vt = tiles + (2 * buf + 1) * Sh::kTileBytes + to + 16 * lane;
+    for (int u = 0; u < kWaveUnits; ++u) all = all && x.ok[u];
+    if (kBytes<T> == 2 && first_key(step) + Sh::kKeys <= tile_first && all) return;
+    char* vt = tile + to + 16 * lane;
 #pragma unroll
-      for (int i = 0; i < Sh::kPerThread; ++i) {
-        // Rows past the sequence and of unnamed pages may hold anything, NaN
-        // among it: zeros in place of their values (their scores are masked).
-        const int r = i * Sh::kRowsPerLoad + srow;
-        U4 v = *reinterpret_cast<const U4*>(vt + 1024 * i);
-        const bool in = ok[i * Sh::kRowsPerLoad / Sh::kUnit] && p0 + r < len;
-        bool odd = !in;
+    for (int i = 0; i < Sh::kPerThread; ++i) {
+      const int r = i * Sh::kRowsPerLoad + srow;
+      U4 v = *reinterpret_cast<const U4*>(vt + 1024 * i);
+      if (!(x.ok[i * Sh::kRowsPerLoad / Sh::kUnit] && p0 + r < len)) {
+        *reinterpret_cast<U4*>(vt + 1024 * i) = U4{};
+        v = U4{};
+      }
+      bool odd = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd = odd || NotFinite<T>(v[e]);
-        if (odd) {
-          const int d0 = (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + r)) * (16 / kBytes<T>);
+      for (int e = 0; e < 4; ++e) odd = odd || NotFinite<T>(v[e]);
+      if (odd) {
+        const int d0 = (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + r)) * (16 / kBytes<T>);
 #pragma unroll 1
-          for (int e = 0; e < 16 / kBytes<T>; ++e) {
-            const int word = e * kBytes<T> / 4, shift = kBytes<T> == 4 ? 0 : 16 * (e & 1);
-            const uint32_t u = kBytes<T> == 4 ? v[word] : (v[word] >> shift) & 0xFFFFu;
-            if (in && NotFinite<T>(u)) {
-              atomicMin(&first_odd[OddKind<T>(u)][d0 + e], p0 + r);
-              any_odd = 1;
-            }
-            if (!in || NotFinite<T>(u)) v[word] &= kBytes<T> == 4 ? 0u : 0xFFFF0000u >> shift;
+        for (int e = 0; e < 16 / kBytes<T>; ++e) {
+          const int word = e * kBytes<T> / 4, shift = kBytes<T> == 4 ? 0 : 16 * (e & 1);
+          const uint32_t u = kBytes<T> == 4 ? v[word] : (v[word] >> shift) & 0xFFFFu;
+          if (NotFinite<T>(u)) {
+            atomicMin(&first_odd[OddKind<T>(u)][d0 + e], p0 + r);
+            any_odd = 1;
+            v[word] &= kBytes<T> == 4 ? 0u : 0xFFFF0000u >> shift;
           }
-          *reinterpret_cast<U4*>(vt + 1024 * i) = v;
         }
+        *reinterpret_cast<U4*>(vt + 1024 * i) = v;
       }
     }
-    if (lane == 0) {
-#pragma unroll
-      for (int u = 0; u < kWaveUnits; ++u)
-        reinterpret_cast<volatile uint8_t*>(&page_ok[grp][buf])[gw * kWaveUnits + u] = ok[u] ? 1 : 0;
-    }
-    if constexpr (Sh::kGroupWaves > 1)
-      __syncthreads();
-    else
-      __builtin_amdgcn_wave_barrier();
   };
 
   // where this lane reads: K row l % 32, chunks 2 i + h; V rows 4 h + 8 u + (0 .. 3),
@@ -320,117 +327,184 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKerne
   const float c = a.scale * 1.44269504088896341f;
   float m = kNegInf, l = 0.0f;
   F16v o[kDim / 32] = {};
-  if (steps > 0) {
-    look_up(0);
-    fetch(0);
-    look_up(1);
-    landed(0);
-  }
-  for (int step = 0; step < steps; ++step) {
-    if (step + 1 < steps) {
-      fetch(step + 1);
-      look_up(step + 2);
-    }
-    const int key0 = first_key(step);
-    if (key0 <= wave_last && key0 < key_end) {
-      const int buf = step & 1;
-      const char* kt = tiles + 2 * buf * Sh::kTileBytes;
-      const char* vt = kt + Sh::kTileBytes;
-      F16v s[Sh::kBlocks];
+  F16v s[Sh::kBlocks];
+  auto scores = [&](const char* kt) {
 #pragma unroll
-      for (int b = 0; b < Sh::kBlocks; ++b) {
+    for (int b = 0; b < Sh::kBlocks; ++b) {
 #pragma unroll
-        for (int i = 0; i < Sh::kQ; ++i) {
-          const char* at = kt + 32 * b * Sh::kRowBytes;
-          if constexpr (kBytes<T> == 4) {
-            const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 64 * i));
-            const U4 y = *reinterpret_cast<const U4*>(at + (k_at ^ (64 * i + 16)));
-            s[b] = i == 0 ? Mfma32x6First(Split8(x, y), q[i]) : Mfma32x6(Split8(x, y), q[i], s[b]);
-          } else {
-            const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 32 * i));
-            s[b] = i == 0 ? Mfma32First<T>(x, q[i]) : Mfma32<T>(x, q[i], s[b]);
-          }
+      for (int i = 0; i < Sh::kQ; ++i) {
+        const char* at = kt + 32 * b * Sh::kRowBytes;
+        if constexpr (kBytes<T> == 4) {
+          const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 64 * i));
+          const U4 y = *reinterpret_cast<const U4*>(at + (k_at ^ (64 * i + 16)));
+          s[b] = i == 0 ? Mfma32x6First(Split8(x, y), q[i]) : Mfma32x6(Split8(x, y), q[i], s[b]);
+        } else {
+          const U4 x = *reinterpret_cast<const U4*>(at + (k_at ^ 32 * i));
+          s[b] = i == 0 ? Mfma32First<T>(x, q[i]) : Mfma32<T>(x, q[i], s[b]);
         }
       }
-      const uint32_t pages = page_ok[grp][buf];
-      if (key0 + Sh::kKeys - 1 > wave_first || pages != 0x01010101u) {
-#pragma unroll
-        for (int b = 0; b < Sh::kBlocks; ++b)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
-            const bool in = key0 + key <= limit && ((pages >> (8 * (key / Sh::kUnit))) & 1);
-            s[b][e] = in ? s[b][e] : kNegInf;
-          }
-      }
-      float top = kNegInf;
-#pragma unroll
-      for (int b = 0; b < Sh::kBlocks; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
-      top = lanes::MaxXor32(top) * c;
-      if (__any(top > m)) {
-        const float now = fmaxf(m, top), f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-        m = now;
-        l *= f;
-#pragma unroll
-        for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
-      }
-      const float base = m == kNegInf ? 0.0f : m;
+    }
+  };
+  // Masks, the running maximum, weights in place of scores.
+  auto weigh = [&](int key0, uint32_t pages) {
+    if (key0 + Sh::kKeys - 1 > wave_first || pages != 0x01010101u) {
 #pragma unroll
       for (int b = 0; b < Sh::kBlocks; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          s[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], c, -base));
-          l += s[b][e];
+          const int key = 32 * b + 8 * (e / 4) + 4 * h + e % 4;
+          const bool in = key0 + key <= limit && ((pages >> (8 * (key / Sh::kUnit))) & 1);
+          s[b][e] = in ? s[b][e] : kNegInf;
         }
-      if constexpr (kBytes<T> == 4) {
-        // dimension (kDim / 32) m + w in row m of output block w
-        const char* vl = vt + 4 * h * Sh::kRowBytes + (kDim / 8) * (lane & 31);
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int b = 0; b < Sh::kBlocks; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
+    top = lanes::MaxXor32(top) * c;
+    // The maximum that weights refer to moves only when one would pass 2^8: most
+    // steps raise some row's, and rescaling costs as much as the exponentials.
+    if (__any(top > m + 8.0f)) {
+      const float now = fmaxf(m, top), f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= f;
+#pragma unroll
+      for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
+    }
+    const float base = m == kNegInf ? 0.0f : m;
+#pragma unroll
+    for (int b = 0; b < Sh::kBlocks; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[b][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], c, -base));
+        l += s[b][e];
+      }
+  };
+  auto add_values = [&](const char* vt) {
+    if constexpr (kBytes<T> == 4) {
+      // dimension (kDim / 32) m + w in row m of output block w
+      const char* vl = vt + 4 * h * Sh::kRowBytes + (kDim / 8) * (lane & 31);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // keys 16 j + 4 h + {0 .. 3, 8 .. 11}, as the scores come
+        Parts8 p, v[kDim / 32];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p.Set(e, Split3(s[0][8 * j + 2 * e], s[0][8 * j + 2 * e + 1]));
+          const int key = 16 * j + 8 * (e / 2) + 2 * (e % 2);
+          const float* x = reinterpret_cast<const float*>(vl + key * Sh::kRowBytes);
+          const float* y = reinterpret_cast<const float*>(vl + (key + 1) * Sh::kRowBytes);
+#pragma unroll
+          for (int w = 0; w < kDim / 32; ++w) v[w].Set(e, Split3(x[w], y[w]));
+        }
+#pragma unroll
+        for (int w = 0; w < kDim / 32; ++w) o[w] = Mfma32x6(v[w], p, o[w]);
+      }
+    } else {
+      // The weights are rounded to the cache's 16 bits for the product (each
+      // by at most half a step, as V itself was); the sum has them unrounded.
+      typedef short S4 __attribute__((ext_vector_type(4)));
+      // A operand: dimensions 32 w .., keys 32 b + 16 j + 4 h + {0 .. 3, 8 .. 11}
+#pragma unroll
+      for (int b = 0; b < Sh::kBlocks; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          // keys 16 j + 4 h + {0 .. 3, 8 .. 11}, as the scores come
-          Parts8 p, v[kDim / 32];
+          U4 p;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p.Set(e, Split3(s[0][8 * j + 2 * e], s[0][8 * j + 2 * e + 1]));
-            const int key = 16 * j + 8 * (e / 2) + 2 * (e % 2);
-            const float* x = reinterpret_cast<const float*>(vl + key * Sh::kRowBytes);
-            const float* y = reinterpret_cast<const float*>(vl + (key + 1) * Sh::kRowBytes);
+          for (int e = 0; e < 4; ++e) p[e] = Pack2<T>(s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
 #pragma unroll
-            for (int w = 0; w < kDim / 32; ++w) v[w].Set(e, Split3(x[w], y[w]));
-          }
+          for (int w = 0; w < kDim / 32; ++w) {
+            U4 v;
 #pragma unroll
-          for (int w = 0; w < kDim / 32; ++w) o[w] = Mfma32x6(v[w], p, o[w]);
-        }
-      } else {
-        // The weights are rounded to the cache's 16 bits for the product (each
-        // by at most half a step, as V itself was); the sum has them unrounded.
-        typedef short S4 __attribute__((ext_vector_type(4)));
-        // A operand: dimensions 32 w .., keys 32 b + 16 j + 4 h + {0 .. 3, 8 .. 11}
-#pragma unroll
-        for (int b = 0; b < Sh::kBlocks; ++b)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            U4 p;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = Pack2<T>(s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
-#pragma unroll
-            for (int w = 0; w < kDim / 32; ++w) {
-              U4 v;
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const char* at = vt + (v_at[u] ^ 64 * w) + (32 * b + 16 * j) * Sh::kRowBytes;
-                const U2 x = __builtin_bit_cast(
-                    U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at));
-                v[2 * u] = x[0], v[2 * u + 1] = x[1];
-              }
-              o[w] = Mfma32<T>(v, p, o[w]);
+            for (int u = 0; u < 2; ++u) {
+              const char* at = vt + (v_at[u] ^ 64 * w) + (32 * b + 16 * j) * Sh::kRowBytes;
+              const U2 x = __builtin_bit_cast(
+                  U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at));
+              v[2 * u] = x[0], v[2 * u + 1] = x[1];
             }
+            o[w] = Mfma32<T>(v, p, o[w]);
           }
-      }
+        }
     }
-    if (step + 1 < steps) landed(step + 1);
+  };
+
+  if constexpr (kSolo) {
+    constexpr int kLoads = Sh::kPerThread;
+    char* kt = tiles;
+    char* vt = tiles + Sh::kTileBytes;
+    Place now, next;
+    if (steps > 0) {
+      look_up(0);
+      now = place_of(0);
+      fetch_k(now, kt);
+      fetch_v(now, vt);
+      look_up(1);
+    }
+    for (int step = 0; step < steps; ++step) {
+      const int key0 = first_key(step);
+      const bool mine = key0 <= wave_last && key0 < key_end, more = step + 1 < steps;
+      next = place_of(step + 1);
+      look_up(step + 2);
+      // in flight: K, then V of this step
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+      if (mine) scores(kt);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
+      if (more) fetch_k(next, kt);
+      uint32_t pages = 0;
+#pragma unroll
+      for (int u = 0; u < kWaveUnits; ++u) pages |= (now.ok[u] ? 1u : 0u) << (8 * u);
+#pragma unroll
+      for (int u = kWaveUnits; u < 4; ++u) pages |= 1u << (8 * u);
+      if (mine) weigh(key0, pages);
+      // in flight: V of this step, then K of the next
+      if (more)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (mine) {
+        settle_v(step, now, vt);
+        add_values(vt);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
+      if (more) fetch_v(next, vt);
+      now = next;
+    }
+  } else {
+    Place x;
+    auto tile_of = [&](int step) { return tiles + (step & 1) * 2 * Sh::kTileBytes; };
+    auto begin = [&](int step) {
+      x = place_of(step);
+      fetch_k(x, tile_of(step));
+      fetch_v(x, tile_of(step) + Sh::kTileBytes);
+      look_up(step + 1);
+    };
+    // the wave's rows have landed, and then all of the group's
+    auto landed = [&](int step) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      settle_v(step, x, tile_of(step) + Sh::kTileBytes);
+      if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < kWaveUnits; ++u)
+          reinterpret_cast<volatile uint8_t*>(&page_ok[grp][step & 1])[gw * kWaveUnits + u] = x.ok[u] ? 1 : 0;
+      }
+      __syncthreads();
+    };
+    if (steps > 0) {
+      look_up(0);
+      begin(0);
+      landed(0);
+    }
+    for (int step = 0; step < steps; ++step) {
+      if (step + 1 < steps) begin(step + 1);
+      const int key0 = first_key(step);
+      if (key0 <= wave_last && key0 < key_end) {
+        scores(tile_of(step));
+        weigh(key0, page_ok[grp][step & 1]);
+        add_values(tile_of(step) + Sh::kTileBytes);
+      }
+      if (step + 1 < steps) landed(step + 1);
+    }
   }
 
   l = lanes::AddXor32(l);
@@ -464,10 +538,10 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 1 ? 2 : 1) void PromptKerne
   } else {
     // The groups' states, joined in LDS where the tiles were.
     __shared__ float sm[kGroups][Sh::kRows], sl[kGroups][Sh::kRows];
-    static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= 4 * Sh::kTileBytes, "a group's state fits its tiles");
+    static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= 2 * kBuffers * Sh::kTileBytes, "a group's state fits its tiles");
     // chunk c (four dimensions) of row r of group g
     auto at = [&](int g, int r, int c) {
-      return reinterpret_cast<F4*>(lds + g * 4 * Sh::kTileBytes + r * kDim * 4 + (c ^ (r & 15)) * 16);
+      return reinterpret_cast<F4*>(lds + g * 2 * kBuffers * Sh::kTileBytes + r * kDim * 4 + (c ^ (r & 15)) * 16);
     };
     const int r = 32 * gw + (lane & 31);
     if (h == 0) sm[grp][r] = m, sl[grp][r] = l;
@@ -588,8 +662,8 @@ int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
 // Groups of a workgroup (its rows: 128 / groups).
 int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes) {
   const int group = n_heads / n_kv;
-  if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 512) return 1;
-  if (bytes == 4 || TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 512) return 2;
+  if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 384) return 1;
+  if (bytes == 4 || TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
   return 4;
 }
 
@@ -598,7 +672,7 @@ int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes
 int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
   if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv, bytes) != 4) return 1;
   const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv;
-  const int64_t want = wgs >= 256 ? 1 : CeilDiv(512, wgs);
+  const int64_t want = wgs >= 128 ? 1 : CeilDiv(256, wgs);
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
 }
 
