@@ -23,17 +23,6 @@ namespace rpg {
 namespace paged {
 namespace {
 
-// the number of j in 1 .. n with starts[j] <= t, over the wave's lanes
-__device__ __forceinline__ int SequenceOf(const Seqs& s, int t) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int j = 0; j < s.n_seqs; j += 64) {
-    const bool le = j + lane < s.n_seqs && s.starts[j + lane + 1] <= t;
-    before += __popcll(__ballot(le));
-  }
-  return before;
-}
-
 // sum over aligned groups of kLanes lanes
 template <int kLanes>
 __device__ __forceinline__ float GroupSum(float v) {
@@ -52,91 +41,121 @@ __device__ __forceinline__ float OtherHalf(float v) {
   return __shfl_xor(v, kLanes / 2, 64);
 }
 
-// grid (token, 256 / kLanes rows of it): the token's rows are its query heads,
-// then its key heads, then its value heads.
-template <typename T, int kDim>
+// grid (token, kEach x 256 / kLanes rows of it): the token's rows are its query
+// heads, then its key heads, then its value heads.
+template <typename T, int kDim, int kEach>
 __global__ __launch_bounds__(256) void AppendKernel(AppendArgs a) {
   constexpr int kPer = 16 / kBytes<T>;      // elements of a lane
   constexpr int kLanes = kDim / kPer;       // lanes of a row
+  constexpr int kRows = 256 / kLanes;       // rows of a pass
   const int t = blockIdx.x;
-  const int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, c = threadIdx.x % kLanes;
-  const int nq = a.q.p != nullptr ? a.n_heads : 0;
-  const bool in = row < nq + 2 * a.c.n_kv;
-  const bool is_q = row < nq, is_v = row >= nq + a.c.n_kv;
-  const int head = is_q ? row : is_v ? row - nq - a.c.n_kv : row - nq;
-  const Rows& from = is_q ? a.q : is_v ? a.v : a.k;
-  U4 raw = {};
-  if (in) raw = Load16(from.p + t * from.token_bytes + head * from.head_bytes + 16 * c);
-  const int seq = SequenceOf(a.s, t);
-  if (seq >= a.s.n_seqs) return;  // behind the last sequence
-  const int first = a.s.starts[seq], n_new = a.s.starts[seq + 1] - first;
-  const int pos = Length(a.s, seq) - n_new + (t - first);
+  const int c = threadIdx.x % kLanes;
+  const int nq = a.q.p != nullptr ? a.n_heads : 0, rows = nq + 2 * a.c.n_kv;
+  const int row0 = blockIdx.y * (kEach * kRows) + threadIdx.x / kLanes;
+  // The rows are on their way while the token's place is found.
+  U4 raw[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int row = min(row0 + k * kRows, rows - 1);
+    const bool is_q = row < nq, is_v = row >= nq + a.c.n_kv;
+    const int head = is_q ? row : is_v ? row - nq - a.c.n_kv : row - nq;
+    const Rows& from = is_q ? a.q : is_v ? a.v : a.k;
+    raw[k] = Load16(from.p + t * from.token_bytes + head * from.head_bytes + 16 * c);
+  }
+  Sequence x;
+  if (!FindSequence(a.s, [&](int end, int) { return end <= t; }, &x)) return;  // behind the last sequence
+  const int pos = x.len - x.n_new + (t - x.first);
   // Tokens before the first sequence or at no position of the cache, and those
   // that the rotation table does not reach, are left out.
-  if (t < first || pos < 0 || (a.rope != nullptr && pos >= a.rope_rows)) return;
-  const int page = PageAt(a.c, a.s.table + seq * a.s.table_stride, pos);
-  U4 out = raw;
-  if (!is_v) {
-    float x[kPer];
-    if constexpr (kPer == 8) {
+  if (t < x.first || pos < 0 || (a.rope != nullptr && pos >= a.rope_rows)) return;
+  const int page = PageAt(a.c, a.s.table + x.seq * a.s.table_stride, pos);
+  const int64_t in_cache =
+      max(page, 0) * a.c.page_bytes + (pos & ((1 << a.c.page_log2) - 1)) * static_cast<int64_t>(a.c.row_bytes) + 16 * c;
+  float cs[kPer], sn[kPer];
+  if (a.rope != nullptr) {
+    const float* r = a.rope + static_cast<int64_t>(pos) * kDim + (kPer * c) % (kDim / 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) Unpack2<T>(raw[i], &x[2 * i], &x[2 * i + 1]);
-    } else {
+    for (int i = 0; i < kPer; i += 4) {
+      const F4 u = *reinterpret_cast<const F4*>(r + i), v = *reinterpret_cast<const F4*>(r + kDim / 2 + i);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(raw[i]);
-    }
-    const float* gain = is_q ? a.q_norm : a.k_norm;
-    if (gain != nullptr) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
-      const float mean = GroupSum<kLanes>(sum) * (1.0f / kDim);
-      const float scale = 1.0f / __builtin_sqrtf(mean + a.eps);
-#pragma unroll
-      for (int i = 0; i < kPer; i += 4) {
-        const F4 g = *reinterpret_cast<const F4*>(gain + kPer * c + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i + e] = x[i + e] * scale * g[e];
-      }
-    }
-    if (a.rope != nullptr) {
-      const float* r = a.rope + static_cast<int64_t>(pos) * kDim + (kPer * c) % (kDim / 2);
-      const float sign = c < kLanes / 2 ? -1.0f : 1.0f;
-#pragma unroll
-      for (int i = 0; i < kPer; i += 4) {
-        const F4 cs = *reinterpret_cast<const F4*>(r + i), sn = *reinterpret_cast<const F4*>(r + kDim / 2 + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float other = OtherHalf<kLanes>(x[i + e]);
-          x[i + e] = __builtin_fmaf(x[i + e], cs[e], sign * other * sn[e]);
-        }
-      }
-    }
-    if constexpr (kPer == 8) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = Pack2<T>(x[2 * i], x[2 * i + 1]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[i] = __float_as_uint(x[i]);
+      for (int e = 0; e < 4; ++e) cs[i + e] = u[e], sn[i + e] = c < kLanes / 2 ? -v[e] : v[e];
     }
   }
-  if (!in || (!is_q && page < 0)) return;
-  char* to = is_q ? a.q_out.p + t * a.q_out.token_bytes + head * a.q_out.head_bytes
-                  : (is_v ? a.c.v : a.c.k) + page * a.c.page_bytes + head * a.c.head_bytes +
-                        (pos & ((1 << a.c.page_log2) - 1)) * static_cast<int64_t>(a.c.row_bytes);
-  *reinterpret_cast<U4*>(to + 16 * c) = out;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int row = row0 + k * kRows;
+    const bool is_q = row < nq, is_v = row >= nq + a.c.n_kv;
+    const int head = is_q ? row : is_v ? row - nq - a.c.n_kv : row - nq;
+    U4 out = raw[k];
+    if (!is_v) {
+      float y[kPer];
+      if constexpr (kPer == 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Unpack2<T>(out[i], &y[2 * i], &y[2 * i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __uint_as_float(out[i]);
+      }
+      const float* gain = is_q ? a.q_norm : a.k_norm;
+      if (gain != nullptr) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
+        const float mean = GroupSum<kLanes>(sum) * (1.0f / kDim);
+        const float scale = 1.0f / __builtin_sqrtf(mean + a.eps);
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) {
+          const F4 g = *reinterpret_cast<const F4*>(gain + kPer * c + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[i + e] = y[i + e] * scale * g[e];
+        }
+      }
+      if (a.rope != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const float other = OtherHalf<kLanes>(y[i]);
+          y[i] = __builtin_fmaf(y[i], cs[i], other * sn[i]);
+        }
+      }
+      if constexpr (kPer == 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = Pack2<T>(y[2 * i], y[2 * i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = __float_as_uint(y[i]);
+      }
+    }
+    if (row >= rows || (!is_q && page < 0)) continue;
+    char* to = is_q ? a.q_out.p + t * a.q_out.token_bytes + head * a.q_out.head_bytes + 16 * c
+                    : (is_v ? a.c.v : a.c.k) + head * a.c.head_bytes + in_cache;
+    *reinterpret_cast<U4*>(to) = out;
+  }
+}
+
+// Rows of a thread: one for a decode step's few tokens, whose time is that of
+// its round trips; three where the tokens alone fill the card, so that a token's
+// place is found by a third as many workgroups (12 sequences, 4060 tokens,
+// bf16: 23 -> EACH us).
+constexpr int kManyTokens = 1024;
+
+template <typename T, int kDim>
+void LaunchDim(const AppendArgs& a, hipStream_t s) {
+  const int rows = (a.q.p != nullptr ? a.n_heads : 0) + 2 * a.c.n_kv;
+  constexpr int kPass = 256 * 16 / (kDim * kBytes<T>);
+  const uint32_t n = static_cast<uint32_t>(a.s.n_tokens);
+  if (a.s.n_tokens >= kManyTokens)
+    AppendKernel<T, kDim, 3><<<dim3(n, static_cast<uint32_t>(CeilDiv(rows, 3 * kPass))), 256, 0, s>>>(a);
+  else
+    AppendKernel<T, kDim, 1><<<dim3(n, static_cast<uint32_t>(CeilDiv(rows, kPass))), 256, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
 }
 
 template <typename T>
 void Launch(const AppendArgs& a, hipStream_t s) {
-  const int rows = (a.q.p != nullptr ? a.n_heads : 0) + 2 * a.c.n_kv;
-  const int lanes_per_row = a.c.head_dim * kBytes<T> / 16;
-  const dim3 grid(static_cast<uint32_t>(a.s.n_tokens), static_cast<uint32_t>(CeilDiv(rows, 256 / lanes_per_row)));
   if (a.c.head_dim == 128)
-    AppendKernel<T, 128><<<grid, 256, 0, s>>>(a);
+    LaunchDim<T, 128>(a, s);
   else
-    AppendKernel<T, 64><<<grid, 256, 0, s>>>(a);
-  HIP_CHECK(hipGetLastError());
+    LaunchDim<T, 64>(a, s);
 }
 
 }  // namespace

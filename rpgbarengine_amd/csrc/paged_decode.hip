@@ -279,7 +279,7 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
 
 int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
   const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));
-  const int64_t want = std::max(CeilDiv(1024, base), CeilDiv(capacity, 2048));
+  const int64_t want = std::max(CeilDiv(256, base), CeilDiv(capacity, 2048));
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, kRangeUnit), int64_t{kMaxSplits}})));
 }
 

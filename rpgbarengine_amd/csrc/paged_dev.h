@@ -30,15 +30,46 @@ inline constexpr int kBytes<F32> = 4;
 
 constexpr float kNegInf = -__builtin_inff();
 
+// Lengths, starts and page tables: nothing writes them while a kernel runs, so a
+// wave-uniform one is read by a scalar load.
+__device__ __forceinline__ int Uniform(const int32_t* p, int64_t i) {
+  return *(const __attribute__((address_space(4))) int32_t*)(p + i);
+}
+
 // Positions of sequence s: 0 .. Length - 1.
-__device__ __forceinline__ int Length(const Seqs& s, int seq) { return max(0, min(s.lens[seq], s.capacity)); }
+__device__ __forceinline__ int ClampLength(const Seqs& s, int len) { return max(0, min(len, s.capacity)); }
+__device__ __forceinline__ int Length(const Seqs& s, int seq) { return ClampLength(s, Uniform(s.lens, seq)); }
+
+// The first sequence that `skip(its end among the packed tokens, its number)` is
+// false for (skip is true up to some sequence): its tokens and length, in one
+// round trip for up to 64 sequences, a lane for each. False: there is none, or
+// its tokens do not lie in [0, n_tokens).
+struct Sequence {
+  int seq, first, n_new, len;
+};
+template <typename F>
+__device__ __forceinline__ bool FindSequence(const Seqs& s, F&& skip, Sequence* out) {
+  const int lane = threadIdx.x & 63;
+  for (int j0 = 0; j0 < s.n_seqs; j0 += 64) {
+    const int j = min(j0 + lane, s.n_seqs - 1);
+    const int begin = s.starts[j], end = s.starts[j + 1], len = s.lens[j];
+    const uint64_t skipped = __ballot(j0 + lane < s.n_seqs && skip(end, j));
+    const int n = __popcll(skipped);
+    if (n >= min(64, s.n_seqs - j0)) continue;
+    out->seq = j0 + n;
+    out->first = __builtin_amdgcn_readlane(begin, n);
+    out->n_new = __builtin_amdgcn_readlane(end, n) - out->first;
+    out->len = ClampLength(s, __builtin_amdgcn_readlane(len, n));
+    return out->first >= 0 && out->n_new > 0 && out->first <= s.n_tokens - out->n_new;
+  }
+  return false;
+}
 
 // The page of the 16 positions from pos on (a page holds a multiple of 16), or
 // -1 where the table names none: such a page is never read or written, and its
 // positions take no part.
-// (Read by a scalar load: nothing writes the table while a kernel runs.)
 __device__ __forceinline__ int PageAt(const Cache& c, const int32_t* row, int pos) {
-  const int page = *(const __attribute__((address_space(4))) int32_t*)(row + (pos >> c.page_log2));
+  const int page = Uniform(row, pos >> c.page_log2);
   return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.n_pages) ? page : -1;
 }
 

@@ -80,19 +80,6 @@ __device__ __forceinline__ Parts8 Split8(U4 x, U4 y) {
   return p;
 }
 
-// The sequence that row tile b belongs to, -1 for none: tiles of sequence s
-// start at floor(starts[s] G / rows) + s, which leaves each its ceil(n_new G /
-// rows) tiles wherever the starts lie.
-__device__ __forceinline__ int SequenceOfTile(const Seqs& s, int group, int rows, int b) {
-  const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int j = 0; j < s.n_seqs; j += 64) {
-    const bool le = j + lane < s.n_seqs && s.starts[j + lane] * group / rows + j + lane <= b;
-    n += __popcll(__ballot(le));
-  }
-  return n - 1;
-}
-
 template <typename T>
 __device__ __forceinline__ bool NotFinite(uint32_t u) {
   if constexpr (kBytes<T> == 4) return (u & 0x7F800000u) == 0x7F800000u;
@@ -149,17 +136,18 @@ struct RowTile {
   int first, row0, n_rows, len, pos0;  // first: the sequence's first token; row0: of the sequence's n_rows
   __device__ __forceinline__ int Position(int row, int group) const { return pos0 + min(row, n_rows - 1) / group; }
 };
-// false: there is no such tile
+// Row tile `tile`: those of sequence s start at floor(starts[s] G / rows) + s,
+// which leaves each its ceil(n_new G / rows) tiles wherever the starts lie. False:
+// there is no such tile.
 __device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int tile, int* seq, RowTile* t) {
-  *seq = SequenceOfTile(s, group, rows, tile);
-  if (*seq < 0) return false;
-  t->first = s.starts[*seq];
-  const int n_new = s.starts[*seq + 1] - t->first;
-  if (t->first < 0 || n_new <= 0 || t->first > s.n_tokens - n_new) return false;
-  t->n_rows = n_new * group;
-  t->row0 = (tile - (t->first * group / rows + *seq)) * rows;
-  t->len = Length(s, *seq);
-  t->pos0 = t->len - n_new;
+  Sequence x;
+  if (!FindSequence(s, [&](int end, int j) { return end * group / rows + j + 1 <= tile; }, &x)) return false;
+  *seq = x.seq;
+  t->first = x.first;
+  t->n_rows = x.n_new * group;
+  t->row0 = (tile - (x.first * group / rows + x.seq)) * rows;
+  t->len = x.len;
+  t->pos0 = x.len - x.n_new;
   return t->row0 >= 0 && t->row0 < t->n_rows;
 }
 
@@ -603,15 +591,10 @@ __global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
   const int64_t row = blockIdx.x;
   const int token = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
   const int group = a.n_heads / a.c.n_kv;
-  // the sequence, and the row's tile there
-  const int lane = threadIdx.x & 63;
-  int seq = 0;
-  for (int j = 0; j < a.s.n_seqs; j += 64)
-    seq += __popcll(__ballot(j + lane < a.s.n_seqs && a.s.starts[j + lane + 1] <= token));
-  if (seq >= a.s.n_seqs) return;
-  const int first = a.s.starts[seq], n_new = a.s.starts[seq + 1] - first;
-  if (token < first || first < 0 || first > a.s.n_tokens - n_new) return;
-  const int len = Length(a.s, seq), pos0 = len - n_new;
+  Sequence x;
+  if (!FindSequence(a.s, [&](int end, int) { return end <= token; }, &x) || token < x.first) return;
+  const int first = x.first, n_new = x.n_new, pos0 = x.len - x.n_new;
+  // the row's tile
   const int tile = ((token - first) * group + head % group) / 32;
   const int keys = pos0 + min(32 * tile + 31, n_new * group - 1) / group + 1;
   const int range = RangeOf(max(keys, 1), a.splits);
