@@ -140,21 +140,25 @@ __device__ __forceinline__ F16v Mfma32First(U4 a, U4 b) {
   return r;
 }
 
-// x = hi + mid + lo exactly, three bf16 parts of a pair of floats: hi truncated
-// (so that no finite value becomes infinite), mid to nearest, lo what is left
-// (8 bits). Not for values that are not finite (inf - inf).
+// x = hi + mid + lo exactly: three bf16 parts of 8 bits each (truncated, so that
+// no finite value becomes infinite), for a pair of floats. Not for values that
+// are not finite: inf - inf.
 struct Parts {
   uint32_t hi, mid, lo;
 };
+__device__ __forceinline__ float Top8(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t Tops(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
 __device__ __forceinline__ Parts Split3(float a, float b) {
   Parts p;
-  p.hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-  const float a1 = a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
-  const float b1 = b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
-  p.mid = Pack2<BF16>(a1, b1);
-  float am, bm;
-  Unpack2<BF16>(p.mid, &am, &bm);
-  p.lo = Pack2<BF16>(a1 - am, b1 - bm);
+  p.hi = Tops(a, b);
+  a -= Top8(a);
+  b -= Top8(b);
+  p.mid = Tops(a, b);
+  a -= Top8(a);
+  b -= Top8(b);
+  p.lo = Tops(a, b);
   return p;
 }
 struct Parts8 {
@@ -162,8 +166,8 @@ struct Parts8 {
   __device__ __forceinline__ void Set(int i, Parts p) { hi[i] = p.hi, mid[i] = p.mid, lo[i] = p.lo; }
 };
 // f32 products on the bf16 matrix units: the six products of parts down to
-// 2^-16 of the whole (the dropped ones, mid lo, lo mid and lo lo, are below 2^-22
-// of it and of either sign, as fp32's own roundings), 192 cycles for 16 keys or
+// 2^-16 of the whole (the dropped ones, mid lo, lo mid and lo lo, are 2^-23 of it
+// on average, less than one rounding of fp32), 192 cycles for 16 keys or
 // dimensions where the f32 instruction takes 512. Smallest first.
 __device__ __forceinline__ F16v Mfma32x5(const Parts8& a, const Parts8& b, F16v c) {
   c = Mfma32<BF16>(a.hi, b.lo, c);

@@ -154,7 +154,7 @@ __device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int t
 // grid (row tile x key head, key range): key heads next to each other, the tiles
 // with the most keys first.
 template <typename T, int kDim, int kGroups>
-__global__ __launch_bounds__(64 * kWaves, kGroups == 2 ? 1 : 2) void PromptKernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4) ? 1 : 2) void PromptKernel(AttentionArgs a) {
   using Sh = Shape<T, kDim, kGroups>;
   // A group of one wave needs no barriers: it takes the next K tile in as soon as
   // the scores are done and the next V tile after the second product, each in the
@@ -623,9 +623,7 @@ void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
 template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
   const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv, kBytes<T>);
-  if constexpr (kBytes<T> == 2) {
-    if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
-  }
+  if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
   if (groups == 2) return LaunchGroups<T, kDim, 2>(a, s);
   LaunchGroups<T, kDim, 1>(a, s);
 }
@@ -646,7 +644,7 @@ int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
 int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes) {
   const int group = n_heads / n_kv;
   if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 384) return 1;
-  if (bytes == 4 || TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
+  if (TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
   return 4;
 }
 
