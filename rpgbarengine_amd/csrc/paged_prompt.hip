@@ -266,14 +266,14 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   // What the wave's rows of a V tile need before they are read: rows past the
   // sequence and of unnamed pages may hold anything, NaN among it, and become
   // zeros (their scores are masked); values that are not finite go to first_odd
-  // where some row does not see all of the step's keys (in f32 always, since the
-  // parts of an infinity are not one).
+  // where some row does not see all of the step's keys (careful: always).
+  bool careful = false;
   auto settle_v = [&](int step, const Place& x, char* tile) {
     const int p0 = first_key(step) + gw * kWaveRows;
     bool all = true;
 #pragma unroll
     for (int u = 0; u < kWaveUnits; ++u) all = all && x.ok[u];
-    if (kBytes<T> == 2 && first_key(step) + Sh::kKeys <= tile_first && all) return;
+    if (!careful && first_key(step) + Sh::kKeys <= tile_first && all) return;
     char* vt = tile + to + 16 * lane;
 #pragma unroll
     for (int i = 0; i < Sh::kPerThread; ++i) {
@@ -417,82 +417,98 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
     }
   };
 
-  if constexpr (kSolo) {
-    constexpr int kLoads = Sh::kPerThread;
-    char* kt = tiles;
-    char* vt = tiles + Sh::kTileBytes;
-    Place now, next;
-    if (steps > 0) {
-      look_up(0);
-      now = place_of(0);
-      fetch_k(now, kt);
-      fetch_v(now, vt);
-      look_up(1);
-    }
-    for (int step = 0; step < steps; ++step) {
-      const int key0 = first_key(step);
-      const bool mine = key0 <= wave_last && key0 < key_end, more = step + 1 < steps;
-      next = place_of(step + 1);
-      look_up(step + 2);
-      // in flight: K, then V of this step
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-      if (mine) scores(kt);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
-      if (more) fetch_k(next, kt);
-      uint32_t pages = 0;
-#pragma unroll
-      for (int u = 0; u < kWaveUnits; ++u) pages |= (now.ok[u] ? 1u : 0u) << (8 * u);
-#pragma unroll
-      for (int u = kWaveUnits; u < 4; ++u) pages |= 1u << (8 * u);
-      if (mine) weigh(key0, pages);
-      // in flight: V of this step, then K of the next
-      if (more)
+  for (;;) {
+    if constexpr (kSolo) {
+      constexpr int kLoads = Sh::kPerThread;
+      char* kt = tiles;
+      char* vt = tiles + Sh::kTileBytes;
+      Place now, next;
+      if (steps > 0) {
+        look_up(0);
+        now = place_of(0);
+        fetch_k(now, kt);
+        fetch_v(now, vt);
+        look_up(1);
+      }
+      for (int step = 0; step < steps; ++step) {
+        const int key0 = first_key(step);
+        const bool mine = key0 <= wave_last && key0 < key_end, more = step + 1 < steps;
+        next = place_of(step + 1);
+        look_up(step + 2);
+        // in flight: K, then V of this step
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-      else
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (mine) {
-        settle_v(step, now, vt);
-        add_values(vt);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
-      if (more) fetch_v(next, vt);
-      now = next;
-    }
-  } else {
-    Place x;
-    auto tile_of = [&](int step) { return tiles + (step & 1) * 2 * Sh::kTileBytes; };
-    auto begin = [&](int step) {
-      x = place_of(step);
-      fetch_k(x, tile_of(step));
-      fetch_v(x, tile_of(step) + Sh::kTileBytes);
-      look_up(step + 1);
-    };
-    // the wave's rows have landed, and then all of the group's
-    auto landed = [&](int step) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      settle_v(step, x, tile_of(step) + Sh::kTileBytes);
-      if (lane == 0) {
+        if (mine) scores(kt);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
+        if (more) fetch_k(next, kt);
+        uint32_t pages = 0;
 #pragma unroll
-        for (int u = 0; u < kWaveUnits; ++u)
-          reinterpret_cast<volatile uint8_t*>(&page_ok[grp][step & 1])[gw * kWaveUnits + u] = x.ok[u] ? 1 : 0;
+        for (int u = 0; u < kWaveUnits; ++u) pages |= (now.ok[u] ? 1u : 0u) << (8 * u);
+#pragma unroll
+        for (int u = kWaveUnits; u < 4; ++u) pages |= 1u << (8 * u);
+        if (mine) weigh(key0, pages);
+        // in flight: V of this step, then K of the next
+        if (more)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (mine) {
+          settle_v(step, now, vt);
+          add_values(vt);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
+        if (more) fetch_v(next, vt);
+        now = next;
       }
-      __syncthreads();
-    };
-    if (steps > 0) {
-      look_up(0);
-      begin(0);
-      landed(0);
-    }
-    for (int step = 0; step < steps; ++step) {
-      if (step + 1 < steps) begin(step + 1);
-      const int key0 = first_key(step);
-      if (key0 <= wave_last && key0 < key_end) {
-        scores(tile_of(step));
-        weigh(key0, page_ok[grp][step & 1]);
-        add_values(tile_of(step) + Sh::kTileBytes);
+    } else {
+      Place x;
+      auto tile_of = [&](int step) { return tiles + (step & 1) * 2 * Sh::kTileBytes; };
+      auto begin = [&](int step) {
+        x = place_of(step);
+        fetch_k(x, tile_of(step));
+        fetch_v(x, tile_of(step) + Sh::kTileBytes);
+        look_up(step + 1);
+      };
+      // the wave's rows have landed, and then all of the group's
+      auto landed = [&](int step) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        settle_v(step, x, tile_of(step) + Sh::kTileBytes);
+        if (lane == 0) {
+#pragma unroll
+          for (int u = 0; u < kWaveUnits; ++u)
+            reinterpret_cast<volatile uint8_t*>(&page_ok[grp][step & 1])[gw * kWaveUnits + u] = x.ok[u] ? 1 : 0;
+        }
+        __syncthreads();
+      };
+      if (steps > 0) {
+        look_up(0);
+        begin(0);
+        landed(0);
       }
-      if (step + 1 < steps) landed(step + 1);
+      for (int step = 0; step < steps; ++step) {
+        if (step + 1 < steps) begin(step + 1);
+        const int key0 = first_key(step);
+        if (key0 <= wave_last && key0 < key_end) {
+          scores(tile_of(step));
+          weigh(key0, page_ok[grp][step & 1]);
+          add_values(tile_of(step) + Sh::kTileBytes);
+        }
+        if (step + 1 < steps) landed(step + 1);
+      }
     }
+    // In f32 an infinite value that every row of its step sees comes out as NaN,
+    // since the parts of an infinity are not one. A tile that ends with a NaN is
+    // gone through again, its values looked at.
+    if (kBytes<T> == 2 || careful) break;
+    bool nan = false;
+#pragma unroll
+    for (int w = 0; w < kDim / 32; ++w)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) nan = nan || o[w][e] != o[w][e];
+    if (!__syncthreads_or(nan)) break;
+    careful = true;
+    m = kNegInf, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDim / 32; ++w) o[w] = F16v{};
   }
 
   l = lanes::AddXor32(l);

@@ -287,6 +287,27 @@ def test_prompt_masked_places_hold_anything(dtype, value):
     close(got, want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("lens,new", [([300], [150]), ([900], [3]), ([700] * 8, [300] * 8)], ids=["mid", "few", "many"])
+def test_prompt_infinities_that_every_query_sees(dtype, lens, new):
+    """Infinite values early in a sequence: every query has them, of either sign,
+    and NaN where both meet."""
+    b = Batch(lens, new, dtype, 2, 128, 16, 8, seed=23)
+    at = int(b.table[0, 0])
+    b.v[at, 0, 2, 5], b.v[at, 0, 9, 6] = math.inf, -math.inf
+    b.v[at, 1, 3, 7], b.v[at, 1, 4, 7] = math.inf, -math.inf
+    q = b.normal(b.tokens, 8, 128)
+    cache, table, lens_d, starts = b.gpu()
+    got = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts).double().cpu()
+    n = new[0]
+    assert bool((got[:n, :4, 5] == math.inf).all()) and bool((got[:n, :4, 6] == -math.inf).all())
+    assert bool(got[:n, 4:, 7].isnan().all())
+    ok = torch.ones_like(got, dtype=torch.bool)
+    ok[:n, :4, 5:7] = False
+    ok[:n, 4:, 7] = False
+    assert bool(got[ok].isfinite().all())
+
+
 def test_prompt_more_tokens_than_positions():
     """Tokens before the cache's first position see no key: zeros."""
     b = Batch([3, 0], [5, 2], torch.float16, seed=10)
