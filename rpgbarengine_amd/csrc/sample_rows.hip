@@ -54,6 +54,7 @@ constexpr int kDrawThreads = 1024;
 constexpr int kList = 1024;      // tokens of the cut's step that Draw ranks in LDS
 constexpr int kUnit = 4096;      // Draw looks for the token in a run of this many; slices are multiples of it
 constexpr int kMaxUnits = 64;    // of a row: 262144 tokens
+constexpr int kGroups = 64;      // groups of tokens of a slice whose maxima are kept (four threads' runs each)
 constexpr float kNone = -__builtin_inff();
 
 struct Bin {
@@ -68,7 +69,7 @@ struct SliceMax {
 
 struct Layout {
   int slices, length;  // tokens per slice
-  int64_t max_at, bins_at, weights_at, lists_at, counts_at, cuts_at, bytes;
+  int64_t max_at, bins_at, weights_at, lists_at, counts_at, cuts_at, groups_at, bytes;
 };
 
 __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
@@ -87,7 +88,8 @@ __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   l.lists_at = l.weights_at + rows * kMaxUnits * 8;
   l.counts_at = l.lists_at + rows * kList * 8;
   l.cuts_at = (l.counts_at + rows * 8 + 63) / 64 * 64;
-  l.bytes = l.cuts_at + rows * 64;
+  l.groups_at = l.cuts_at + rows * 64;
+  l.bytes = l.groups_at + rows * l.slices * kGroups * 4;
   return l;
 }
 
@@ -99,13 +101,15 @@ struct Work {
   uint64_t* list;  // rank keys
   uint32_t* count;  // tokens listed; slices counted
   Cut* cut;
+  float* groups;
   __device__ Work(const SampleArgs& a, const Layout& l, int row)
       : bins(reinterpret_cast<Bin*>(a.work + l.bins_at) + static_cast<int64_t>(row) * kBins),
         max(reinterpret_cast<SliceMax*>(a.work + l.max_at) + static_cast<int64_t>(row) * l.slices),
         weights(reinterpret_cast<uint64_t*>(a.work + l.weights_at) + static_cast<int64_t>(row) * kMaxUnits),
         list(reinterpret_cast<uint64_t*>(a.work + l.lists_at) + static_cast<int64_t>(row) * kList),
         count(reinterpret_cast<uint32_t*>(a.work + l.counts_at) + 2 * row),
-        cut(reinterpret_cast<Cut*>(a.work + l.cuts_at + static_cast<int64_t>(row) * 64)) {}
+        cut(reinterpret_cast<Cut*>(a.work + l.cuts_at + static_cast<int64_t>(row) * 64)),
+        groups(reinterpret_cast<float*>(a.work + l.groups_at) + static_cast<int64_t>(row) * l.slices * kGroups) {}
 };
 
 template <typename T>
@@ -128,11 +132,15 @@ __device__ __forceinline__ float One(const char* row, int i) {
 // Two neighbouring values of a run: those of its first dword (16-bit types) or
 // dwords (f32). Next moves on to the two behind them.
 template <typename T>
-__device__ __forceinline__ void Two(U4 v, float* a, float* b) {
+__device__ __forceinline__ void RawTwo(U4 v, float* a, float* b) {
   if constexpr (paged::kBytes<T> == 4)
     *a = __uint_as_float(v[0]), *b = __uint_as_float(v[1]);
   else
     Unpack2<T>(v[0], a, b);
+}
+template <typename T>
+__device__ __forceinline__ void Two(U4 v, float* a, float* b) {
+  RawTwo<T>(v, a, b);
   *a = Clean(*a);
   *b = Clean(*b);
 }
@@ -172,6 +180,12 @@ struct Row {
   // top_k so small that the tokens up to the k-th are listed whole: only their
   // number is needed of the histogram
   __device__ __forceinline__ bool Lean() const { return k > 0 && k <= kList / 2; }
+
+  // top_k so small against the groups whose maxima are kept that the k-th largest
+  // of those, which is no more than the k-th token, has few tokens above it: they
+  // are listed without a histogram (192 rows of 151936, top_k 40: 37 us in
+  // CountKernel with one, 18 without).
+  __device__ __forceinline__ bool Direct(int slices) const { return k > 0 && k <= min(128, slices * kGroups / 4); }
 
   // w 2^44, at most half a unit off when rounded; 0 where it would be less
   // than half of one.
@@ -296,17 +310,30 @@ __device__ __forceinline__ void ForTwo(U4 run, int i, F&& f) {
     run = Next<T>(run);
   }
 }
+// The largest value of a run, and the smallest (fmax and fmin pass NaN over).
 template <typename T>
 __device__ __forceinline__ float Top(U4 run) {
   float top = kNone;
 #pragma unroll
   for (int e = 0; e < kPer<T>; e += 2) {
     float x, y;
-    Two<T>(run, &x, &y);
+    RawTwo<T>(run, &x, &y);
     top = fmaxf(top, fmaxf(x, y));
     run = Next<T>(run);
   }
   return top;
+}
+template <typename T>
+__device__ __forceinline__ float Bottom(U4 run) {
+  float low = -kNone;
+#pragma unroll
+  for (int e = 0; e < kPer<T>; e += 2) {
+    float x, y;
+    RawTwo<T>(run, &x, &y);
+    low = fminf(low, fminf(x, y));
+    run = Next<T>(run);
+  }
+  return low;
 }
 
 // grid (slice, row)
@@ -318,18 +345,29 @@ __global__ __launch_bounds__(kThreads) void MaxKernel(SampleArgs a, Layout l) {
   for (int i = slice * kThreads + tid; i < kBins; i += l.slices * kThreads) w.bins[i] = Bin{0, 0, 0};
   if (slice == 0 && tid == 0) w.count[0] = w.count[1] = 0;
   float most = kNone, least = -kNone;
-  int at = INT32_MAX;
-  ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int) {  // (a token met twice changes nothing)
-#pragma unroll
-    for (int e = 0; e < kPer<T>; e += 2) {
-      float y, z;
-      Two<T>(run, &y, &z);
-      if (y > most) most = y, at = i + e;
-      if (z > most) most = z, at = i + e + 1;
-      least = fminf(least, fminf(y > kNone ? y : -kNone, z > kNone ? z : -kNone));
-      run = Next<T>(run);
+  int at = INT32_MAX;  // the first run that holds `most`
+  ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
+    float top = Top<T>(run);
+    if (__any(i != lo)) {  // the row's end: a token counts in one group only
+      top = kNone;
+      ForTwo<T>(run, i, [&](float y, float z, int t) {
+        top = fmaxf(top, fmaxf(t >= lo ? y : kNone, t + 1 >= lo ? z : kNone));
+      });
     }
+    if (top > most) most = top, at = i;
+    least = fminf(least, Bottom<T>(run));
   });
+  if (__syncthreads_or(least == kNone)) {  // the least above -inf: a row with tokens ruled out
+    least = -kNone;
+    ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int) {
+      ForTwo<T>(run, i, [&](float y, float z, int) {
+        least = fminf(least, fminf(y > kNone ? y : -kNone, z > kNone ? z : -kNone));
+      });
+    });
+  }
+  float quad = fmaxf(most, lanes::DppF<lanes::kQuadXor1>(most));
+  quad = fmaxf(quad, lanes::DppF<lanes::kQuadXor2>(quad));
+  if (tid % 4 == 0) w.groups[slice * kGroups + tid / 4] = quad;
   __shared__ SliceMax s[kThreads / 64];
   const float top = lanes::WaveMaxF(most);
   const float low = -lanes::WaveMaxF(-least);
@@ -338,13 +376,17 @@ __global__ __launch_bounds__(kThreads) void MaxKernel(SampleArgs a, Layout l) {
   for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
   if ((tid & 63) == 0) s[tid >> 6] = SliceMax{top, low, first, 0};
   __syncthreads();
-  if (tid != 0) return;
+  if (tid >= 64) return;
   SliceMax m = s[0];
+#pragma unroll
   for (int i = 1; i < kThreads / 64; ++i) {
     if (s[i].max > m.max || (s[i].max == m.max && s[i].index < m.index)) m.max = s[i].max, m.index = s[i].index;
     m.min = fminf(m.min, s[i].min);
   }
-  w.max[slice] = m;
+  // the token in its run
+  const bool here = m.max > kNone && tid < kPer<T> && m.index + tid < a.vocab && One<T>(x, m.index + tid) == m.max;
+  m.index += __ffsll(static_cast<unsigned long long>(__ballot(here))) - 1;
+  if (tid == 0) w.max[slice] = m;
 }
 
 __device__ __forceinline__ void LoadPow2(double* pow2) {
@@ -405,7 +447,7 @@ struct Cut {
   uint64_t all;                 // the row's weight
   // (words: a copy of a struct with padding would go through private memory,
   // which the compiler puts into LDS by reading the dispatch packet, 14 us away)
-  uint32_t whole;  // all tokens down to the cut's step are listed (there are at most kList)
+  uint32_t whole;  // all tokens down to the cut's step are to be listed (there are at most kList), or (2) are already
   uint32_t slow;   // the histogram does not tell
   __device__ __forceinline__ int End() const { return min(k_bin, p_bin); }
 };
@@ -495,6 +537,45 @@ __device__ __forceinline__ Cut FindCut(const Row& r, const Bin* bins) {
   return s;
 }
 
+// Lists the tokens of a slice down to step `last`. They gather in LDS (`found`,
+// kList of them) and go to the row's list together: a place in it for each would
+// be a round trip to memory.
+struct Lister {
+  uint64_t* found;
+  uint32_t* n_found;
+  uint32_t* at;
+  __device__ __forceinline__ void Begin() {
+    if (threadIdx.x == 0) *n_found = 0;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void Add(float v, int i) {
+    const uint32_t k = atomicAdd(n_found, 1u);
+    if (k < kList) found[k] = RankKey(v, i);
+  }
+  __device__ __forceinline__ void End(const Work& w) {
+    __syncthreads();
+    const uint32_t n = *n_found;
+    if (n == 0) return;
+    if (threadIdx.x == 0) *at = atomicAdd(w.count, n);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(n, static_cast<uint32_t>(kList)); i += kThreads)
+      if (*at + i < kList) w.list[*at + i] = found[i];
+  }
+};
+template <typename T>
+__device__ __forceinline__ void ListDown(const SampleArgs& a, const Layout& l, const Work& w, const Row& r, const char* x,
+                                         int slice, int last, Lister list) {
+  list.Begin();
+  ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
+    if (!__any(r.Bin(Top<T>(run)) <= last)) return;  // few runs hold a listed token
+    ForTwo<T>(run, i, [&](float y, float z, int at) {
+      if (at >= lo && y > kNone && r.Bin(y) <= last) list.Add(y, at);
+      if (at + 1 >= lo && z > kNone && r.Bin(z) <= last) list.Add(z, at + 1);
+    });
+  });
+  list.End(w);
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) {
   const int slice = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
@@ -505,10 +586,47 @@ __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) 
   __shared__ unsigned long long weight[kBins];
   __shared__ uint32_t count[kBins];
   __shared__ double pow2[32];
+  __shared__ int s_last;
+  constexpr int kEach = kBins / kThreads;
+  const uint32_t k = static_cast<uint32_t>(r.k);
   LoadPow2(pow2);
   for (int i = tid; i < kBins; i += kThreads) weight[i] = 0, count[i] = 0;
+  if (tid == 0) s_last = -1;
   __syncthreads();
   const char* x = a.logits + row * a.row_bytes;
+  if (r.Direct(l.slices)) {
+    for (int i = tid; i < l.slices * kGroups; i += kThreads) {
+      const float top = w.groups[i];
+      if (top > kNone) atomicAdd(&count[r.Bin(top)], 1u);
+    }
+    __syncthreads();
+    uint32_t n = 0, before;
+    uint64_t unused;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) n += count[tid * kEach + i];
+    Before<kThreads>(0, &unused, n, &before);
+    if (before < k && before + n >= k) {
+      uint32_t c = before;
+      int bin = -1;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        c += count[tid * kEach + i];
+        if (bin < 0 && c >= k) bin = tid * kEach + i;
+      }
+      // (without weight from there on: no limit)
+      s_last = r.weightless_end && bin == kBins - 1 ? kBins - 2 : bin;
+    }
+    __syncthreads();
+    if (s_last >= 0) {
+      __shared__ uint32_t n_found, s_at;
+      ListDown<T>(a, l, w, r, x, slice, s_last, Lister{reinterpret_cast<uint64_t*>(weight), &n_found, &s_at});
+      if (slice == 0 && tid == 0) *w.cut = Cut{s_last, kBins, 0, 0, 0, 0, 0, 2, 0};
+      return;
+    }
+    // fewer groups than k hold a token: the histogram
+    for (int i = tid; i < kBins; i += kThreads) count[i] = 0;
+    __syncthreads();
+  }
   const bool lean = r.Lean();
   ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
     ForTwo<T>(run, i, [&](float y, float z, int at) {
@@ -529,15 +647,12 @@ __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) 
   // lies no further down, and those steps get every slice's counts.
   int last = kBins - 1;
   if (lean) {
-    __shared__ int s_last;
     if (tid == 0) s_last = last;
-    constexpr int kEach = kBins / kThreads;
     uint32_t n = 0, before;
     uint64_t unused;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) n += count[tid * kEach + i];
     Before<kThreads>(0, &unused, n, &before);
-    const uint32_t k = static_cast<uint32_t>(r.k);
     if (before < k && before + n >= k) s_last = tid * kEach + kEach - 1;
     __syncthreads();
     last = s_last;
@@ -573,36 +688,15 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
   if (cut.slow) return;
   const int end_bin = cut.End();
   const char* x = a.logits + row * a.row_bytes;
-  // Listed tokens gather in LDS and go to the row's list together: a place in it
-  // for each would be a round trip to memory.
+  if (cut.whole == 2) return;
   __shared__ uint64_t found[kList];
   __shared__ uint32_t n_found, s_at;
-  if (tid == 0) n_found = 0;
-  __syncthreads();
-  auto list = [&](float v, int i) {
-    const uint32_t at = atomicAdd(&n_found, 1u);
-    if (at < kList) found[at] = RankKey(v, i);
-  };
-  auto flush = [&] {
-    __syncthreads();
-    const uint32_t n = n_found;
-    if (n == 0) return;
-    if (tid == 0) s_at = atomicAdd(w.count, n);
-    __syncthreads();
-    for (uint32_t i = tid; i < min(n, static_cast<uint32_t>(kList)); i += kThreads)
-      if (s_at + i < kList) w.list[s_at + i] = found[i];
-  };
+  Lister list{found, &n_found, &s_at};
   if (cut.whole) {
-    ForRuns<T>(a, x, slice * l.length, l.length, [&](U4 run, int i, int lo) {
-      if (!__any(r.Bin(Top<T>(run)) <= end_bin)) return;  // few runs hold a listed token
-      ForTwo<T>(run, i, [&](float y, float z, int at) {
-        if (at >= lo && y > kNone && r.Bin(y) <= end_bin) list(y, at);
-        if (at + 1 >= lo && z > kNone && r.Bin(z) <= end_bin) list(z, at + 1);
-      });
-    });
-    flush();
+    ListDown<T>(a, l, w, r, x, slice, end_bin, list);
     return;
   }
+  list.Begin();
   const int listed_last = max(cut.k_bin < kBins ? cut.k_bin : -1, cut.p_bin < kBins ? cut.p_bin : -1);
   __shared__ uint64_t part[kThreads / 64];
   for (int start = slice * l.length; start < min(a.vocab, (slice + 1) * l.length); start += kUnit) {
@@ -616,8 +710,8 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
         const double fy = r.Weight(y, pow2), fz = r.Weight(z, pow2);
         sum += by < end_bin && fy >= r.floor ? Row::Units(fy) : 0;
         sum += bz < end_bin && fz >= r.floor ? Row::Units(fz) : 0;
-        if (by < kBins && (by == cut.k_bin || by == cut.p_bin)) list(y, at);
-        if (bz < kBins && (bz == cut.k_bin || bz == cut.p_bin)) list(z, at + 1);
+        if (by < kBins && (by == cut.k_bin || by == cut.p_bin)) list.Add(y, at);
+        if (bz < kBins && (bz == cut.k_bin || bz == cut.p_bin)) list.Add(z, at + 1);
       });
     });
     sum = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(sum));
@@ -626,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
     __syncthreads();
     if (tid == 0) w.weights[start / kUnit] = part[0] + part[1] + part[2] + part[3];
   }
-  flush();
+  list.End(w);
 }
 
 // The rank key of the last token kept when tokens are taken from the best on

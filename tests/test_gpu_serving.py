@@ -568,6 +568,29 @@ def test_sample_full_vocabulary(dtype):
     check_samples(x.to(dtype), torch.rand(rows, generator=g), t, k, p, m)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("vocab", [4099, 20011, 65541])
+def test_sample_small_top_k(dtype, vocab):
+    """Few tokens of many: the best ones side by side at the row's end, in
+    order, spread, alike, among NaN of every kind."""
+    g = torch.Generator().manual_seed(vocab + 1)
+    x = torch.randn(7, vocab, generator=g)
+    x[0, -3:] += 20
+    x[1] = torch.arange(vocab) * (40.0 / vocab)
+    x[2] = torch.arange(vocab, 0, -1) * (40.0 / vocab)
+    x[3] = torch.arange(vocab) % 2
+    x[4, ::2] = -math.inf
+    x[5, 7:] = -math.inf
+    x = x.to(dtype)
+    bits = x.view(torch.int32 if dtype == torch.float32 else torch.int16)
+    one = {torch.float32: 0x7F800001, torch.float16: 0x7C01, torch.bfloat16: 0x7F81}[dtype]  # a signalling NaN
+    bits[6, ::3], x[6, 1::3] = one, math.nan
+    for k in (1, 2, 3, 5, 16, 40, 64, 100, 128):
+        rows = x.shape[0]
+        check_samples(x, torch.rand(rows, generator=g), torch.full((rows,), 0.8), torch.full((rows,), k, dtype=torch.int32),
+                      torch.tensor([1.0, 0.9, 1.0, 0.5, 1.0, 0.9, 0.7]), torch.tensor([0.0, 0.0, 0.1, 0.0, 0.2, 0.0, 0.0]))
+
+
 def test_sample_ties_and_flat_rows():
     """Equal values: the lowest indices stay; lists longer than the kernel ranks in
     shared memory; temperatures that flatten or sharpen everything."""
