@@ -251,11 +251,11 @@ typedef struct {
 } rpg_hip_paged_cache;
 
 /* n_seqs sequences. Sequence s holds lens[s] positions (at most pages *
- * page_size, 0 and less: none), the new tokens among them; position p lies in
+ * page_size, which is at most 2^30; 0 and less: none), the new tokens among them; position p lies in
  * page table[s * table_stride + p / page_size]. A page number outside [0,
  * n_pages) is never followed: its positions take no part. The new tokens of
- * sequence s are the packed rows starts[s] .. starts[s + 1] (starts[n_seqs + 1],
- * not decreasing), at its last positions; rows of no sequence are left as they
+ * sequence s are the packed rows starts[s] .. starts[s + 1] (n_seqs + 1
+ * of them, not decreasing), at its last positions; rows of no sequence are left as they
  * are. starts is not read by rpg_hip_paged_decode (one token each). */
 typedef struct {
   const int32_t* table;

@@ -42,6 +42,9 @@ struct Rows {
   int64_t token_bytes = 0, head_bytes = 0;
 };
 
+// Workgroups of one launch, at 256 threads each.
+constexpr int64_t kMaxGroups = (int64_t{1} << 24) - 1;
+
 struct AppendArgs {
   Cache c;
   Seqs s;

@@ -143,6 +143,7 @@ void LaunchDim(const AppendArgs& a, hipStream_t s) {
   const int rows = (a.q.p != nullptr ? a.n_heads : 0) + 2 * a.c.n_kv;
   constexpr int kPass = 256 * 16 / (kDim * kBytes<T>);
   const uint32_t n = static_cast<uint32_t>(a.s.n_tokens);
+  RPG_CHECK(n <= kMaxGroups, "%u new tokens in one launch", n);
   if (a.s.n_tokens >= kManyTokens)
     AppendKernel<T, kDim, 3><<<dim3(n, static_cast<uint32_t>(CeilDiv(rows, 3 * kPass))), 256, 0, s>>>(a);
   else

@@ -87,6 +87,12 @@ __device__ __forceinline__ int DimOf(int w, int m) {
   return (kDim / 16) * m + w;
 }
 
+// Weights are held times 2^kLift, their sums too. f16 has steps of 2^-24 at the
+// least: without it, keys whose weight is below 2^-25 of the largest would count
+// in the sum and not in the output, and a long cache has many of those.
+template <typename T>
+constexpr float kLift = __is_same(T, F16) ? 15.0f : 0.0f;
+
 // A query head's running state in a lane: maximum (of scale log2(e) q.k) and
 // the output of its column, alike over the lanes of a column; the sum of the
 // lane's own keys.
@@ -144,7 +150,7 @@ struct State {
 #pragma unroll
       for (int w = 0; w < kDim / 16; ++w) o[w] *= f;
     }
-    const float base = m == kNegInf ? 0.0f : m;
+    const float base = m == kNegInf ? 0.0f : m - kLift<T>;
 #pragma unroll
     for (int h = 0; h < Tl::kHalves; ++h)
 #pragma unroll
@@ -260,6 +266,8 @@ template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
   const int group = a.n_heads / a.c.n_kv;
   const int64_t x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(group, kCols);
+  RPG_CHECK(static_cast<int64_t>(a.s.n_seqs) * a.n_heads <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs,
+            a.n_heads);
   DecodeKernel<T, kDim><<<dim3(static_cast<uint32_t>(x), a.splits), 64 * kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
   if (a.splits == 1) return;

@@ -124,7 +124,12 @@ __device__ __forceinline__ F4 Mfma16F32(float a, float b, F4 c) {
   return r;
 }
 // D[8 (e / 4) + 4 (l / 32) + e % 4][l % 32] += sum_k A[l % 32][k] B[k][l % 32]; a
-// lane holds the eight k of its l / 32.
+// lane holds the eight k of its l / 32 (16-bit types), the one k = l / 32 (f32).
+__device__ __forceinline__ F16v Mfma32F32(float a, float b, F16v c) {
+  const F16v r = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+  asm volatile("" ::"v"(a), "v"(b), "v"(r));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ F16v Mfma32(U4 a, U4 b, F16v c) {
   if constexpr (__is_same(T, BF16))

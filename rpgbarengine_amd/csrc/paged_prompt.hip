@@ -113,6 +113,16 @@ __device__ __forceinline__ int DimOf(int w, int m) {
   return kBytes<T> == 4 ? (kDim / 32) * m + w : 32 * w + m;
 }
 
+// The maximum that weights refer to moves only when one would pass 2^kLazy: most
+// steps raise some row's, and rescaling costs as much as the exponentials (4000
+// tokens, bf16: 164 us with a rescaling whenever a maximum rises, 152 without).
+// Weights are held times 2^kLift, their sums too: f16 has steps of 2^-24 at the
+// least, and keys whose weight is below half of that would count in the sum and
+// not in the output. The largest is 2^15.
+constexpr float kLazy = 8.0f;
+template <typename T>
+constexpr float kLift = __is_same(T, F16) ? 15.0f - kLazy : 0.0f;
+
 // A buffer resource (wave-uniform) over `bytes` bytes from p.
 __device__ __forceinline__ U4 Resource(const char* p, uint32_t bytes) {
   const uint64_t u = reinterpret_cast<uint64_t>(p);
@@ -317,6 +327,23 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   F16v o[kDim / 32] = {};
   F16v s[Sh::kBlocks];
   auto scores = [&](const char* kt) {
+    if constexpr (kBytes<T> == 4) {
+      if (careful) {  // in f32 products: what is infinite stays that
+        const char* qp = a.q.p + (first + token) * a.q.token_bytes + head * a.q.head_bytes + 8 * h * kBytes<T>;
+        s[0] = F16v{};
+#pragma unroll 1
+        for (int i = 0; i < Sh::kQ; ++i) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const U4 x = *reinterpret_cast<const U4*>(kt + (k_at ^ (64 * i + 16 * half)));
+            const U4 y = Load16(qp + 64 * i + 16 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0] = Mfma32F32(__uint_as_float(x[e]), __uint_as_float(y[e]), s[0]);
+          }
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int b = 0; b < Sh::kBlocks; ++b) {
 #pragma unroll
@@ -351,16 +378,14 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[b][e]);
     top = lanes::MaxXor32(top) * c;
-    // The maximum that weights refer to moves only when one would pass 2^8: most
-    // steps raise some row's, and rescaling costs as much as the exponentials.
-    if (__any(top > m + 8.0f)) {
+    if (__any(top > m + kLazy)) {
       const float now = fmaxf(m, top), f = m == now ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
       l *= f;
 #pragma unroll
       for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
     }
-    const float base = m == kNegInf ? 0.0f : m;
+    const float base = m == kNegInf ? 0.0f : m - kLift<T>;
 #pragma unroll
     for (int b = 0; b < Sh::kBlocks; ++b)
 #pragma unroll
@@ -495,9 +520,9 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
         if (step + 1 < steps) landed(step + 1);
       }
     }
-    // In f32 an infinite value that every row of its step sees comes out as NaN,
+    // In f32 an infinite key, query or value that a row sees comes out as NaN,
     // since the parts of an infinity are not one. A tile that ends with a NaN is
-    // gone through again, its values looked at.
+    // gone through again, its values looked at and its scores in f32 products.
     if (kBytes<T> == 2 || careful) break;
     bool nan = false;
 #pragma unroll
@@ -625,7 +650,9 @@ int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes
 template <typename T, int kDim, int kGroups>
 void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
   const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, kGroups);
-  RPG_CHECK(tiles * a.c.n_kv < (int64_t{1} << 31), "paged_prompt: too many rows for one launch");
+  RPG_CHECK(tiles * a.c.n_kv <= kMaxGroups &&
+                (a.splits == 1 || static_cast<int64_t>(a.s.n_tokens) * a.n_heads <= kMaxGroups),
+            "%d x %d query rows in one launch", a.s.n_tokens, a.n_heads);
   PromptKernel<T, kDim, kGroups>
       <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());

@@ -37,6 +37,9 @@ int ElementBytes(int32_t type) {
 // Byte strides of this size keep every product with a 32-bit count in 64 bits.
 constexpr int64_t kMaxStride = int64_t{1} << 31;
 
+// Of a sequence: a kernel's steps may count some thousand past them.
+constexpr int32_t kMaxPositions = 1 << 30;
+
 int64_t StrideBytes(const char* what, int64_t elements, int bytes) {
   RPG_CHECK(elements >= -kMaxStride && elements <= kMaxStride, "%s of %lld elements", what, (long long)elements);
   RPG_CHECK(elements * bytes % 16 == 0, "%s of %lld elements is not a multiple of 16 bytes", what,
@@ -90,7 +93,7 @@ paged::Seqs SeqSizes(const rpg_hip_sequences* s, const rpg_hip_paged_cache* c) {
   RPG_CHECK(s != nullptr, "the sequences are null");
   paged::Seqs out;
   RPG_CHECK(s->n_seqs >= 0 && s->n_tokens >= 0, "%d sequences of %d new tokens", s->n_seqs, s->n_tokens);
-  RPG_CHECK(s->pages >= 0 && s->pages <= (INT32_MAX - 4096) / c->page_size,
+  RPG_CHECK(s->pages >= 0 && s->pages <= kMaxPositions / c->page_size,
             "%d pages of %d positions for a sequence", s->pages, c->page_size);
   out.n_seqs = s->n_seqs;
   out.n_tokens = s->n_tokens;

@@ -76,6 +76,7 @@ class PagedCache:
         _need(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
         _need(k.dtype in _TYPES and v.dtype == k.dtype, "k and v are both float32, float16 or bfloat16")
         _need(k.is_cuda and v.device == k.device, "k and v lie on one GPU")
+        _need(not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)), "the cache requires gradients: there is no backward pass")
         _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
         self.k, self.v = k, v
         self.device, self.dtype = k.device, k.dtype
@@ -126,6 +127,8 @@ def _vector(x, name, n, dtype, device):
     """The address of a contiguous vector; None stays None."""
     if x is None:
         return None
+    if x.requires_grad and torch.is_grad_enabled():
+        raise EngineError(f"{name} requires gradients: there is no backward pass")
     if x.dtype is not dtype or x.shape != (n,) or x.device != device or (n > 1 and x.stride(0) != 1):
         raise EngineError(f"{name} is {dtype} [{n}], contiguous, on the same GPU")
     return x.data_ptr()
@@ -157,25 +160,26 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
     given; may be q). Keys and queries are RMS-normed per head with the gains
     k_norm and q_norm (float32 [dim]) and rotated by rope (float32 [positions,
     dim]: cos | sin) where those are given. Returns q_out."""
+    kr, vr = _rows(k, "k", cache), _rows(v, "v", cache)
     n = k.shape[0]
     seqs = _seqs(cache, table, lens, starts, n)[0]
-    kr, vr = _rows(k, "k", cache), _rows(v, "v", cache)
     if v.shape != k.shape or k.shape[1] != cache.n_kv:
         raise EngineError("k and v are [tokens, key heads of the cache, head dim]")
     heads, qr, qo = 0, None, None
     if q is not None:
+        qr = _rows(q, "q", cache)
         heads = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if q.shape[0] != n or q_out.shape != q.shape:
             raise EngineError("q, q_out and k are of one number of tokens")
-        qr, qo = _rows(q, "q", cache), _rows(q_out, "q_out", cache)
+        qo = _rows(q_out, "q_out", cache)
     dev, dim = cache.device, cache.head_dim
     rp, rope_rows = None, 0
     if rope is not None:
         if (rope.dtype is not torch.float32 or rope.dim() != 2 or rope.shape[1] != dim or not rope.is_contiguous()
-                or rope.device != dev):
-            raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU")
+                or rope.device != dev or (rope.requires_grad and torch.is_grad_enabled())):
+            raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU, without gradients")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
     _enqueue(dev, _lib().rpg_hip_paged_append, cache._c, seqs, kr, vr, qr, qo, heads,
              _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
@@ -191,8 +195,7 @@ def _work_bytes(n_kv, page_size, head_dim, kind, pages, n_seqs, n_tokens, heads,
     return _ok(_lib().rpg_hip_paged_work(c, _SEQS.pack(0, pages, 0, 0, pages, n_seqs, n_tokens), heads, prompt))
 
 
-def _attention(f, q, cache, seqs, n_seqs, pages, n_tokens, scale, out, prompt):
-    qr = _rows(q, "q", cache)
+def _attention(f, q, qr, cache, seqs, n_seqs, pages, n_tokens, scale, out, prompt):
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
@@ -209,19 +212,24 @@ def decode_attention(q, cache: PagedCache, table, lens, scale=None, out=None):
     """Attention of one token per sequence, q [sequences, heads, dim], over all of
     its sequence's positions. scale: 1 / sqrt(dim) when not given. out (may be q)
     is made when not given."""
+    qr = _rows(q, "q", cache)
     seqs, n, pages = _seqs(cache, table, lens, None, 0)
     if q.shape[0] != n:
         raise EngineError("q has a row for each sequence")
-    return _attention(_lib().rpg_hip_paged_decode, q, cache, seqs, n, pages, 0, scale, out, 0)
+    return _attention(_lib().rpg_hip_paged_decode, q, qr, cache, seqs, n, pages, 0, scale, out, 0)
 
 
 def prompt_attention(q, cache: PagedCache, table, lens, starts, scale=None, out=None):
     """Causal attention of the packed new tokens, q [tokens, heads, dim]: the token
     at position p of its sequence over positions 0 .. p, whose keys and values
-    lie in the cache (the new tokens' own too)."""
+    lie in the cache (the new tokens' own too). out (may be q) is made when not
+    given; rows of no sequence are not written."""
+    qr = _rows(q, "q", cache)
     tokens = q.shape[0]
+    if starts is None:
+        raise EngineError("starts is needed")
     seqs, n, pages = _seqs(cache, table, lens, starts, tokens)
-    return _attention(_lib().rpg_hip_paged_prompt, q, cache, seqs, n, pages, tokens, scale, out, 1)
+    return _attention(_lib().rpg_hip_paged_prompt, q, qr, cache, seqs, n, pages, tokens, scale, out, 1)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -64,11 +64,11 @@ def attention(q, k, v, seen, scale, dtype):
         ds = float((kk.abs() @ qq.abs()).max()) * scale * (dim + 4) * 2.0 ** -24 + float(s.abs().max()) * 2.0 ** -21
         rel = math.expm1(2 * ds) + (len(s) + 16) * 2.0 ** -23
         if dtype != torch.float32:
-            # A 16-bit weight below the type's normal range (f16: 2^-14) is off by
-            # at most 2^-25 absolutely; the largest weight is 1.
+            # An f16 weight is held times 2^7 at the least; below the type's normal
+            # range it is off by at most 2^-25 absolutely; the largest weight is 1.
             rel += EPS[dtype]
             if dtype == torch.float16:
-                bound[h] += 2.0 ** -25 * vv.abs().sum(0) * float(p.max())
+                bound[h] += 2.0 ** -32 * vv.abs().sum(0) * float(p.max())
         bound[h] += rel * mass
     return out, bound + EPS[dtype] * (out.abs() + bound) + TINY[dtype]
 

@@ -117,6 +117,21 @@ def test_starts_and_work_memory():
     assert L.rpg_hip_paged_work(ref(c), ref(seqs(pages=1, n_seqs=1)), 8, 0) == 0  # one range: none
 
 
+def test_more_than_one_launch_holds():
+    """2^24 workgroups and more, and positions that a step would count past 2^31."""
+    L = serving._lib()
+    c, r = cache(), rows(token_stride=1024)
+    s = seqs(n_seqs=1 << 22, n_tokens=1 << 22)
+    refused(L.rpg_hip_paged_decode(ref(c), ref(s), ref(r), ref(r), 8, 0.1, A, 1 << 60, None), "query rows in one launch")
+    refused(L.rpg_hip_paged_prompt(ref(c), ref(s), ref(r), ref(r), 8, 0.1, A, 1 << 60, None), "query rows in one launch")
+    s = seqs(n_tokens=1 << 24)
+    refused(L.rpg_hip_paged_append(ref(c), ref(s), ref(r), ref(r), None, None, 0, None, None, 0.0, None, 0, None),
+            "new tokens in one launch")
+    most = (1 << 30) // 16
+    assert L.rpg_hip_paged_work(ref(c), ref(seqs(pages=most, table_stride=most)), 8, 0) > 0
+    refused(L.rpg_hip_paged_work(ref(c), ref(seqs(pages=most + 1, table_stride=most + 1)), 8, 0), "pages")
+
+
 BAD_APPENDS = [
     (dict(k=None), "k is null"), (dict(v=rows(data=None)), "v is null"), (dict(q_out=None), "q_out is null"),
     (dict(q_out=rows(head_stride=256, token_stride=4096)), "other strides"), (dict(heads=5), "query heads"),

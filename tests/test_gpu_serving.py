@@ -308,6 +308,81 @@ def test_prompt_infinities_that_every_query_sees(dtype, lens, new):
     assert bool(got[ok].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("lens,new", [([300], [150]), ([900], [3]), ([700] * 8, [300] * 8)], ids=["mid", "few", "many"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_an_infinite_key(dtype, lens, new, value):
+    """A score of -inf gives its key no weight; one of +inf makes the row NaN
+    (inf - inf). The same for one new token."""
+    b = Batch(lens, new, dtype, 2, 128, 16, 8, seed=24)
+    d, pos = 37, 5
+    b.k[int(b.table[0, 0]), :, pos, d] = value
+    q = b.normal(b.tokens, 8, 128)
+    q[:, :, d] = torch.where(q[:, :, d] < 0, -1.0, 1.0).to(dtype)
+    cache, table, lens_d, starts = b.gpu()
+    last = starts[1:].long() - 1
+    many = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts)
+    one = serving.decode_attention(q.cuda()[last], cache, table, lens_d)
+    kk, there = plain.sequence_rows(b.k, b.table[0], lens[0])
+    vv, _ = plain.sequence_rows(b.v, b.table[0], lens[0])
+    kk[:, pos] = 0.0
+    for j in (0, new[0] // 2, new[0] - 1):
+        seen = there & (torch.arange(lens[0]) <= lens[0] - new[0] + j)
+        seen[pos] = False
+        want, bound = plain.attention(q[j], kk, vv, seen, 128 ** -0.5, dtype)
+        up = q[j, :, d].double() * value > 0
+        for got in [many[j]] + ([one[0]] if j == new[0] - 1 else []):
+            assert bool(got.cpu()[up].isnan().all())
+            close(got.cpu()[~up], want[~up], bound[~up])
+    assert bool(many[new[0]:].isfinite().all()) and bool(one[1:].isfinite().all())
+
+
+@pytest.mark.parametrize("tokens", [1, 2])
+def test_f16_many_light_keys_beside_a_heavy_one(tokens):
+    """One key takes nearly all the weight, 20000 others have 2^-25.4 of it each:
+    less than half of f16's smallest step, and together all of the output."""
+    n, page = 20000, 16
+    k, v = torch.zeros(2, 1, page, 64, dtype=torch.float16), torch.ones(2, 1, page, 64, dtype=torch.float16)
+    k[0, 0, 0, :16] = 1.1
+    v[0, 0, 0] = 0.0
+    table = torch.ones(1, n // page, dtype=torch.int32)
+    table[0, 0] = 0
+    q = torch.zeros(tokens, 1, 64, dtype=torch.float16)
+    q[:, :, :16] = 8.0
+    cache = serving.PagedCache(k.cuda(), v.cuda())
+    lens = torch.tensor([n], dtype=torch.int32)
+    if tokens == 1:
+        got = serving.decode_attention(q.cuda(), cache, table.cuda(), lens.cuda()).double().cpu()
+    else:
+        starts = torch.tensor([0, tokens], dtype=torch.int32)
+        got = serving.prompt_attention(q.cuda(), cache, table.cuda(), lens.cuda(), starts.cuda()).double().cpu()
+    heavy = float(k[0, 0, 0, 0].double()) * 8.0 * 16 * 0.125
+    assert 2.0 ** -26 < math.exp(-heavy) < 2.0 ** -25
+    for t in range(tokens):
+        rest = (n - tokens + t) * math.exp(-heavy)
+        want = rest / (1.0 + rest)
+        # A weight's rounding: half a step of 2^-24 / 2^7 (the least lift) of the
+        # heaviest; sums of 20000 in fp32; the score (18 roundings of at most 2^-24
+        # of it, twice); the output's rounding.
+        rel = 2.0 ** -32 / math.exp(-heavy) + n * 2.0 ** -23 + 36 * heavy * 2.0 ** -24 + 2.0 ** -11
+        assert float((got[t] - want).abs().max()) <= rel * want
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("lens,new", [([70, 30], [70, 12]), ([900, 40], [3, 1]), ([500] * 9, [140] * 9)])
+def test_attention_in_place(dtype, lens, new):
+    """out = q: the same bits as out of its own."""
+    b = Batch(lens, new, dtype, 2, 64, 16, 8, seed=25)
+    q = b.normal(b.tokens, 8, 64).cuda()
+    cache, table, lens_d, starts = b.gpu()
+    want = serving.prompt_attention(q, cache, table, lens_d, starts)
+    one = q[: len(lens)].clone()
+    want_one = serving.decode_attention(one, cache, table, lens_d)
+    assert serving.prompt_attention(q, cache, table, lens_d, starts, out=q) is q
+    serving.decode_attention(one, cache, table, lens_d, out=one)
+    assert torch.equal(q, want) and torch.equal(one, want_one)
+
+
 def test_prompt_more_tokens_than_positions():
     """Tokens before the cache's first position see no key: zeros."""
     b = Batch([3, 0], [5, 2], torch.float16, seed=10)
@@ -703,6 +778,31 @@ def test_refusals():
             pytest.fail(f"call {i} was not refused")
     with torch.no_grad():
         serving.decode_attention(q.detach().requires_grad_(), cache, table, lens)
+
+
+def test_parameters_that_require_gradients_are_refused():
+    b = Batch([4], [1], torch.float32, 1, 64, 16, 2)
+    cache, table, lens, starts = b.gpu()
+    k, q = b.normal(1, 1, 64).cuda(), b.normal(1, 2, 64).cuda()
+    gain = torch.nn.Parameter(torch.ones(64, device="cuda"))
+    rope = torch.nn.Parameter(torch.ones(64, 64, device="cuda"))
+    one = torch.nn.Parameter(torch.ones(1, device="cuda"))
+    x = torch.zeros(1, 5, device="cuda")
+    for call in (lambda: serving.append(cache, table, lens, starts, k, k, q=q, q_norm=gain),
+                 lambda: serving.append(cache, table, lens, starts, k, k, k_norm=gain),
+                 lambda: serving.append(cache, table, lens, starts, k, k, rope=rope),
+                 lambda: serving.sample(x, one.detach(), temperature=one),
+                 lambda: serving.PagedCache(torch.nn.Parameter(cache.k), cache.v)):
+        with pytest.raises(eng.EngineError, match="gradients"):
+            call()
+    with torch.no_grad():
+        serving.append(cache, table, lens, starts, k, k, q=q, q_norm=gain, k_norm=gain, rope=rope)
+    for call in (lambda: serving.append(cache, table, lens, starts, k[0], k[0]),
+                 lambda: serving.append(cache, table, lens, starts, k, k, q=q[0, 0]),
+                 lambda: serving.decode_attention(q[0, 0], cache, table, lens),
+                 lambda: serving.prompt_attention(q, cache, table, lens, None)):
+        with pytest.raises(eng.EngineError):
+            call()
 
 
 def test_nothing_to_do():
