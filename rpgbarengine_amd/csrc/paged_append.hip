@@ -10,7 +10,9 @@
 // dependent round trips (the sequence's place, then the rows and the page). A
 // row is one 16-byte load of 8, 16 or 32 adjacent lanes: the sum of squares
 // and the rotation's partner half cross lanes by DPP, nothing goes through
-// LDS, and a row is stored as it was loaded.
+// LDS, and a row is stored as it was loaded. Measured: 4060 tokens of 12
+// sequences, 32 heads on 8 of 128, bf16, 101 MB in 24 us (a large copy's rate: 20);
+// 8 tokens, f32: 3.5 us in the kernel, 10 in the call.
 
 #include <hip/hip_runtime.h>
 

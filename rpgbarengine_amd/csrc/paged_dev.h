@@ -188,7 +188,9 @@ __device__ __forceinline__ F16v Mfma32x6First(const Parts8& a, const Parts8& b) 
   return Mfma32x5(a, b, Mfma32First<BF16>(a.lo, b.hi));
 }
 
-constexpr int kRangeUnit = 128;  // a key range's positions are a multiple of this, a workgroup's step
+// A key range's positions are a multiple of this, a step of a decode workgroup (8 x
+// 1088 bf16: 12.4 us, with 64 13.3).
+constexpr int kRangeUnit = 128;
 
 // Positions of one key range of a sequence of len positions.
 __device__ __forceinline__ int RangeOf(int len, int splits) {
@@ -199,8 +201,7 @@ __device__ __forceinline__ int RangeOf(int len, int splits) {
 __device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
 
 // Work: [row][splits] (maximum, sum), then [row][splits][kDim] outputs that are
-// not yet divided by the sum; row = query
-// token x head.
+// not yet divided by the sum; row = query token x head.
 __device__ __forceinline__ F2* PartStats(const AttentionArgs& a, int64_t row) {
   return reinterpret_cast<F2*>(a.work) + row * a.splits;
 }

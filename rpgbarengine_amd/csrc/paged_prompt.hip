@@ -14,6 +14,22 @@
 // the second product as they stand, and the key order that they come in is
 // the one that V is read in (16-bit types: ds_read_b64_tr_b16 reads four keys
 // of a dimension).
+//
+// Few rows: the waves form 2 or 4 groups (32 rows each then) that take the key
+// steps in turn and join their states in LDS; for fewer still the keys are cut into
+// ranges over workgroups, joined by a second kernel.
+//
+// f32 goes to the bf16 units in three parts a value (Split3): 512 tokens 78 us
+// with f32 products, 39 so. Its splitting costs the vector unit as much as the
+// products cost the matrix unit.
+//
+// Bound: the matrix products, for few rows the chain of steps of a tile. Measured,
+// 32 heads on 8 of 128: 4000 tokens of one sequence 147 us in bf16 (892 TFLOP/s; a
+// large product of a library reaches 1194), 793 in f32 (165; 153 in f32
+// instructions); 512 tokens 13 and 39 us; six turns of 12 to 40 tokens behind 400
+// to 1700 16 us in f16; documents of 376 GFLOP, bf16, 407 us. Matrix units are
+// busy for half the cycles, the exponentials and maxima share the rest; no LDS bank
+// conflicts.
 
 #include <hip/hip_runtime.h>
 
@@ -645,7 +661,7 @@ __global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
 }
 
 int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups);
-int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes);
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv);
 
 template <typename T, int kDim, int kGroups>
 void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
@@ -665,7 +681,7 @@ void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
 
 template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
-  const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv, kBytes<T>);
+  const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv);
   if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
   if (groups == 2) return LaunchGroups<T, kDim, 2>(a, s);
   LaunchGroups<T, kDim, 1>(a, s);
@@ -683,8 +699,12 @@ int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
   return n_tokens * group / (128 / groups) + n_seqs;
 }
 
-// Groups of a workgroup (its rows: 128 / groups).
-int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes) {
+// Groups of a workgroup (its rows: 128 / groups): one where that makes three
+// workgroups for every two compute units, or else as many as it takes. bf16, us
+// with 1 / 2 / 4: 512 tokens 17.9 / 16.5 / 13.8; 1000 30.9 / 28.9 / 33.5; 2000 56.8 /
+// 63.5 / 75.7; 4 x 300 18.5 / 21.7 / 28.1; 16 x 60 behind 640 31.3 / 26.9 / 34.8; six
+// turns 43.8 / 35.5 / 23.5; 203 behind 1297 38.8 / 31.5 / 20.4.
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv) {
   const int group = n_heads / n_kv;
   if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 384) return 1;
   if (TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
@@ -693,8 +713,11 @@ int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes
 
 }  // namespace
 
-int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
-  if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv, bytes) != 4) return 1;
+// Key ranges where not even half the compute units have a workgroup (12 tokens
+// behind 30000: 304 us with one, 37 with ranges; 203 behind 1297, 208 workgroups:
+// 20 us with one, 38 with three), of 512 positions at least.
+int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
+  if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv) != 4) return 1;
   const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv;
   const int64_t want = wgs >= 128 ? 1 : CeilDiv(256, wgs);
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));

@@ -14,12 +14,14 @@
 // polynomial of degree 5, 1.5e-13 relative).
 //
 // Four launches over (row, slice of the vocabulary), without a sort:
-//   Max    largest value (and its first index) and least finite one per slice
+//   Max    largest value (and its first index) and least finite one per slice,
+//          the largest of every group of four threads' tokens
 //   Count  histogram of 2048 equal steps of x below the row's maximum: count
 //          and weight, slices added by atomics; the row's last slice looks up
-//          the step that holds the cut
-//   Split  a list of the tokens down to that step; where those are more than kList, the list of its
-//          own tokens and the weight above it per 4096 tokens
+//          the step that holds the cut. For a small top_k the list below at once,
+//          down to the step of the k-th largest group
+//   Split  a list of the tokens down to the cut's step; where those are more than
+//          kList, the list of its own tokens and the weight above it per 4096 tokens
 //   Draw   one workgroup a row: the list sorted and cut, then the draw, among
 //          the list's tokens by index or in the unit that it falls into
 // A step of more than kList tokens (thousands of equal values) and a cut whose
@@ -27,7 +29,11 @@
 // top_p's) are found by Draw over the whole row, digit by digit.
 //
 // Bound: the logits' bytes, read once from HBM (later launches find them in
-// the memory-side cache); a single row is bound by its four launches.
+// the memory-side cache); for few rows the four launches. Measured, vocabulary of
+// 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 52,
+// min_p 49, temperature alone 91, top_p 131 (a weight in double and two LDS atomics
+// for nearly every token), all mixed 104; 8 f32 rows with min_p 18.5; one row with
+// top_p 41, its kernels 4, 13, 7 and 15.
 
 #include <hip/hip_runtime.h>
 
