@@ -60,7 +60,6 @@ constexpr int kDrawThreads = 1024;
 constexpr int kList = 1024;      // tokens of the cut's step that Draw ranks in LDS
 constexpr int kUnit = 4096;      // Draw looks for the token in a run of this many; slices are multiples of it
 constexpr int kMaxUnits = 64;    // of a row: 262144 tokens
-constexpr int kGroups = 64;      // groups of tokens of a slice whose maxima are kept (four threads' runs each)
 constexpr float kNone = -__builtin_inff();
 
 struct Bin {
@@ -75,19 +74,23 @@ struct SliceMax {
 
 struct Layout {
   int slices, length;  // tokens per slice
+  int groups;          // of a slice's tokens, whose maxima are kept: a thread's, or four threads'
   int64_t max_at, bins_at, weights_at, lists_at, counts_at, cuts_at, groups_at, bytes;
 };
 
 __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   Layout l;
-  // About 1500 workgroups where there are many rows, slices of 4096 tokens
-  // where there are few.
+  // About 1500 workgroups where there are many rows, as many as the card holds at a
+  // time, slices of 4096 tokens where there are few. 192 rows, us with 768 / 1536 /
+  // 3072: mixed parameters 136 / 104 / 100, top_p alone 119 / 132 / 160 (each
+  // slice adds its histogram to the row's).
   const int64_t most = (vocab + kUnit - 1) / kUnit;
   int64_t want = rows < 1 ? 1 : (1536 + rows - 1) / rows;
   want = want < 1 ? 1 : want > most ? most : want;
   want = want > kMaxUnits ? kMaxUnits : want;
   l.length = static_cast<int>(((vocab + want - 1) / want + kUnit - 1) / kUnit * kUnit);
   l.slices = static_cast<int>((vocab + l.length - 1) / l.length);
+  l.groups = l.slices <= 8 ? kThreads : kThreads / 4;
   l.bins_at = 0;
   l.max_at = l.bins_at + rows * kBins * static_cast<int64_t>(sizeof(Bin));
   l.weights_at = l.max_at + rows * l.slices * static_cast<int64_t>(sizeof(SliceMax));
@@ -95,7 +98,7 @@ __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   l.counts_at = l.lists_at + rows * kList * 8;
   l.cuts_at = (l.counts_at + rows * 8 + 63) / 64 * 64;
   l.groups_at = l.cuts_at + rows * 64;
-  l.bytes = l.groups_at + rows * l.slices * kGroups * 4;
+  l.bytes = l.groups_at + rows * l.slices * l.groups * 4;
   return l;
 }
 
@@ -115,7 +118,7 @@ struct Work {
         list(reinterpret_cast<uint64_t*>(a.work + l.lists_at) + static_cast<int64_t>(row) * kList),
         count(reinterpret_cast<uint32_t*>(a.work + l.counts_at) + 2 * row),
         cut(reinterpret_cast<Cut*>(a.work + l.cuts_at + static_cast<int64_t>(row) * 64)),
-        groups(reinterpret_cast<float*>(a.work + l.groups_at) + static_cast<int64_t>(row) * l.slices * kGroups) {}
+        groups(reinterpret_cast<float*>(a.work + l.groups_at) + static_cast<int64_t>(row) * l.slices * l.groups) {}
 };
 
 template <typename T>
@@ -190,8 +193,11 @@ struct Row {
   // top_k so small against the groups whose maxima are kept that the k-th largest
   // of those, which is no more than the k-th token, has few tokens above it: they
   // are listed without a histogram (192 rows of 151936, top_k 40: 37 us in
-  // CountKernel with one, 18 without).
-  __device__ __forceinline__ bool Direct(int slices) const { return k > 0 && k <= min(128, slices * kGroups / 4); }
+  // CountKernel with one, 18 without). Where at most a quarter of the groups hold one,
+  // 1.15 k tokens spread over them do, and k more that crowd in a few: within kList.
+  __device__ __forceinline__ bool Direct(const Layout& l) const {
+    return k > 0 && k <= min(kList * 7 / 16, l.slices * l.groups / 4);
+  }
 
   // w 2^44, at most half a unit off when rounded; 0 where it would be less
   // than half of one.
@@ -373,7 +379,10 @@ __global__ __launch_bounds__(kThreads) void MaxKernel(SampleArgs a, Layout l) {
   }
   float quad = fmaxf(most, lanes::DppF<lanes::kQuadXor1>(most));
   quad = fmaxf(quad, lanes::DppF<lanes::kQuadXor2>(quad));
-  if (tid % 4 == 0) w.groups[slice * kGroups + tid / 4] = quad;
+  if (l.groups == kThreads)
+    w.groups[slice * kThreads + tid] = most;
+  else if (tid % 4 == 0)
+    w.groups[slice * l.groups + tid / 4] = quad;
   __shared__ SliceMax s[kThreads / 64];
   const float top = lanes::WaveMaxF(most);
   const float low = -lanes::WaveMaxF(-least);
@@ -600,8 +609,8 @@ __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) 
   if (tid == 0) s_last = -1;
   __syncthreads();
   const char* x = a.logits + row * a.row_bytes;
-  if (r.Direct(l.slices)) {
-    for (int i = tid; i < l.slices * kGroups; i += kThreads) {
+  if (r.Direct(l)) {
+    for (int i = tid; i < l.slices * l.groups; i += kThreads) {
       const float top = w.groups[i];
       if (top > kNone) atomicAdd(&count[r.Bin(top)], 1u);
     }
