@@ -11,7 +11,7 @@
 // at most 2^18 of them in 64 bits): sums are the same in any order, so atomics
 // and slices cannot change a draw, and each is within half a unit of the exact
 // weight. A weight itself is computed in double (a table of 2^(-j/32) and a
-// polynomial of degree 5, 1.5e-13 relative).
+// polynomial of degree 5, 3e-15 relative).
 //
 // Four launches over (row, slice of the vocabulary), without a sort:
 //   Max    largest value (and its first index) and least finite one per slice,
@@ -179,7 +179,7 @@ struct Row {
   float max;     // -inf: nothing to draw from
   int32_t best;  // its first index
   float scale;   // histogram steps per unit of x
-  double c;      // log2(e) / T
+  double c32;    // 32 log2(e) / T
   bool greedy;
   int32_t k;      // 0: no limit
   double p, floor;  // 0: no limit; min_p in weight units
@@ -205,26 +205,25 @@ struct Row {
   // without). A step spans a 65th of its weight; the margin is for the
   // rounding of Bin.
   __device__ __forceinline__ uint32_t Most(int bin, uint64_t q) const {
-    const float low = __builtin_amdgcn_exp2f(44.0f - static_cast<float>(c) * (static_cast<float>(bin + 1) / scale)) * 0.98f;
+    const float low = __builtin_amdgcn_exp2f(44.0f - static_cast<float>(c32) * 0.03125f * (static_cast<float>(bin + 1) / scale)) * 0.98f;
     return q == 0 ? 0u : low >= 64.0f ? static_cast<uint32_t>(fminf(static_cast<float>(q) / low, 1e6f)) + 1u : 1u << 20;
   }
 
-  // w 2^44, at most half a unit off when rounded; 0 where it would be less
-  // than half of one.
+  // w 2^44, at most half a unit off when rounded (below half a unit: somewhere
+  // there). 2^-y = 2^-(n / 32) 2^-(y - n / 32) with n the integer next to 32 y, found
+  // by adding what leaves no bits for a fraction.
   __device__ __forceinline__ double Weight(float x, const double* pow2) const {
     const double d = x == max ? 0.0 : static_cast<double>(max) - static_cast<double>(x);
-    const double far = d == 0.0 ? 0.0 : d * c;
-    const bool in = far < 45.5;
-    const double y = in ? far : 0.0;  // (no branch: a run's weights are computed side by side)
-    const int n = static_cast<int>(y * 32.0);
-    const double z = (static_cast<double>(n) * 0.03125 - y) * 0.69314718055994530942;  // (-ln 2 / 32, 0]
+    const double y = fmin(d * c32, 46.0 * 32.0);  // (no branch: a run's weights are computed side by side)
+    const double t = y + 0x1.8p52, z = ((t - 0x1.8p52) - y) * (0.69314718055994530942 / 32.0);  // ln 2 / 64 at most
+    const int n = static_cast<int>(__builtin_bit_cast(uint64_t, t));
     double e = __builtin_fma(z, 1.0 / 120.0, 1.0 / 24.0);
     e = __builtin_fma(z, e, 1.0 / 6.0);
     e = __builtin_fma(z, e, 0.5);
     e = __builtin_fma(z, e, 1.0);
     e = __builtin_fma(z, e, 1.0);
-    const uint64_t t = __builtin_bit_cast(uint64_t, pow2[n & 31]) + (static_cast<uint64_t>(44 - (n >> 5)) << 52);
-    return in ? e * __builtin_bit_cast(double, t) : 0.0;
+    const uint64_t p = __builtin_bit_cast(uint64_t, pow2[n & 31]) + (static_cast<uint64_t>(44 - (n >> 5)) << 52);
+    return e * __builtin_bit_cast(double, p);
   }
   // rounded to an integer (weights are below 2^52)
   static __device__ __forceinline__ uint64_t Units(double w) {
@@ -258,7 +257,7 @@ __device__ __forceinline__ Row RowOf(const SampleArgs& a, const Layout& l, const
   r.best = __shfl(m.index, __ffsll(static_cast<unsigned long long>(at)) - 1, 64);  // (slices in order)
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
-  r.c = 1.4426950408889634074 / static_cast<double>(t);
+  r.c32 = 32.0 * 1.4426950408889634074 / static_cast<double>(t);
   const float span = fminf(31.6f * t, max - min);
   r.weightless_end = 31.6f * t <= max - min;
   r.scale = span > 0.0f ? static_cast<float>(kBins) / span : 0.0f;
