@@ -30,10 +30,10 @@
 //
 // Bound: the logits' bytes, read once from HBM (later launches find them in
 // the memory-side cache); for few rows the four launches. Measured, vocabulary of
-// 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 52,
-// min_p 49, temperature alone 91, top_p 131 (a weight in double and two LDS atomics
-// for nearly every token), all mixed 104; 8 f32 rows with min_p 18.5; one row with
-// top_p 41, its kernels 4, 13, 7 and 15.
+// 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 55,
+// min_p 48, temperature alone 75, top_p 99 (a weight in double and an LDS atomic
+// for nearly every token), all mixed 91; 8 f32 rows with min_p 18.5; one row with
+// top_p 38.
 
 #include <hip/hip_runtime.h>
 
@@ -82,7 +82,7 @@ __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   Layout l;
   // About 1500 workgroups where there are many rows, as many as the card holds at a
   // time, slices of 4096 tokens where there are few. 192 rows, us with 768 / 1536 /
-  // 3072: mixed parameters 136 / 104 / 100, top_p alone 119 / 132 / 160 (each
+  // 3072: mixed parameters 136 / 104 / 100, top_p 0.9 119 / 132 / 160 (each
   // slice adds its histogram to the row's).
   const int64_t most = (vocab + kUnit - 1) / kUnit;
   int64_t want = rows < 1 ? 1 : (1536 + rows - 1) / rows;
@@ -173,6 +173,8 @@ __device__ const double kPow2[32] = {
     0x1.172b83c7d517bp-1, 0x1.11301d0125b51p-1, 0x1.0b5586cf9890fp-1, 0x1.059b0d3158574p-1};
 
 constexpr double kOne = 17592186044416.0;  // 2^44: the largest weight
+
+__device__ __forceinline__ uint64_t Mask(bool x) { return x ? ~uint64_t{0} : 0; }
 
 // A row's parameters, from its slices' maxima.
 struct Row {
@@ -659,7 +661,7 @@ __global__ __launch_bounds__(kThreads) void CountKernel(SampleArgs a, Layout l) 
       const bool cy = at >= lo && r.Counted(y, by), cz = at + 1 >= lo && r.Counted(z, bz);
       if (!__any(cy || cz)) return;
       if (!lean) {
-        const uint64_t qy = cy ? Row::Units(r.Weight(y, pow2)) : 0, qz = cz ? Row::Units(r.Weight(z, pow2)) : 0;
+        const uint64_t qy = Row::Units(r.Weight(y, pow2)) & Mask(cy), qz = Row::Units(r.Weight(z, pow2)) & Mask(cz);
         if (qy != 0) atomicAdd(&weight[by], static_cast<unsigned long long>(qy));
         if (qz != 0) atomicAdd(&weight[bz], static_cast<unsigned long long>(qz));
       }
@@ -723,6 +725,7 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
     return;
   }
   list.Begin();
+  const bool limited = end_bin < kBins;
   const int listed_last = max(cut.k_bin < kBins ? cut.k_bin : -1, cut.p_bin < kBins ? cut.p_bin : -1);
   __shared__ uint64_t part[kThreads / 64];
   for (int start = slice * l.length; start < min(a.vocab, (slice + 1) * l.length); start += kUnit) {
@@ -731,13 +734,22 @@ __global__ __launch_bounds__(kThreads) void SplitKernel(SampleArgs a, Layout l) 
       const float top = Top<T>(run);
       if (!__any(r.MayReach(top) || r.Bin(top) <= listed_last)) return;
       ForTwo<T>(run, i, [&](float y, float z, int at) {
-        const int by = at >= lo && y > kNone ? r.Bin(y) : kBins;
-        const int bz = at + 1 >= lo && z > kNone ? r.Bin(z) : kBins;
+        // (masks, no branches: a branch would take the two weights one after the other)
         const double fy = r.Weight(y, pow2), fz = r.Weight(z, pow2);
-        sum += by < end_bin && fy >= r.floor ? Row::Units(fy) : 0;
-        sum += bz < end_bin && fz >= r.floor ? Row::Units(fz) : 0;
-        if (by < kBins && (by == cut.k_bin || by == cut.p_bin)) list.Add(y, at);
-        if (bz < kBins && (bz == cut.k_bin || bz == cut.p_bin)) list.Add(z, at + 1);
+        bool ty = at >= lo, tz = at + 1 >= lo;
+        if (limited) {
+          const int by = r.Bin(y), bz = r.Bin(z);
+          const bool ly = ty & (y > kNone) & ((by == cut.k_bin) | (by == cut.p_bin));
+          const bool lz = tz & (z > kNone) & ((bz == cut.k_bin) | (bz == cut.p_bin));
+          if (__any(ly | lz)) {
+            if (ly) list.Add(y, at);
+            if (lz) list.Add(z, at + 1);
+          }
+          ty &= by < end_bin;
+          tz &= bz < end_bin;
+        }
+        sum += Row::Units(fy) & Mask(ty & (fy >= r.floor));
+        sum += Row::Units(fz) & Mask(tz & (fz >= r.floor));
       });
     });
     sum = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(sum));
