@@ -20,13 +20,13 @@
 // ranges over workgroups, joined by a second kernel.
 //
 // f32 goes to the bf16 units in three parts a value (Split3): 512 tokens 78 us
-// with f32 products, 39 so. Its splitting costs the vector unit as much as the
+// with f32 products, 34 so. Its splitting costs the vector unit as much as the
 // products cost the matrix unit.
 //
 // Bound: the matrix products, for few rows the chain of steps of a tile. Measured,
 // 32 heads on 8 of 128: 4000 tokens of one sequence 147 us in bf16 (892 TFLOP/s; a
 // large product of a library reaches 1194), 793 in f32 (165; 153 in f32
-// instructions); 512 tokens 13 and 39 us; six turns of 12 to 40 tokens behind 400
+// instructions); 512 tokens 13 and 34 us; six turns of 12 to 40 tokens behind 400
 // to 1700 16 us in f16; documents of 376 GFLOP, bf16, 407 us. Matrix units are
 // busy for half the cycles, the exponentials and maxima share the rest; no LDS bank
 // conflicts.
@@ -179,16 +179,19 @@ __device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int t
 
 // grid (row tile x key head, key range): key heads next to each other, the tiles
 // with the most keys first.
-template <typename T, int kDim, int kGroups>
-__global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4) ? 1 : 2) void PromptKernel(AttentionArgs a) {
+template <typename T, int kDim, int kGroups, bool kShared>
+__global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4 && !kShared) ? 1 : 2) void PromptKernel(AttentionArgs a) {
   using Sh = Shape<T, kDim, kGroups>;
   // A group of one wave needs no barriers: it takes the next K tile in as soon as
   // the scores are done and the next V tile after the second product, each in the
   // place of the last (half the LDS: two workgroups per compute unit). Groups of
   // several waves have two of each in turn.
   constexpr bool kSolo = Sh::kGroupWaves == 1;
-  constexpr int kBuffers = kSolo ? 1 : 2;
-  __shared__ __align__(256) char lds[kGroups * 2 * kBuffers * Sh::kTileBytes];  // per group [buffer][K tile, V tile]
+  // kShared: K and V take turns in one place, so that two workgroups fit a compute
+  // unit even in f32: the other's products run while a tile is on its way.
+  static_assert(kSolo || !kShared, "groups of one wave");
+  constexpr int kTiles = kShared ? 1 : kSolo ? 2 : 4;
+  __shared__ __align__(256) char lds[kGroups * kTiles * Sh::kTileBytes];  // per group [buffer][K tile, V tile]
   __shared__ uint32_t page_ok[kGroups][2];     // per buffer: a byte for each unit of rows
   __shared__ int any_odd, first_odd[kOddKinds][kDim];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -245,7 +248,7 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   const int k_from = 16 * (sc ^ KSwizzle<T, kDim>(gw * kWaveRows + srow));
   const int v_from = 16 * (sc ^ VSwizzle<T, kDim>(gw * kWaveRows + srow));
   const int to = gw * kWaveRows * Sh::kRowBytes;
-  char* tiles = lds + grp * 2 * kBuffers * Sh::kTileBytes;
+  char* tiles = lds + grp * kTiles * Sh::kTileBytes;
   // the first key of the group's part of a step
   auto first_key = [&](int step) { return key_begin + (step * kGroups + grp) * Sh::kKeys; };
   // Where a step's rows of this wave lie. Page numbers are looked up a step ahead.
@@ -462,13 +465,13 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
     if constexpr (kSolo) {
       constexpr int kLoads = Sh::kPerThread;
       char* kt = tiles;
-      char* vt = tiles + Sh::kTileBytes;
+      char* vt = tiles + (kShared ? 0 : Sh::kTileBytes);
       Place now, next;
       if (steps > 0) {
         look_up(0);
         now = place_of(0);
         fetch_k(now, kt);
-        fetch_v(now, vt);
+        if (!kShared) fetch_v(now, vt);
         look_up(1);
       }
       for (int step = 0; step < steps; ++step) {
@@ -476,19 +479,22 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
         const bool mine = key0 <= wave_last && key0 < key_end, more = step + 1 < steps;
         next = place_of(step + 1);
         look_up(step + 2);
-        // in flight: K, then V of this step
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+        // in flight: K, then V of this step (shared: K alone)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kShared ? 0 : kLoads) : "memory");
         if (mine) scores(kt);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read
-        if (more) fetch_k(next, kt);
+        if (kShared)
+          fetch_v(now, vt);
+        else if (more)
+          fetch_k(next, kt);
         uint32_t pages = 0;
 #pragma unroll
         for (int u = 0; u < kWaveUnits; ++u) pages |= (now.ok[u] ? 1u : 0u) << (8 * u);
 #pragma unroll
         for (int u = kWaveUnits; u < 4; ++u) pages |= 1u << (8 * u);
         if (mine) weigh(key0, pages);
-        // in flight: V of this step, then K of the next
-        if (more)
+        // in flight: V of this step, then K of the next (shared: V alone)
+        if (more && !kShared)
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
         else
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -497,7 +503,8 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
           add_values(vt);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
-        if (more) fetch_v(next, vt);
+        if (more && kShared) fetch_k(next, kt);
+        if (more && !kShared) fetch_v(next, vt);
         now = next;
       }
     } else {
@@ -583,10 +590,10 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   } else {
     // The groups' states, joined in LDS where the tiles were.
     __shared__ float sm[kGroups][Sh::kRows], sl[kGroups][Sh::kRows];
-    static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= 2 * kBuffers * Sh::kTileBytes, "a group's state fits its tiles");
+    static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= kTiles * Sh::kTileBytes, "a group's state fits its tiles");
     // chunk c (four dimensions) of row r of group g
     auto at = [&](int g, int r, int c) {
-      return reinterpret_cast<F4*>(lds + g * 2 * kBuffers * Sh::kTileBytes + r * kDim * 4 + (c ^ (r & 15)) * 16);
+      return reinterpret_cast<F4*>(lds + g * kTiles * Sh::kTileBytes + r * kDim * 4 + (c ^ (r & 15)) * 16);
     };
     const int r = 32 * gw + (lane & 31);
     if (h == 0) sm[grp][r] = m, sl[grp][r] = l;
@@ -663,13 +670,13 @@ __global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
 int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups);
 int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv);
 
-template <typename T, int kDim, int kGroups>
+template <typename T, int kDim, int kGroups, bool kShared = false>
 void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
   const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, kGroups);
   RPG_CHECK(tiles * a.c.n_kv <= kMaxGroups &&
                 (a.splits == 1 || static_cast<int64_t>(a.s.n_tokens) * a.n_heads <= kMaxGroups),
             "%d x %d query rows in one launch", a.s.n_tokens, a.n_heads);
-  PromptKernel<T, kDim, kGroups>
+  PromptKernel<T, kDim, kGroups, kShared>
       <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
   if constexpr (kGroups == 4) {
@@ -679,9 +686,20 @@ void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
   }
 }
 
+// f32 rows of 128: K and V share a place above this many workgroups, one for each
+// compute unit and the few that TilesFor counts too many. With two places / one, us:
+// 256 tokens (264 workgroups) 19.0 / 21.9, 350 (352) 31.2 / 27.8, 512 (520) 39.4 /
+// 34.5, 700 (704) 65 / 55, 300 behind 1700 (304) 116 / 94; 12 behind 30000 (256 with
+// their ranges) 84 / 107, 40 (288) 274 / 237.
+constexpr int64_t kCrowd = 280;
+
 template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
   const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv);
+  if constexpr (kBytes<T> == 4 && kDim == 128) {
+    const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, 4);
+    if (groups == 4 && tiles * a.c.n_kv * a.splits > kCrowd) return LaunchGroups<T, kDim, 4, true>(a, s);
+  }
   if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
   if (groups == 2) return LaunchGroups<T, kDim, 2>(a, s);
   LaunchGroups<T, kDim, 1>(a, s);

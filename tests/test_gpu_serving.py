@@ -383,6 +383,30 @@ def test_attention_in_place(dtype, lens, new):
     assert torch.equal(q, want) and torch.equal(one, want_one)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_prompt_many_short_turns(dtype):
+    """More row tiles than compute units, most of them partly filled: ragged ends,
+    pages that are not named, NaN in every place that no query sees."""
+    lens = [5 + 7 * i % 101 for i in range(44)]
+    new = [min(n, 1 + 5 * i % 13) for i, n in enumerate(lens)]
+    b = Batch(lens, new, dtype, 8, 128, 16, 8, seed=26)
+    used = torch.zeros(b.n_pages, 16, dtype=torch.bool)
+    for i, n in enumerate(lens):
+        if i % 9 == 4 and n > 16:
+            b.table[i, 0] = b.n_pages + i
+        for p in range(n):
+            at = int(b.table[i, p // 16])
+            if at < b.n_pages:
+                used[at, p % 16] = True
+    hold = (~used)[:, None, :, None]
+    k2, v2 = b.k.masked_fill(hold, 0.0), b.v.masked_fill(hold, 0.0)
+    b.k, b.v = b.k.masked_fill(hold, math.nan), b.v.masked_fill(hold, math.nan)
+    q = b.normal(b.tokens, 8, 128)
+    cache, table, lens_d, starts = b.gpu()
+    want, bound = expect_prompt(b, q, 128 ** -0.5, k2, v2)
+    close(serving.prompt_attention(q.cuda(), cache, table, lens_d, starts), want, bound)
+
+
 def test_prompt_more_tokens_than_positions():
     """Tokens before the cache's first position see no key: zeros."""
     b = Batch([3, 0], [5, 2], torch.float16, seed=10)
