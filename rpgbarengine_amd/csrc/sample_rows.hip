@@ -30,9 +30,9 @@
 //
 // Bound: the logits' bytes, read once from HBM (later launches find them in
 // the memory-side cache); for few rows the four launches. Measured, vocabulary of
-// 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 55,
-// min_p 48, temperature alone 75, top_p 99 (a weight in double and an LDS atomic
-// for nearly every token), all mixed 91; 8 f32 rows with min_p 18.5; one row with
+// 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 50,
+// min_p 48, temperature alone 75, top_p 95 (a weight in double and an LDS atomic
+// for nearly every token), all mixed 83; 8 f32 rows with min_p 18.5; one row with
 // top_p 38.
 
 #include <hip/hip_runtime.h>
@@ -894,9 +894,11 @@ __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout 
   __shared__ double pow2[32];
   __shared__ uint64_t keys[kDrawThreads];
   __shared__ unsigned long long unit_weight[kMaxUnits];
-  __shared__ double weights[kDrawThreads];
   __shared__ uint64_t s_taken, s_last;
+  __shared__ uint32_t s_there;
   LoadPow2(pow2);
+  if (tid < kMaxUnits) unit_weight[tid] = 0;
+  if (tid == 0) s_there = 0;
   const char* x = a.logits + row * a.row_bytes;
   Cut cut{kBins, kBins, 0, 0, 0, 0, 0, 0, 0};
   if (r.k != 0 || r.p != 0.0) cut = stored;
@@ -906,22 +908,18 @@ __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout 
   const bool slow = cut.slow || n > kList;
   __syncthreads();
 
-  // The list, best first: this thread's token and the weight before it. Where
-  // the list holds all that can be kept, those that are, by index: a second
-  // round of the same code.
+  // The list, best first: this thread's token and the weight before it.
   uint64_t key = 0, q = 0, before = 0, sum = 0;
   double f = 0.0;
   if (n > 0 && !slow) {
-    key = tid < static_cast<int>(n) ? item : 0;
-    int here = static_cast<int>(n);
-#pragma unroll 1
-    for (int round = 0;; ++round) {
-      key = SortDown(key, PowerFor(here), keys);
-      f = round == 0 ? (tid < here ? r.Weight(ValueOf(key), pow2) : 0.0)
-                     : (tid < here ? weights[key & 0xFFFFFFFFu] : 0.0);
-      q = Row::Units(f);
-      before = Before<kDrawThreads>(q, &sum);
-      if (!cut.whole || round == 1) break;
+    const int here = static_cast<int>(n);
+    key = SortDown(tid < here ? item : 0, PowerFor(here), keys);
+    f = tid < here ? r.Weight(ValueOf(key), pow2) : 0.0;
+    q = Row::Units(f);
+    before = Before<kDrawThreads>(q, &sum);
+    if (cut.whole) {
+      // It holds all that can be kept. The draw among those that are: the 64th
+      // part of the vocabulary that it falls into, then the token there.
       uint64_t taken = cut.all;
       if (r.k != 0) {
         if (tid == min(here, r.k) - 1) s_taken = before + q;
@@ -930,15 +928,27 @@ __global__ __launch_bounds__(kDrawThreads) void DrawKernel(SampleArgs a, Layout 
       }
       const bool in = tid < here && (r.k == 0 || tid < r.k) && q != 0 && f >= r.floor &&
                       (r.p == 0.0 || static_cast<double>(before) < r.p * static_cast<double>(taken));
-      weights[tid] = f;
-      here = __syncthreads_count(in);  // kept are the first threads
-      key = in ? key << 32 | tid : 0;
-    }
-    if (cut.whole) {
-      const double mark = u * static_cast<double>(sum);
-      const bool past = static_cast<double>(before + q) > mark || tid == here - 1;
-      if (tid < here && past && (tid == 0 || !(static_cast<double>(before) > mark)))
-        Write(a, row, static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key >> 32)), f, sum);
+      const int index = IndexOf(key);
+      const int part = min(static_cast<int>(static_cast<float>(index) * (64.0f / static_cast<float>(a.vocab))), 63);
+      if (in) atomicAdd(&unit_weight[part], static_cast<unsigned long long>(q));
+      __syncthreads();
+      const uint64_t mine = unit_weight[tid & 63];
+      const uint64_t up_to = lanes::WaveInclusiveAdd(static_cast<unsigned long long>(mine));
+      const uint64_t total = lanes::ReadLaneT(up_to, 63);
+      const double mark = u * static_cast<double>(total);
+      uint64_t hit = __ballot(mine != 0 && static_cast<double>(up_to) > mark);
+      if (hit == 0) hit = 1ull << (63 - __clzll(static_cast<long long>(__ballot(mine != 0))));  // u = 1: the last one
+      const int at = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+      const uint64_t end = lanes::ReadLaneT(up_to, at);
+      const bool there = in && part == at;
+      if (there) keys[atomicAdd(&s_there, 1u)] = static_cast<uint64_t>(index) << 45 | q;  // (18 bits, 45 bits)
+      __syncthreads();
+      if (!there) return;
+      uint64_t up = end - lanes::ReadLaneT(mine, at);
+      for (uint32_t i = 0; i < s_there; ++i)
+        if (static_cast<int>(keys[i] >> 45) < index) up += keys[i] & ((uint64_t{1} << 45) - 1);
+      if ((static_cast<double>(up + q) > mark || up + q == end) && !(static_cast<double>(up) > mark))
+        Write(a, row, index, f, total);
       return;
     }
   }
