@@ -81,9 +81,9 @@ struct Layout {
 __host__ __device__ inline Layout LayoutOf(int64_t rows, int64_t vocab) {
   Layout l;
   // About 1500 workgroups where there are many rows, as many as the card holds at a
-  // time, slices of 4096 tokens where there are few. 192 rows, us with 768 / 1536 /
-  // 3072: mixed parameters 136 / 104 / 100, top_p 0.9 119 / 132 / 160 (each
-  // slice adds its histogram to the row's).
+  // time, slices of 4096 tokens where there are few. 192 rows, us with half as
+  // many / these / twice as many: mixed parameters 136 / 104 / 100, top_p 0.9 119 /
+  // 132 / 160 (each slice adds its histogram to the row's).
   const int64_t most = (vocab + kUnit - 1) / kUnit;
   int64_t want = rows < 1 ? 1 : (1536 + rows - 1) / rows;
   want = want < 1 ? 1 : want > most ? most : want;
