@@ -18,9 +18,9 @@
 // Bound: the K and V bytes, each read once (16 columns are computed for any
 // group size: at 8 heads f32 the products would take 1/2 of the time the bytes
 // do, the 16-bit types' 1/10). Measured, 32 heads on 8 of 128: 64 sequences of
-// 100 to 6000 positions, bf16, 862 MB in 165-171 us (the rate of a large copy:
-// 171); one of 131072, f16, 537 MB in 95 us (107); 8 of 1088, f32, 71 MB in 18.5
-// us (14, and two launches); one of 97, f16: 7 us, the call itself. Ranges: see
+// 201 to 11167 positions, bf16, 861 MB in 165-171 us (the rate of a large copy:
+// 171); one of 131000, f16, 537 MB in 95 us (107); 8 of about 1073, f32, 70 MB in 18.5
+// us (14, and two launches); one of 95, f16: 7 us, the call itself. Ranges: see
 // DecodeSplits.
 
 #include <hip/hip_runtime.h>
@@ -290,8 +290,8 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
 }  // namespace
 
 // Ranges for a workgroup per compute unit, and of 2048 positions at most, so that
-// the longest sequence of a ragged batch does not end alone: 64 ragged ones of up
-// to 6000 take 152 us, 162 with 1024. More workgroups only add joins: 32 x 2000
+// the longest sequence of a ragged batch does not end alone: 64 of 200
+// to 12000 take 152 us, 162 with 1024. More workgroups only add joins: 32 x 2000
 // bf16 48.2 us aiming at 256, 52.1 at 512, 53.5 at 1024; 8 x 1088 f32 18.7, 22.1,
 // 21.1. The rule knows the sequences' capacity, not their lengths, which are on
 // the device: ranges behind a sequence's end return at once.

@@ -26,8 +26,8 @@
 // Bound: the matrix products, for few rows the chain of steps of a tile. Measured,
 // 32 heads on 8 of 128: 4000 tokens of one sequence 147 us in bf16 (892 TFLOP/s; a
 // large product of a library reaches 1194), 793 in f32 (165; 153 in f32
-// instructions); 512 tokens 13 and 34 us; six turns of 12 to 40 tokens behind 400
-// to 1700 16 us in f16; documents of 376 GFLOP, bf16, 407 us. Matrix units are
+// instructions); 512 tokens 13 and 34 us; six turns of 13 to 50 tokens behind 400
+// to 1000 16 us in f16; four documents of about 3000, 376 GFLOP, bf16, 407 us. Matrix units are
 // busy for half the cycles, the exponentials and maxima share the rest; no LDS bank
 // conflicts.
 
