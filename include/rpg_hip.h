@@ -279,7 +279,8 @@ typedef struct {
  * QK-norm and RoPE (reference src/qwen3.cc:139-167), computed in f32 and
  * rounded once. A token whose position is below 0 (more new tokens than
  * positions) or at or past rope_rows is left out: no key, value or query of
- * it is written. */
+ * it is written. Two new tokens whose tables lead to one place leave nothing
+ * defined there. */
 RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
                                          const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm,
