@@ -15,9 +15,9 @@
 // the one that V is read in (16-bit types: ds_read_b64_tr_b16 reads four keys
 // of a dimension).
 //
-// Few rows: the waves form 2 or 4 groups (32 rows each then) that take the key
-// steps in turn and join their states in LDS; for fewer still the keys are cut into
-// ranges over workgroups, joined by a second kernel.
+// Few rows: the waves form 2, 4 or 8 groups (of two waves or of one) that take the
+// key steps in turn and join their states in LDS; for fewer still the keys are cut
+// into ranges over workgroups, joined by a second kernel.
 //
 // f32 goes to the bf16 units in three parts a value (Split3): 512 tokens 78 us
 // with f32 products, 34 so. Its splitting costs the vector unit as much as the
@@ -27,7 +27,7 @@
 // 32 heads on 8 of 128: 4000 tokens of one sequence 147 us in bf16 (892 TFLOP/s; a
 // large product of a library reaches 1194), 793 in f32 (165; 153 in f32
 // instructions); 512 tokens 13 and 34 us; six turns of 13 to 50 tokens behind 400
-// to 1000 16 us in f16; four documents of about 3000, 376 GFLOP, bf16, 407 us. Matrix units are
+// to 1000 14 us in f16; four documents of about 3000, 376 GFLOP, bf16, 407 us. Matrix units are
 // busy for half the cycles, the exponentials and maxima share the rest; no LDS bank
 // conflicts.
 
@@ -44,10 +44,9 @@ namespace rpg {
 namespace paged {
 namespace {
 
-constexpr int kWaves = 4;
-
 template <typename T, int kDim, int kGroups>
 struct Shape {
+  static constexpr int kWaves = kGroups == 8 ? 8 : 4;
   static constexpr int kGroupWaves = kWaves / kGroups;
   static constexpr int kRows = 32 * kGroupWaves;              // rows of a workgroup's tile
   static constexpr int kKeys = kBytes<T> == 4 || kGroups > 1 ? 32 : 64;  // keys of a group's step
@@ -180,7 +179,7 @@ __device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int t
 // grid (row tile x key head, key range): key heads next to each other, the tiles
 // with the most keys first.
 template <typename T, int kDim, int kGroups, bool kShared>
-__global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4 && !kShared) ? 1 : 2) void PromptKernel(AttentionArgs a) {
+__global__ __launch_bounds__(kGroups == 8 ? 512 : 256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4 && !kShared) ? 1 : 2) void PromptKernel(AttentionArgs a) {
   using Sh = Shape<T, kDim, kGroups>;
   // A group of one wave needs no barriers: it takes the next K tile in as soon as
   // the scores are done and the next V tile after the second product, each in the
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   const int wave_first = t.Position(row0 + 32 * gw, group), wave_last = t.Position(row0 + 32 * gw + 31, group);
   const int tile_first = t.Position(row0, group), keys = t.Position(row0 + Sh::kRows - 1, group) + 1;
   int key_begin = 0, key_end = max(keys, 0);
-  if constexpr (kGroups == 4) {
+  if constexpr (kGroups >= 4) {
     const int range = RangeOf(max(keys, 1), a.splits);
     key_begin = blockIdx.y * range;
     key_end = min(key_end, key_begin + range);
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
   const int in_page = (1 << a.c.page_log2) - 1;
   if (tid == 0) any_odd = 0;
   if (tid < 2 * kGroups) page_ok[tid / 2][tid % 2] = 0x01010101u;
-  for (int i = tid; i < kOddKinds * kDim; i += 64 * kWaves) first_odd[i / kDim][i % kDim] = INT32_MAX;
+  for (int i = tid; i < kOddKinds * kDim; i += 64 * Sh::kWaves) first_odd[i / kDim][i % kDim] = INT32_MAX;
   __syncthreads();
 
   // Staging by LDS DMA: a wave brings kWaveRows rows, a lane kPerThread chunks
@@ -619,7 +618,7 @@ __global__ __launch_bounds__(64 * kWaves, kGroups == 2 || (kGroups == 4 && kByte
     __syncthreads();
     const bool odd = any_odd != 0;
     const bool alone = a.splits == 1 || RangeOf(max(keys, 1), a.splits) >= keys;
-    for (int i = tid; i < Sh::kRows * (kDim / 4); i += 64 * kWaves) {
+    for (int i = tid; i < Sh::kRows * (kDim / 4); i += 64 * Sh::kWaves) {
       const int ri = i / (kDim / 4), d = i % (kDim / 4) * 4, row_i = row0 + ri;
       if (row_i >= n_rows) break;
       float mi = sm[0][ri], li = 0.0f;
@@ -668,7 +667,18 @@ __global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
 }
 
 int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups);
-int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv);
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
+
+// Key ranges where not even half the compute units have a workgroup (12 tokens
+// behind 30000: 304 us with one, 37 with ranges; 203 behind 1297, 208 workgroups:
+// 20 us with one, 38 with three), of 512 positions at least. In 16 bits eight groups
+// go through 1536 positions in the time that the ranges and their join take (100
+// behind 1400, 104 workgroups: 24.3 us with three ranges of four groups, 16.3 with
+// one of eight; a token each behind 1000, 72: 15.6, 13.3).
+int RangesFor(int64_t wgs, int bytes, int64_t capacity) {
+  if (wgs >= 128 || (bytes == 2 && capacity <= 1536)) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min({CeilDiv(256, wgs), CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
+}
 
 template <typename T, int kDim, int kGroups, bool kShared = false>
 void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
@@ -677,9 +687,9 @@ void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
                 (a.splits == 1 || static_cast<int64_t>(a.s.n_tokens) * a.n_heads <= kMaxGroups),
             "%d x %d query rows in one launch", a.s.n_tokens, a.n_heads);
   PromptKernel<T, kDim, kGroups, kShared>
-      <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * kWaves, 0, s>>>(a);
+      <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * Shape<T, kDim, kGroups>::kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
-  if constexpr (kGroups == 4) {
+  if constexpr (kGroups >= 4) {
     if (a.splits == 1) return;
     PromptJoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_tokens) * a.n_heads, 256, 0, s>>>(a);
     HIP_CHECK(hipGetLastError());
@@ -695,7 +705,10 @@ constexpr int64_t kCrowd = 280;
 
 template <typename T, int kDim>
 void Launch(const AttentionArgs& a, hipStream_t s) {
-  const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv);
+  const int groups = GroupsFor(a.s.n_tokens, a.s.n_seqs, a.n_heads, a.c.n_kv, kBytes<T>, a.s.capacity);
+  if constexpr (kBytes<T> == 2) {
+    if (groups == 8) return LaunchGroups<T, kDim, 8>(a, s);
+  }
   if constexpr (kBytes<T> == 4 && kDim == 128) {
     const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, 4);
     if (groups == 4 && tiles * a.c.n_kv * a.splits > kCrowd) return LaunchGroups<T, kDim, 4, true>(a, s);
@@ -714,31 +727,31 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
 }
 
 int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
-  return n_tokens * group / (128 / groups) + n_seqs;
+  return n_tokens * group / (128 / std::min(groups, 4)) + n_seqs;
 }
 
-// Groups of a workgroup (its rows: 128 / groups): one where that makes three
-// workgroups for every two compute units, or else as many as it takes. bf16, us
-// with 1 / 2 / 4: 512 tokens 17.9 / 16.5 / 13.8; 1000 30.9 / 28.9 / 33.5; 2000 56.8 /
-// 63.5 / 75.7; 4 x 300 18.5 / 21.7 / 28.1; 16 x 60 behind 640 31.3 / 26.9 / 34.8; six
-// turns 43.8 / 35.5 / 23.5; 203 behind 1297 38.8 / 31.5 / 20.4.
-int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv) {
+// Groups of a workgroup (its rows: 128 / groups, 32 at the least): one where that
+// makes three workgroups for every two compute units, or else as many as it
+// takes. bf16, us with 1 / 2 / 4: 512 tokens 17.9 / 16.5 / 13.8; 1000 30.9 / 28.9 /
+// 33.5; 2000 56.8 / 63.5 / 75.7; 4 x 300 18.5 / 21.7 / 28.1; 16 x 60 behind 640 31.3 /
+// 26.9 / 34.8; six turns 43.8 / 35.5 / 23.5; 203 behind 1297 38.8 / 31.5 / 20.4.
+// 16-bit types: eight, of a wave each, where those workgroups find a compute unit
+// to themselves and the keys are many and not cut into ranges (4 / 8: six turns
+// 16.8 / 14.9, 200 behind 1300 19.4 / 16.9; 200 alone 10.0 / 10.6, 300 11.9 / 17.7).
+constexpr int64_t kUnits = 256;  // compute units
+int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
   const int group = n_heads / n_kv;
   if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 384) return 1;
   if (TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
-  return 4;
+  const int64_t wgs = TilesFor(n_tokens, n_seqs, group, 4) * n_kv;
+  return bytes == 2 && wgs <= kUnits && capacity > 512 && RangesFor(wgs, bytes, capacity) == 1 ? 8 : 4;
 }
 
 }  // namespace
 
-// Key ranges where not even half the compute units have a workgroup (12 tokens
-// behind 30000: 304 us with one, 37 with ranges; 203 behind 1297, 208 workgroups:
-// 20 us with one, 38 with three), of 512 positions at least.
-int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
-  if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv) != 4) return 1;
-  const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv;
-  const int64_t want = wgs >= 128 ? 1 : CeilDiv(256, wgs);
-  return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
+int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
+  if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv, bytes, capacity) != 4) return 1;
+  return RangesFor(TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv, bytes, capacity);
 }
 
 void Prompt(const AttentionArgs& a, hipStream_t s) {

@@ -142,7 +142,8 @@ void CheckHeads(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads) {
 
 int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
   if (prompt)
-    return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, s.capacity);
+    return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, ElementBytes(static_cast<int32_t>(c.type)),
+                               s.capacity);
   return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, s.capacity);
 }
 

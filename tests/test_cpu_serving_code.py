@@ -77,8 +77,8 @@ def test_counted_waits_of_one_wave_groups(functions):
     """A wave waits for K with as many loads outstanding as V has, and for V with
     as many as the next K: every tile's loads number what the waits count (others
     in between would only make them wait longer)."""
-    solo = {n: t for n, t in functions.items() if re.search(r"PromptKernelI\S+ELi\d+ELi4ELb0E", n)}
-    assert len(solo) == 6
+    solo = {n: t for n, t in functions.items() if re.search(r"PromptKernelI\S+ELi\d+ELi[48]ELb0E", n)}
+    assert len(solo) == 10
     shared = [t for n, t in functions.items() if re.search(r"PromptKernelI\S+ELi\d+ELi4ELb1E", n)]
     assert len(shared) == 1  # K and V in one place: nothing else in flight, waits for all
     loop = re.findall(r"buffer_load_dwordx4 [^\n]* lds|s_waitcnt vmcnt\(0\)", shared[0])

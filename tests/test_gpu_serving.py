@@ -407,6 +407,36 @@ def test_prompt_many_short_turns(dtype):
     close(serving.prompt_attention(q.cuda(), cache, table, lens_d, starts), want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("lens", [[530, 690, 41], [2300, 1700, 3]], ids=["groups", "ranges"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_few_rows_of_many_keys(dtype, lens, dim):
+    """Turns behind long histories, a page of each not named, NaN in the places that
+    no query sees, and a value of the history infinite."""
+    new = [9, 4, 2]
+    b = Batch(lens, new, dtype, 2, dim, 32, 6, seed=27)
+    used = torch.zeros(b.n_pages, 32, dtype=torch.bool)
+    for i, n in enumerate(lens):
+        if n > 100:
+            b.table[i, 3] = -5
+        for p in range(n):
+            at = int(b.table[i, p // 32])
+            if at >= 0:
+                used[at, p % 32] = True
+    hold = (~used)[:, None, :, None]
+    k2, v2 = b.k.masked_fill(hold, 0.0), b.v.masked_fill(hold, 0.0)
+    b.k, b.v = b.k.masked_fill(hold, math.nan), b.v.masked_fill(hold, math.nan)
+    at, d = int(b.table[0, 8]), 33
+    b.v[at, 1, 7, d] = -math.inf
+    q = b.normal(b.tokens, 6, dim)
+    cache, table, lens_d, starts = b.gpu()
+    got = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts).double().cpu()
+    want, bound = expect_prompt(b, q, dim ** -0.5, k2, v2)
+    assert bool((got[:9, 3:, d] == -math.inf).all())
+    got[:9, 3:, d] = want[:9, 3:, d]
+    close(got, want, bound)
+
+
 def test_prompt_more_tokens_than_positions():
     """Tokens before the cache's first position see no key: zeros."""
     b = Batch([3, 0], [5, 2], torch.float16, seed=10)
