@@ -70,7 +70,7 @@ struct AttentionArgs {
 
 // The key ranges that a batch of this shape is cut into at most, and the bytes
 // of their partials (0 for one range).
-int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity);
+int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
 int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
 int64_t WorkBytes(int64_t rows, int head_dim, int splits);
 void Decode(const AttentionArgs& a, hipStream_t s);

@@ -289,15 +289,19 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Ranges for a workgroup per compute unit, and of 2048 positions at most, so that
-// the longest sequence of a ragged batch does not end alone: 64 of 200
-// to 12000 take 152 us, 162 with 1024. More workgroups only add joins: 32 x 2000
-// bf16 48.2 us aiming at 256, 52.1 at 512, 53.5 at 1024; 8 x 1088 f32 18.7, 22.1,
-// 21.1. The rule knows the sequences' capacity, not their lengths, which are on
-// the device: ranges behind a sequence's end return at once.
-int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
+// Ranges for a workgroup per compute unit and none with two (9 x 1000 f32: 27.0 us
+// with 288 workgroups, 20.0 with 216; 11 x 4000 bf16 51 with 264, 39 with 176), and
+// of 2048 positions at most, so that the longest sequence of a ragged batch does not
+// end alone: 64 of 200 to 12000 take 152 us, 162 with 1024. Aiming higher only adds
+// joins: 32 x 2000 bf16 48.2 us aiming at 256, 52.1 at 512, 53.5 at 1024; 8 x 1088 f32
+// 18.7, 22.1, 21.1. Rows of a few steps stay whole, a join takes as long: one of 200
+// bf16 12.0 us in ranges, 7.6 whole, 500 11.7 and 8.4, 700 11.9 and 10.3; f32 200 11.7
+// and 10.1, 400 11.6 and 13.7. The rule knows the sequences' capacity, not their
+// lengths, which are on the device: ranges behind a sequence's end return at once.
+int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
+  if (capacity * bytes <= 1280) return 1;
   const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));
-  const int64_t want = std::max(CeilDiv(256, base), CeilDiv(capacity, 2048));
+  const int64_t want = std::max(256 / base, CeilDiv(capacity, 2048));
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, kRangeUnit), int64_t{kMaxSplits}})));
 }
 

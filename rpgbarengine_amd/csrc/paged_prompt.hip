@@ -674,10 +674,13 @@ int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes
 // 20 us with one, 38 with three), of 512 positions at least. In 16 bits eight groups
 // go through 1536 positions in the time that the ranges and their join take (100
 // behind 1400, 104 workgroups: 24.3 us with three ranges of four groups, 16.3 with
-// one of eight; a token each behind 1000, 72: 15.6, 13.3).
+// one of eight; a token each behind 1000, 72: 15.6, 13.3). In f32, a workgroup to a
+// compute unit, as many as find one free (40 behind 30000, 48 workgroups: 237 us with
+// six, 176 with five), in 16 bits one more (68 and 72).
 int RangesFor(int64_t wgs, int bytes, int64_t capacity) {
   if (wgs >= 128 || (bytes == 2 && capacity <= 1536)) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min({CeilDiv(256, wgs), CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
+  const int64_t want = bytes == 4 ? 256 / wgs : CeilDiv(256, wgs);
+  return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
 }
 
 template <typename T, int kDim, int kGroups, bool kShared = false>
@@ -700,7 +703,7 @@ void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
 // compute unit and the few that TilesFor counts too many. With two places / one, us:
 // 256 tokens (264 workgroups) 19.0 / 21.9, 350 (352) 31.2 / 27.8, 512 (520) 39.4 /
 // 34.5, 700 (704) 65 / 55, 300 behind 1700 (304) 116 / 94; 12 behind 30000 (256 with
-// their ranges) 84 / 107, 40 (288) 274 / 237.
+// their ranges) 84 / 107.
 constexpr int64_t kCrowd = 280;
 
 template <typename T, int kDim>

@@ -141,10 +141,9 @@ void CheckHeads(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads) {
 }
 
 int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
-  if (prompt)
-    return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, ElementBytes(static_cast<int32_t>(c.type)),
-                               s.capacity);
-  return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, s.capacity);
+  const int bytes = ElementBytes(static_cast<int32_t>(c.type));
+  if (prompt) return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
+  return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
 }
 
 int64_t AttentionWork(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
