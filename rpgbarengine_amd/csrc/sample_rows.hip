@@ -1046,7 +1046,8 @@ void Launch(const SampleArgs& a, hipStream_t s) {
   const Layout l = LayoutOf(a.rows, a.vocab);
   const dim3 grid(l.slices, a.rows);
   MaxKernel<T><<<grid, kThreads, 0, s>>>(a, l);
-  CountKernel<T><<<grid, kThreads, 0, s>>>(a, l);
+  // (min_p needs no cut: 8 f32 rows 17 us a call without the launch, 21 with it)
+  if (a.top_k != nullptr || a.top_p != nullptr) CountKernel<T><<<grid, kThreads, 0, s>>>(a, l);
   SplitKernel<T><<<grid, kThreads, 0, s>>>(a, l);
   DrawKernel<T><<<a.rows, kDrawThreads, 0, s>>>(a, l);
   HIP_CHECK(hipGetLastError());

@@ -778,6 +778,21 @@ def test_sample_numbers_outside_and_absent_parameters():
     assert a.tolist() == [0, 0, 999, 999, 999]  # no limits
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_sample_limits_that_are_absent(dtype):
+    """No top_k and top_p: as arrays that set none; other calls in between."""
+    g = torch.Generator().manual_seed(22)
+    x = (torch.randn(9, 20011, generator=g) * 3).to(dtype).cuda()
+    u, t = torch.rand(9, generator=g).cuda(), torch.full((9,), 0.9).cuda()
+    k, p, m = torch.zeros(9, dtype=torch.int32).cuda(), torch.ones(9).cuda(), torch.full((9,), 0.05).cuda()
+    for min_p in (None, m):
+        want = serving.sample(x, u, t, k, p, min_p)
+        serving.sample(x, u, t, k + 5, p * 0.5, min_p)
+        for top_k, top_p in ((None, None), (k, None), (None, p)):
+            got = serving.sample(x, u, t, top_k, top_p, min_p)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_sample_strided_rows_and_repeats():
     g = torch.Generator().manual_seed(21)
     big = (torch.randn(6, 5000, generator=g) * 2).to(torch.bfloat16)
