@@ -146,7 +146,11 @@ int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool pr
   return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
 }
 
+// Calls without sequences or new tokens have nothing to do.
+bool Empty(const paged::Seqs& s, bool packed) { return s.n_seqs == 0 || (packed && s.n_tokens == 0); }
+
 int64_t AttentionWork(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
+  if (Empty(s, prompt)) return 0;
   const int64_t rows = static_cast<int64_t>(prompt ? s.n_tokens : s.n_seqs) * n_heads;
   return paged::WorkBytes(rows, c.head_dim, Splits(c, s, n_heads, prompt));
 }
@@ -157,7 +161,7 @@ int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seq
   paged::AttentionArgs a;
   a.c = CacheOf(cache);
   a.s = SeqsOf(seqs, cache, prompt);
-  if (a.s.n_seqs == 0 || (prompt && a.s.n_tokens == 0)) return 0;
+  if (Empty(a.s, prompt)) return 0;
   CheckHeads(a.c, a.s, n_heads);
   const int n_tokens = prompt ? a.s.n_tokens : a.s.n_seqs;
   a.q = RowsOf("q", q, a.c, n_tokens, n_heads, false);
@@ -196,7 +200,7 @@ int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const rpg_hip_seq
         paged::AppendArgs a;
         a.c = CacheOf(cache);
         a.s = SeqsOf(seqs, cache, true);
-        if (a.s.n_seqs == 0 || a.s.n_tokens == 0) return 0;
+        if (Empty(a.s, true)) return 0;
         a.k = RowsOf("k", k, a.c, a.s.n_tokens, a.c.n_kv, false);
         a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, false);
         if (q != nullptr && q->data != nullptr) {

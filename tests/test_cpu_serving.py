@@ -117,6 +117,22 @@ def test_starts_and_work_memory():
     assert L.rpg_hip_paged_work(ref(c), ref(seqs(pages=1, n_seqs=1)), 8, 0) == 0  # one range: none
 
 
+@pytest.mark.parametrize("kind", [0, 1, 30])
+@pytest.mark.parametrize("pages", [1, 64, 256, 8192])
+@pytest.mark.parametrize("n_seqs,n_tokens,prompt", [(0, 0, 0), (0, 0, 1), (0, 3, 0), (0, 3, 1), (5, 0, 1)])
+def test_nothing_to_do_takes_no_work_memory(kind, pages, n_seqs, n_tokens, prompt):
+    """No sequences, with tokens or without, or no tokens: no bytes and no refusal,
+    and a call that returns at once with no work memory."""
+    L = serving._lib()
+    r = rows()
+    s = seqs(pages=pages, table_stride=pages, n_seqs=n_seqs, n_tokens=n_tokens)
+    for c in (cache(type=kind), cache(type=kind, n_kv=1)):
+        assert L.rpg_hip_paged_work(ref(c), ref(s), 8, prompt) == 0
+        call = L.rpg_hip_paged_prompt if prompt else L.rpg_hip_paged_decode
+        assert call(ref(c), ref(s), ref(r), ref(r), 8, 0.1, None, 0, None) == 0
+    assert serving._work_bytes(8, 16, 128, kind, pages, n_seqs, n_tokens, 32, prompt) == 0
+
+
 def test_more_than_one_launch_holds():
     """2^24 workgroups and more, and positions that a step would count past 2^31."""
     L = serving._lib()

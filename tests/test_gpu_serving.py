@@ -888,3 +888,20 @@ def test_nothing_to_do():
                                     torch.ones(1, **i32))
     assert bool((none == 0).all())  # a table without pages
     assert serving.sample(torch.zeros(0, 9, device="cuda"), torch.zeros(0, device="cuda"))[0].shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_no_sequences(dtype, tokens):
+    """Tables of any width and no sequence: rows of none are left as they were."""
+    cache = serving.PagedCache.zeros(2, 16, 2, 128, dtype)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, starts = torch.zeros(0, **i32), torch.zeros(1, **i32)
+    for pages in (1, 64, 256):
+        table = torch.zeros(0, pages, **i32)
+        q = torch.ones(tokens, 8, 128, dtype=dtype, device="cuda")
+        out = torch.full_like(q, 7.0)
+        serving.prompt_attention(q, cache, table, lens, starts, out=out)
+        assert serving.decode_attention(q[:0], cache, table, lens).shape == (0, 8, 128)
+        serving.append(cache, table, lens, starts, q[:, :2], q[:, :2], q=q, q_out=out)
+        assert bool((out == 7).all()) and bool((cache.k == 0).all()) and bool((cache.v == 0).all())
