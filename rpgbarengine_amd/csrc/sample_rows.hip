@@ -262,7 +262,9 @@ __device__ __forceinline__ Row RowOf(const SampleArgs& a, const Layout& l, const
   r.c32 = 32.0 * 1.4426950408889634074 / static_cast<double>(t);
   const float span = fminf(31.6f * t, max - min);
   r.weightless_end = 31.6f * t <= max - min;
-  r.scale = span > 0.0f ? static_cast<float>(kBins) / span : 0.0f;
+  // (finite: the maximum's own step is 0 x scale. Below a span of 6e-36, a temperature
+  // of 1.9e-37, the steps are wider than they could be)
+  r.scale = span > 0.0f ? fminf(static_cast<float>(kBins) / span, __FLT_MAX__) : 0.0f;
   const int32_t k = a.top_k != nullptr ? a.top_k[row] : 0;
   r.k = k > 0 && k < a.vocab ? k : 0;
   const float p = a.top_p != nullptr ? a.top_p[row] : 1.0f;

@@ -746,6 +746,51 @@ def test_sample_ties_and_flat_rows():
                   torch.tensor(m))
 
 
+def sample_into(x, u, t, k, p, m, fill):
+    """serving.sample's call with work memory and outputs that hold `fill` in every byte."""
+    rows, vocab = x.shape
+    L = serving._lib()
+    size = L.rpg_hip_sample_rows_work(rows, vocab)
+    work = torch.full((size,), fill, dtype=torch.uint8, device="cuda")
+    tokens, lp = (torch.full((4 * rows,), fill, dtype=torch.uint8, device="cuda").view(d) for d in (torch.int32, torch.float32))
+    dev = [v.cuda() for v in (x, t, k, p, m, u)]
+    rc = L.rpg_hip_sample_rows(serving._TYPES[x.dtype], dev[0].data_ptr(), rows, vocab, vocab, *[v.data_ptr() for v in dev[1:]],
+                               tokens.data_ptr(), lp.data_ptr(), work.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    return tokens.cpu(), lp.cpu()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("vocab", [700, 20011, 151936])
+def test_sample_temperatures_next_to_zero(dtype, vocab):
+    """Down to the smallest number above 0 they are temperatures: the best token,
+    or a draw among those that are equal, or nearly so, to it. Nothing is taken
+    from what work memory and outputs held."""
+    g = torch.Generator().manual_seed(vocab + 3)
+    base = torch.randn(4, vocab, generator=g) * 2.5
+    base[1, [5, vocab // 2, vocab - 1]] = 30.0  # equal ones
+    base[2, ::3] = 25.0                         # more of them than a list holds
+    base[3] = torch.where(torch.rand(vocab, generator=g) < 0.01, torch.randn(vocab, generator=g) * 1e-37, -1.0)
+    x, u, t, k, p, m = [], [], [], [], [], []
+    for row, tt, (kk, pp, mm) in itertools.product(base, [1e-30, 1e-36, 2e-37, 1e-37, torch.finfo(torch.float32).tiny, 1e-39, 1e-45], [
+            (0, 1.0, 0.0), (1, 1.0, 0.0), (40, 1.0, 0.0), (5000, 1.0, 0.0), (0, 0.9, 0.0), (1, 0.9, 0.0), (40, 0.9, 0.0),
+            (5000, 0.9, 0.0), (0, 1.0, 0.5), (40, 0.5, 0.5)]):
+        x.append(row)
+        for v, w in zip((u, t, k, p, m), (float(torch.rand(1, generator=g)), tt, kk, pp, mm)):
+            v.append(w)
+    x = torch.stack(x).to(dtype)
+    u, t, p, m = (torch.tensor(v) for v in (u, t, p, m))
+    k = torch.tensor(k, dtype=torch.int32)
+    assert bool((t > 0).all())
+    want = [plain.sample(x[i], float(u[i]), float(t[i]), int(k[i]), float(p[i]), float(m[i])) for i in range(len(u))]
+    for fill in (0x7F, 0xFF):
+        tokens, lp = sample_into(x, u, t, k, p, m, fill)
+        for i, (token, logp) in enumerate(want):
+            assert int(tokens[i]) == token, (i, float(t[i]), int(k[i]), float(p[i]), float(m[i]))
+            # as in check_samples
+            assert abs(float(lp[i]) - logp) <= 2.0 ** -24 * abs(logp) + vocab * 2.0 ** -44 + 1e-10, i
+
+
 def test_sample_rows_that_hold_little():
     """Infinities, NaN, rows with one value, with none."""
     inf, nan = math.inf, math.nan
