@@ -147,13 +147,14 @@ __device__ __forceinline__ U4 Resource(const char* p, uint32_t bytes) {
 // 16 bytes per lane from the resource to LDS, a wave's lanes side by side. In
 // assembly, since the compiler holds every LDS read after the builtin until the
 // load is done, though the reads are of another buffer: the waits are
-// written out, before the tile's first read. It writes no register.
+// written out, before the tile's first read. Of the registers it overwrites m0 alone.
 __device__ __forceinline__ void LdsDma(U4 src, char* to, int voff, int soff) {
   const uint32_t at = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to));
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(at), "v"(voff), "s"(src), "s"(soff));
+               : "s"(at), "v"(voff), "s"(src), "s"(soff)
+               : "m0");
 }
 
 // A row tile: its sequence and rows, and the positions it stands for.

@@ -1,6 +1,7 @@
 """What the serving kernels' built code has to keep, read from the library: no
 matrix instruction's result over its own A or B operands (wrong sums on gfx950),
-and as many LDS loads in flight as the counted waits of the one-wave groups say."""
+and as many LDS loads in flight as the counted waits of the one-wave groups say.
+And what their inline assembly has to name: the registers that it overwrites."""
 
 import os
 import re
@@ -89,3 +90,56 @@ def test_counted_waits_of_one_wave_groups(functions):
         waits = re.findall(r"s_waitcnt vmcnt\((\d+)\)\s", text)
         assert dma % 4 == 0 and waits.count(str(dma // 4)) >= 2, (name, dma, waits)
         assert "scratch_" not in text, name
+
+
+def statements(text):
+    """(assembly, clobbers) of every asm statement of a source file."""
+    text = re.sub(r"//[^\n]*", "", text)
+    for m in re.finditer(r"\basm volatile\s*\(", text):
+        at, depth = m.end(), 1
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[at], 0)
+            at += 1
+        body = text[m.end():at - 1]
+        code = re.match(r'\s*((?:"(?:[^"\\]|\\.)*"\s*)+)', body)
+        fields = re.split(r":", re.sub(r'"(?:[^"\\]|\\.)*"', lambda q: q.group(0).replace(":", ";"), body[code.end():]))
+        yield "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', code.group(1))), fields[3] if len(fields) > 3 else ""
+
+
+def unnamed(text):
+    """The fixed registers that asm statements write and do not name as clobbered."""
+    bad = []
+    for code, clobbers in statements(text):
+        for line in code.split(r"\n\t"):
+            m = re.match(r"\s*[sv]_\w+\s+(m0|vcc\w*|exec\w*|[sv]\d+|[sv]\[\d+:\d+\])\s*,", line)
+            if m and f'"{m.group(1)}"' not in clobbers:
+                bad.append((m.group(1), code))
+    return bad
+
+
+def test_assembly_names_the_registers_it_overwrites():
+    src = os.path.join(os.path.dirname(eng.LIB_PATH), "csrc")
+    seen = 0
+    for f in sorted(os.listdir(src)):
+        with open(os.path.join(src, f), encoding="utf-8") as h:
+            text = h.read()
+        seen += len(list(statements(text)))
+        assert not unnamed(text), (f, unnamed(text))
+    assert seen >= 20
+
+
+def test_the_check_sees_an_unnamed_register():
+    line = 'asm volatile("s_mov_b32 m0, %0\\n\\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(f(a)), "v"(b), "s"(c), "s"(d)'
+    assert [r for r, _ in unnamed(line + ");")] == ["m0"]
+    assert unnamed(line + ' : "m0");') == [] and unnamed(line + ' : "m0", "memory");') == []
+
+
+def test_m0_serves_the_loads_to_lds_alone(functions):
+    """Nothing else in the prompt kernels sets or reads it."""
+    for name, text in functions.items():
+        if "PromptKernel" not in name:
+            continue
+        lines = [x.split("//")[0].strip() for x in text.splitlines()]
+        uses = [x for x in lines if re.search(r"\bm0\b", x)]
+        loads = [x for x in lines if re.match(r"buffer_load_dwordx4 .* lds$", x)]
+        assert loads and len(uses) == len(loads) and all(re.match(r"s_mov_b32 m0, s\d+$", x) for x in uses), (name, uses[:5])
