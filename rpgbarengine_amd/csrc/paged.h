@@ -73,6 +73,10 @@ struct AttentionArgs {
 int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
 int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
 int64_t WorkBytes(int64_t rows, int head_dim, int splits);
+
+// Floats of the partials' maxima and sums, in front of their outputs, which are
+// read and written 16 bytes at a time.
+__host__ __device__ inline int64_t StatFloats(int64_t rows, int splits) { return (2 * rows * splits + 3) / 4 * 4; }
 void Decode(const AttentionArgs& a, hipStream_t s);
 
 void Prompt(const AttentionArgs& a, hipStream_t s);

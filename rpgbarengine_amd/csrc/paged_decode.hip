@@ -306,7 +306,7 @@ int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capac
 }
 
 int64_t WorkBytes(int64_t rows, int head_dim, int splits) {
-  return splits == 1 ? 0 : rows * splits * (2 + head_dim) * 4;
+  return splits == 1 ? 0 : (StatFloats(rows, splits) + rows * splits * head_dim) * 4;
 }
 
 void Decode(const AttentionArgs& a, hipStream_t s) {

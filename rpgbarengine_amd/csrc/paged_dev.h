@@ -200,14 +200,14 @@ __device__ __forceinline__ int RangeOf(int len, int splits) {
 // x - y of maxima that may both be -inf (no key yet): then 0.
 __device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
 
-// Work: [row][splits] (maximum, sum), then [row][splits][kDim] outputs that are
-// not yet divided by the sum; row = query token x head.
+// Work: [row][splits] (maximum, sum), then (StatFloats) [row][splits][kDim] outputs
+// that are not yet divided by the sum; row = query token x head.
 __device__ __forceinline__ F2* PartStats(const AttentionArgs& a, int64_t row) {
   return reinterpret_cast<F2*>(a.work) + row * a.splits;
 }
 template <int kDim>
 __device__ __forceinline__ float* PartOut(const AttentionArgs& a, int64_t rows, int64_t row) {
-  return a.work + 2 * rows * a.splits + row * a.splits * kDim;
+  return a.work + StatFloats(rows, a.splits) + row * a.splits * kDim;
 }
 
 template <typename T>

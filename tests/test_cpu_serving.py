@@ -133,6 +133,25 @@ def test_nothing_to_do_takes_no_work_memory(kind, pages, n_seqs, n_tokens, promp
     assert serving._work_bytes(8, 16, 128, kind, pages, n_seqs, n_tokens, 32, prompt) == 0
 
 
+@pytest.mark.parametrize("kind,pages,prompt", [(30, 72, 0), (1, 200, 0), (0, 72, 0), (0, 90, 1), (1, 160, 1), (30, 288, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_partial_outputs_lie_at_multiples_of_16_bytes(kind, pages, prompt, dim):
+    """An odd number of (maximum, sum) pairs in front of them: rows of five heads in
+    an odd number of ranges. Work memory is in whole 16 bytes then, as the outputs are."""
+    L = serving._lib()
+    c = cache(type=kind, n_kv=1, head_dim=dim, row_stride=dim)
+    odd = 0
+    for tokens in (1, 3):
+        s = seqs(pages=pages, table_stride=pages, n_seqs=tokens if prompt == 0 else 1, n_tokens=tokens)
+        size = L.rpg_hip_paged_work(ref(c), ref(s), 5, prompt)
+        pairs = size // (4 * (dim + 2))
+        odd += pairs % 2
+        assert size > 0 and pairs % (5 * tokens) == 0
+        assert size == 4 * (pairs * dim + (2 * pairs + 3) // 4 * 4)
+        assert size % 16 == 0
+    assert odd > 0
+
+
 def test_more_than_one_launch_holds():
     """2^24 workgroups and more, and positions that a step would count past 2^31."""
     L = serving._lib()

@@ -202,6 +202,30 @@ def test_decode_long_and_split(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("prompt", [0, 1], ids=["decode", "prompt"])
+def test_an_odd_number_of_partials(dtype, dim, prompt):
+    """Five rows in an odd number of ranges, in work memory of exactly the size asked
+    for, the bytes behind it as they were."""
+    n = 1300 if dtype == torch.float32 else 2300
+    b = Batch([n], [1], dtype, 1, dim, 16, 5, seed=28)
+    q = b.normal(1, 5, dim, by=1.5).cuda()
+    cache, table, lens, starts = b.gpu()
+    L = serving._lib()
+    size = serving._work_bytes(1, 16, dim, serving._TYPES[dtype], table.shape[1], 1, prompt, 5, prompt)
+    assert size // (4 * (dim + 2)) % 2 == 1
+    work = torch.full((size + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    args = (cache._c, serving._seqs(cache, table, lens, starts, prompt)[0], serving._rows(q, "q", cache),
+            serving._rows(out, "out", cache), 5, 0.1, work.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    assert (L.rpg_hip_paged_prompt if prompt else L.rpg_hip_paged_decode)(*args) == 0
+    kk, there = plain.sequence_rows(b.k, b.table[0], n)
+    vv, _ = plain.sequence_rows(b.v, b.table[0], n)
+    close(out[0], *plain.attention(q[0].cpu(), kk, vv, there, float(torch.tensor(0.1)), dtype))
+    assert bool((work[size:] == 0xA5).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_decode_masked_places_hold_anything(dtype, value):
     """Rows past the length, spare pages and pages that the table names no more."""
