@@ -272,7 +272,7 @@ typedef struct {
 } rpg_hip_rows;
 
 /* Stores the new tokens' keys and values in their pages. Keys, and queries
- * from q into q_out (which may be q; q->data NULL: no queries), are RMS-normed
+ * from q into q_out (which may be q, with its strides; q->data NULL: no queries), are RMS-normed
  * per head with the gains k_norm and q_norm (f32 [head_dim]; NULL: not normed)
  * and rotated by row `position` of rope (f32 [rope_rows][head_dim], cos |
  * sin, as rpg_hip_model_rope_row; NULL: not rotated), as the engine's own
@@ -292,7 +292,7 @@ RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const
  * .. sharing key head kv (reference src/qwen3.cc:79-117). scale > 0. Sums and
  * softmax in f32; for 16-bit types the weights are rounded to that type before
  * they multiply the values. A sequence without positions gives zeros. out may
- * be q. work: rpg_hip_paged_work bytes, read and written by this call alone
+ * be q, with its strides. work: rpg_hip_paged_work bytes, read and written by this call alone
  * until it is complete (any contents; may be NULL when that is 0). */
 RPG_HIP_API int32_t rpg_hip_paged_decode(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,

@@ -134,6 +134,14 @@ paged::Rows RowsOf(const char* what, const rpg_hip_rows* r, const paged::Cache& 
   return out;
 }
 
+// Rows that are written where others are read: those of one token and head lie in
+// one place, or else some are overwritten before they are read.
+void CheckInPlace(const char* out_is_in, const paged::Rows& out, const paged::Rows& in, int n_tokens, int n_heads) {
+  RPG_CHECK(out.p != in.p || ((n_tokens == 1 || out.token_bytes == in.token_bytes) &&
+                              (n_heads == 1 || out.head_bytes == in.head_bytes)),
+            "%s with other strides", out_is_in);
+}
+
 void CheckHeads(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads) {
   RPG_CHECK(n_heads >= c.n_kv && n_heads % c.n_kv == 0, "%d query heads on %d key heads", n_heads, c.n_kv);
   RPG_CHECK(static_cast<int64_t>(n_heads) * std::max(s.n_tokens, s.n_seqs) < (int64_t{1} << 31) - 4096,
@@ -166,6 +174,7 @@ int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seq
   const int n_tokens = prompt ? a.s.n_tokens : a.s.n_seqs;
   a.q = RowsOf("q", q, a.c, n_tokens, n_heads, false);
   a.out = RowsOf("out", out, a.c, n_tokens, n_heads, true);
+  CheckInPlace("out is q", a.out, a.q, n_tokens, n_heads);
   RPG_CHECK(scale > 0.0f && std::isfinite(scale), "scale %g is not positive and finite", scale);
   a.n_heads = n_heads;
   a.scale = scale;
@@ -208,9 +217,7 @@ int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const rpg_hip_seq
           RPG_CHECK(n_heads <= 65536 && a.c.n_kv <= 65536, "%d query heads on %d key heads", n_heads, a.c.n_kv);
           a.q = RowsOf("q", q, a.c, a.s.n_tokens, n_heads, false);
           a.q_out = RowsOf("q_out", q_out, a.c, a.s.n_tokens, n_heads, true);
-          RPG_CHECK(a.q_out.p != a.q.p || (a.q_out.token_bytes == a.q.token_bytes &&
-                                           (n_heads == 1 || a.q_out.head_bytes == a.q.head_bytes)),
-                    "q_out is q with other strides");
+          CheckInPlace("q_out is q", a.q_out, a.q, a.s.n_tokens, n_heads);
           a.n_heads = n_heads;
         } else {
           RPG_CHECK(a.c.n_kv <= 65536, "%d key heads", a.c.n_kv);

@@ -103,6 +103,18 @@ def test_bad_attention_calls(over, word):
                      None), word)
 
 
+@pytest.mark.parametrize("over", [dict(head_stride=256, token_stride=2048), dict(head_stride=512), dict(token_stride=4096)],
+                         ids=["both", "heads", "tokens"])
+def test_outputs_at_the_queries_with_other_strides(over):
+    """They would overwrite queries that are not read yet."""
+    L = serving._lib()
+    c, s, r = cache(), seqs(), rows()
+    for call in (L.rpg_hip_paged_decode, L.rpg_hip_paged_prompt):
+        refused(call(ref(c), ref(s), ref(r), ref(rows(**over)), 8, 0.1, A, 1 << 50, None), "out is q with other strides")
+    refused(L.rpg_hip_paged_append(ref(c), ref(s), ref(r), ref(r), ref(r), ref(rows(**over)), 8, None, None, 0.0, None, 0,
+                                   None), "q_out is q with other strides")
+
+
 def test_starts_and_work_memory():
     L = serving._lib()
     c, r = cache(), rows()

@@ -408,6 +408,25 @@ def test_attention_in_place(dtype, lens, new):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_one_token_in_place_with_another_token_stride(dtype):
+    """The distance of tokens says nothing where there is one."""
+    b = Batch([70], [1], dtype, 2, 64, 16, 8, seed=29)
+    q = b.normal(1, 8, 64).cuda()
+    cache, table, lens, starts = b.gpu()
+    L = serving._lib()
+    wants = [(L.rpg_hip_paged_decode, serving.decode_attention(q, cache, table, lens)),
+             (L.rpg_hip_paged_prompt, serving.prompt_attention(q, cache, table, lens, starts))]
+    seqs = serving._seqs(cache, table, lens, starts, 1)[0]
+    stream = torch.cuda.current_stream().cuda_stream
+    for call, want in wants:
+        x = q.clone()
+        r, o = (serving._ROWS.pack(x.data_ptr(), n, 64) for n in (512, 4096))
+        assert serving._work_bytes(2, 16, 64, serving._TYPES[dtype], table.shape[1], 1, 1, 8, 1) == 0
+        assert call(cache._c, seqs, r, o, 8, 0.125, None, 0, stream) == 0
+        assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 def test_prompt_many_short_turns(dtype):
     """More row tiles than compute units, most of them partly filled: ragged ends,
     pages that are not named, NaN in every place that no query sees."""
