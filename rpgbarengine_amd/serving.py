@@ -145,6 +145,11 @@ def _enqueue(device, f, *args):
         _ok(rc)
 
 
+# What a call writes in place is a new version of the tensor to autograd: a
+# backward pass that saved the old one refuses.
+_written = torch.autograd.graph.increment_version
+
+
 def _stream(index):
     return torch.cuda.current_stream(index).cuda_stream
 
@@ -184,6 +189,7 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
     _enqueue(dev, _lib().rpg_hip_paged_append, cache._c, seqs, kr, vr, qr, qo, heads,
              _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
              rp, rope_rows)
+    _written((cache.k, cache.v) if qo is None else (cache.k, cache.v, q_out))
     return q_out
 
 
@@ -205,6 +211,7 @@ def _attention(f, q, qr, cache, seqs, n_seqs, pages, n_tokens, scale, out, promp
     work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
     _enqueue(cache.device, f, cache._c, seqs, qr, _rows(out, "out", cache), heads, dim ** -0.5 if scale is None else scale,
              work.data_ptr() if size else None, size)
+    _written(out)
     return out
 
 

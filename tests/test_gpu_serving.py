@@ -962,6 +962,33 @@ def test_parameters_that_require_gradients_are_refused():
             call()
 
 
+def test_tensors_written_in_place_are_new_versions():
+    """The pool, out and q_out: a backward pass that saved one of them refuses,
+    instead of taking what was written over it."""
+    b = Batch([20], [2], torch.float32, 2, 64, 16, 4, seed=30)
+    cache, table, lens, starts = b.gpu()
+    k, q = b.normal(2, 2, 64).cuda(), b.normal(2, 4, 64).cuda()
+    calls = [(lambda: serving.append(cache, table, lens, starts, k, k), [cache.k, cache.v]),
+             (lambda: serving.append(cache, table, lens, starts, k, k, q=q, q_out=q), [cache.k, cache.v, q]),
+             (lambda: serving.decode_attention(q[:1], cache, table, lens, out=q[:1]), [q]),
+             (lambda: serving.prompt_attention(q, cache, table, lens, starts, out=q), [q])]
+    for i, (call, written) in enumerate(calls):
+        for x in written:
+            leaf = torch.ones_like(x, requires_grad=True)
+            loss = (leaf * x).sum()  # saves x
+            was = x._version
+            call()
+            assert x._version > was, i
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+    with torch.inference_mode():  # tensors without versions
+        out = torch.empty_like(q)
+        serving.append(cache, table, lens, starts, k, k, q=q, q_out=out)
+        serving.prompt_attention(q, cache, table, lens, starts, out=out)
+        pool = serving.PagedCache.zeros(2, 16, 2, 64)
+        serving.append(pool, table, lens, starts, k, k)
+
+
 def test_nothing_to_do():
     """No sequence, no token, no row."""
     cache = serving.PagedCache.zeros(2, 16, 1, 64, torch.float32)
