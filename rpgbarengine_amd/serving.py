@@ -16,8 +16,9 @@ packed rows at which each sequence's new tokens start (and the last ones end).
 The work is enqueued on the current torch stream of the tensors' GPU; work
 memory comes from torch's allocator on that stream. Lengths, pages, starts and
 sampling parameters are read on the GPU, so a call captured into a graph takes
-the values of each replay. There is no backward pass: tensors that require
-gradients are refused while gradients are recorded.
+the values of each replay. There is no backward pass and no forward-mode one:
+tensors that require gradients are refused while gradients are recorded, and
+those that carry a tangent always.
 """
 
 from __future__ import annotations
@@ -27,6 +28,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import EngineError, lib
 
@@ -68,6 +70,14 @@ def _need(cond, what):
         raise EngineError(what)
 
 
+def _plain(x, name):
+    """No derivative is asked of x."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise EngineError(f"{name} requires gradients: there is no backward pass")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise EngineError(f"{name} carries a tangent: there are no forward-mode gradients")
+
+
 class PagedCache:
     """A pool of key and value pages, [pages, key heads, page size, head dim] each
     (f32, f16 or bf16; views of a larger pool are fine)."""
@@ -76,7 +86,8 @@ class PagedCache:
         _need(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
         _need(k.dtype in _TYPES and v.dtype == k.dtype, "k and v are both float32, float16 or bfloat16")
         _need(k.is_cuda and v.device == k.device, "k and v lie on one GPU")
-        _need(not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad)), "the cache requires gradients: there is no backward pass")
+        _plain(k, "the cache's k")
+        _plain(v, "the cache's v")
         _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
         self.k, self.v = k, v
         self.device, self.dtype = k.device, k.dtype
@@ -117,8 +128,7 @@ def _rows(x, name, cache):
     if (len(shape) != 3 or x.dtype is not cache.dtype or x.device != cache.device or shape[2] != cache.head_dim
             or strides[2] != 1):
         raise EngineError(f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise EngineError(f"{name} requires gradients: there is no backward pass")
+    _plain(x, name)
     n, heads, dim = shape
     return _ROWS.pack(x.data_ptr(), strides[0] if n > 1 else heads * dim, strides[1] if heads > 1 else dim)
 
@@ -127,8 +137,7 @@ def _vector(x, name, n, dtype, device):
     """The address of a contiguous vector; None stays None."""
     if x is None:
         return None
-    if x.requires_grad and torch.is_grad_enabled():
-        raise EngineError(f"{name} requires gradients: there is no backward pass")
+    _plain(x, name)
     if x.dtype is not dtype or x.shape != (n,) or x.device != device or (n > 1 and x.stride(0) != 1):
         raise EngineError(f"{name} is {dtype} [{n}], contiguous, on the same GPU")
     return x.data_ptr()
@@ -183,8 +192,9 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
     rp, rope_rows = None, 0
     if rope is not None:
         if (rope.dtype is not torch.float32 or rope.dim() != 2 or rope.shape[1] != dim or not rope.is_contiguous()
-                or rope.device != dev or (rope.requires_grad and torch.is_grad_enabled())):
-            raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU, without gradients")
+                or rope.device != dev):
+            raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU")
+        _plain(rope, "rope")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
     _enqueue(dev, _lib().rpg_hip_paged_append, cache._c, seqs, kr, vr, qr, qo, heads,
              _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
@@ -252,8 +262,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     if (logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda
             or (logits.shape[1] > 1 and logits.stride(1) != 1)):
         raise EngineError("logits are [rows, vocab] float32, float16 or bfloat16 on a GPU, contiguous in the last dimension")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise EngineError("logits require gradients: there is no backward pass")
+    _plain(logits, "logits")
     if u is None:
         raise EngineError("u is needed")
     rows, vocab = logits.shape

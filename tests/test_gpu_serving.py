@@ -962,6 +962,39 @@ def test_parameters_that_require_gradients_are_refused():
             call()
 
 
+def test_tensors_with_tangents_are_refused():
+    """Forward-mode gradients, which the outputs would lose without a word."""
+    from torch.autograd import forward_ad
+    b = Batch([4], [1], torch.float32, 1, 64, 16, 2, seed=31)
+    cache, table, lens, starts = b.gpu()
+    k, q, gain, rope, x, one = (torch.ones(*s, device="cuda") for s in ((1, 1, 64), (1, 2, 64), (64,), (64, 64), (1, 5), (1,)))
+    calls = [
+        (k, lambda t: serving.append(cache, table, lens, starts, t, k)),
+        (k, lambda t: serving.append(cache, table, lens, starts, k, t)),
+        (q, lambda t: serving.append(cache, table, lens, starts, k, k, q=t)),
+        (q, lambda t: serving.append(cache, table, lens, starts, k, k, q=q, q_out=t)),
+        (gain, lambda t: serving.append(cache, table, lens, starts, k, k, q=q, q_norm=t)),
+        (gain, lambda t: serving.append(cache, table, lens, starts, k, k, k_norm=t)),
+        (rope, lambda t: serving.append(cache, table, lens, starts, k, k, rope=t)),
+        (q, lambda t: serving.decode_attention(t, cache, table, lens)),
+        (q, lambda t: serving.decode_attention(q, cache, table, lens, out=t)),
+        (q, lambda t: serving.prompt_attention(t, cache, table, lens, starts)),
+        (cache.k, lambda t: serving.PagedCache(t, cache.v)),
+        (cache.v, lambda t: serving.PagedCache(cache.k, t)),
+        (x, lambda t: serving.sample(t, one)),
+        (one, lambda t: serving.sample(x, t)),
+        (one, lambda t: serving.sample(x, one, temperature=t)),
+    ]
+    with forward_ad.dual_level():
+        for i, (value, call) in enumerate(calls):
+            call(value.clone())  # without one, in the same place
+            with pytest.raises(eng.EngineError, match="tangent"):
+                call(forward_ad.make_dual(value.clone(), torch.ones_like(value)))
+                pytest.fail(f"call {i} was not refused")
+    for value, call in calls:
+        call(value.clone())
+
+
 def test_tensors_written_in_place_are_new_versions():
     """The pool, out and q_out: a backward pass that saved one of them refuses,
     instead of taking what was written over it."""
