@@ -260,8 +260,9 @@ __device__ __forceinline__ Row RowOf(const SampleArgs& a, const Layout& l, const
   const float t = a.temperature != nullptr ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
   r.c32 = 32.0 * 1.4426950408889634074 / static_cast<double>(t);
-  const float span = fminf(31.6f * t, max - min);
-  r.weightless_end = 31.6f * t <= max - min;
+  const float weighty = 31.6f * t, span = fminf(weighty, max - min);
+  // (both infinite: values further apart than a float reaches have weight too)
+  r.weightless_end = weighty <= max - min && weighty < -kNone;
   // (finite: the maximum's own step is 0 x scale. Below a span of 6e-36, a temperature
   // of 1.9e-37, the steps are wider than they could be)
   r.scale = span > 0.0f ? fminf(static_cast<float>(kBins) / span, __FLT_MAX__) : 0.0f;

@@ -834,6 +834,27 @@ def test_sample_temperatures_next_to_zero(dtype, vocab):
             assert abs(float(lp[i]) - logp) <= 2.0 ** -24 * abs(logp) + vocab * 2.0 ** -44 + 1e-10, i
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ident)
+def test_sample_temperatures_next_to_infinity(dtype):
+    """Rows whose values lie further apart than a float reaches, at temperatures at
+    which all of them, or many, have weight."""
+    vocab = 3000
+    g = torch.Generator().manual_seed(32)
+    # (in float64: the step of one in float32 is infinite, and an infinite value
+    # over an infinite temperature is nothing)
+    rows = [torch.linspace(-3e38, 3e38, vocab, dtype=torch.float64).float(), torch.where(torch.rand(vocab, generator=g) < 0.5, -3.3e38, 3.3e38),
+            torch.randn(vocab, generator=g)]
+    x, u, t, k, p, m = [], [], [], [], [], []
+    for row, tt, (kk, pp, mm) in itertools.product(rows, [5e36, 1.2e37, 3e37, 1e38, 3e38, math.inf], [
+            (0, 1.0, 0.0), (5, 1.0, 0.0), (450, 0.9, 0.0), (2900, 1.0, 0.0), (0, 0.9, 0.0), (2500, 0.7, 0.0), (0, 1.0, 0.1),
+            (0, 0.99, 0.5)]):
+        x.append(row)
+        for v, w in zip((u, t, k, p, m), (float(torch.rand(1, generator=g)), tt, kk, pp, mm)):
+            v.append(w)
+    check_samples(torch.stack(x).to(dtype), torch.tensor(u), torch.tensor(t), torch.tensor(k, dtype=torch.int32),
+                  torch.tensor(p), torch.tensor(m))
+
+
 def test_sample_rows_that_hold_little():
     """Infinities, NaN, rows with one value, with none."""
     inf, nan = math.inf, math.nan
