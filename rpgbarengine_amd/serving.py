@@ -80,7 +80,8 @@ def _plain(x, name):
 
 class PagedCache:
     """A pool of key and value pages, [pages, key heads, page size, head dim] each
-    (f32, f16 or bf16; views of a larger pool are fine)."""
+    (f32, f16 or bf16; views of a larger pool are fine). A larger pool is a new
+    PagedCache; one whose tensors were given other memory since is refused."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         _need(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
@@ -89,12 +90,21 @@ class PagedCache:
         _plain(k, "the cache's k")
         _plain(v, "the cache's v")
         _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
         self.device, self.dtype = k.device, k.dtype
         n_pages, n_kv, page, dim = k.shape
         self.n_kv, self.head_dim, self.page_size = n_kv, dim, page
         strides = [s if n > 1 else page * dim * 16 for n, s in zip(k.shape, k.stride())]
-        self._c = _CACHE.pack(k.data_ptr(), v.data_ptr(), *strides[:3], n_pages, page, n_kv, dim, _TYPES[k.dtype])
+        self._at = k.data_ptr(), v.data_ptr()
+        self._c = _CACHE.pack(*self._at, *strides[:3], n_pages, page, n_kv, dim, _TYPES[k.dtype])
+
+    k = property(lambda self: self._k, doc="the pool of keys")
+    v = property(lambda self: self._v, doc="the pool of values")
+
+    def _packed(self):
+        if (self._k.data_ptr(), self._v.data_ptr()) != self._at:
+            raise EngineError("the cache's tensors lie elsewhere than when it was made: make a new PagedCache")
+        return self._c
 
     @classmethod
     def zeros(cls, n_pages: int, page_size: int, n_kv: int, head_dim: int, dtype=torch.float32,
@@ -196,10 +206,10 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
             raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU")
         _plain(rope, "rope")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
-    _enqueue(dev, _lib().rpg_hip_paged_append, cache._c, seqs, kr, vr, qr, qo, heads,
+    _enqueue(dev, _lib().rpg_hip_paged_append, cache._packed(), seqs, kr, vr, qr, qo, heads,
              _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
              rp, rope_rows)
-    _written((cache.k, cache.v) if qo is None else (cache.k, cache.v, q_out))
+    _written((cache._k, cache._v) if qo is None else (cache._k, cache._v, q_out))
     return q_out
 
 
@@ -219,7 +229,7 @@ def _attention(f, q, qr, cache, seqs, n_seqs, pages, n_tokens, scale, out, promp
     heads, dim = q.shape[1], cache.head_dim
     size = _work_bytes(cache.n_kv, cache.page_size, dim, _TYPES[cache.dtype], pages, n_seqs, n_tokens, heads, prompt)
     work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
-    _enqueue(cache.device, f, cache._c, seqs, qr, _rows(out, "out", cache), heads, dim ** -0.5 if scale is None else scale,
+    _enqueue(cache.device, f, cache._packed(), seqs, qr, _rows(out, "out", cache), heads, dim ** -0.5 if scale is None else scale,
              work.data_ptr() if size else None, size)
     _written(out)
     return out

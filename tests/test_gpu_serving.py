@@ -983,6 +983,28 @@ def test_parameters_that_require_gradients_are_refused():
             call()
 
 
+def test_a_cache_whose_tensors_moved_is_refused():
+    """Its k and v are those that it was made of, and where they were."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, lens, starts = torch.zeros(1, 1, **i32), torch.ones(1, **i32), torch.tensor([0, 1], **i32)
+    k, q = torch.ones(1, 1, 64, device="cuda"), torch.ones(1, 2, 64, device="cuda")
+    for move in (lambda t: setattr(t, "data", torch.zeros(4, 1, 16, 64, device="cuda")),
+                 lambda t: t.untyped_storage().resize_(0)):
+        for which in ("k", "v"):
+            cache = serving.PagedCache.zeros(2, 16, 1, 64)
+            with pytest.raises(AttributeError):
+                setattr(cache, which, torch.zeros(4, 1, 16, 64, device="cuda"))
+            calls = (lambda: serving.append(cache, table, lens, starts, k, k),
+                     lambda: serving.decode_attention(q, cache, table, lens),
+                     lambda: serving.prompt_attention(q, cache, table, lens, starts))
+            for call in calls:
+                call()
+            move(getattr(cache, which))
+            for call in calls:
+                with pytest.raises(eng.EngineError, match="lie elsewhere"):
+                    call()
+
+
 def test_tensors_with_tangents_are_refused():
     """Forward-mode gradients, which the outputs would lose without a word."""
     from torch.autograd import forward_ad
