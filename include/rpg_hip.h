@@ -290,8 +290,8 @@ RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const
 /* Attention of one token per sequence, row s of q, over all of the sequence's
  * positions: out = softmax(scale q . k) v per head, heads kv * (n_heads / n_kv)
  * .. sharing key head kv (reference src/qwen3.cc:79-117). scale > 0. Sums and
- * softmax in f32; for 16-bit types the weights are rounded to that type before
- * they multiply the values. A sequence without positions gives zeros. out may
+ * softmax in f32; for 16-bit types the weights multiply the values in two parts
+ * of that type, which together keep 16 (bf16) or 22 bits. A sequence without positions gives zeros. out may
  * be q, with its strides. work: rpg_hip_paged_work bytes, read and written by this call alone
  * until it is complete (any contents; may be NULL when that is 0). */
 RPG_HIP_API int32_t rpg_hip_paged_decode(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
@@ -299,7 +299,8 @@ RPG_HIP_API int32_t rpg_hip_paged_decode(const rpg_hip_paged_cache* cache, const
                                          void* work, int64_t work_bytes, void* stream);
 
 /* Causal attention of the packed new tokens: as rpg_hip_paged_decode, the token
- * at position p over positions 0 .. p. */
+ * at position p over positions 0 .. p; for 16-bit types the weights are rounded
+ * to that type before they multiply the values. */
 RPG_HIP_API int32_t rpg_hip_paged_prompt(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
                                          void* work, int64_t work_bytes, void* stream);

@@ -99,11 +99,25 @@ constexpr float kLift = __is_same(T, F16) ? 15.0f : 0.0f;
 
 // A query head's running state in a lane: maximum (of scale log2(e) q.k) and
 // the output of its column, alike over the lanes of a column; the sum of the
-// lane's own keys.
+// lane's own keys. 16-bit types: the weights go to the products in two parts, each
+// of 8 or 11 bits, and the second parts' products have a sum of their own, `rest`,
+// so that a weight which is its first part alone makes no NaN of an infinite value
+// (0 x inf). With one part the output is 1.1 to 1.3 times as far from exact as its
+// own rounding leaves it; two take hardly longer, for the bytes are what takes the
+// time (64 ragged bf16 172 us either way, 131000 f16 95, 8 x 1000 f16 12.6 and 12.8).
 template <typename T, int kDim>
 struct State {
+  static constexpr int kBlocks = kDim / 16, kRest = kBytes<T> == 4 ? 0 : kBlocks;
   float m = kNegInf, l = 0.0f;
-  F4 o[kDim / 16] = {};
+  F4 o[kBlocks] = {}, rest[kRest ? kRest : 1] = {};
+
+  // The output, not yet divided by the sum. Where a value that is not finite came
+  // in, the first parts' sum says what comes out.
+  __device__ __forceinline__ float Out(int w, int e) const {
+    if constexpr (kRest == 0) return o[w][e];
+    const float x = o[w][e];
+    return __builtin_isfinite(x) ? x + rest[w][e] : x;
+  }
 
   // Adds a tile whose first position is pos.
   __device__ __forceinline__ void Add(Tile<T, kDim>& t, const U4 (&q)[Tile<T, kDim>::kChunks], float c, int pos,
@@ -152,7 +166,9 @@ struct State {
       m = now;
       l *= f;
 #pragma unroll
-      for (int w = 0; w < kDim / 16; ++w) o[w] *= f;
+      for (int w = 0; w < kBlocks; ++w) o[w] *= f;
+#pragma unroll
+      for (int w = 0; w < kRest; ++w) rest[w] *= f;
     }
     const float base = m == kNegInf ? 0.0f : m - kLift<T>;
 #pragma unroll
@@ -168,10 +184,11 @@ struct State {
 #pragma unroll
         for (int w = 0; w < kDim / 16; ++w) o[w] = Mfma16F32(__uint_as_float(t.v[0][r][w]), s[0][r], o[w]);
     } else {
-      // The weights are rounded to the cache's 16 bits for the product (each by
-      // at most half a step, as V itself was); the sum takes them unrounded.
+      // (the sum takes the weights unrounded)
       const U4 p = {Pack2<T>(s[0][0], s[0][1]), Pack2<T>(s[0][2], s[0][3]), Pack2<T>(s[1][0], s[1][1]),
                     Pack2<T>(s[1][2], s[1][3])};
+      const U4 p2 = {Rest2<T>(s[0][0], s[0][1], p[0]), Rest2<T>(s[0][2], s[0][3], p[1]),
+                     Rest2<T>(s[1][0], s[1][1], p[2]), Rest2<T>(s[1][2], s[1][3], p[3])};
 #pragma unroll
       for (int w = 0; w < kDim / 16; ++w) {
         const uint32_t sel = w % 2 ? 0x07060302u : 0x05040100u;
@@ -180,14 +197,17 @@ struct State {
         for (int j = 0; j < 4; ++j)
           a[j] = __builtin_amdgcn_perm(t.v[j / 2][2 * (j % 2) + 1][w / 2], t.v[j / 2][2 * (j % 2)][w / 2], sel);
         o[w] = Mfma16<T>(a, p, o[w]);
+        rest[w] = Mfma16<T>(a, p2, rest[w]);
       }
     }
   }
 };
 
-// grid (sequence x key head x block of 16 query heads, key range)
+// grid (sequence x key head x block of 16 query heads, key range). Four waves to a
+// SIMD unit for 16-bit rows of 64, by 128 registers; the compiler alone takes 134
+// (64 x 4000 bf16 99 us, 96 so).
 template <typename T, int kDim>
-__global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kDim == 64 && kBytes<T> == 2 ? 4 : 2) void DecodeKernel(AttentionArgs a) {
   using Tl = Tile<T, kDim>;
   __shared__ float sm[kWaves][kCols], sl[kWaves][kCols];
   __shared__ __align__(16) float so[kWaves][kCols][kDim + 4];
@@ -229,7 +249,7 @@ __global__ __launch_bounds__(64 * kWaves) void DecodeKernel(AttentionArgs a) {
 #pragma unroll
     for (int w = 0; w < kDim / 16; ++w)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) so[wave][col][DimOf<T, kDim>(w, 4 * g + e)] = st.o[w][e] * f;
+      for (int e = 0; e < 4; ++e) so[wave][col][DimOf<T, kDim>(w, 4 * g + e)] = st.Out(w, e) * f;
   }
   __syncthreads();
   const bool alone = range >= len;

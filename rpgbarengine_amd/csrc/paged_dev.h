@@ -101,6 +101,14 @@ __device__ __forceinline__ void Unpack2(uint32_t u, float* a, float* b) {
   }
 }
 
+// What rounding to 16 bits took off two floats, rounded and packed the same way.
+template <typename T>
+__device__ __forceinline__ uint32_t Rest2(float a, float b, uint32_t rounded) {
+  float x, y;
+  Unpack2<T>(rounded, &x, &y);
+  return Pack2<T>(a - x, b - y);
+}
+
 // An MFMA whose destination aliases its A or B registers gives wrong sums on
 // gfx950, and the compiler allows it where the sum starts or moves to other
 // registers. The empty asm behind such a product holds the sources past it. It

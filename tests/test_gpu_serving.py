@@ -201,6 +201,49 @@ def test_decode_long_and_split(dtype):
         close(got[i], want, bound)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ident)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_weights_keep_more_bits_than_the_type(dtype, dim):
+    """Values +-1, whose weighted sums cancel down to near nothing: what a weight's
+    rounding to 16 bits takes off would stand out. Two parts leave its square."""
+    b = Batch([40, 300, 3000], [1] * 3, dtype, 2, dim, 16, 8, seed=33)
+    b.v = torch.where(b.v < 0, -1.0, 1.0).to(dtype)
+    q = b.normal(3, 8, dim, by=1.5)
+    cache, table, lens, _ = b.gpu()
+    got = serving.decode_attention(q.cuda(), cache, table, lens)
+    half = plain.EPS[dtype]
+    for i, n in enumerate(b.lens):
+        kk, there = plain.sequence_rows(b.k, b.table[i], n)
+        vv, _ = plain.sequence_rows(b.v, b.table[i], n)
+        want, bound = plain.attention(q[i], kk, vv, there, dim ** -0.5, torch.float32)
+        # The weights sum to 1 and the values are 1: a first part is within half of
+        # a step, relative, and the second part within half a step of what is left;
+        # an f16 second part, held times 2^15, not closer than 2^-25.
+        bound += half * half + (n * 2.0 ** -40 if dtype == torch.float16 else 0.0)
+        close(got[i], want, bound + half * (want.abs() + bound) + plain.TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("n", [37, 3000])
+def test_decode_infinities(dtype, n):
+    """Infinite values that a token sees, of either sign, beside weights that are
+    whole numbers of steps and others; NaN where both signs meet."""
+    b = Batch([n, 20], [1, 1], dtype, 2, 128, 16, 8, seed=34)
+    at = int(b.table[0, 1])
+    b.v[at, 0, 2, 5], b.v[at, 0, 9, 6] = math.inf, -math.inf
+    b.v[at, 1, 3, 7], b.v[at, 1, 4, 7] = math.inf, -math.inf
+    q = b.normal(2, 8, 128)
+    q[0, 0] = 0.0  # every weight is the largest
+    cache, table, lens, _ = b.gpu()
+    got = serving.decode_attention(q.cuda(), cache, table, lens).double().cpu()
+    assert bool((got[0, :4, 5] == math.inf).all()) and bool((got[0, :4, 6] == -math.inf).all())
+    assert bool(got[0, 4:, 7].isnan().all())
+    ok = torch.ones_like(got, dtype=torch.bool)
+    ok[0, :4, 5:7] = False
+    ok[0, 4:, 7] = False
+    assert bool(got[ok].isfinite().all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("prompt", [0, 1], ids=["decode", "prompt"])
