@@ -71,7 +71,8 @@ def _need(cond, what):
 
 
 def _plain(x, name):
-    """No derivative is asked of x."""
+    """No derivative is asked of x. (Called where it may be: a call's seven tensors
+    otherwise cost 0.5 us.)"""
     if x.requires_grad and torch.is_grad_enabled():
         raise EngineError(f"{name} requires gradients: there is no backward pass")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
@@ -138,7 +139,8 @@ def _rows(x, name, cache):
     if (len(shape) != 3 or x.dtype is not cache.dtype or x.device != cache.device or shape[2] != cache.head_dim
             or strides[2] != 1):
         raise EngineError(f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension")
-    _plain(x, name)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _plain(x, name)
     n, heads, dim = shape
     return _ROWS.pack(x.data_ptr(), strides[0] if n > 1 else heads * dim, strides[1] if heads > 1 else dim)
 
@@ -147,7 +149,8 @@ def _vector(x, name, n, dtype, device):
     """The address of a contiguous vector; None stays None."""
     if x is None:
         return None
-    _plain(x, name)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _plain(x, name)
     if x.dtype is not dtype or x.shape != (n,) or x.device != device or (n > 1 and x.stride(0) != 1):
         raise EngineError(f"{name} is {dtype} [{n}], contiguous, on the same GPU")
     return x.data_ptr()
@@ -204,7 +207,8 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
         if (rope.dtype is not torch.float32 or rope.dim() != 2 or rope.shape[1] != dim or not rope.is_contiguous()
                 or rope.device != dev):
             raise EngineError("rope is float32 [positions, head dim], contiguous, on the same GPU")
-        _plain(rope, "rope")
+        if rope.requires_grad or forward_ad._current_level >= 0:
+            _plain(rope, "rope")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
     _enqueue(dev, _lib().rpg_hip_paged_append, cache._packed(), seqs, kr, vr, qr, qo, heads,
              _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
@@ -272,7 +276,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
     if (logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda
             or (logits.shape[1] > 1 and logits.stride(1) != 1)):
         raise EngineError("logits are [rows, vocab] float32, float16 or bfloat16 on a GPU, contiguous in the last dimension")
-    _plain(logits, "logits")
+    if logits.requires_grad or forward_ad._current_level >= 0:
+        _plain(logits, "logits")
     if u is None:
         raise EngineError("u is needed")
     rows, vocab = logits.shape
