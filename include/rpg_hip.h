@@ -240,8 +240,8 @@ RPG_HIP_API int32_t rpg_hip_bench_matmul(uint32_t type, const uint8_t* w, int64_
  * elements are contiguous; pointers and strides are multiples of 16 bytes,
  * strides are counted in elements. */
 
-/* A pool of n_pages pages, each of page_size positions (a power of two, 16 or
- * more) of n_kv heads of head_dim (64 or 128) elements: position r of head h of
+/* A pool of n_pages pages, each of page_size positions (a power of two, 16 to
+ * 65536) of n_kv heads of head_dim (64 or 128) elements: position r of head h of
  * page p at p * page_stride + h * head_stride + r * row_stride, alike in k and v. */
 typedef struct {
   void* k;
@@ -290,7 +290,9 @@ RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const
 /* Attention of one token per sequence, row s of q, over all of the sequence's
  * positions: out = softmax(scale q . k) v per head, heads kv * (n_heads / n_kv)
  * .. sharing key head kv (reference src/qwen3.cc:79-117). scale > 0. Sums and
- * softmax in f32; for 16-bit types the weights multiply the values in two parts
+ * softmax in f32, weights up to 1 (in prompts 256) before the division by their
+ * sum: a float has to hold the keys' number times the largest value times that.
+ * For 16-bit types the weights multiply the values in two parts
  * of that type, which together keep 16 (bf16) or 22 bits. A sequence without positions gives zeros. out may
  * be q, with its strides. work: rpg_hip_paged_work bytes, read and written by this call alone
  * until it is complete (any contents; may be NULL when that is 0). */

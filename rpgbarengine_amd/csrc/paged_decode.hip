@@ -18,10 +18,10 @@
 // Bound: the K and V bytes, each read once (16 columns are computed for any
 // group size: at 8 heads f32 the products would take 1/2 of the time the bytes
 // do, the 16-bit types' 1/10). Measured, 32 heads on 8 of 128: 64 sequences of
-// 201 to 11167 positions, bf16, 861 MB in 165-171 us (the rate of a large copy:
+// 201 to 11167 positions, bf16, 861 MB in 172 us (the rate of a large copy:
 // 171); one of 131000, f16, 537 MB in 95 us (107); 8 of about 1073, f32, 70 MB in 18.5
-// us (14, and two launches); one of 95, f16: 7 us, the call itself. Ranges: see
-// DecodeSplits.
+// us (14, and two launches); one of 95, f16: 7.2 us, the call itself (5.4 in a captured
+// graph). Ranges: see DecodeSplits.
 
 #include <hip/hip_runtime.h>
 
@@ -318,6 +318,9 @@ void LaunchDim(const AttentionArgs& a, hipStream_t s) {
 // bf16 12.0 us in ranges, 7.6 whole, 500 11.7 and 8.4, 700 11.9 and 10.3; f32 200 11.7
 // and 10.1, 400 11.6 and 13.7. The rule knows the sequences' capacity, not their
 // lengths, which are on the device: ranges behind a sequence's end return at once.
+// So a table wider than its sequences costs the join's launch: one of 95 positions
+// f16 7.8 us a call in a table of its own width, 11.7 in one for 4096 or for 131072
+// (5.3 and 6.7 in a captured graph), one of 300 8.3 and 11.8 (8.0 and 8.4).
 int DecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
   if (capacity * bytes <= 1280) return 1;
   const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));

@@ -13,7 +13,8 @@
 // weight. A weight itself is computed in double (a table of 2^(-j/32) and a
 // polynomial of degree 5, 3e-15 relative).
 //
-// Four launches over (row, slice of the vocabulary), without a sort:
+// Four launches over (row, slice of the vocabulary), three where neither top_k nor
+// top_p are given, without a sort:
 //   Max    largest value (and its first index) and least finite one per slice,
 //          the largest of every group of four threads' tokens
 //   Count  histogram of 2048 equal steps of x below the row's maximum: count
@@ -29,11 +30,14 @@
 // top_p's) are found by Draw over the whole row, digit by digit.
 //
 // Bound: the logits' bytes, read once from HBM (later launches find them in
-// the memory-side cache); for few rows the four launches. Measured, vocabulary of
+// the memory-side cache); for few rows what a row takes whatever its length: the
+// launches, a histogram's 2048 steps, sorting a list. Measured, vocabulary of
 // 151936: 192 bf16 rows, 58 MB (12 us for a large copy), greedy 24 us, top_k 40 50,
 // min_p 48, temperature alone 75, top_p 95 (a weight in double and an LDS atomic
-// for nearly every token), all mixed 83; 8 f32 rows with min_p 18.5; one row with
-// top_p 38.
+// for nearly every token), all mixed 84-92; 8 f32 rows with min_p 19 where the
+// launches are four, 17 where they are three. One f32 row, in a captured graph:
+// greedy 8.5 us (all that the four launches and one look at the logits take), no
+// limits 16, top_k 40 22, top_p 27 (peaked) to 36 (flat), of which 31 with 4096 tokens.
 
 #include <hip/hip_runtime.h>
 
@@ -1049,7 +1053,7 @@ void Launch(const SampleArgs& a, hipStream_t s) {
   const Layout l = LayoutOf(a.rows, a.vocab);
   const dim3 grid(l.slices, a.rows);
   MaxKernel<T><<<grid, kThreads, 0, s>>>(a, l);
-  // (min_p needs no cut: 8 f32 rows 17 us a call without the launch, 21 with it)
+  // (min_p needs no cut: 8 f32 rows 17 us a call without the launch, 19.5 with it)
   if (a.top_k != nullptr || a.top_p != nullptr) CountKernel<T><<<grid, kThreads, 0, s>>>(a, l);
   SplitKernel<T><<<grid, kThreads, 0, s>>>(a, l);
   DrawKernel<T><<<a.rows, kDrawThreads, 0, s>>>(a, l);
