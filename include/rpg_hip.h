@@ -251,12 +251,13 @@ typedef struct {
 } rpg_hip_paged_cache;
 
 /* n_seqs sequences. Sequence s holds lens[s] positions (at most pages *
- * page_size, which is at most 2^30; 0 and less: none), the new tokens among them; position p lies in
- * page table[s * table_stride + p / page_size]. A page number outside [0,
- * n_pages) is never followed: its positions take no part. The new tokens of
- * sequence s are the packed rows starts[s] .. starts[s + 1] (n_seqs + 1
- * of them, not decreasing), at its last positions; rows of no sequence are left as they
- * are. starts is not read by rpg_hip_paged_decode (one token each). */
+ * page_size, which is at most 2^30; 0 and less: none), the new tokens among
+ * them; position p lies in page table[s * table_stride + p / page_size]. A page
+ * number outside [0, n_pages) is never followed: its positions take no part.
+ * The new tokens of sequence s are the packed rows starts[s] .. starts[s + 1]
+ * (n_seqs + 1 of them, not decreasing), at its last positions; rows of no
+ * sequence are left as they are. starts is not read by rpg_hip_paged_decode
+ * (one token each). Without sequences a call does nothing. */
 typedef struct {
   const int32_t* table;
   int64_t table_stride;
@@ -272,8 +273,8 @@ typedef struct {
 } rpg_hip_rows;
 
 /* Stores the new tokens' keys and values in their pages. Keys, and queries
- * from q into q_out (which may be q, with its strides; q->data NULL: no queries), are RMS-normed
- * per head with the gains k_norm and q_norm (f32 [head_dim]; NULL: not normed)
+ * from q into q_out (which may be q, with its strides; q->data NULL: no
+ * queries), are RMS-normed per head with the gains k_norm and q_norm (f32 [head_dim]; NULL: not normed)
  * and rotated by row `position` of rope (f32 [rope_rows][head_dim], cos |
  * sin, as rpg_hip_model_rope_row; NULL: not rotated), as the engine's own
  * QK-norm and RoPE (reference src/qwen3.cc:139-167), computed in f32 and
@@ -292,10 +293,11 @@ RPG_HIP_API int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const
  * .. sharing key head kv (reference src/qwen3.cc:79-117). scale > 0. Sums and
  * softmax in f32, weights up to 1 (in prompts 256) before the division by their
  * sum: a float has to hold the keys' number times the largest value times that.
- * For 16-bit types the weights multiply the values in two parts
- * of that type, which together keep 16 (bf16) or 22 bits. A sequence without positions gives zeros. out may
- * be q, with its strides. work: rpg_hip_paged_work bytes, read and written by this call alone
- * until it is complete (any contents; may be NULL when that is 0). */
+ * For 16-bit types the weights multiply the values in two parts of that type,
+ * which together keep 16 (bf16) or 22 bits. A sequence without positions gives
+ * zeros. out may be q, with its strides. work: rpg_hip_paged_work bytes, read
+ * and written by this call alone until it is complete (any contents; may be
+ * NULL when that is 0). */
 RPG_HIP_API int32_t rpg_hip_paged_decode(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
                                          void* work, int64_t work_bytes, void* stream);
@@ -309,7 +311,7 @@ RPG_HIP_API int32_t rpg_hip_paged_prompt(const rpg_hip_paged_cache* cache, const
 
 /* Bytes of work memory that rpg_hip_paged_decode (prompt = 0) or
  * rpg_hip_paged_prompt (prompt = 1) takes for these sizes; -1 when they are
- * refused. Host only; reads the sizes of *cache and *seqs, no pointers. */
+ * refused; 0 for batches with nothing to do. Host only; reads the sizes of *cache and *seqs, no pointers. */
 RPG_HIP_API int64_t rpg_hip_paged_work(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                        int32_t n_heads, int32_t prompt);
 
