@@ -315,6 +315,86 @@ RPG_HIP_API int32_t rpg_hip_paged_prompt(const rpg_hip_paged_cache* cache, const
 RPG_HIP_API int64_t rpg_hip_paged_work(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                        int32_t n_heads, int32_t prompt);
 
+/* ---- a cache held in 8 bits. Position r of head h of page p is a row of
+ * head_dim codes (k, v: one byte each, strides in bytes, multiples of 16) and a
+ * scale (k_scale, v_scale: f32 at p * scale_page_stride + h * scale_head_stride + r,
+ * strides in elements, multiples of 4): element = code * scale. code:
+ * RPG_HIP_I8 = whole numbers up to 127 either way, RPG_HIP_E4M3 = 8-bit floats of
+ * 4 exponent and 3 mantissa bits, up to 448, without infinities. As
+ * rpg_hip_paged_cache in all else; the rows that go in and come out are f32, f16 or
+ * bf16 (`type`, a ggml id), all of a call alike. */
+enum { RPG_HIP_I8 = 0, RPG_HIP_E4M3 = 1 };
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t page_stride, head_stride, row_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  int32_t n_pages, page_size, n_kv, head_dim, code;
+} rpg_hip_quant_cache;
+
+/* rpg_hip_paged_append into such a cache. A row y (keys: as normed and rotated in
+ * f32; values: as they are) with the largest magnitude a is held as scale a / M, M
+ * the largest code, and codes y M / a, to the nearest, even at ties. Where a is below
+ * 2^-112 scale and codes are 0; where y is not finite the scale is NaN, the codes 0:
+ * the whole row reads as NaN. */
+RPG_HIP_API int32_t rpg_hip_quant_append(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                                         const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
+                                         const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm,
+                                         const float* k_norm, float eps, const float* rope, int64_t rope_rows,
+                                         void* stream);
+
+/* The last positions of each sequence as rows: those of sequence s go to the packed
+ * rows starts[s] .. starts[s + 1] of k and v ([token][n_kv] rows), computed in f32 and
+ * rounded once. Positions of pages that the table does not name give zeros; rows of no
+ * sequence and of positions below 0 are left as they are. */
+RPG_HIP_API int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                                       const rpg_hip_rows* k, const rpg_hip_rows* v, void* stream);
+
+/* Edits of logits before a draw. All device pointers; arrays of one element per
+ * row unless a stride (in elements) is given.
+ *
+ * history: the tokens of each row so far ([rows][history_size], of which
+ * history_lens counts the first ones that are there; NULL: all), the first
+ * prompts[row] of them its prompt (NULL: none). Tokens outside [0, vocab) count for
+ * nothing. x being a token's logit and c the times that it was made behind the prompt:
+ *   x = x > 0 ? x / repetition : x * repetition   where the history holds it
+ *   x = x - frequency c - presence                where c > 0
+ *   x = x + bias                                  where bias_ids lists it
+ *   x = -inf                                      where its mask's bit is 0
+ * in f32, rounded once. repetition, presence, frequency may be NULL: none of it; a
+ * repetition that is not above 0 counts as 1. bias_ids, bias: [rows][n_biases];
+ * numbers outside [0, vocab) are no entries, of several for one token the last
+ * counts. mask: [n_masks] rows of ceil(vocab / 32) words, bit t % 32 of word t / 32
+ * set where token t may come; row r goes by mask mask_rows[r] (NULL: r), by none
+ * where that is outside [0, n_masks). */
+typedef struct {
+  const int32_t* history;
+  int64_t history_stride;
+  const int32_t* history_lens;
+  const int32_t* prompts;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids;
+  int64_t bias_ids_stride;
+  const float* bias;
+  int64_t bias_stride;
+  const int32_t* mask;
+  int64_t mask_stride;
+  const int32_t* mask_rows;
+  int32_t history_size, n_biases, n_masks;
+} rpg_hip_edits;
+
+/* logits [rows][vocab], row_stride elements apart, edited into out (which may be
+ * logits, with its stride: then rows without a mask are touched only where tokens
+ * change). Any alignment of the type; vocab <= 2^24, rows <= 65535, history_size
+ * <= 2^24. No work memory. */
+RPG_HIP_API int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t rows, int64_t vocab,
+                                        int64_t row_stride, const rpg_hip_edits* edits, void* out,
+                                        int64_t out_stride, void* stream);
+
 /* One token per row of logits ([rows][vocab], row_stride elements apart, any
  * alignment of the type): weights exp((x - max) / temperature), tokens ranked
  * by value, equal ones by index; kept are the first top_k of them, of those

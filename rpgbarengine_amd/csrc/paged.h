@@ -58,6 +58,32 @@ struct AppendArgs {
 };
 void Append(const AppendArgs& a, hipStream_t s);
 
+// A cache of 8-bit codes: its k and v (and their strides) are the codes, `type`
+// the element type of the rows that go in and come out; position r of head h of
+// page p has its scales at p * page_bytes + h * head_bytes + 4 r.
+enum Code : uint32_t { kI8 = 0, kE4M3 = 1 };
+struct Scales {
+  char* k = nullptr;
+  char* v = nullptr;
+  int64_t page_bytes = 0, head_bytes = 0;
+};
+
+struct CodesAppendArgs {
+  AppendArgs a;
+  Scales scales;
+  int64_t code = kI8;
+};
+void AppendCodes(const CodesAppendArgs& a, hipStream_t s);
+
+struct CodesReadArgs {
+  Cache c;
+  Scales scales;
+  Seqs s;
+  Rows k, v;
+  int64_t code = kI8;
+};
+void ReadCodes(const CodesReadArgs& a, hipStream_t s);
+
 struct AttentionArgs {
   Cache c;
   Seqs s;

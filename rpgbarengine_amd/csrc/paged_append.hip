@@ -25,24 +25,6 @@ namespace rpg {
 namespace paged {
 namespace {
 
-// sum over aligned groups of kLanes lanes
-template <int kLanes>
-__device__ __forceinline__ float GroupSum(float v) {
-  v += lanes::DppF<lanes::kQuadXor1>(v);
-  v += lanes::DppF<lanes::kQuadXor2>(v);
-  v += lanes::DppF<lanes::kRowHalfMirror>(v);
-  if constexpr (kLanes >= 16) v += lanes::DppF<lanes::kRowMirror>(v);
-  if constexpr (kLanes >= 32) v = lanes::AddXor16(v);
-  return v;
-}
-
-// the value of the lane kLanes / 2 further in its group of kLanes
-template <int kLanes>
-__device__ __forceinline__ float OtherHalf(float v) {
-  if constexpr (kLanes == 16) return lanes::DppF<lanes::kRowRor8>(v);
-  return __shfl_xor(v, kLanes / 2, 64);
-}
-
 // grid (token, kEach x 256 / kLanes rows of it): the token's rows are its query
 // heads, then its key heads, then its value heads.
 template <typename T, int kDim, int kEach>

@@ -77,6 +77,24 @@ __device__ __forceinline__ U4 Load16(const char* p) {
   return *(const __attribute__((address_space(1))) U4*)p;
 }
 
+// sum over aligned groups of kLanes lanes
+template <int kLanes>
+__device__ __forceinline__ float GroupSum(float v) {
+  v += lanes::DppF<lanes::kQuadXor1>(v);
+  v += lanes::DppF<lanes::kQuadXor2>(v);
+  v += lanes::DppF<lanes::kRowHalfMirror>(v);
+  if constexpr (kLanes >= 16) v += lanes::DppF<lanes::kRowMirror>(v);
+  if constexpr (kLanes >= 32) v = lanes::AddXor16(v);
+  return v;
+}
+
+// the value of the lane kLanes / 2 further in its group of kLanes
+template <int kLanes>
+__device__ __forceinline__ float OtherHalf(float v) {
+  if constexpr (kLanes == 16) return lanes::DppF<lanes::kRowRor8>(v);
+  return __shfl_xor(v, kLanes / 2, 64);
+}
+
 // two floats rounded to nearest even, packed
 template <typename T>
 __device__ __forceinline__ uint32_t Pack2(float a, float b) {

@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "common.h"
+#include "edit_rows.h"
 #include "paged.h"
 #include "rpg_hip.h"
 #include "sample_rows.h"
@@ -52,30 +53,39 @@ void CheckPointer(const char* what, const void* p, int align) {
   RPG_CHECK(reinterpret_cast<uintptr_t>(p) % align == 0, "%s does not lie at a multiple of %d bytes", what, align);
 }
 
+void CheckSizes(int32_t head_dim, int32_t page_size, int32_t n_pages, int32_t n_kv) {
+  RPG_CHECK(head_dim == 64 || head_dim == 128, "head_dim %d is neither 64 nor 128", head_dim);
+  RPG_CHECK(page_size >= 16 && page_size <= 65536 && (page_size & (page_size - 1)) == 0,
+            "page_size %d is not a power of two from 16 to 65536", page_size);
+  RPG_CHECK(n_pages >= 1, "a cache of %d pages", n_pages);
+  RPG_CHECK(n_kv >= 1, "%d key heads", n_kv);
+}
+
+// The strides and sizes of rows of `bytes` bytes an element.
+void PageStrides(int64_t page_stride, int64_t head_stride, int64_t row_stride, int32_t head_dim, int32_t page_size,
+                 int32_t n_pages, int32_t n_kv, int bytes, paged::Cache* out) {
+  out->page_bytes = StrideBytes("page_stride", page_stride, bytes);
+  out->head_bytes = StrideBytes("head_stride", head_stride, bytes);
+  const int64_t row = StrideBytes("row_stride", row_stride, bytes);
+  // positions of a page are addressed by 32-bit offsets; no two of them overlap
+  RPG_CHECK(row >= head_dim * bytes && row * page_size < kMaxStride, "row_stride %lld", (long long)row_stride);
+  RPG_CHECK((n_kv == 1 || std::abs(out->head_bytes) >= head_dim * bytes) &&
+                (n_pages == 1 || std::abs(out->page_bytes) >= head_dim * bytes),
+            "head_stride %lld or page_stride %lld is less than a row", (long long)head_stride,
+            (long long)page_stride);
+  out->row_bytes = static_cast<int32_t>(row);
+  out->n_pages = n_pages;
+  out->n_kv = n_kv;
+  out->page_log2 = __builtin_ctz(static_cast<unsigned>(page_size));
+  out->head_dim = head_dim;
+}
+
 paged::Cache CacheSizes(const rpg_hip_paged_cache* c) {
   RPG_CHECK(c != nullptr, "the cache is null");
   paged::Cache out;
   const int bytes = ElementBytes(c->type);
-  RPG_CHECK(c->head_dim == 64 || c->head_dim == 128, "head_dim %d is neither 64 nor 128", c->head_dim);
-  RPG_CHECK(c->page_size >= 16 && c->page_size <= 65536 && (c->page_size & (c->page_size - 1)) == 0,
-            "page_size %d is not a power of two from 16 to 65536", c->page_size);
-  RPG_CHECK(c->n_pages >= 1, "a cache of %d pages", c->n_pages);
-  RPG_CHECK(c->n_kv >= 1, "%d key heads", c->n_kv);
-  out.page_bytes = StrideBytes("page_stride", c->page_stride, bytes);
-  out.head_bytes = StrideBytes("head_stride", c->head_stride, bytes);
-  const int64_t row = StrideBytes("row_stride", c->row_stride, bytes);
-  // positions of a page are addressed by 32-bit offsets; no two of them overlap
-  RPG_CHECK(row >= c->head_dim * bytes && row * c->page_size < kMaxStride, "row_stride %lld",
-            (long long)c->row_stride);
-  RPG_CHECK((c->n_kv == 1 || std::abs(out.head_bytes) >= c->head_dim * bytes) &&
-                (c->n_pages == 1 || std::abs(out.page_bytes) >= c->head_dim * bytes),
-            "head_stride %lld or page_stride %lld is less than a row", (long long)c->head_stride,
-            (long long)c->page_stride);
-  out.row_bytes = static_cast<int32_t>(row);
-  out.n_pages = c->n_pages;
-  out.n_kv = c->n_kv;
-  out.page_log2 = __builtin_ctz(static_cast<unsigned>(c->page_size));
-  out.head_dim = c->head_dim;
+  CheckSizes(c->head_dim, c->page_size, c->n_pages, c->n_kv);
+  PageStrides(c->page_stride, c->head_stride, c->row_stride, c->head_dim, c->page_size, c->n_pages, c->n_kv, bytes, &out);
   out.type = static_cast<uint32_t>(c->type);
   return out;
 }
@@ -89,20 +99,51 @@ paged::Cache CacheOf(const rpg_hip_paged_cache* c) {
   return out;
 }
 
-paged::Seqs SeqSizes(const rpg_hip_sequences* s, const rpg_hip_paged_cache* c) {
-  RPG_CHECK(s != nullptr, "the sequences are null");
-  paged::Seqs out;
-  RPG_CHECK(s->n_seqs >= 0 && s->n_tokens >= 0, "%d sequences of %d new tokens", s->n_seqs, s->n_tokens);
-  RPG_CHECK(s->pages >= 0 && s->pages <= kMaxPositions / c->page_size,
-            "%d pages of %d positions for a sequence", s->pages, c->page_size);
-  out.n_seqs = s->n_seqs;
-  out.n_tokens = s->n_tokens;
-  out.capacity = s->pages * c->page_size;
+// A cache of codes; `type`: of the rows.
+paged::Cache QuantSizes(const rpg_hip_quant_cache* c, int32_t type, paged::Scales* scales) {
+  RPG_CHECK(c != nullptr, "the cache is null");
+  paged::Cache out;
+  ElementBytes(type);
+  RPG_CHECK(c->code == RPG_HIP_I8 || c->code == RPG_HIP_E4M3, "code %d is neither i8 (0) nor e4m3 (1)", c->code);
+  CheckSizes(c->head_dim, c->page_size, c->n_pages, c->n_kv);
+  PageStrides(c->page_stride, c->head_stride, c->row_stride, c->head_dim, c->page_size, c->n_pages, c->n_kv, 1, &out);
+  scales->page_bytes = StrideBytes("scale_page_stride", c->scale_page_stride, 4);
+  scales->head_bytes = StrideBytes("scale_head_stride", c->scale_head_stride, 4);
+  RPG_CHECK((c->n_kv == 1 || std::abs(c->scale_head_stride) >= c->page_size) &&
+                (c->n_pages == 1 || std::abs(c->scale_page_stride) >= c->page_size),
+            "scale_head_stride %lld or scale_page_stride %lld is less than a page's positions",
+            (long long)c->scale_head_stride, (long long)c->scale_page_stride);
+  out.type = static_cast<uint32_t>(type);
   return out;
 }
 
-paged::Seqs SeqsOf(const rpg_hip_sequences* s, const rpg_hip_paged_cache* c, bool packed) {
-  paged::Seqs out = SeqSizes(s, c);
+paged::Cache QuantOf(const rpg_hip_quant_cache* c, int32_t type, paged::Scales* scales) {
+  paged::Cache out = QuantSizes(c, type, scales);
+  CheckPointer("the cache's k", c->k, 16);
+  CheckPointer("the cache's v", c->v, 16);
+  CheckPointer("the cache's k_scale", c->k_scale, 16);
+  CheckPointer("the cache's v_scale", c->v_scale, 16);
+  out.k = static_cast<char*>(c->k);
+  out.v = static_cast<char*>(c->v);
+  scales->k = reinterpret_cast<char*>(c->k_scale);
+  scales->v = reinterpret_cast<char*>(c->v_scale);
+  return out;
+}
+
+paged::Seqs SeqSizes(const rpg_hip_sequences* s, int page_size) {
+  RPG_CHECK(s != nullptr, "the sequences are null");
+  paged::Seqs out;
+  RPG_CHECK(s->n_seqs >= 0 && s->n_tokens >= 0, "%d sequences of %d new tokens", s->n_seqs, s->n_tokens);
+  RPG_CHECK(s->pages >= 0 && s->pages <= kMaxPositions / page_size,
+            "%d pages of %d positions for a sequence", s->pages, page_size);
+  out.n_seqs = s->n_seqs;
+  out.n_tokens = s->n_tokens;
+  out.capacity = s->pages * page_size;
+  return out;
+}
+
+paged::Seqs SeqsOf(const rpg_hip_sequences* s, int page_size, bool packed) {
+  paged::Seqs out = SeqSizes(s, page_size);
   if (s->n_seqs == 0) return out;
   if (s->pages > 0) CheckPointer("the page table", s->table, 4);
   RPG_CHECK(s->n_seqs == 1 || s->table_stride >= s->pages, "table_stride %lld is less than %d pages",
@@ -168,7 +209,7 @@ int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seq
                   bool prompt) {
   paged::AttentionArgs a;
   a.c = CacheOf(cache);
-  a.s = SeqsOf(seqs, cache, prompt);
+  a.s = SeqsOf(seqs, cache->page_size, prompt);
   if (Empty(a.s, prompt)) return 0;
   CheckHeads(a.c, a.s, n_heads);
   const int n_tokens = prompt ? a.s.n_tokens : a.s.n_seqs;
@@ -193,6 +234,40 @@ int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seq
   return 0;
 }
 
+void AppendRows(paged::AppendArgs* to, const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
+                const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm, const float* k_norm, float eps,
+                const float* rope, int64_t rope_rows) {
+  paged::AppendArgs& a = *to;
+  a.k = RowsOf("k", k, a.c, a.s.n_tokens, a.c.n_kv, false);
+  a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, false);
+  if (q != nullptr && q->data != nullptr) {
+    CheckHeads(a.c, a.s, n_heads);
+    RPG_CHECK(n_heads <= 65536 && a.c.n_kv <= 65536, "%d query heads on %d key heads", n_heads, a.c.n_kv);
+    a.q = RowsOf("q", q, a.c, a.s.n_tokens, n_heads, false);
+    a.q_out = RowsOf("q_out", q_out, a.c, a.s.n_tokens, n_heads, true);
+    CheckInPlace("q_out is q", a.q_out, a.q, a.s.n_tokens, n_heads);
+    a.n_heads = n_heads;
+  } else {
+    RPG_CHECK(a.c.n_kv <= 65536, "%d key heads", a.c.n_kv);
+  }
+  if (q_norm != nullptr) CheckPointer("q_norm", q_norm, 16);
+  if (k_norm != nullptr) CheckPointer("k_norm", k_norm, 16);
+  if (rope != nullptr) CheckPointer("rope", rope, 16);
+  RPG_CHECK(rope == nullptr || rope_rows >= 0, "%lld rotation rows", (long long)rope_rows);
+  RPG_CHECK(eps >= 0.0f, "eps %g", eps);
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.eps = eps;
+  a.rope = rope;
+  a.rope_rows = rope_rows;
+}
+
+// Rows of 4-byte elements that may be given more than once (stride 0).
+void CheckList(const char* what, const void* p, int64_t stride) {
+  CheckPointer(what, p, 4);
+  RPG_CHECK(stride >= 0 && stride <= kMaxStride, "%s: rows %lld elements apart", what, (long long)stride);
+}
+
 }  // namespace
 }  // namespace rpg
 
@@ -208,30 +283,9 @@ int32_t rpg_hip_paged_append(const rpg_hip_paged_cache* cache, const rpg_hip_seq
       [&] {
         paged::AppendArgs a;
         a.c = CacheOf(cache);
-        a.s = SeqsOf(seqs, cache, true);
+        a.s = SeqsOf(seqs, cache->page_size, true);
         if (Empty(a.s, true)) return 0;
-        a.k = RowsOf("k", k, a.c, a.s.n_tokens, a.c.n_kv, false);
-        a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, false);
-        if (q != nullptr && q->data != nullptr) {
-          CheckHeads(a.c, a.s, n_heads);
-          RPG_CHECK(n_heads <= 65536 && a.c.n_kv <= 65536, "%d query heads on %d key heads", n_heads, a.c.n_kv);
-          a.q = RowsOf("q", q, a.c, a.s.n_tokens, n_heads, false);
-          a.q_out = RowsOf("q_out", q_out, a.c, a.s.n_tokens, n_heads, true);
-          CheckInPlace("q_out is q", a.q_out, a.q, a.s.n_tokens, n_heads);
-          a.n_heads = n_heads;
-        } else {
-          RPG_CHECK(a.c.n_kv <= 65536, "%d key heads", a.c.n_kv);
-        }
-        if (q_norm != nullptr) CheckPointer("q_norm", q_norm, 16);
-        if (k_norm != nullptr) CheckPointer("k_norm", k_norm, 16);
-        if (rope != nullptr) CheckPointer("rope", rope, 16);
-        RPG_CHECK(rope == nullptr || rope_rows >= 0, "%lld rotation rows", (long long)rope_rows);
-        RPG_CHECK(eps >= 0.0f, "eps %g", eps);
-        a.q_norm = q_norm;
-        a.k_norm = k_norm;
-        a.eps = eps;
-        a.rope = rope;
-        a.rope_rows = rope_rows;
+        AppendRows(&a, k, v, q, q_out, n_heads, q_norm, k_norm, eps, rope, rope_rows);
         paged::Append(a, static_cast<hipStream_t>(stream));
         return 0;
       },
@@ -255,7 +309,7 @@ int64_t rpg_hip_paged_work(const rpg_hip_paged_cache* cache, const rpg_hip_seque
   return Guard(
       [&]() -> int64_t {
         const paged::Cache c = CacheSizes(cache);
-        const paged::Seqs s = SeqSizes(seqs, cache);
+        const paged::Seqs s = SeqSizes(seqs, cache->page_size);
         CheckHeads(c, s, n_heads);
         return AttentionWork(c, s, n_heads, prompt != 0);
       },
@@ -311,6 +365,114 @@ int64_t rpg_hip_sample_rows_work(int64_t n_rows, int64_t vocab) {
         RPG_CHECK(n_rows >= 0 && n_rows <= 65535, "%lld rows outside [0, 65535]", (long long)n_rows);
         RPG_CHECK(vocab >= 1 && vocab <= 262144, "%lld logits outside [1, 262144]", (long long)vocab);
         return rows::WorkBytes(n_rows, vocab);
+      },
+      -1);
+}
+
+int32_t rpg_hip_quant_append(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                             const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
+                             const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm, const float* k_norm,
+                             float eps, const float* rope, int64_t rope_rows, void* stream) {
+  return Guard(
+      [&] {
+        paged::CodesAppendArgs a;
+        a.a.c = QuantOf(cache, type, &a.scales);
+        a.code = cache->code;
+        a.a.s = SeqsOf(seqs, cache->page_size, true);
+        if (Empty(a.a.s, true)) return 0;
+        AppendRows(&a.a, k, v, q, q_out, n_heads, q_norm, k_norm, eps, rope, rope_rows);
+        paged::AppendCodes(a, static_cast<hipStream_t>(stream));
+        return 0;
+      },
+      -1);
+}
+
+int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                           const rpg_hip_rows* k, const rpg_hip_rows* v, void* stream) {
+  return Guard(
+      [&] {
+        paged::CodesReadArgs a;
+        a.c = QuantOf(cache, type, &a.scales);
+        a.code = cache->code;
+        a.s = SeqsOf(seqs, cache->page_size, true);
+        if (Empty(a.s, true)) return 0;
+        RPG_CHECK(a.c.n_kv <= 65536, "%d key heads", a.c.n_kv);
+        a.k = RowsOf("k", k, a.c, a.s.n_tokens, a.c.n_kv, true);
+        a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, true);
+        paged::ReadCodes(a, static_cast<hipStream_t>(stream));
+        return 0;
+      },
+      -1);
+}
+
+int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t n_rows, int64_t vocab, int64_t row_stride,
+                            const rpg_hip_edits* edits, void* out, int64_t out_stride, void* stream) {
+  return Guard(
+      [&] {
+        const int bytes = ElementBytes(type);
+        RPG_CHECK(edits != nullptr, "the edits are null");
+        const rpg_hip_edits& e = *edits;
+        RPG_CHECK(n_rows >= 0 && n_rows <= 65535, "%lld rows outside [0, 65535]", (long long)n_rows);
+        RPG_CHECK(vocab >= 1 && vocab <= 1 << 24, "%lld logits outside [1, 2^24]", (long long)vocab);
+        if (n_rows == 0) return 0;
+        CheckPointer("logits", logits, bytes);
+        CheckPointer("out", out, bytes);
+        RPG_CHECK(n_rows == 1 || (row_stride >= 0 && row_stride <= kMaxStride), "row_stride %lld",
+                  (long long)row_stride);
+        RPG_CHECK(n_rows == 1 || (out_stride >= vocab && out_stride <= kMaxStride), "out_stride %lld",
+                  (long long)out_stride);
+        RPG_CHECK(out != logits || n_rows == 1 || out_stride == row_stride, "out is logits with another stride");
+        rows::EditArgs a;
+        a.logits = static_cast<const char*>(logits);
+        a.out = static_cast<char*>(out);
+        a.row_bytes = n_rows == 1 ? 0 : row_stride * bytes;
+        a.out_bytes = n_rows == 1 ? 0 : out_stride * bytes;
+        a.type = static_cast<uint32_t>(type);
+        a.rows = static_cast<int32_t>(n_rows);
+        a.vocab = static_cast<int32_t>(vocab);
+        for (const void* p : {static_cast<const void*>(e.history_lens), static_cast<const void*>(e.prompts),
+                              static_cast<const void*>(e.repetition), static_cast<const void*>(e.presence),
+                              static_cast<const void*>(e.frequency), static_cast<const void*>(e.mask_rows)})
+          if (p != nullptr) CheckPointer("a row parameter", p, 4);
+        if (e.history != nullptr) {
+          CheckList("history", e.history, n_rows == 1 ? 0 : e.history_stride);
+          RPG_CHECK(e.history_size >= 0 && e.history_size <= 1 << 24, "a history of %d tokens", e.history_size);
+          a.history = e.history;
+          a.history_stride = n_rows == 1 ? 0 : e.history_stride;
+          a.history_size = e.history_size;
+          a.history_lens = e.history_lens;
+          a.prompts = e.prompts;
+          a.repetition = e.repetition;
+          a.presence = e.presence;
+          a.frequency = e.frequency;
+        } else {
+          RPG_CHECK(e.history_lens == nullptr && e.prompts == nullptr && e.repetition == nullptr &&
+                        e.presence == nullptr && e.frequency == nullptr,
+                    "penalties without a history");
+        }
+        RPG_CHECK((e.bias_ids == nullptr) == (e.bias == nullptr), "bias_ids without bias, or bias without bias_ids");
+        if (e.bias_ids != nullptr) {
+          CheckList("bias_ids", e.bias_ids, n_rows == 1 ? 0 : e.bias_ids_stride);
+          CheckList("bias", e.bias, n_rows == 1 ? 0 : e.bias_stride);
+          RPG_CHECK(e.n_biases >= 0 && e.n_biases <= 1 << 24, "%d biases", e.n_biases);
+          a.bias_ids = e.bias_ids;
+          a.bias = e.bias;
+          a.bias_ids_stride = n_rows == 1 ? 0 : e.bias_ids_stride;
+          a.bias_stride = n_rows == 1 ? 0 : e.bias_stride;
+          a.n_biases = e.n_biases;
+        }
+        if (e.mask != nullptr) {
+          RPG_CHECK(e.n_masks >= 0, "%d masks", e.n_masks);
+          CheckList("mask", e.mask, e.n_masks <= 1 ? 0 : e.mask_stride);
+          a.mask = e.mask;
+          a.mask_stride = e.n_masks <= 1 ? 0 : e.mask_stride;
+          a.mask_rows = e.mask_rows;
+          a.n_masks = e.n_masks;
+        } else {
+          RPG_CHECK(e.mask_rows == nullptr, "mask_rows without a mask");
+        }
+        rows::Edit(a, static_cast<hipStream_t>(stream));
+        return 0;
       },
       -1);
 }

@@ -6,7 +6,10 @@ of many rows, for hosts that schedule sessions themselves.
     serving.append(cache, table, lens, starts, k, v, q=q, q_norm=..., k_norm=..., rope=...)
     out = serving.prompt_attention(q, cache, table, lens, starts)   # prompts, packed
     out = serving.decode_attention(q, cache, table, lens)           # one token each
+    logits = serving.edit_logits(logits, history, history_lens, repetition=..., mask=...)
     tokens, logprobs = serving.sample(logits, u, temperature, top_k, top_p, min_p)
+
+A QuantCache in the cache's place holds its rows in 8 bits.
 
 `table` is int32 [sequences, pages]: position p of a sequence lies in page
 table[s, p // page_size]; `lens` int32 [sequences] counts a sequence's
@@ -36,12 +39,18 @@ _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_f
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml ids
 # rpg_hip_paged_cache, rpg_hip_sequences, rpg_hip_rows, packed as C lays them out
 _CACHE, _SEQS, _ROWS = struct.Struct("PPqqqiiiii"), struct.Struct("PqPPiii"), struct.Struct("Pqq")
+# rpg_hip_quant_cache, rpg_hip_edits
+_QUANT, _EDITS = struct.Struct("PPPPqqqqqiiiii"), struct.Struct("PqPPPPPPqPqPqPiii")
+_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 _SIGS = {
     "rpg_hip_paged_append": ([_P, _P, _P, _P, _P, _P, _I32, _P, _P, _F, _P, _I64, _P], _I32),
     "rpg_hip_paged_decode": ([_P, _P, _P, _P, _I32, _F, _P, _I64, _P], _I32),
     "rpg_hip_paged_prompt": ([_P, _P, _P, _P, _I32, _F, _P, _I64, _P], _I32),
     "rpg_hip_paged_work": ([_P, _P, _I32, _I32], _I64),
+    "rpg_hip_quant_append": ([_P, _P, _I32, _P, _P, _P, _P, _I32, _P, _P, _F, _P, _I64, _P], _I32),
+    "rpg_hip_quant_read": ([_P, _P, _I32, _P, _P, _P], _I32),
+    "rpg_hip_edit_logits": ([_I32, _P, _I64, _I64, _I64, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows": ([_I32, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows_work": ([_I64, _I64], _I64),
 }
@@ -114,6 +123,53 @@ class PagedCache:
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
 
 
+class QuantCache:
+    """A pool of pages held in 8 bits: k and v [pages, key heads, page size, head dim]
+    of codes (torch.int8 or torch.float8_e4m3fn) and k_scale and v_scale [pages, key
+    heads, page size] float32; an element is its code times its row's scale. Views of
+    larger pools are fine, rows at multiples of 16 bytes. What goes in and comes out is
+    float32, float16 or bfloat16."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        _need(k.dim() == 4 and v.shape == k.shape, "k and v are [pages, key heads, page size, head dim]")
+        _need(k.dtype in _CODES and v.dtype == k.dtype, "k and v are both int8 or float8_e4m3fn")
+        _need(k_scale.shape == k.shape[:3] and v_scale.shape == k.shape[:3]
+              and k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32,
+              "k_scale and v_scale are float32 [pages, key heads, page size]")
+        _need(k.is_cuda and all(x.device == k.device for x in (v, k_scale, v_scale)),
+              "k, v, k_scale and v_scale lie on one GPU")
+        for x, name in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            _plain(x, "the cache's " + name)
+        _need(k.stride(3) == 1 and k.stride() == v.stride(), "k and v have the same strides, 1 in the last dimension")
+        _need(k_scale.stride(2) == 1 and k_scale.stride() == v_scale.stride(),
+              "k_scale and v_scale have the same strides, 1 in the last dimension")
+        self._held = k, v, k_scale, v_scale
+        self.device, self.codes = k.device, k.dtype
+        n_pages, n_kv, page, dim = k.shape
+        self.n_kv, self.head_dim, self.page_size = n_kv, dim, page
+        strides = [s if n > 1 else page * dim * 16 for n, s in zip(k.shape, k.stride())]
+        scales = [s if n > 1 else page for n, s in zip(k_scale.shape, k_scale.stride())]
+        self._at = [x.data_ptr() for x in self._held]
+        self._c = _QUANT.pack(*self._at, *strides[:3], *scales[:2], n_pages, page, n_kv, dim, _CODES[k.dtype])
+
+    k = property(lambda self: self._held[0], doc="the pool of the keys' codes")
+    v = property(lambda self: self._held[1], doc="the pool of the values' codes")
+    k_scale = property(lambda self: self._held[2], doc="the keys' scales")
+    v_scale = property(lambda self: self._held[3], doc="the values' scales")
+
+    def _packed(self):
+        if [x.data_ptr() for x in self._held] != self._at:
+            raise EngineError("the cache's tensors lie elsewhere than when it was made: make a new QuantCache")
+        return self._c
+
+    @classmethod
+    def zeros(cls, n_pages: int, page_size: int, n_kv: int, head_dim: int, codes=torch.float8_e4m3fn,
+              device="cuda") -> "QuantCache":
+        shape = (n_pages, n_kv, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=torch.int8, device=device).view(codes) for _ in "kv")
+        return cls(k, v, *(torch.zeros(shape[:3], device=device) for _ in "kv"))
+
+
 def _ints(x, name, dims, device):
     shape = x.shape
     if x.dtype is not torch.int32 or len(shape) != dims or x.device != device or (shape[-1] > 1 and x.stride(-1) != 1):
@@ -134,11 +190,14 @@ def _seqs(cache, table, lens, starts, n_tokens):
     return _SEQS.pack(table.data_ptr(), table.stride(0), lens.data_ptr(), at, pages, n, n_tokens), n, pages
 
 
-def _rows(x, name, cache):
+def _rows(x, name, cache, dtype=None):
+    """dtype: of the call's rows, where the cache is a QuantCache."""
     shape, strides = x.shape, x.stride()
-    if (len(shape) != 3 or x.dtype is not cache.dtype or x.device != cache.device or shape[2] != cache.head_dim
-            or strides[2] != 1):
-        raise EngineError(f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension")
+    if (len(shape) != 3 or x.dtype is not (dtype or cache.dtype) or x.device != cache.device
+            or shape[2] != cache.head_dim or strides[2] != 1):
+        raise EngineError(f"{name} is [tokens, heads, head dim] of the cache's type and GPU, contiguous in the last dimension"
+                          if dtype is None else
+                          f"{name} is [tokens, heads, head dim] of {dtype} on the cache's GPU, contiguous in the last dimension")
     if x.requires_grad or forward_ad._current_level >= 0:
         _plain(x, name)
     n, heads, dim = shape
@@ -167,6 +226,13 @@ def _enqueue(device, f, *args):
         _ok(rc)
 
 
+def _row_type(x, name):
+    """The type of a call's rows on a QuantCache."""
+    if x.dtype not in _TYPES:
+        raise EngineError(f"{name} is float32, float16 or bfloat16")
+    return x.dtype
+
+
 # What a call writes in place is a new version of the tensor to autograd: a
 # backward pass that saved the old one refuses.
 _written = torch.autograd.graph.increment_version
@@ -180,27 +246,30 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same without a Stream 
     _stream = torch._C._cuda_getCurrentRawStream
 
 
-def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_norm=None, k_norm=None,
+def append(cache, table, lens, starts, k, v, q=None, q_out=None, q_norm=None, k_norm=None,
            eps: float = 1e-6, rope=None):
     """Stores the packed new tokens' keys and values, k and v [tokens, key heads,
     dim], in their pages; q [tokens, heads, dim] goes to q_out (made when not
     given; may be q). Keys and queries are RMS-normed per head with the gains
     k_norm and q_norm (float32 [dim]) and rotated by rope (float32 [positions,
-    dim]: cos | sin) where those are given. Returns q_out."""
-    kr, vr = _rows(k, "k", cache), _rows(v, "v", cache)
+    dim]: cos | sin) where those are given. A QuantCache holds each row as codes and
+    a scale; k, v and q are of one type. Returns q_out."""
+    quant = type(cache) is QuantCache
+    kind = _row_type(k, "k") if quant else None
+    kr, vr = _rows(k, "k", cache, kind), _rows(v, "v", cache, kind)
     n = k.shape[0]
     seqs = _seqs(cache, table, lens, starts, n)[0]
     if v.shape != k.shape or k.shape[1] != cache.n_kv:
         raise EngineError("k and v are [tokens, key heads of the cache, head dim]")
     heads, qr, qo = 0, None, None
     if q is not None:
-        qr = _rows(q, "q", cache)
+        qr = _rows(q, "q", cache, kind)
         heads = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if q.shape[0] != n or q_out.shape != q.shape:
             raise EngineError("q, q_out and k are of one number of tokens")
-        qo = _rows(q_out, "q_out", cache)
+        qo = _rows(q_out, "q_out", cache, kind)
     dev, dim = cache.device, cache.head_dim
     rp, rope_rows = None, 0
     if rope is not None:
@@ -210,11 +279,34 @@ def append(cache: PagedCache, table, lens, starts, k, v, q=None, q_out=None, q_n
         if rope.requires_grad or forward_ad._current_level >= 0:
             _plain(rope, "rope")
         rp, rope_rows = rope.data_ptr(), rope.shape[0]
-    _enqueue(dev, _lib().rpg_hip_paged_append, cache._packed(), seqs, kr, vr, qr, qo, heads,
-             _vector(q_norm, "q_norm", dim, torch.float32, dev), _vector(k_norm, "k_norm", dim, torch.float32, dev), eps,
-             rp, rope_rows)
-    _written((cache._k, cache._v) if qo is None else (cache._k, cache._v, q_out))
+    rest = (kr, vr, qr, qo, heads, _vector(q_norm, "q_norm", dim, torch.float32, dev),
+            _vector(k_norm, "k_norm", dim, torch.float32, dev), eps, rp, rope_rows)
+    if quant:
+        _enqueue(dev, _lib().rpg_hip_quant_append, cache._packed(), seqs, _TYPES[kind], *rest)
+        _written(cache._held if qo is None else (*cache._held, q_out))
+    else:
+        _enqueue(dev, _lib().rpg_hip_paged_append, cache._packed(), seqs, *rest)
+        _written((cache._k, cache._v) if qo is None else (cache._k, cache._v, q_out))
     return q_out
+
+
+def read_rows(cache: QuantCache, table, lens, starts, k_out, v_out):
+    """The last positions of each sequence out of a QuantCache: those of sequence s
+    go to rows starts[s] .. starts[s + 1] of k_out and v_out [tokens, key heads, dim],
+    both of one type. Rows of no sequence are left as they are; positions whose pages
+    the table does not name read as zeros. Returns (k_out, v_out)."""
+    if type(cache) is not QuantCache:
+        raise EngineError("cache is a QuantCache")
+    kind = _row_type(k_out, "k_out")
+    kr, vr = _rows(k_out, "k_out", cache, kind), _rows(v_out, "v_out", cache, kind)
+    if v_out.shape != k_out.shape or k_out.shape[1] != cache.n_kv:
+        raise EngineError("k_out and v_out are [tokens, key heads of the cache, head dim]")
+    if starts is None:
+        raise EngineError("starts is needed")
+    seqs = _seqs(cache, table, lens, starts, k_out.shape[0])[0]
+    _enqueue(cache.device, _lib().rpg_hip_quant_read, cache._packed(), seqs, _TYPES[kind], kr, vr)
+    _written((k_out, v_out))
+    return k_out, v_out
 
 
 @functools.lru_cache(maxsize=4096)
@@ -291,3 +383,80 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
              _vector(top_p, "top_p", rows, f32, dev), _vector(min_p, "min_p", rows, f32, dev), _vector(u, "u", rows, f32, dev),
              tokens.data_ptr(), logprobs.data_ptr(), work.data_ptr(), size)
     return tokens, logprobs
+
+
+def _list(x, name, rows, dtype, device):
+    """(address, elements between rows, row length) of a [rows, n] matrix whose rows
+    are contiguous; rows may be one and the same (an expanded view)."""
+    if (x.dim() != 2 or x.dtype is not dtype or x.device != device or (rows is not None and x.shape[0] != rows)
+            or (x.shape[1] > 1 and x.stride(1) != 1) or x.stride(0) < 0):
+        raise EngineError(f"{name} is {dtype} [{'masks' if rows is None else 'rows'}, n], contiguous in the last dimension, on the logits' GPU")
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _plain(x, name)
+    return x.data_ptr(), x.stride(0), x.shape[1]
+
+
+def edit_logits(logits, history=None, history_lens=None, prompts=None, repetition=None, presence=None, frequency=None,
+                bias_ids=None, bias=None, mask=None, mask_rows=None, out=None):
+    """logits [rows, vocab] with penalties, biases and masks, into out (made when not
+    given; may be logits). In this order, where c counts how often a row's history
+    holds a token behind the row's prompt:
+
+        x = x / repetition if x > 0 else x * repetition   tokens of the history
+        x = x - frequency * c - presence                  tokens with c > 0
+        x = x + bias                                      tokens of bias_ids
+        x = -inf                                          tokens whose mask bit is 0
+
+    history int32 [rows, n], of which the first history_lens [rows] tokens are there,
+    the first prompts [rows] of those the prompt; repetition, presence and frequency
+    float32 [rows]; bias_ids int32 and bias float32 [rows, m] (numbers outside the
+    vocabulary are no entries, of several for a token the last counts); mask int32
+    [masks, ceil(vocab / 32)], token t at bit t % 32 of word t / 32; row r goes by mask
+    mask_rows[r] (int32 [rows]; r when not given), by none where that names no mask.
+    None leaves an edit out. Returns out."""
+    if (logits.dim() != 2 or logits.dtype not in _TYPES or not logits.is_cuda
+            or (logits.shape[1] > 1 and logits.stride(1) != 1)):
+        raise EngineError("logits are [rows, vocab] float32, float16 or bfloat16 on a GPU, contiguous in the last dimension")
+    if logits.requires_grad or forward_ad._current_level >= 0:
+        _plain(logits, "logits")
+    rows, vocab = logits.shape
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    elif (out.shape != logits.shape or out.dtype is not logits.dtype or out.device != dev
+          or (vocab > 1 and out.stride(1) != 1)):
+        raise EngineError("out is of the logits' shape, type and GPU, contiguous in the last dimension")
+    elif out.requires_grad or forward_ad._current_level >= 0:
+        _plain(out, "out")
+    if history is None and not (history_lens is prompts is repetition is presence is frequency is None):
+        raise EngineError("history_lens, prompts and penalties go with a history")
+    if (bias_ids is None) != (bias is None):
+        raise EngineError("bias_ids and bias go together")
+    if mask is None and mask_rows is not None:
+        raise EngineError("mask_rows goes with a mask")
+    h = b = w = m = (None, 0, 0)
+    if history is not None:
+        h = _list(history, "history", rows, i32, dev)
+    if bias is not None:
+        b, w = _list(bias_ids, "bias_ids", rows, i32, dev), _list(bias, "bias", rows, f32, dev)
+        if b[2] != w[2]:
+            raise EngineError("bias_ids and bias are of one shape")
+    masks = 0
+    if mask is not None:
+        m, masks = _list(mask, "mask", None, i32, dev), mask.shape[0]
+        if m[2] != (vocab + 31) // 32:
+            raise EngineError("mask has a bit for each token: ceil(vocab / 32) words a row")
+        if mask_rows is None and masks < rows:
+            raise EngineError("mask has a row for each row of logits, or mask_rows says which")
+    row = [_vector(x, name, rows, t, dev) or 0 for x, name, t in (
+        (history_lens, "history_lens", i32), (prompts, "prompts", i32), (repetition, "repetition", f32),
+        (presence, "presence", f32), (frequency, "frequency", f32), (mask_rows, "mask_rows", i32))]
+    if not h[2]:  # no token: no penalty
+        h, row[:5] = (0, 0, 0), [0] * 5
+    if not b[2]:
+        b = w = (0, 0, 0)
+    edits = _EDITS.pack(h[0], h[1], *row[:5], b[0], b[1], w[0], w[1], m[0] or 0, m[1], row[5], h[2], b[2], masks)
+    _enqueue(dev, _lib().rpg_hip_edit_logits, _TYPES[logits.dtype], logits.data_ptr(), rows, vocab, logits.stride(0), edits,
+             out.data_ptr(), out.stride(0))
+    _written(out)
+    return out

@@ -1,0 +1,240 @@
+"""A cache held in 8 bits (rpgbarengine_amd.serving.QuantCache): rows in and out,
+against their definitions in float64."""
+
+import math
+
+import pytest
+import torch
+
+import rpgbarengine_amd as eng
+import serving_more_plain as more
+import serving_plain as plain
+from rpgbarengine_amd import serving
+from test_gpu_serving import DTYPES, IDS, Batch, close
+
+pytestmark = pytest.mark.gpu
+
+CODES = [torch.int8, torch.float8_e4m3fn]
+NAMES = {**IDS, torch.int8: "i8", torch.float8_e4m3fn: "e4m3"}
+
+
+def ident(x):
+    return NAMES.get(x, None) if isinstance(x, torch.dtype) else None
+
+
+def empty_cache(b, codes, fill=0x33):
+    """A QuantCache over the batch's pages whose every byte is `fill`, scales 7."""
+    shape = (b.n_pages, b.kv, b.page, b.dim)
+    k, v = (torch.full(shape, fill, dtype=torch.int8, device="cuda").view(codes) for _ in "kv")
+    return serving.QuantCache(k, v, *(torch.full(shape[:3], 7.0, device="cuda") for _ in "kv"))
+
+
+def held(cache):
+    return [x.cpu() for x in (cache.k.view(torch.int8), cache.v.view(torch.int8), cache.k_scale, cache.v_scale)]
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 32, 8, 16), (128, 5, 1, 64), (64, 6, 3, 32)])
+def test_append(codes, dtype, dim, heads, kv, page):
+    b = Batch([37, 16, 1, 200, 33], [5, 16, 1, 0, 33], dtype, kv, dim, page, heads, seed=1)
+    behind = 4  # rows behind the last sequence
+    n = b.tokens + behind
+    qkv = b.normal(n, heads + 2 * kv, dim, by=3.0)
+    qn, kn = 1 + 0.2 * torch.randn(dim, generator=b.gen), 1 + 0.2 * torch.randn(dim, generator=b.gen)
+    ang = torch.rand(256, dim // 2, generator=b.gen) * 6
+    rope = torch.cat([ang.cos(), ang.sin()], 1)
+    _, table, lens, starts = b.gpu()
+    cache = empty_cache(b, codes)
+    before = held(cache)
+    x = qkv.cuda()
+    out = torch.full((n, heads, dim), 7.0, dtype=dtype, device="cuda")
+    got = serving.append(cache, table, lens, starts, x[:, heads:heads + kv], x[:, heads + kv:], q=x[:, :heads], q_out=out,
+                         q_norm=qn.cuda(), k_norm=kn.cuda(), eps=1e-5, rope=rope.cuda())
+    assert got is out
+    after = held(cache)
+    k, v = cache.k.cpu().double(), cache.v.cpu().double()
+    ks, vs = after[2].double(), after[3].double()
+    touched = torch.zeros(b.n_pages, page, dtype=torch.bool)
+    for i, (ln, m) in enumerate(zip(b.lens, b.new)):
+        for j in range(m):
+            t, pos = int(b.starts[i]) + j, ln - m + j
+            at, r = int(b.table[i, pos // page]), pos % page
+            touched[at, r] = True
+            want, mag = plain.turned(qkv[t, heads:heads + kv], kn, 1e-5, rope[pos])
+            more.check_row(k[at, :, r], ks[at, :, r], want, plain.turned_bound(torch.float32, 0 * want, mag), codes)
+            y = qkv[t, heads + kv:].double()
+            more.check_row(v[at, :, r], vs[at, :, r], y, 0 * y, codes)
+            if dtype != torch.float32:  # y M is exact, the quotient rounded once: the codes are the nearest
+                assert torch.equal(v[at, :, r], more.nearest(y * more.LARGEST[codes] / y.abs().amax(-1, keepdim=True), codes))
+            want, mag = plain.turned(qkv[t, :heads], qn, 1e-5, rope[pos])
+            close(out[t], want, plain.turned_bound(dtype, want, mag))
+    for was, now in zip(before, after):  # every other row as it was
+        assert torch.equal(now.transpose(1, 2)[~touched], was.transpose(1, 2)[~touched])
+    assert bool((out[b.tokens:] == 7).all())
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_append_odd_rows(codes, dtype):
+    """Zeros, a single value, the type's largest and smallest magnitudes, rows that are
+    not finite; signs of zero and of the largest."""
+    b = Batch([40], [12], dtype, 2, 128, 16, 4, seed=2)
+    rows = b.normal(12, 2, 128)
+    big = torch.finfo(dtype).max
+    rows[0] = 0.0
+    rows[1], rows[1, 0, 5], rows[1, 1, 7] = 0.0, -3.0, 1e-3
+    rows[2] *= big / 8
+    rows[2, :, 3] = -big
+    rows[3] = (rows[3].double() * 1e-3 * float(torch.finfo(dtype).smallest_normal)).to(dtype)
+    rows[4, 0, 9], rows[4, 1, 9] = math.inf, -math.inf
+    rows[5, 0, 0], rows[5, 1, 127] = math.nan, -math.nan
+    rows[6] = (rows[6].double() * 2.0 ** -70).to(dtype)  # f16: zeros
+    rows[7] = torch.where(rows[7] < 0, -2.5, 2.5).to(dtype)
+    rows[8] = (rows[8].double() * (2.0 ** 90 if dtype != torch.float16 else 1000)).to(dtype)
+    _, table, lens, starts = b.gpu()
+    cache = empty_cache(b, codes)
+    x = rows.cuda()
+    assert serving.append(cache, table, lens, starts, x, x) is None
+    k, v, ks, vs = cache.k.cpu().double(), cache.v.cpu().double(), cache.k_scale.cpu().double(), cache.v_scale.cpu().double()
+    assert torch.equal(k, v) or codes == torch.float8_e4m3fn
+    assert torch.equal(cache.k.view(torch.int8), cache.v.view(torch.int8))
+    assert torch.equal(ks.nan_to_num(-1.0), vs.nan_to_num(-1.0))
+    for j in range(12):
+        pos = 28 + j
+        at, r = int(b.table[0, pos // 16]), pos % 16
+        for h in range(2):
+            y = rows[j, h].double()
+            if not bool(y.isfinite().all()):
+                assert math.isnan(float(ks[at, h, r])) and bool((k[at, h, r] == 0).all())
+            elif float(y.abs().max()) < 2.0 ** -112:
+                assert float(ks[at, h, r]) == 0.0 and bool((k[at, h, r] == 0).all())
+            else:
+                more.check_row(k[at, h, r], ks[at, h, r], y, 0 * y, codes)
+    kr, vr = torch.empty_like(x), torch.empty_like(x)
+    serving.read_rows(cache, table, lens, starts, kr, vr)
+    for j in (4, 5):
+        assert bool(kr[j].isnan().all()) and bool(vr[j].isnan().all())
+    assert bool((kr[0] == 0).all()) and bool(kr[[1, 2, 6, 7, 8, 9, 10, 11]].isfinite().all())
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+def test_append_leaves_out_tokens_without_a_place(codes):
+    """More new tokens than positions, positions past the rotation table, pages
+    that the table does not name; queries in place."""
+    b = Batch([3, 40, 20], [5, 2, 20], torch.bfloat16, seed=3)
+    b.table[2, 0] = b.n_pages  # no such page
+    b.table[2, 1] = -7
+    _, table, lens, starts = b.gpu()
+    cache = empty_cache(b, codes)
+    before = held(cache)
+    k, v, q = (b.normal(b.tokens, h, 128).cuda() for h in (2, 2, 4))
+    rope = torch.ones(39, 128).cuda()
+    apart = torch.full_like(q, 9.0)
+    serving.append(cache, table, lens, starts, k, v, q=q, q_out=apart, rope=rope)
+    same = [int(b.starts[0]), int(b.starts[0]) + 1, int(b.starts[1]) + 1]  # positions -2, -1; 39
+    for t in range(b.tokens):
+        assert bool((apart[t] == 9).all()) == (t in same), t
+    want = torch.zeros(b.n_pages, 16, dtype=torch.bool)
+    for pos in range(3):
+        want[int(b.table[0, 0]), pos] = True
+    want[int(b.table[1, 2]), 38 - 32] = True
+    for was, now in zip(before, held(cache)):
+        changed = now != was
+        changed = (changed if changed.dim() == 3 else changed.any(-1)).any(1)
+        assert torch.equal(changed, want)
+    mine = q.clone()
+    assert serving.append(cache, table, lens, starts, k, v, q=mine, q_out=mine, rope=rope) is mine
+    there = [t for t in range(b.tokens) if t not in same]
+    assert torch.equal(mine[there], apart[there]) and torch.equal(mine[same], q[same])
+
+
+def random_cache(b, codes, by=1.0):
+    """Codes of any value (NaN apart) and scales over some orders of magnitude."""
+    shape = (b.n_pages, b.kv, b.page, b.dim)
+
+    def pool():
+        if codes == torch.int8:
+            return torch.randint(-127, 128, shape, generator=b.gen, dtype=torch.int8)
+        x = torch.randint(0, 254, shape, generator=b.gen)
+        return torch.where(x >= 127, x + 1, x).to(torch.uint8).view(codes)
+
+    def scales():
+        return torch.exp(torch.randn(shape[:3], generator=b.gen)) * by / more.LARGEST[codes]
+
+    return serving.QuantCache(pool().cuda(), pool().cuda(), scales().cuda(), scales().cuda())
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,kv,page", [(128, 8, 16), (128, 1, 64), (64, 3, 32)])
+def test_read(codes, dtype, dim, kv, page):
+    b = Batch([37, 16, 1, 200, 33, 3], [5, 16, 1, 0, 33, 5], dtype, kv, dim, page, kv, seed=4)
+    b.table[4, 0] = -1
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    ko, vo = (torch.full((b.tokens + 3, kv, dim), 7.0, dtype=dtype, device="cuda") for _ in "kv")
+    got = serving.read_rows(cache, table, lens, starts, ko, vo)
+    assert got[0] is ko and got[1] is vo
+    for out, pool, scale in ((ko, cache.k, cache.k_scale), (vo, cache.v, cache.v_scale)):
+        want = torch.full((b.tokens + 3, kv, dim), 7.0, dtype=torch.float64)
+        rows = more.values(pool.cpu(), scale.cpu())
+        for i, (ln, m) in enumerate(zip(b.lens, b.new)):
+            for j in range(m):
+                pos = ln - m + j
+                if pos < 0:
+                    continue
+                at = int(b.table[i, pos // page])
+                want[int(b.starts[i]) + j] = rows[at, :, pos % page] if at >= 0 else 0.0
+        # The product of a code (8 bits) and a scale (24) is exact in float64. The kernel
+        # rounds it to f32, by 2^-24 at most, and then to the type, or to the type at
+        # once (the compiler may join the two); to f32 once.
+        twice = 0.0 if dtype == torch.float32 else 2.0 ** -24
+        bound = (plain.EPS[dtype] * (1 + twice) + twice) * want.abs() + plain.TINY[dtype]
+        close(out, want, bound)
+
+
+def test_every_code_reads_as_its_value():
+    for codes in CODES:
+        b = Batch([16], [16], torch.float32, 1, 128, 16, 1, seed=5)
+        _, table, lens, starts = b.gpu()
+        every = torch.arange(256, dtype=torch.uint8).repeat(b.n_pages * 8).view(b.n_pages, 1, 16, 128)
+        k = every.view(codes).cuda()
+        one = torch.ones(b.n_pages, 1, 16, device="cuda")
+        cache = serving.QuantCache(k, k.clone(), one, one.clone())
+        for dtype in DTYPES:
+            ko, vo = (torch.empty(16, 1, 128, dtype=dtype, device="cuda") for _ in "kv")
+            serving.read_rows(cache, table, lens, starts, ko, vo)
+            want = every[int(b.table[0, 0]), 0].view(codes).float().view(16, 1, 128)
+            assert torch.equal(ko.cpu().float().nan_to_num(1e9), want.nan_to_num(1e9))
+
+
+def test_views_of_larger_pools():
+    """Pages, heads and positions at any strides of 16 bytes, rows behind one another."""
+    b = Batch([50, 20], [50, 20], torch.bfloat16, 3, 64, 16, 3, seed=6)
+    _, table, lens, starts = b.gpu()
+    pool = torch.zeros(b.n_pages, 16, 2, 3, 80, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(2, b.n_pages, 5, 16, device="cuda")
+    k, v = (pool[:, :, i, :, :64].transpose(1, 2) for i in range(2))
+    ks, vs = (scales[i, :, 1:4] for i in range(2))
+    cache = serving.QuantCache(k, v, ks, vs)
+    rows = b.normal(70, 3, 64).cuda()
+    serving.append(cache, table, lens, starts, rows, -rows)
+    flat = serving.QuantCache.zeros(b.n_pages, 16, 3, 64, torch.int8)
+    serving.append(flat, table, lens, starts, rows, -rows)
+    for x, y in ((cache.k, flat.k), (cache.v, flat.v), (cache.k_scale, flat.k_scale), (cache.v_scale, flat.v_scale)):
+        assert torch.equal(x, y)
+    assert bool((pool[..., 64:] == 0).all()) and bool((scales[:, :, [0, 4]] == 0).all())
+    ko, vo = torch.empty_like(rows), torch.empty_like(rows)
+    serving.read_rows(cache, table, lens, starts, ko, vo)
+    assert torch.equal(ko, -vo)
+
+
+def test_a_cache_whose_tensors_moved_is_refused():
+    cache = serving.QuantCache.zeros(4, 16, 2, 64)
+    b = Batch([5], [5], torch.float32, 2, 64, 16, 2)
+    _, table, lens, starts = b.gpu()
+    rows = b.normal(5, 2, 64).cuda()
+    cache.k_scale.set_(torch.zeros(4, 2, 16, device="cuda"))
+    with pytest.raises(eng.EngineError, match="lie elsewhere"):
+        serving.append(cache, table, lens, starts, rows, rows)
