@@ -352,6 +352,22 @@ RPG_HIP_API int32_t rpg_hip_quant_append(const rpg_hip_quant_cache* cache, const
 RPG_HIP_API int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
                                        const rpg_hip_rows* k, const rpg_hip_rows* v, void* stream);
 
+/* rpg_hip_paged_decode and rpg_hip_paged_prompt over such a cache, q and out rows of
+ * `type`. Scales are applied in f32 to scores and weights, codes are multiplied as
+ * they are; weights times scales go to the product in two parts of 8 bits, for f32
+ * rows in three. Queries are finite; a row whose scale is NaN makes NaN of what sees
+ * it, and of nothing else. In places that no query sees codes and scales may be
+ * anything, but for the NaN codes of e4m3 (which rpg_hip_quant_append never writes)
+ * behind a prompt's token in its own sequence. work: rpg_hip_quant_work bytes. */
+RPG_HIP_API int32_t rpg_hip_quant_decode(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                                         const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
+                                         void* work, int64_t work_bytes, void* stream);
+RPG_HIP_API int32_t rpg_hip_quant_prompt(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                                         const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale,
+                                         void* work, int64_t work_bytes, void* stream);
+RPG_HIP_API int64_t rpg_hip_quant_work(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                                       int32_t n_heads, int32_t prompt);
+
 /* Edits of logits before a draw. All device pointers; arrays of one element per
  * row unless a stride (in elements) is given.
  *

@@ -6,6 +6,7 @@
 
 #include <cstdint>
 
+#include "paged.h"
 #include "paged_dev.h"
 
 namespace rpg {
@@ -44,6 +45,73 @@ __device__ __forceinline__ uint32_t Halves2(uint32_t u) {
     const F2 x = Floats2<I8, kHigh>(u);
     return __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u);
   }
+}
+
+// eight codes as a product's operand
+template <typename C, typename T>
+__device__ __forceinline__ U4 Operand8(uint32_t x, uint32_t y) {
+  return U4{Halves2<C, T, false>(x), Halves2<C, T, true>(x), Halves2<C, T, false>(y), Halves2<C, T, true>(y)};
+}
+
+// For rows of type T: what the keys' codes are multiplied as, the parts that a query
+// takes (f32: three exact bf16 parts, Split3), and those of a weight times a
+// value's scale, in bf16: of 8 bits each, so two are as fine as an f16 output's
+// rounding, and three are all of an f32.
+template <typename T>
+struct KeyTypeOf {
+  typedef BF16 type;
+};
+template <>
+struct KeyTypeOf<F16> {
+  typedef F16 type;
+};
+template <typename T>
+using KeyType = typename KeyTypeOf<T>::type;
+template <typename T>
+constexpr int kQueryParts = kBytes<T> == 4 ? 3 : 1;
+template <typename T>
+constexpr int kWeightParts = kBytes<T> == 4 ? 3 : 2;
+
+// eight elements of a query from p on: operand i of its parts
+template <typename T, int kParts, int kQ>
+__device__ __forceinline__ void LoadQuery(const char* p, int i, U4 (&q)[kParts][kQ]) {
+  if constexpr (kBytes<T> == 4) {
+    const U4 x = Load16(p), y = Load16(p + 16);
+    Parts8 parts;
+    parts.Set(0, Split3(__uint_as_float(x[0]), __uint_as_float(x[1])));
+    parts.Set(1, Split3(__uint_as_float(x[2]), __uint_as_float(x[3])));
+    parts.Set(2, Split3(__uint_as_float(y[0]), __uint_as_float(y[1])));
+    parts.Set(3, Split3(__uint_as_float(y[2]), __uint_as_float(y[3])));
+    q[0][i] = parts.hi, q[1][i] = parts.mid, q[2][i] = parts.lo;
+  } else {
+    q[0][i] = Load16(p);
+  }
+}
+
+// Eight weights (times scales) as the parts of an operand.
+template <typename T>
+struct WeightParts {
+  U4 x[kWeightParts<T>];
+  __device__ __forceinline__ void Set(int j, float a, float b) {
+    if constexpr (kBytes<T> == 4) {
+      const Parts p = Split3(a, b);
+      x[0][j] = p.hi, x[1][j] = p.mid, x[2][j] = p.lo;
+    } else {
+      x[0][j] = Pack2<BF16>(a, b);
+      x[1][j] = Rest2<BF16>(a, b, x[0][j]);
+    }
+  }
+};
+
+// f(code, row type, dimensions) of a cache
+template <typename F>
+void ByTypes(int64_t code, const Cache& c, F&& f) {
+  ByRows(c, [&](auto type, auto dim) {
+    if (code == kI8)
+      f(I8{}, type, dim);
+    else
+      f(E4M3{}, type, dim);
+  });
 }
 
 }  // namespace paged

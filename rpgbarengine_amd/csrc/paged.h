@@ -104,8 +104,19 @@ int64_t WorkBytes(int64_t rows, int head_dim, int splits);
 // read and written 16 bytes at a time.
 __host__ __device__ inline int64_t StatFloats(int64_t rows, int splits) { return (2 * rows * splits + 3) / 4 * 4; }
 void Decode(const AttentionArgs& a, hipStream_t s);
+void DecodeJoin(const AttentionArgs& a, hipStream_t s);  // of a.splits > 1 ranges, of any cache
+
+struct CodesAttentionArgs {
+  AttentionArgs a;
+  Scales scales;
+  int64_t code = kI8;
+};
+void DecodeCodes(const CodesAttentionArgs& a, hipStream_t s);
+int CodesPromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity);
+void PromptCodes(const CodesAttentionArgs& a, hipStream_t s);
 
 void Prompt(const AttentionArgs& a, hipStream_t s);
+void PromptJoin(const AttentionArgs& a, hipStream_t s);  // of a.splits > 1 ranges of tiles of 32 rows
 
 }  // namespace paged
 }  // namespace rpg

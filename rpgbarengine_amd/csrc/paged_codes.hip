@@ -281,29 +281,6 @@ void LaunchRead(const CodesReadArgs& a, hipStream_t s) {
   HIP_CHECK(hipGetLastError());
 }
 
-// f(code, row type, dimensions) of a cache
-template <typename F>
-void ByTypes(int64_t code, const Cache& c, F&& f) {
-  auto by_dim = [&](auto code_type, auto type) {
-    if (c.head_dim == 128)
-      f(code_type, type, std::integral_constant<int, 128>{});
-    else
-      f(code_type, type, std::integral_constant<int, 64>{});
-  };
-  auto by_type = [&](auto code_type) {
-    if (c.type == kF32)
-      by_dim(code_type, F32{});
-    else if (c.type == kF16)
-      by_dim(code_type, F16{});
-    else
-      by_dim(code_type, BF16{});
-  };
-  if (code == kI8)
-    by_type(I8{});
-  else
-    by_type(E4M3{});
-}
-
 }  // namespace
 
 void AppendCodes(const CodesAppendArgs& a, hipStream_t s) {

@@ -4,7 +4,9 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
+#include "common.h"
 #include "lanes.h"
 #include "paged.h"
 
@@ -292,6 +294,23 @@ __device__ __forceinline__ void JoinRow(const AttentionArgs& a, int64_t rows, in
 #pragma unroll
   for (int p = 1; p < kParts; ++p) o += *reinterpret_cast<const F4*>(&so[p][d]);
   Store4<T>(out + d * kBytes<T>, o * Inverse(top, l));
+}
+
+// f(row type, dimensions) of a cache
+template <typename F>
+void ByRows(const Cache& c, F&& f) {
+  auto by_dim = [&](auto type) {
+    if (c.head_dim == 128)
+      f(type, std::integral_constant<int, 128>{});
+    else
+      f(type, std::integral_constant<int, 64>{});
+  };
+  if (c.type == kF32)
+    by_dim(F32{});
+  else if (c.type == kF16)
+    by_dim(F16{});
+  else
+    by_dim(BF16{});
 }
 
 }  // namespace paged

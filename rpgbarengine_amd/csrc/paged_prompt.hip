@@ -39,6 +39,7 @@
 #include "lanes.h"
 #include "paged.h"
 #include "paged_dev.h"
+#include "row_tile.h"
 
 namespace rpg {
 namespace paged {
@@ -155,26 +156,6 @@ __device__ __forceinline__ void LdsDma(U4 src, char* to, int voff, int soff) {
                :
                : "s"(at), "v"(voff), "s"(src), "s"(soff)
                : "m0");
-}
-
-// A row tile: its sequence and rows, and the positions it stands for.
-struct RowTile {
-  int first, row0, n_rows, len, pos0;  // first: the sequence's first token; row0: of the sequence's n_rows
-  __device__ __forceinline__ int Position(int row, int group) const { return pos0 + min(row, n_rows - 1) / group; }
-};
-// Row tile `tile`: those of sequence s start at floor(starts[s] G / rows) + s,
-// which leaves each its ceil(n_new G / rows) tiles wherever the starts lie. False:
-// there is no such tile.
-__device__ __forceinline__ bool TileOf(const Seqs& s, int group, int rows, int tile, int* seq, RowTile* t) {
-  Sequence x;
-  if (!FindSequence(s, [&](int end, int j) { return end * group / rows + j + 1 <= tile; }, &x)) return false;
-  *seq = x.seq;
-  t->first = x.first;
-  t->n_rows = x.n_new * group;
-  t->row0 = (tile - (x.first * group / rows + x.seq)) * rows;
-  t->len = x.len;
-  t->pos0 = x.len - x.n_new;
-  return t->row0 >= 0 && t->row0 < t->n_rows;
 }
 
 // grid (row tile x key head, key range): key heads next to each other, the tiles
@@ -671,7 +652,6 @@ __global__ __launch_bounds__(256) void PromptJoinKernel(AttentionArgs a) {
                    a.out.p + token * a.out.token_bytes + head * a.out.head_bytes);
 }
 
-int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups);
 int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity);
 
 // Key ranges where not even half the compute units have a workgroup (12 tokens
@@ -690,18 +670,20 @@ int RangesFor(int64_t wgs, int bytes, int64_t capacity) {
 
 template <typename T, int kDim, int kGroups, bool kShared = false>
 void LaunchGroups(const AttentionArgs& a, hipStream_t s) {
-  const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, kGroups);
+  const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, 128 / std::min(kGroups, 4));
   RPG_CHECK(tiles * a.c.n_kv <= kMaxGroups &&
                 (a.splits == 1 || static_cast<int64_t>(a.s.n_tokens) * a.n_heads <= kMaxGroups),
             "%d x %d query rows in one launch", a.s.n_tokens, a.n_heads);
   PromptKernel<T, kDim, kGroups, kShared>
       <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 64 * Shape<T, kDim, kGroups>::kWaves, 0, s>>>(a);
   HIP_CHECK(hipGetLastError());
-  if constexpr (kGroups >= 4) {
-    if (a.splits == 1) return;
-    PromptJoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_tokens) * a.n_heads, 256, 0, s>>>(a);
-    HIP_CHECK(hipGetLastError());
-  }
+  if (a.splits > 1) PromptJoin(a, s);
+}
+
+template <typename T, int kDim>
+void LaunchJoin(const AttentionArgs& a, hipStream_t s) {
+  PromptJoinKernel<T, kDim><<<static_cast<uint32_t>(a.s.n_tokens) * a.n_heads, 256, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
 }
 
 // f32 rows of 128: K and V share a place above this many workgroups, one for each
@@ -718,24 +700,12 @@ void Launch(const AttentionArgs& a, hipStream_t s) {
     if (groups == 8) return LaunchGroups<T, kDim, 8>(a, s);
   }
   if constexpr (kBytes<T> == 4 && kDim == 128) {
-    const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, 4);
+    const int64_t tiles = TilesFor(a.s.n_tokens, a.s.n_seqs, a.n_heads / a.c.n_kv, 32);
     if (groups == 4 && tiles * a.c.n_kv * a.splits > kCrowd) return LaunchGroups<T, kDim, 4, true>(a, s);
   }
   if (groups == 4) return LaunchGroups<T, kDim, 4>(a, s);
   if (groups == 2) return LaunchGroups<T, kDim, 2>(a, s);
   LaunchGroups<T, kDim, 1>(a, s);
-}
-
-template <typename T>
-void LaunchDim(const AttentionArgs& a, hipStream_t s) {
-  if (a.c.head_dim == 128)
-    Launch<T, 128>(a, s);
-  else
-    Launch<T, 64>(a, s);
-}
-
-int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
-  return n_tokens * group / (128 / std::min(groups, 4)) + n_seqs;
 }
 
 // Groups of a workgroup (its rows: 128 / groups, 32 at the least): one where that
@@ -749,9 +719,9 @@ int64_t TilesFor(int64_t n_tokens, int64_t n_seqs, int group, int groups) {
 constexpr int64_t kUnits = 256;  // compute units
 int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
   const int group = n_heads / n_kv;
-  if (TilesFor(n_tokens, n_seqs, group, 1) * n_kv >= 384) return 1;
-  if (TilesFor(n_tokens, n_seqs, group, 2) * n_kv >= 384) return 2;
-  const int64_t wgs = TilesFor(n_tokens, n_seqs, group, 4) * n_kv;
+  if (TilesFor(n_tokens, n_seqs, group, 128) * n_kv >= 384) return 1;
+  if (TilesFor(n_tokens, n_seqs, group, 64) * n_kv >= 384) return 2;
+  const int64_t wgs = TilesFor(n_tokens, n_seqs, group, 32) * n_kv;
   return bytes == 2 && wgs <= kUnits && capacity > 512 && RangesFor(wgs, bytes, capacity) == 1 ? 8 : 4;
 }
 
@@ -759,17 +729,16 @@ int GroupsFor(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes
 
 int PromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int bytes, int64_t capacity) {
   if (GroupsFor(n_tokens, n_seqs, n_heads, n_kv, bytes, capacity) != 4) return 1;
-  return RangesFor(TilesFor(n_tokens, n_seqs, n_heads / n_kv, 4) * n_kv, bytes, capacity);
+  return RangesFor(TilesFor(n_tokens, n_seqs, n_heads / n_kv, 32) * n_kv, bytes, capacity);
 }
 
 void Prompt(const AttentionArgs& a, hipStream_t s) {
   if (a.s.n_tokens == 0 || a.s.n_seqs == 0) return;
-  if (a.c.type == kF32)
-    LaunchDim<F32>(a, s);
-  else if (a.c.type == kF16)
-    LaunchDim<F16>(a, s);
-  else
-    LaunchDim<BF16>(a, s);
+  ByRows(a.c, [&](auto type, auto dim) { Launch<decltype(type), decltype(dim)::value>(a, s); });
+}
+
+void PromptJoin(const AttentionArgs& a, hipStream_t s) {
+  ByRows(a.c, [&](auto type, auto dim) { LaunchJoin<decltype(type), decltype(dim)::value>(a, s); });
 }
 
 }  // namespace paged

@@ -189,8 +189,10 @@ void CheckHeads(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads) {
             "%d x %d query rows", std::max(s.n_tokens, s.n_seqs), n_heads);
 }
 
-int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
+int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt, bool codes) {
   const int bytes = ElementBytes(static_cast<int32_t>(c.type));
+  if (codes && prompt) return paged::CodesPromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, s.capacity);
+  if (codes) return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, 2, s.capacity);
   if (prompt) return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
   return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
 }
@@ -198,10 +200,35 @@ int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool pr
 // Calls without sequences or new tokens have nothing to do.
 bool Empty(const paged::Seqs& s, bool packed) { return s.n_seqs == 0 || (packed && s.n_tokens == 0); }
 
-int64_t AttentionWork(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt) {
+int64_t AttentionWork(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt, bool codes) {
   if (Empty(s, prompt)) return 0;
   const int64_t rows = static_cast<int64_t>(prompt ? s.n_tokens : s.n_seqs) * n_heads;
-  return paged::WorkBytes(rows, c.head_dim, Splits(c, s, n_heads, prompt));
+  return paged::WorkBytes(rows, c.head_dim, Splits(c, s, n_heads, prompt, codes));
+}
+
+void CheckWork(void* work, int64_t work_bytes, int64_t need) {
+  if (need == 0) return;
+  CheckPointer("work", work, 16);
+  RPG_CHECK(work_bytes >= need, "%lld bytes of work memory, %lld are needed", (long long)work_bytes, (long long)need);
+}
+
+// Queries and outputs of a call on a.c and a.s, one for each of n_tokens.
+void AttentionRows(paged::AttentionArgs* to, const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_tokens,
+                   int32_t n_heads, float scale) {
+  paged::AttentionArgs& a = *to;
+  CheckHeads(a.c, a.s, n_heads);
+  a.q = RowsOf("q", q, a.c, n_tokens, n_heads, false);
+  a.out = RowsOf("out", out, a.c, n_tokens, n_heads, true);
+  CheckInPlace("out is q", a.out, a.q, n_tokens, n_heads);
+  RPG_CHECK(scale > 0.0f && std::isfinite(scale), "scale %g is not positive and finite", scale);
+  a.n_heads = n_heads;
+  a.scale = scale;
+}
+
+void AttentionParts(paged::AttentionArgs* a, bool prompt, bool codes, void* work, int64_t work_bytes) {
+  a->splits = Splits(a->c, a->s, a->n_heads, prompt, codes);
+  CheckWork(work, work_bytes, AttentionWork(a->c, a->s, a->n_heads, prompt, codes));
+  a->work = static_cast<float*>(work);
 }
 
 int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs, const rpg_hip_rows* q,
@@ -211,26 +238,29 @@ int32_t Attention(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seq
   a.c = CacheOf(cache);
   a.s = SeqsOf(seqs, cache->page_size, prompt);
   if (Empty(a.s, prompt)) return 0;
-  CheckHeads(a.c, a.s, n_heads);
-  const int n_tokens = prompt ? a.s.n_tokens : a.s.n_seqs;
-  a.q = RowsOf("q", q, a.c, n_tokens, n_heads, false);
-  a.out = RowsOf("out", out, a.c, n_tokens, n_heads, true);
-  CheckInPlace("out is q", a.out, a.q, n_tokens, n_heads);
-  RPG_CHECK(scale > 0.0f && std::isfinite(scale), "scale %g is not positive and finite", scale);
-  a.n_heads = n_heads;
-  a.scale = scale;
-  a.splits = Splits(a.c, a.s, n_heads, prompt);
-  const int64_t need = AttentionWork(a.c, a.s, n_heads, prompt);
-  if (need > 0) {
-    CheckPointer("work", work, 16);
-    RPG_CHECK(work_bytes >= need, "%lld bytes of work memory, %lld are needed", (long long)work_bytes,
-              (long long)need);
-  }
-  a.work = static_cast<float*>(work);
+  AttentionRows(&a, q, out, prompt ? a.s.n_tokens : a.s.n_seqs, n_heads, scale);
+  AttentionParts(&a, prompt, false, work, work_bytes);
   if (prompt)
     paged::Prompt(a, static_cast<hipStream_t>(stream));
   else
     paged::Decode(a, static_cast<hipStream_t>(stream));
+  return 0;
+}
+
+int32_t QuantAttention(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                       const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale, void* work,
+                       int64_t work_bytes, void* stream, bool prompt) {
+  paged::CodesAttentionArgs a;
+  a.a.c = QuantOf(cache, type, &a.scales);
+  a.code = cache->code;
+  a.a.s = SeqsOf(seqs, cache->page_size, prompt);
+  if (Empty(a.a.s, prompt)) return 0;
+  AttentionRows(&a.a, q, out, prompt ? a.a.s.n_tokens : a.a.s.n_seqs, n_heads, scale);
+  AttentionParts(&a.a, prompt, true, work, work_bytes);
+  if (prompt)
+    paged::PromptCodes(a, static_cast<hipStream_t>(stream));
+  else
+    paged::DecodeCodes(a, static_cast<hipStream_t>(stream));
   return 0;
 }
 
@@ -311,7 +341,7 @@ int64_t rpg_hip_paged_work(const rpg_hip_paged_cache* cache, const rpg_hip_seque
         const paged::Cache c = CacheSizes(cache);
         const paged::Seqs s = SeqSizes(seqs, cache->page_size);
         CheckHeads(c, s, n_heads);
-        return AttentionWork(c, s, n_heads, prompt != 0);
+        return AttentionWork(c, s, n_heads, prompt != 0, false);
       },
       -1);
 }
@@ -401,6 +431,33 @@ int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const rpg_hip_seque
         a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, true);
         paged::ReadCodes(a, static_cast<hipStream_t>(stream));
         return 0;
+      },
+      -1);
+}
+
+int32_t rpg_hip_quant_decode(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                             const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale, void* work,
+                             int64_t work_bytes, void* stream) {
+  return Guard(
+      [&] { return QuantAttention(cache, seqs, type, q, out, n_heads, scale, work, work_bytes, stream, false); }, -1);
+}
+
+int32_t rpg_hip_quant_prompt(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                             const rpg_hip_rows* q, const rpg_hip_rows* out, int32_t n_heads, float scale, void* work,
+                             int64_t work_bytes, void* stream) {
+  return Guard(
+      [&] { return QuantAttention(cache, seqs, type, q, out, n_heads, scale, work, work_bytes, stream, true); }, -1);
+}
+
+int64_t rpg_hip_quant_work(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
+                           int32_t n_heads, int32_t prompt) {
+  return Guard(
+      [&]() -> int64_t {
+        paged::Scales scales;
+        const paged::Cache c = QuantSizes(cache, type, &scales);
+        const paged::Seqs s = SeqSizes(seqs, cache->page_size);
+        CheckHeads(c, s, n_heads);
+        return AttentionWork(c, s, n_heads, prompt != 0, true);
       },
       -1);
 }

@@ -50,6 +50,9 @@ _SIGS = {
     "rpg_hip_paged_work": ([_P, _P, _I32, _I32], _I64),
     "rpg_hip_quant_append": ([_P, _P, _I32, _P, _P, _P, _P, _I32, _P, _P, _F, _P, _I64, _P], _I32),
     "rpg_hip_quant_read": ([_P, _P, _I32, _P, _P, _P], _I32),
+    "rpg_hip_quant_decode": ([_P, _P, _I32, _P, _P, _I32, _F, _P, _I64, _P], _I32),
+    "rpg_hip_quant_prompt": ([_P, _P, _I32, _P, _P, _I32, _F, _P, _I64, _P], _I32),
+    "rpg_hip_quant_work": ([_P, _P, _I32, _I32, _I32], _I64),
     "rpg_hip_edit_logits": ([_I32, _P, _I64, _I64, _I64, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows": ([_I32, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows_work": ([_I64, _I64], _I64),
@@ -317,42 +320,57 @@ def _work_bytes(n_kv, page_size, head_dim, kind, pages, n_seqs, n_tokens, heads,
     return _ok(_lib().rpg_hip_paged_work(c, _SEQS.pack(0, pages, 0, 0, pages, n_seqs, n_tokens), heads, prompt))
 
 
-def _attention(f, q, qr, cache, seqs, n_seqs, pages, n_tokens, scale, out, prompt):
+@functools.lru_cache(maxsize=4096)
+def _quant_work_bytes(n_kv, page_size, head_dim, kind, pages, n_seqs, n_tokens, heads, prompt):
+    """rpg_hip_quant_work of these sizes."""
+    wide = page_size * head_dim
+    c = _QUANT.pack(0, 0, 0, 0, n_kv * wide, wide, head_dim, n_kv * page_size, page_size, 1, page_size, n_kv, head_dim, 0)
+    return _ok(_lib().rpg_hip_quant_work(c, _SEQS.pack(0, pages, 0, 0, pages, n_seqs, n_tokens), kind, heads, prompt))
+
+
+def _attention(q, cache, table, lens, starts, scale, out, prompt):
+    quant = type(cache) is QuantCache
+    kind = _row_type(q, "q") if quant else None
+    qr = _rows(q, "q", cache, kind)
+    n_tokens = q.shape[0] if prompt else 0
+    seqs, n_seqs, pages = _seqs(cache, table, lens, starts, n_tokens)
+    if not prompt and q.shape[0] != n_seqs:
+        raise EngineError("q has a row for each sequence")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
         raise EngineError("out has the shape of q")
     heads, dim = q.shape[1], cache.head_dim
-    size = _work_bytes(cache.n_kv, cache.page_size, dim, _TYPES[cache.dtype], pages, n_seqs, n_tokens, heads, prompt)
+    size = (_quant_work_bytes if quant else _work_bytes)(
+        cache.n_kv, cache.page_size, dim, _TYPES[q.dtype], pages, n_seqs, n_tokens, heads, prompt)
     work = torch.empty(size, dtype=torch.uint8, device=cache.device) if size else None
-    _enqueue(cache.device, f, cache._packed(), seqs, qr, _rows(out, "out", cache), heads, dim ** -0.5 if scale is None else scale,
-             work.data_ptr() if size else None, size)
+    rest = (qr, _rows(out, "out", cache, kind), heads, dim ** -0.5 if scale is None else scale,
+            work.data_ptr() if size else None, size)
+    if quant:
+        f = _lib().rpg_hip_quant_prompt if prompt else _lib().rpg_hip_quant_decode
+        _enqueue(cache.device, f, cache._packed(), seqs, _TYPES[kind], *rest)
+    else:
+        f = _lib().rpg_hip_paged_prompt if prompt else _lib().rpg_hip_paged_decode
+        _enqueue(cache.device, f, cache._packed(), seqs, *rest)
     _written(out)
     return out
 
 
-def decode_attention(q, cache: PagedCache, table, lens, scale=None, out=None):
+def decode_attention(q, cache, table, lens, scale=None, out=None):
     """Attention of one token per sequence, q [sequences, heads, dim], over all of
     its sequence's positions. scale: 1 / sqrt(dim) when not given. out (may be q)
     is made when not given."""
-    qr = _rows(q, "q", cache)
-    seqs, n, pages = _seqs(cache, table, lens, None, 0)
-    if q.shape[0] != n:
-        raise EngineError("q has a row for each sequence")
-    return _attention(_lib().rpg_hip_paged_decode, q, qr, cache, seqs, n, pages, 0, scale, out, 0)
+    return _attention(q, cache, table, lens, None, scale, out, 0)
 
 
-def prompt_attention(q, cache: PagedCache, table, lens, starts, scale=None, out=None):
+def prompt_attention(q, cache, table, lens, starts, scale=None, out=None):
     """Causal attention of the packed new tokens, q [tokens, heads, dim]: the token
     at position p of its sequence over positions 0 .. p, whose keys and values
     lie in the cache (the new tokens' own too). out (may be q) is made when not
     given; rows of no sequence are not written."""
-    qr = _rows(q, "q", cache)
-    tokens = q.shape[0]
     if starts is None:
         raise EngineError("starts is needed")
-    seqs, n, pages = _seqs(cache, table, lens, starts, tokens)
-    return _attention(_lib().rpg_hip_paged_prompt, q, qr, cache, seqs, n, pages, tokens, scale, out, 1)
+    return _attention(q, cache, table, lens, starts, scale, out, 1)
 
 
 @functools.lru_cache(maxsize=4096)

@@ -238,3 +238,228 @@ def test_a_cache_whose_tensors_moved_is_refused():
     cache.k_scale.set_(torch.zeros(4, 2, 16, device="cuda"))
     with pytest.raises(eng.EngineError, match="lie elsewhere"):
         serving.append(cache, table, lens, starts, rows, rows)
+
+
+# ---- attention
+
+
+def attention(q, k, v, ks, vs, seen, scale, dtype, weight_bits):
+    """q [heads, dim] over codes k, v [kv, n, dim] with scales ks, vs [kv, n], where
+    seen [n]: (out, bound), float64. weight_bits: of a weight times its scale in the
+    second product."""
+    heads, dim = q.shape
+    group = heads // k.shape[0]
+    out, bound = torch.zeros(heads, dim, dtype=torch.float64), torch.zeros(heads, dim, dtype=torch.float64)
+    if not bool(seen.any()):
+        return out, bound
+    for h in range(heads):
+        kv = h // group
+        kk, vv = k[kv][seen].double(), v[kv][seen].double()
+        ss, tt = ks[kv][seen].double(), vs[kv][seen].double()
+        qq = q[h].double()
+        s = (kk @ qq) * ss * scale
+        p = torch.softmax(s, 0)
+        out[h] = ((p * tt)[:, None] * vv).sum(0)
+        mass = ((p * tt)[:, None] * vv.abs()).sum(0)
+        # A score: dim products in fp32, added in any order (three parts of an f32
+        # query are exact), two products with scales, the difference from the maximum;
+        # 2^x; the weight's product with its scale; sums over the keys and the ranges'
+        # joins; the weight's rounding.
+        ds = float(((kk.abs() @ qq.abs()) * ss).max()) * scale * (3 * dim + 6) * 2.0 ** -24 + float(s.abs().max()) * 2.0 ** -21
+        rel = math.expm1(2 * ds) + (3 * len(s) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
+        bound[h] = rel * mass + 2.0 ** -140 * len(s) * 448
+    return out, bound + plain.EPS[dtype] * (out.abs() + bound) + plain.TINY[dtype]
+
+
+def rows_of(pool, b, i, n):
+    return plain.sequence_rows(pool, b.table[i], n)
+
+
+def scales_of(pool, b, i, n):
+    rows, there = plain.sequence_rows(pool[..., None], b.table[i], n)
+    return rows[..., 0], there
+
+
+def on_cpu(cache):
+    return cache.k.cpu().float(), cache.v.cpu().float(), cache.k_scale.cpu(), cache.v_scale.cpu()
+
+
+def expect(b, cache, q, scale, i, pos, row):
+    """(out, bound) of the token at position pos of sequence i, row `row` of q."""
+    k, v, ks, vs = cache
+    n = b.lens[i]
+    kk, there = rows_of(k, b, i, n)
+    seen = there & (torch.arange(n) <= pos)
+    return attention(q[row], kk, rows_of(v, b, i, n)[0], scales_of(ks, b, i, n)[0], scales_of(vs, b, i, n)[0], seen, scale,
+                     b.dtype, 24 if b.dtype == torch.float32 else 16)
+
+
+LENS = [1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 300, 0]
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 8, 2, 16), (128, 3, 3, 64), (64, 40, 2, 32), (64, 8, 1, 16),
+                                               (128, 17, 1, 256)])
+def test_decode(codes, dtype, dim, heads, kv, page):
+    b = Batch(LENS, [1] * len(LENS), dtype, kv, dim, page, heads, seed=7)
+    q = b.normal(len(LENS), heads, dim, by=0.3)
+    _, table, lens, _ = b.gpu()
+    cache = random_cache(b, codes)
+    out = torch.full((len(LENS), heads, dim), 5.0, dtype=dtype, device="cuda")
+    assert serving.decode_attention(q.cuda(), cache, table, lens, scale=0.11, out=out) is out
+    held_ = on_cpu(cache)
+    for i, n in enumerate(LENS):
+        close(out[i], *expect(b, held_, q, 0.11, i, n - 1, i))
+    assert torch.equal(serving.decode_attention(q.cuda(), cache, table, lens, scale=0.11), out)  # the same bits
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_decode_long_and_split(codes, dtype):
+    """Many ranges joined; lengths next to a range's border in a table that has room
+    for more; peaked scores (the maximum moves from range to range)."""
+    b = Batch([3001, 1, 640, 513, 2049], [1] * 5, dtype, 1, 64, 16, 2, seed=8, extra_pages=70)
+    q = b.normal(5, 2, 64, by=0.4)
+    _, table, lens, _ = b.gpu()
+    cache = random_cache(b, codes)
+    cache.k_scale[int(b.table[0, 100]), 0, 3] *= 6
+    got = serving.decode_attention(q.cuda(), cache, table, lens)
+    held_ = on_cpu(cache)
+    for i, n in enumerate(b.lens):
+        close(got[i], *expect(b, held_, q, 64 ** -0.5, i, n - 1, i))
+
+
+def spoil(b, cache, used, odd_scale):
+    """Every place that no position uses: NaN codes, scales of odd_scale."""
+    hold = (~used)[:, None, :].expand(-1, b.kv, -1).cuda()
+    for x in (cache.k, cache.v):
+        bits = x.view(torch.uint8)
+        bits[hold] = 0x7F if x.dtype == torch.float8_e4m3fn else 0x80
+    for x in (cache.k_scale, cache.v_scale):
+        x[hold] = odd_scale
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("prompt", [0, 1], ids=["decode", "prompt"])
+def test_masked_places_hold_anything(codes, dtype, value, prompt):
+    """Rows past the length, spare pages and pages that the table names no more."""
+    new = [3, 40, 1, 2] if prompt else [1] * 4
+    b = Batch([37, 130, 16, 700], new, dtype, 2, 128, 16, 8, seed=9)
+    used = torch.zeros(b.n_pages, 16, dtype=torch.bool)
+    b.table[1, 3] = -1
+    b.table[3, 20] = b.n_pages + 5
+    b.table[2, 0] = 1 << 30  # the whole of a sequence
+    for i, n in enumerate(b.lens):
+        for p in range(n):
+            at = int(b.table[i, p // 16])
+            if 0 <= at < b.n_pages:
+                used[at, p % 16] = True
+    q = b.normal(b.tokens, 8, 128, by=0.3)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    held_ = on_cpu(cache)
+    spoil(b, cache, used, value)
+    if prompt:
+        got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
+    else:
+        got = serving.decode_attention(q.cuda(), cache, table, lens)
+    for i, n in enumerate(b.lens):
+        for j in range(b.new[i]):
+            row = int(b.starts[i]) + j
+            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row))
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_a_row_that_was_not_finite(codes, dtype):
+    """NaN for the tokens that see it, nothing for those before it and for other
+    sequences; keys' and values' rows."""
+    for name in ("k_scale", "v_scale"):
+        b = Batch([90, 50], [60, 50], dtype, 2, 64, 16, 4, seed=10)
+        q = b.normal(b.tokens, 4, 64, by=0.3)
+        _, table, lens, starts = b.gpu()
+        cache = random_cache(b, codes)
+        held_ = on_cpu(cache)
+        getattr(cache, name)[int(b.table[0, 70 // 16]), 1, 70 % 16] = math.nan
+        got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
+        one = serving.decode_attention(q[[59, 109]].cuda(), cache, table, lens)
+        for i in range(2):
+            for j in range(b.new[i]):
+                row, pos = int(b.starts[i]) + j, b.lens[i] - b.new[i] + j
+                hit = i == 0 and pos >= 70
+                want, bound = expect(b, held_, q, 64 ** -0.5, i, pos, row)
+                heads = slice(0, 2) if hit else slice(0, 4)
+                close(got[row, heads], want[heads], bound[heads])
+                assert not hit or bool(got[row, 2:].isnan().all())
+        assert bool(one[0, 2:].isnan().all()) and bool(one[0, :2].isfinite().all()) and bool(one[1].isfinite().all())
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("power", [-100, -60, 60, 90])
+def test_scales_of_any_size(codes, dtype, power):
+    """Values' scales far from 1, where an f16 product's operands would not hold them."""
+    if dtype == torch.float16:
+        power //= 10
+    b = Batch([33, 200], [1, 1], dtype, 2, 128, 16, 4, seed=11)
+    q = b.normal(2, 4, 128, by=0.3)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    cache.v_scale.mul_(2.0 ** power)
+    held_ = on_cpu(cache)
+    for got in (serving.decode_attention(q.cuda(), cache, table, lens),
+                serving.prompt_attention(q.cuda(), cache, table, lens, starts)):
+        for i, n in enumerate(b.lens):
+            close(got[i], *expect(b, held_, q, 128 ** -0.5, i, n - 1, i))
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 3, 3, 64), (64, 34, 2, 16)])
+def test_prompt(codes, dtype, dim, heads, kv, page):
+    lens, new = [70, 33, 1, 5, 130, 64, 0, 100], [70, 3, 1, 0, 40, 64, 0, 1]
+    b = Batch(lens, new, dtype, kv, dim, page, heads, seed=12)
+    q = b.normal(b.tokens + 3, heads, dim, by=0.3)
+    _, table, lens_d, starts = b.gpu()
+    cache = random_cache(b, codes)
+    out = torch.full((b.tokens + 3, heads, dim), 5.0, dtype=dtype, device="cuda")
+    assert serving.prompt_attention(q.cuda(), cache, table, lens_d, starts, scale=0.1, out=out) is out
+    held_ = on_cpu(cache)
+    for i, n in enumerate(b.lens):
+        for j in range(b.new[i]):
+            row = int(b.starts[i]) + j
+            close(out[row], *expect(b, held_, q, 0.1, i, n - b.new[i] + j, row))
+    assert bool((out[b.tokens:] == 5).all())  # rows behind the last sequence
+    again = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts, scale=0.1)
+    assert torch.equal(again[:b.tokens], out[:b.tokens])
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_prompt_behind_a_long_history(codes, dtype):
+    b = Batch([900, 1500, 333], [7, 1, 20], dtype, 1, 128, 64, 2, seed=13)
+    q = b.normal(b.tokens, 2, 128, by=0.3)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    cache.k_scale[int(b.table[0, 5]), 0, 3] *= 5  # the maximum moves
+    got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
+    held_ = on_cpu(cache)
+    for i, n in enumerate(b.lens):
+        for j in range(b.new[i]):
+            row = int(b.starts[i]) + j
+            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row))
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_more_new_tokens_than_positions(codes, dtype):
+    """Tokens at positions below 0 see nothing: zeros."""
+    b = Batch([3, 20], [8, 20], dtype, 2, 64, 16, 4, seed=14)
+    q = b.normal(b.tokens, 4, 64)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
+    assert bool((got[:5] == 0).all()) and bool((got[5:] != 0).any(-1).all())
