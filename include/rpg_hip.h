@@ -368,6 +368,34 @@ RPG_HIP_API int32_t rpg_hip_quant_prompt(const rpg_hip_quant_cache* cache, const
 RPG_HIP_API int64_t rpg_hip_quant_work(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
                                        int32_t n_heads, int32_t prompt);
 
+/* Groups of sequences whose first positions lie in the same pages (a prompt that
+ * many sessions share): group g is sequences starts[g] .. starts[g + 1] (n_groups + 1
+ * starts, not decreasing), and the tables of those of them that have positions name
+ * the same pages for the first shared[g] positions. A sequence may belong to no group.
+ * Where tables differ there, it is not defined whose pages are read for which
+ * sequence of the group. */
+typedef struct {
+  const int32_t* starts;
+  const int32_t* shared;
+  int32_t n_groups;
+} rpg_hip_groups;
+
+/* rpg_hip_paged_decode (rpg_hip_quant_decode) that reads what a group has in common
+ * once. For 16-bit rows the weights are rounded over a group's common positions as
+ * rpg_hip_paged_prompt has them. Group starts and shared positions are read on the
+ * device. work: rpg_hip_paged_shared_work (rpg_hip_quant_shared_work) bytes. */
+RPG_HIP_API int32_t rpg_hip_paged_shared(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                         const rpg_hip_groups* groups, const rpg_hip_rows* q, const rpg_hip_rows* out,
+                                         int32_t n_heads, float scale, void* work, int64_t work_bytes, void* stream);
+RPG_HIP_API int64_t rpg_hip_paged_shared_work(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                                              int32_t n_groups, int32_t n_heads);
+RPG_HIP_API int32_t rpg_hip_quant_shared(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs,
+                                         const rpg_hip_groups* groups, int32_t type, const rpg_hip_rows* q,
+                                         const rpg_hip_rows* out, int32_t n_heads, float scale, void* work,
+                                         int64_t work_bytes, void* stream);
+RPG_HIP_API int64_t rpg_hip_quant_shared_work(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs,
+                                              int32_t n_groups, int32_t type, int32_t n_heads);
+
 /* Edits of logits before a draw. All device pointers; arrays of one element per
  * row unless a stride (in elements) is given.
  *

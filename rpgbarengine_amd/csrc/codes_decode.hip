@@ -18,6 +18,7 @@
 #include "codes_dev.h"
 #include "common.h"
 #include "decode_body.h"
+#include "groups.h"
 #include "paged.h"
 #include "paged_dev.h"
 
@@ -193,6 +194,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void CodesDecodeKernel(CodesAttenti
   DecodeCodeRows<C, T, kDim>(a, at, range);
 }
 
+// The positions of a sequence behind those that its group has in common.
+template <typename C, typename T, int kDim>
+__global__ __launch_bounds__(64 * kWaves, 2) void CodesOwnKernel(CodesSharedArgs a) {
+  const DecodePlace at = PlaceOf(a.c.a);
+  DecodeRange range;
+  if (!OwnRange(a.c.a, a.groups, static_cast<int>(a.prefix_splits), at.seq, 0.0f, &range)) return;
+  DecodeCodeRows<C, T, kDim>(a.c, at, range);
+}
+
+template <typename C, typename T, int kDim>
+void LaunchOwn(const CodesSharedArgs& args, hipStream_t s) {
+  const AttentionArgs& a = args.c.a;
+  const int64_t x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(a.n_heads / a.c.n_kv, kCols);
+  RPG_CHECK(static_cast<int64_t>(a.s.n_seqs) * a.n_heads <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs,
+            a.n_heads);
+  CodesOwnKernel<C, T, kDim>
+      <<<dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(a.splits - args.prefix_splits)), 64 * kWaves, 0, s>>>(args);
+  HIP_CHECK(hipGetLastError());
+}
+
 template <typename C, typename T, int kDim>
 void Launch(const CodesAttentionArgs& args, hipStream_t s) {
   const AttentionArgs& a = args.a;
@@ -212,6 +233,19 @@ void DecodeCodes(const CodesAttentionArgs& a, hipStream_t s) {
   ByTypes(a.code, a.a.c, [&](auto code, auto type, auto dim) {
     Launch<decltype(code), decltype(type), decltype(dim)::value>(a, s);
   });
+}
+
+void SharedCodes(const CodesSharedArgs& a, hipStream_t s) {
+  if (a.c.a.s.n_seqs == 0) return;
+  if (a.groups.n_seqs > 0) PrefixCodes(a, s);
+  ByTypes(a.c.code, a.c.a.c, [&](auto code, auto type, auto dim) {
+    LaunchOwn<decltype(code), decltype(type), decltype(dim)::value>(a, s);
+  });
+  SharedArgs join;
+  join.a = a.c.a;
+  join.groups = a.groups;
+  join.prefix_splits = a.prefix_splits;
+  SharedJoin(join, s);
 }
 
 }  // namespace paged

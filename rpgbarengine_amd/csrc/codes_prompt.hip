@@ -16,6 +16,7 @@
 
 #include "codes_dev.h"
 #include "common.h"
+#include "groups.h"
 #include "lanes.h"
 #include "paged.h"
 #include "paged_dev.h"
@@ -75,9 +76,9 @@ struct Block {
 };
 
 // grid (row tile x key head, key range): key heads next to each other, the tiles
-// with the most keys first.
-template <typename C, typename T, int kDim, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttentionArgs args) {
+// with the most keys first. kPrefix: as PromptBody's (prompt_body.h).
+template <typename C, typename T, int kDim, int kWaves, bool kPrefix>
+__device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const Seqs& groups, int prefix_splits) {
   const AttentionArgs& a = args.a;
   using K = KeyType<T>;
   constexpr int kQ = kDim / 16, kBlocks = kDim / 32;
@@ -88,15 +89,23 @@ __global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttention
   const int kh = blockIdx.x % a.c.n_kv;
   int seq;
   RowTile t;
-  if (!TileOf(a.s, group, kRows, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.c.n_kv), &seq, &t)) return;
+  if (!TileOf(kPrefix ? groups : a.s, group, kRows, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.c.n_kv), &seq, &t))
+    return;
+  if constexpr (kPrefix) {
+    const Common common = CommonOf(a.s, t.first, t.n_rows / group, t.len);
+    if (common.keys == 0) return;
+    seq = common.seq;
+    t.len = common.keys;
+  }
   const int h = lane >> 5;
   const int row = min(t.row0 + (lane & 31), t.n_rows - 1);
   const int token = row / group, head = kh * group + row % group;
-  const int limit = t.pos0 + token;  // the last key that the lane's row sees (< len)
-  const int first_limit = t.Position(t.row0, group), keys = t.Position(t.row0 + kRows - 1, group) + 1;
-  const int range = RangeOf(max(keys, 1), a.splits);
+  const int limit = kPrefix ? t.len - 1 : t.pos0 + token;  // the last key that the lane's row sees (< len)
+  const int first_limit = kPrefix ? t.len - 1 : t.Position(t.row0, group);
+  const int keys = kPrefix ? t.len : t.Position(t.row0 + kRows - 1, group) + 1;
+  const int range = RangeOf(max(keys, 1), kPrefix ? prefix_splits : a.splits);
   const int begin = blockIdx.y * range, end = min(max(keys, 0), begin + range);
-  if (begin >= end && blockIdx.y > 0) return;
+  if (begin >= end && (kPrefix || blockIdx.y > 0)) return;
   const int32_t* table = a.s.table + seq * a.s.table_stride;
 
   U4 q[kQueryParts<T>][kQ];  // operand i: dimensions 32 (i / 2) + 16 h + 8 (i % 2) ..
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttention
       *at(wave, r, (8 * (e / 4) + 4 * h + e % 4) / 2) = F4{o[0][e], o[1][e], o[0][e + 1], o[1][e + 1]} * f;
   }
   __syncthreads();
-  const bool alone = range >= keys;
+  const bool alone = !kPrefix && range >= keys;
   for (int i = tid; i < kRows * (kDim / 4); i += 64 * kWaves) {
     const int ri = i / (kDim / 4), d = i % (kDim / 4) * 4, row_i = t.row0 + ri;
     if (row_i >= t.n_rows) break;
@@ -227,12 +236,32 @@ __global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttention
       Store4<T>(a.out.p + (t.first + token_i) * a.out.token_bytes + head_i * a.out.head_bytes + d * kBytes<T>,
                 x * Inverse(mi, li));
     } else {
-      const int64_t rows = static_cast<int64_t>(a.s.n_tokens) * a.n_heads;
+      const int64_t rows = static_cast<int64_t>(kPrefix ? a.s.n_seqs : a.s.n_tokens) * a.n_heads;
       const int64_t out_row = static_cast<int64_t>(t.first + token_i) * a.n_heads + head_i;
       if (d == 0) PartStats(a, out_row)[blockIdx.y] = F2{mi, li};
       *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(blockIdx.y) * kDim + d) = x;
     }
   }
+}
+
+template <typename C, typename T, int kDim, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttentionArgs a) {
+  SoloBody<C, T, kDim, kWaves, false>(a, a.a.s, 1);
+}
+
+template <typename C, typename T, int kDim, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 1) void CodesPrefixKernel(CodesSharedArgs a) {
+  SoloBody<C, T, kDim, kWaves, true>(a.c, a.groups, static_cast<int>(a.prefix_splits));
+}
+
+template <typename C, typename T, int kDim>
+void LaunchPrefix(const CodesSharedArgs& args, hipStream_t s) {
+  const AttentionArgs& a = args.c.a;
+  const int64_t tiles = TilesFor(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv, kRows);
+  RPG_CHECK(tiles * a.c.n_kv <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs, a.n_heads);
+  CodesPrefixKernel<C, T, kDim, 4>
+      <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), static_cast<uint32_t>(args.prefix_splits)), 256, 0, s>>>(args);
+  HIP_CHECK(hipGetLastError());
 }
 
 template <typename C, typename T, int kDim>
@@ -259,6 +288,12 @@ void PromptCodes(const CodesAttentionArgs& a, hipStream_t s) {
   if (a.a.s.n_tokens == 0 || a.a.s.n_seqs == 0) return;
   ByTypes(a.code, a.a.c, [&](auto code, auto type, auto dim) {
     Launch<decltype(code), decltype(type), decltype(dim)::value>(a, s);
+  });
+}
+
+void PrefixCodes(const CodesSharedArgs& a, hipStream_t s) {
+  ByTypes(a.c.code, a.c.a.c, [&](auto code, auto type, auto dim) {
+    LaunchPrefix<decltype(code), decltype(type), decltype(dim)::value>(a, s);
   });
 }
 

@@ -60,11 +60,11 @@ struct Tile {
   }
 };
 
-// Weights are held times 2^kLift, their sums too. f16 has steps of 2^-24 at the
+// Weights are held times 2^kDecodeLift, their sums too. f16 has steps of 2^-24 at the
 // least: without it, keys whose weight is below 2^-25 of the largest would count
 // in the sum and not in the output, and a long cache has many of those.
 template <typename T>
-constexpr float kLift = __is_same(T, F16) ? 15.0f : 0.0f;
+constexpr float kDecodeLift = __is_same(T, F16) ? 15.0f : 0.0f;
 
 // A query head's running state in a lane: maximum (of scale log2(e) q.k) and
 // the output of its column, alike over the lanes of a column; the sum of the
@@ -148,7 +148,7 @@ struct State {
 #pragma unroll
       for (int w = 0; w < kRest; ++w) rest[w] *= f;
     }
-    const float base = m == kNegInf ? 0.0f : m - kLift<T>;
+    const float base = m == kNegInf ? 0.0f : m - kDecodeLift<T>;
 #pragma unroll
     for (int h = 0; h < Tl::kHalves; ++h)
 #pragma unroll
@@ -179,15 +179,6 @@ struct State {
       }
     }
   }
-};
-
-// A workgroup's range of positions: [start, end) of a sequence, and where what comes
-// out goes: the output, or partials in a slot of the row's (then other ranges add
-// to it).
-struct DecodeRange {
-  int start, end;
-  bool alone;
-  int slot;
 };
 
 // Tiles of the range are brought by load(tile, pos), the queries by load_q(q, column),
@@ -244,7 +235,7 @@ __device__ __forceinline__ void DecodeBody(const AttentionArgs& a, int seq, int 
       Store4<T>(a.out.p + seq * a.out.token_bytes + (h0 + h) * a.out.head_bytes + d * kBytes<T>, o);
     } else {
       const int64_t row = static_cast<int64_t>(seq) * a.n_heads + h0 + h;
-      if (d == 0) PartStats(a, row)[range.slot] = F2{m, l};
+      if (d == 0) PartStats(a, row)[range.slot] = F2{m - range.off, l};
       *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, row) + static_cast<int64_t>(range.slot) * kDim + d) = o;
     }
   }
@@ -265,7 +256,7 @@ __device__ __forceinline__ DecodePlace PlaceOf(const AttentionArgs& a) {
 __device__ __forceinline__ bool WholeRange(const AttentionArgs& a, int seq, DecodeRange* out) {
   const int len = Length(a.s, seq);
   const int range = RangeOf(max(len, 1), a.splits), start = blockIdx.y * range;
-  *out = {start, min(len, start + range), range >= len, static_cast<int>(blockIdx.y)};
+  *out = {start, min(len, start + range), range >= len, static_cast<int>(blockIdx.y), 0.0f};
   return out->start < out->end || blockIdx.y == 0;
 }
 

@@ -1,0 +1,61 @@
+// Groups of sequences whose first positions lie in the same pages (SharedArgs).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "paged.h"
+#include "paged_dev.h"
+
+namespace rpg {
+namespace paged {
+
+// What a group's sequences have in common: `keys` positions, a multiple of 16 (the
+// unit that pages are looked up in), read through the table of sequence `seq`.
+// Sequences without positions (a batch's empty places) do not count.
+struct Common {
+  int keys, seq;
+};
+
+__device__ __forceinline__ Common CommonOf(const Seqs& s, int first, int n, int shared) {
+  const int lane = threadIdx.x & 63;
+  int least = shared, seq = -1;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int len = i0 + lane < n ? ClampLength(s, s.lens[first + i0 + lane]) : 0;
+    const uint64_t some = __ballot(len > 0);
+    if (some == 0) continue;
+    if (seq < 0) seq = first + i0 + __builtin_ctzll(some);
+    least = min(least, lanes::WaveReduce(len > 0 ? len : INT32_MAX, [](int x, int y) { return min(x, y); }));
+  }
+  return Common{seq < 0 ? 0 : max(least, 0) & ~15, max(seq, first)};
+}
+
+// Of a sequence's group; sequences of no group have nothing in common.
+__device__ __forceinline__ int CommonKeys(const Seqs& s, const Seqs& groups, int seq) {
+  Sequence x;
+  if (!FindSequence(groups, [&](int end, int) { return end <= seq; }, &x) || seq < x.first) return 0;
+  return CommonOf(s, x.first, x.n_new, x.len).keys;
+}
+
+// The ranges that `len` positions are cut into, of `splits` at most.
+__device__ __forceinline__ int RangesOf(int len, int splits) {
+  if (len <= 0) return 0;
+  const int range = RangeOf(len, splits);
+  return (len + range - 1) / range;
+}
+
+// Range blockIdx.y of a sequence's own positions, behind the common ones; false:
+// there is no such range. off: DecodeRange's.
+__device__ __forceinline__ bool OwnRange(const AttentionArgs& a, const Seqs& groups, int prefix_splits, int seq, float off,
+                                         DecodeRange* out) {
+  const int len = Length(a.s, seq);
+  if (len <= 0) return false;
+  const int from = CommonKeys(a.s, groups, seq), own = len - from;
+  const int range = RangeOf(max(own, 1), a.splits - prefix_splits), start = from + blockIdx.y * range;
+  *out = {start, min(len, start + range), false, RangesOf(from, prefix_splits) + static_cast<int>(blockIdx.y), off};
+  return out->start < out->end;
+}
+
+}  // namespace paged
+}  // namespace rpg

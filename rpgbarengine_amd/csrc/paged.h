@@ -118,5 +118,30 @@ void PromptCodes(const CodesAttentionArgs& a, hipStream_t s);
 void Prompt(const AttentionArgs& a, hipStream_t s);
 void PromptJoin(const AttentionArgs& a, hipStream_t s);  // of a.splits > 1 ranges of tiles of 32 rows
 
+// One token per sequence, sequences in groups: those of group g are groups.starts[g]
+// .. groups.starts[g + 1], the first groups.lens[g] positions of each lie in the same
+// pages. (Seqs, for the groups are searched as sequences are: n_seqs groups of
+// n_tokens sequences.) a.splits: the ranges of the common positions, at most
+// prefix_splits, and of a sequence's own.
+struct SharedArgs {
+  AttentionArgs a;
+  Seqs groups;
+  int64_t prefix_splits = 1;
+};
+struct CodesSharedArgs {
+  CodesAttentionArgs c;
+  Seqs groups;
+  int64_t prefix_splits = 1;
+};
+struct SharedSplits {
+  int prefix, own;
+};
+SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity);
+void Shared(const SharedArgs& a, hipStream_t s);
+void SharedCodes(const CodesSharedArgs& a, hipStream_t s);
+void PrefixCodes(const CodesSharedArgs& a, hipStream_t s);  // its first part
+// Joins what the ranges of either kind leave, of any cache.
+void SharedJoin(const SharedArgs& a, hipStream_t s);
+
 }  // namespace paged
 }  // namespace rpg

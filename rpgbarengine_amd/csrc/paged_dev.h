@@ -225,6 +225,17 @@ __device__ __forceinline__ int RangeOf(int len, int splits) {
   return ((len - 1) / splits / kRangeUnit + 1) * kRangeUnit;
 }
 
+// A workgroup's range of positions: [start, end) of a sequence, and where what comes
+// out goes: the output, or partials in a slot of the row's (then other ranges add
+// to it). off: what the range's weights are held above those of other kernels' ranges
+// that it is joined with (a power of two, taken off its maximum).
+struct DecodeRange {
+  int start, end;
+  bool alone;
+  int slot;
+  float off;
+};
+
 // x - y of maxima that may both be -inf (no key yet): then 0.
 __device__ __forceinline__ float MaxDiff(float x, float y) { return x == y ? 0.0f : x - y; }
 

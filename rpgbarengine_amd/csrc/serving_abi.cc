@@ -264,6 +264,38 @@ int32_t QuantAttention(const rpg_hip_quant_cache* cache, const rpg_hip_sequences
   return 0;
 }
 
+paged::SharedSplits SharedSizes(const paged::Cache& c, const paged::Seqs& s, int32_t n_groups, int32_t n_heads,
+                                int64_t* bytes) {
+  RPG_CHECK(n_groups >= 0, "%d groups", n_groups);
+  CheckHeads(c, s, n_heads);
+  const paged::SharedSplits n = paged::SplitsOfShared(s.n_seqs, n_groups, n_heads, c.n_kv, s.capacity);
+  *bytes = paged::WorkBytes(static_cast<int64_t>(s.n_seqs) * n_heads, c.head_dim, n.prefix + n.own);
+  return n;
+}
+
+// The groups, splits and work memory of a call whose rows `a` has.
+paged::Seqs GroupsOf(const rpg_hip_groups* g, paged::AttentionArgs* a, int64_t* prefix_splits, void* work,
+                     int64_t work_bytes) {
+  RPG_CHECK(g != nullptr, "the groups are null");
+  int64_t need;
+  const paged::SharedSplits n = SharedSizes(a->c, a->s, g->n_groups, a->n_heads, &need);
+  if (g->n_groups > 0) {
+    CheckPointer("the groups' starts", g->starts, 4);
+    CheckPointer("shared", g->shared, 4);
+  }
+  CheckWork(work, work_bytes, need);
+  a->work = static_cast<float*>(work);
+  a->splits = n.prefix + n.own;
+  *prefix_splits = n.prefix;
+  paged::Seqs out;
+  out.starts = g->starts;
+  out.lens = g->shared;
+  out.n_seqs = g->n_groups;
+  out.n_tokens = a->s.n_seqs;
+  out.capacity = a->s.capacity;
+  return out;
+}
+
 void AppendRows(paged::AppendArgs* to, const rpg_hip_rows* k, const rpg_hip_rows* v, const rpg_hip_rows* q,
                 const rpg_hip_rows* q_out, int32_t n_heads, const float* q_norm, const float* k_norm, float eps,
                 const float* rope, int64_t rope_rows) {
@@ -458,6 +490,69 @@ int64_t rpg_hip_quant_work(const rpg_hip_quant_cache* cache, const rpg_hip_seque
         const paged::Seqs s = SeqSizes(seqs, cache->page_size);
         CheckHeads(c, s, n_heads);
         return AttentionWork(c, s, n_heads, prompt != 0, true);
+      },
+      -1);
+}
+
+int32_t rpg_hip_paged_shared(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
+                             const rpg_hip_groups* groups, const rpg_hip_rows* q, const rpg_hip_rows* out,
+                             int32_t n_heads, float scale, void* work, int64_t work_bytes, void* stream) {
+  return Guard(
+      [&] {
+        paged::SharedArgs a;
+        a.a.c = CacheOf(cache);
+        a.a.s = SeqsOf(seqs, cache->page_size, false);
+        if (Empty(a.a.s, false)) return 0;
+        AttentionRows(&a.a, q, out, a.a.s.n_seqs, n_heads, scale);
+        a.groups = GroupsOf(groups, &a.a, &a.prefix_splits, work, work_bytes);
+        paged::Shared(a, static_cast<hipStream_t>(stream));
+        return 0;
+      },
+      -1);
+}
+
+int64_t rpg_hip_paged_shared_work(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs, int32_t n_groups,
+                                  int32_t n_heads) {
+  return Guard(
+      [&]() -> int64_t {
+        const paged::Cache c = CacheSizes(cache);
+        const paged::Seqs s = SeqSizes(seqs, cache->page_size);
+        int64_t bytes;
+        SharedSizes(c, s, n_groups, n_heads, &bytes);
+        return Empty(s, false) ? 0 : bytes;
+      },
+      -1);
+}
+
+int32_t rpg_hip_quant_shared(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs,
+                             const rpg_hip_groups* groups, int32_t type, const rpg_hip_rows* q,
+                             const rpg_hip_rows* out, int32_t n_heads, float scale, void* work, int64_t work_bytes,
+                             void* stream) {
+  return Guard(
+      [&] {
+        paged::CodesSharedArgs a;
+        a.c.a.c = QuantOf(cache, type, &a.c.scales);
+        a.c.code = cache->code;
+        a.c.a.s = SeqsOf(seqs, cache->page_size, false);
+        if (Empty(a.c.a.s, false)) return 0;
+        AttentionRows(&a.c.a, q, out, a.c.a.s.n_seqs, n_heads, scale);
+        a.groups = GroupsOf(groups, &a.c.a, &a.prefix_splits, work, work_bytes);
+        paged::SharedCodes(a, static_cast<hipStream_t>(stream));
+        return 0;
+      },
+      -1);
+}
+
+int64_t rpg_hip_quant_shared_work(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t n_groups,
+                                  int32_t type, int32_t n_heads) {
+  return Guard(
+      [&]() -> int64_t {
+        paged::Scales scales;
+        const paged::Cache c = QuantSizes(cache, type, &scales);
+        const paged::Seqs s = SeqSizes(seqs, cache->page_size);
+        int64_t bytes;
+        SharedSizes(c, s, n_groups, n_heads, &bytes);
+        return Empty(s, false) ? 0 : bytes;
       },
       -1);
 }

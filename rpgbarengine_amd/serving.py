@@ -6,6 +6,7 @@ of many rows, for hosts that schedule sessions themselves.
     serving.append(cache, table, lens, starts, k, v, q=q, q_norm=..., k_norm=..., rope=...)
     out = serving.prompt_attention(q, cache, table, lens, starts)   # prompts, packed
     out = serving.decode_attention(q, cache, table, lens)           # one token each
+    out = serving.shared_attention(q, cache, table, lens, groups, shared)  # with prefixes in common
     logits = serving.edit_logits(logits, history, history_lens, repetition=..., mask=...)
     tokens, logprobs = serving.sample(logits, u, temperature, top_k, top_p, min_p)
 
@@ -39,8 +40,8 @@ _P, _I32, _I64, _F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_f
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # ggml ids
 # rpg_hip_paged_cache, rpg_hip_sequences, rpg_hip_rows, packed as C lays them out
 _CACHE, _SEQS, _ROWS = struct.Struct("PPqqqiiiii"), struct.Struct("PqPPiii"), struct.Struct("Pqq")
-# rpg_hip_quant_cache, rpg_hip_edits
-_QUANT, _EDITS = struct.Struct("PPPPqqqqqiiiii"), struct.Struct("PqPPPPPPqPqPqPiii")
+# rpg_hip_quant_cache, rpg_hip_edits, rpg_hip_groups
+_QUANT, _EDITS, _GROUPS = struct.Struct("PPPPqqqqqiiiii"), struct.Struct("PqPPPPPPqPqPqPiii"), struct.Struct("PPi")
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 _SIGS = {
@@ -53,6 +54,10 @@ _SIGS = {
     "rpg_hip_quant_decode": ([_P, _P, _I32, _P, _P, _I32, _F, _P, _I64, _P], _I32),
     "rpg_hip_quant_prompt": ([_P, _P, _I32, _P, _P, _I32, _F, _P, _I64, _P], _I32),
     "rpg_hip_quant_work": ([_P, _P, _I32, _I32, _I32], _I64),
+    "rpg_hip_paged_shared": ([_P, _P, _P, _P, _P, _I32, _F, _P, _I64, _P], _I32),
+    "rpg_hip_paged_shared_work": ([_P, _P, _I32, _I32], _I64),
+    "rpg_hip_quant_shared": ([_P, _P, _P, _I32, _P, _P, _I32, _F, _P, _I64, _P], _I32),
+    "rpg_hip_quant_shared_work": ([_P, _P, _I32, _I32, _I32], _I64),
     "rpg_hip_edit_logits": ([_I32, _P, _I64, _I64, _I64, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows": ([_I32, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P], _I32),
     "rpg_hip_sample_rows_work": ([_I64, _I64], _I64),
@@ -371,6 +376,51 @@ def prompt_attention(q, cache, table, lens, starts, scale=None, out=None):
     if starts is None:
         raise EngineError("starts is needed")
     return _attention(q, cache, table, lens, starts, scale, out, 1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_bytes(quant, n_kv, page_size, head_dim, kind, pages, n_seqs, n_groups, heads):
+    """rpg_hip_paged_shared_work or rpg_hip_quant_shared_work of these sizes."""
+    wide = page_size * head_dim
+    s = _SEQS.pack(0, pages, 0, 0, pages, n_seqs, 0)
+    if quant:
+        c = _QUANT.pack(0, 0, 0, 0, n_kv * wide, wide, head_dim, n_kv * page_size, page_size, 1, page_size, n_kv, head_dim, 0)
+        return _ok(_lib().rpg_hip_quant_shared_work(c, s, n_groups, kind, heads))
+    c = _CACHE.pack(0, 0, n_kv * wide, wide, head_dim, 1, page_size, n_kv, head_dim, kind)
+    return _ok(_lib().rpg_hip_paged_shared_work(c, s, n_groups, heads))
+
+
+def shared_attention(q, cache, table, lens, groups, shared, scale=None, out=None):
+    """decode_attention where the first positions of a group's sequences lie in the
+    same pages, which are read once for the group: group g is sequences groups[g] ..
+    groups[g + 1] (int32 [groups + 1]), and the tables of those that have positions
+    name the same pages for the first shared[g] (int32 [groups]) positions. out (may
+    be q) is made when not given."""
+    quant = type(cache) is QuantCache
+    kind = _row_type(q, "q") if quant else None
+    qr = _rows(q, "q", cache, kind)
+    seqs, n_seqs, pages = _seqs(cache, table, lens, None, 0)
+    if q.shape[0] != n_seqs:
+        raise EngineError("q has a row for each sequence")
+    dev, heads, dim = cache.device, q.shape[1], cache.head_dim
+    n_groups = _ints(shared, "shared", 1, dev)[0]
+    if _ints(groups, "groups", 1, dev)[0] != n_groups + 1:
+        raise EngineError("groups has one value more than shared")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise EngineError("out has the shape of q")
+    size = _shared_bytes(quant, cache.n_kv, cache.page_size, dim, _TYPES[q.dtype], pages, n_seqs, n_groups, heads)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    of = _GROUPS.pack(groups.data_ptr(), shared.data_ptr(), n_groups)
+    rest = (qr, _rows(out, "out", cache, kind), heads, dim ** -0.5 if scale is None else scale,
+            work.data_ptr() if size else None, size)
+    if quant:
+        _enqueue(dev, _lib().rpg_hip_quant_shared, cache._packed(), seqs, of, _TYPES[kind], *rest)
+    else:
+        _enqueue(dev, _lib().rpg_hip_paged_shared, cache._packed(), seqs, of, *rest)
+    _written(out)
+    return out
 
 
 @functools.lru_cache(maxsize=4096)

@@ -1,0 +1,233 @@
+"""Attention of sequences whose first positions lie in the same pages
+(rpgbarengine_amd.serving.shared_attention) against the definition in float64: that
+of decode_attention, whatever is said to be shared."""
+
+import math
+
+import pytest
+import torch
+
+import serving_plain as plain
+from rpgbarengine_amd import serving
+from test_gpu_serving import DTYPES, Batch, close
+from test_gpu_serving_codes import CODES, expect, ident, on_cpu, random_cache, spoil
+
+pytestmark = pytest.mark.gpu
+
+
+class Shared(Batch):
+    """Sequences in groups: `sizes` sequences each, the first `common[g]` positions of
+    group g's in the same pages."""
+
+    def __init__(self, sizes, common, lens, dtype, kv=2, dim=128, page=16, heads=8, seed=0, extra_pages=2, before=0):
+        super().__init__(lens, [1] * len(lens), dtype, kv, dim, page, heads, seed, extra_pages=extra_pages)
+        first = before
+        self.groups = torch.tensor([before + sum(sizes[:i]) for i in range(len(sizes) + 1)], dtype=torch.int32)
+        self.common = torch.tensor(common, dtype=torch.int32)
+        for n, shared in zip(sizes, common):
+            members = range(first, first + n)
+            pages = -(-shared // page)  # the last of them may end inside: no two write there here
+            src = max(members, key=lambda i: lens[i], default=None)
+            for i in members:
+                here = min(pages, -(-lens[i] // page))
+                self.table[i, :here] = self.table[src, :here]
+            first += n
+
+    def call(self, q, cache, table, lens, **kw):
+        return serving.shared_attention(q.cuda(), cache, table, lens, self.groups.cuda(), self.common.cuda(), **kw)
+
+
+def want(b, q, i, scale, k=None, v=None):
+    n = b.lens[i]
+    kk, there = plain.sequence_rows(b.k if k is None else k, b.table[i], n)
+    vv, _ = plain.sequence_rows(b.v if v is None else v, b.table[i], n)
+    return plain.attention(q[i], kk, vv, there, scale, b.dtype)
+
+
+SHAPES = [
+    # one small group
+    ([3], [48], [50, 70, 49]),
+    # common positions that are no whole unit, none at all, one group of one
+    ([2, 3, 1], [37, 0, 64], [40, 38, 20, 1, 5, 70]),
+    # sequences shorter than what is said to be shared, empty ones among them
+    ([4, 2], [200, 100], [200, 150, 0, 333, 0, 0]),
+    # many of them, and long
+    ([20, 9], [300, 640], [300 + 13 * i for i in range(20)] + [641 + i for i in range(9)]),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 3, 3, 64), (64, 34, 2, 16)])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_shared(dtype, dim, heads, kv, page, shape):
+    b = Shared(*SHAPES[shape], dtype, kv, dim, page, heads, seed=shape)
+    n = len(b.lens)
+    q = b.normal(n, heads, dim, by=1.5)
+    cache, table, lens, _ = b.gpu()
+    out = torch.full((n, heads, dim), 5.0, dtype=dtype, device="cuda")
+    assert b.call(q, cache, table, lens, scale=0.1, out=out) is out
+    for i in range(n):
+        close(out[i], *want(b, q, i, 0.1))
+    assert torch.equal(b.call(q, cache, table, lens, scale=0.1), out)  # the same bits
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 8, 2, 16), (64, 5, 1, 32), (64, 34, 2, 64)])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_shared_codes(codes, dtype, dim, heads, kv, page, shape):
+    b = Shared(*SHAPES[shape], dtype, kv, dim, page, heads, seed=shape)
+    n = len(b.lens)
+    q = b.normal(n, heads, dim, by=0.3)
+    _, table, lens, _ = b.gpu()
+    cache = random_cache(b, codes)
+    out = torch.full((n, heads, dim), 5.0, dtype=dtype, device="cuda")
+    assert b.call(q, cache, table, lens, scale=0.1, out=out) is out
+    held = on_cpu(cache)
+    for i in range(n):
+        close(out[i], *expect(b, held, q, 0.1, i, b.lens[i] - 1, i))
+    assert torch.equal(b.call(q, cache, table, lens, scale=0.1), out)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_long_common_positions(dtype):
+    """Many ranges of common positions, the maximum in one of them or in a sequence's
+    own; room in the table for more."""
+    lens = [3000 + 7 * i for i in range(5)] + [2100, 2900]
+    b = Shared([5, 2], [2999, 2048], lens, dtype, 1, 64, 16, 4, seed=5, extra_pages=90)
+    b.k[int(b.table[0, 100]), 0, 3] *= 6
+    b.k[int(b.table[6, -(-2900 // 16) - 1]), 0, 1] *= 6
+    q = b.normal(7, 4, 64, by=1.5)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    for i in range(7):
+        close(got[i], *want(b, q, i, 64 ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("members", [1, 17, 40])
+def test_groups_of_any_size(dtype, members):
+    """Rows of one tile and of several, of 32 rows and of 128."""
+    lens = [130 + (5 * i) % 40 for i in range(members)]
+    b = Shared([members], [128], lens, dtype, 1, 128, 16, 8, seed=members)
+    q = b.normal(members, 8, 128, by=1.5)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    for i in range(members):
+        close(got[i], *want(b, q, i, 128 ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_sequences_of_no_group(dtype):
+    """In front of the first group and behind the last; no groups at all; shared counts
+    past what the table holds, and below 0."""
+    lens = [70, 33, 90, 95, 20, 64]
+    b = Shared([2], [80], lens, dtype, before=2, seed=7)
+    q = b.normal(6, 8, 128, by=1.5)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    for i in range(6):
+        close(got[i], *want(b, q, i, 128 ** -0.5))
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    alone = serving.shared_attention(q.cuda(), cache, table, l, torch.zeros(1, dtype=torch.int32, device="cuda"), none)
+    for i in range(6):
+        close(alone[i], *want(b, q, i, 128 ** -0.5))
+    one = Shared([1], [20], [20], dtype, seed=8)
+    q = one.normal(1, 8, 128, by=1.5)
+    cache, table, l, _ = one.gpu()
+    for shared in (10 ** 9, -5, 16):
+        one.common[0] = shared
+        close(one.call(q, cache, table, l)[0], *want(one, q, 0, 128 ** -0.5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_masked_places_hold_anything(dtype, value):
+    """Rows past lengths, spare pages, unnamed pages among the common ones and a
+    sequence's own, tables of empty sequences."""
+    lens = [90, 130, 0, 101]
+    b = Shared([4], [80], lens, dtype, 2, 128, 16, 8, seed=9)
+    b.table[:, 2] = -1  # among the common pages
+    b.table[1, 6] = b.n_pages + 5
+    b.table[2, :] = -7
+    used = torch.zeros(b.n_pages, 16, dtype=torch.bool)
+    for i, n in enumerate(lens):
+        for p in range(n):
+            at = int(b.table[i, p // 16])
+            if 0 <= at < b.n_pages:
+                used[at, p % 16] = True
+    kb, vb = b.k.clone(), b.v.clone()
+    hold = (~used)[:, None, :, None]
+    b.k, b.v = b.k.masked_fill(hold, value), b.v.masked_fill(hold, value)
+    q = b.normal(4, 8, 128)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    for i in range(4):
+        close(got[i], *want(b, q, i, 128 ** -0.5, kb, vb))
+    for codes in CODES:
+        quant = random_cache(b, codes)
+        held = on_cpu(quant)
+        spoil(b, quant, used, value)
+        got = b.call(q, quant, table, l)
+        for i in range(4):
+            close(got[i], *expect(b, held, q, 128 ** -0.5, i, lens[i] - 1, i))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+def test_infinite_values_that_are_seen(dtype):
+    """Among the common positions and in one sequence's own."""
+    b = Shared([3], [64], [70, 80, 65], dtype, 2, 128, 16, 8, seed=10)
+    b.v[int(b.table[0, 1]), 0, 3, 5] = math.inf
+    b.v[int(b.table[1, 4]), 1, 2, 6] = -math.inf
+    q = b.normal(3, 8, 128)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l).double().cpu()
+    ok = torch.ones_like(got, dtype=torch.bool)
+    ok[:, :4, 5] = False
+    ok[1, 4:, 6] = False
+    assert bool((got[:, :4, 5] == math.inf).all()) and bool((got[1, 4:, 6] == -math.inf).all())
+    assert bool(got[ok].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", ["rows", "codes"])
+def test_captured_and_replayed(kind):
+    """A replay takes lengths, tables, groups and shared counts of its moment; eager
+    calls on other memory in between."""
+    dtype = torch.bfloat16
+    b = Shared([3, 2], [64, 48], [80, 90, 70, 60, 200], dtype, seed=11)
+    q = b.normal(5, 8, 128, by=0.3).cuda()
+    rows, table, lens, _ = b.gpu()
+    cache = rows if kind == "rows" else random_cache(b, torch.int8)
+    held = None if kind == "rows" else on_cpu(cache)
+    groups, common, out = b.groups.cuda(), b.common.cuda(), torch.empty_like(q)
+    serving.shared_attention(q, cache, table, lens, groups, common, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        serving.shared_attention(q, cache, table, lens, groups, common, out=out)
+    for step in range(4):
+        b.lens = [80 - step, 90, 70, max(0, 60 - 20 * step), 200 - 30 * step]
+        b.common = torch.tensor([64 - 16 * step, 48])
+        if step == 2:
+            b.groups = torch.tensor([0, 2, 2])
+        lens.copy_(torch.tensor(b.lens, dtype=torch.int32)), common.copy_(b.common), groups.copy_(b.groups)
+        out.fill_(9)
+        graph.replay()
+        serving.decode_attention(q, cache, table, lens)
+        torch.cuda.synchronize()
+        for i in range(5):
+            if kind == "rows":
+                close(out[i], *want(b, q.cpu(), i, 128 ** -0.5))
+            else:
+                close(out[i], *expect(b, held, q.cpu(), 128 ** -0.5, i, b.lens[i] - 1, i))
+
+
+def test_queries_in_place_and_strided():
+    b = Shared([3], [64], [70, 80, 65], torch.float16, seed=12)
+    wide = b.normal(3, 20, 128, by=0.5).cuda()
+    cache, table, lens, _ = b.gpu()
+    q = wide[:, 5:13]
+    apart = b.call(q, cache, table, lens)
+    keep = wide.clone()
+    assert serving.shared_attention(q, cache, table, lens, b.groups.cuda(), b.common.cuda(), out=q) is q
+    assert torch.equal(q, apart) and torch.equal(wide[:, :5], keep[:, :5]) and torch.equal(wide[:, 13:], keep[:, 13:])
