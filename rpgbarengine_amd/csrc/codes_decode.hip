@@ -27,15 +27,15 @@ namespace paged {
 namespace {
 
 // A wave's keys of one step, as two halves of 16: K as 16 codes of key l % 16 per 64
-// dimensions, V as the lane's dimensions (kDim / 16) (l % 16) .. of keys 4 (l / 16) + r,
-// the scales of those keys.
+// dimensions, V as the lane's dimensions (kDim / 16) (l % 16) .. of keys 4 (l / 16) + r;
+// of key 4 (l / 16) + l % 4 the scales.
 template <int kDim>
 struct CodesTile {
   static constexpr int kKeys = 32;
   static constexpr int kChunks = kDim / 64;  // K: 16-byte pieces; V: dwords per key
   U4 k[2][kChunks];
   uint32_t v[2][4][kChunks];
-  F4 ks[2], vs[2];
+  float ks[2], vs[2];
   bool ok[2];  // its page is there
 
   // Rows of positions pos .. of the sequence whose last one is `last`; those
@@ -54,8 +54,8 @@ struct CodesTile {
       const char* vb = c.v + at;
 #pragma unroll
       for (int i = 0; i < kChunks; ++i) k[h][i] = Load16(kb + static_cast<uint32_t>(l16 * c.row_bytes + 64 * i + 16 * g));
-      ks[h] = __builtin_bit_cast(F4, Load16(sc.k + scale_at + static_cast<uint32_t>(16 * g)));
-      vs[h] = __builtin_bit_cast(F4, Load16(sc.v + scale_at + static_cast<uint32_t>(16 * g)));
+      ks[h] = *(const __attribute__((address_space(1))) float*)(sc.k + scale_at + 16 * g + 4 * (lane & 3));
+      vs[h] = *(const __attribute__((address_space(1))) float*)(sc.v + scale_at + 16 * g + 4 * (lane & 3));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const char* row = vb + static_cast<uint32_t>((4 * g + r) * c.row_bytes);
@@ -100,9 +100,11 @@ struct CodesState {
 #pragma unroll
         for (int p = kQueryParts<T> - 1; p >= 0; --p) x = Mfma16<K>(a, q.x[p][i], x);
       }
-      s[h] = x * (t.ks[h] * c);
+      s[h] = x;
+      ScaleBy<0, 4>(s[h], t.ks[h] * c);
     }
-    if (!(pos + Tl::kKeys - 1 <= last && t.ok[0] && t.ok[1])) {
+    const bool masked = !(pos + Tl::kKeys - 1 <= last && t.ok[0] && t.ok[1]);
+    if (masked) {
       // Masked keys: no weight, and nothing of what their rows hold (which may
       // be anything, NaN among it) reaches the second product.
 #pragma unroll
@@ -111,7 +113,6 @@ struct CodesState {
         for (int r = 0; r < 4; ++r) {
           const bool in = t.ok[h] && pos + 16 * h + 4 * g + r <= last;
           s[h][r] = in ? s[h][r] : kNegInf;
-          t.vs[h][r] = in ? t.vs[h][r] : 0.0f;
 #pragma unroll
           for (int w = 0; w < Tl::kChunks; ++w) t.v[h][r][w] = in ? t.v[h][r][w] : 0u;
         }
@@ -134,11 +135,16 @@ struct CodesState {
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p = __builtin_amdgcn_exp2f(s[h][r] - base);
-        l += p;  // (the sum takes the weights unrounded)
-        s[h][r] = p * t.vs[h][r];
+        s[h][r] = __builtin_amdgcn_exp2f(s[h][r] - base);
+        l += s[h][r];  // (the sum takes the weights unrounded)
       }
-    WeightParts<T> p;
+    if (masked) {  // 0 x NaN must not reach the product
+#pragma unroll
+      for (int h = 0; h < 2; ++h) t.vs[h] = t.ok[h] && pos + 16 * h + 4 * g + (lane & 3) <= last ? t.vs[h] : 0.0f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) ScaleBy<0, 4>(s[h], t.vs[h]);
+    WeightParts<kWeightParts<T>> p;
 #pragma unroll
     for (int j = 0; j < 4; ++j) p.Set(j, s[j / 2][2 * (j % 2)], s[j / 2][2 * (j % 2) + 1]);
 #pragma unroll

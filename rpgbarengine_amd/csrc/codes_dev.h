@@ -47,6 +47,22 @@ __device__ __forceinline__ uint32_t Halves2(uint32_t u) {
   }
 }
 
+// The value of lane i of each 16, to all of them: an operand modifier of the
+// instruction that takes it. Scales of the rows that a lane's scores belong to come
+// that way, a register for 16 of them.
+template <int i>
+__device__ __forceinline__ float OfLane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + i, 0xF, 0xF, true));
+}
+// x[e] * (v of lane e of the 16)
+template <int e, int n, typename V>
+__device__ __forceinline__ void ScaleBy(V& x, float v) {
+  if constexpr (e < n) {
+    x[e] *= OfLane<e>(v);
+    ScaleBy<e + 1, n>(x, v);
+  }
+}
+
 // eight codes as a product's operand
 template <typename C, typename T>
 __device__ __forceinline__ U4 Operand8(uint32_t x, uint32_t y) {
@@ -89,16 +105,16 @@ __device__ __forceinline__ void LoadQuery(const char* p, int i, U4 (&q)[kParts][
 }
 
 // Eight weights (times scales) as the parts of an operand.
-template <typename T>
+template <int kParts>
 struct WeightParts {
-  U4 x[kWeightParts<T>];
+  U4 x[kParts];
   __device__ __forceinline__ void Set(int j, float a, float b) {
-    if constexpr (kBytes<T> == 4) {
+    if constexpr (kParts == 3) {
       const Parts p = Split3(a, b);
       x[0][j] = p.hi, x[1][j] = p.mid, x[2][j] = p.lo;
     } else {
       x[0][j] = Pack2<BF16>(a, b);
-      x[1][j] = Rest2<BF16>(a, b, x[0][j]);
+      if constexpr (kParts == 2) x[1][j] = Rest2<BF16>(a, b, x[0][j]);
     }
   }
 };

@@ -57,13 +57,6 @@ __global__ __launch_bounds__(256) void SharedJoinKernel(SharedArgs args) {
                    a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes);
 }
 
-// Waves of a workgroup's tile that share its rows: all of them (32 rows) for small
-// groups, none (128 rows) for large ones.
-int GroupsOf(int64_t n_seqs, int64_t n_groups, int group) {
-  const int64_t rows = n_seqs * group / std::max<int64_t>(n_groups, 1);
-  return rows > 64 ? 1 : rows > 32 ? 2 : 4;
-}
-
 template <typename T, int kDim, int kGroups>
 void LaunchPrefix(const SharedArgs& args, hipStream_t s) {
   const AttentionArgs& a = args.a;
@@ -81,11 +74,11 @@ void Launch(const SharedArgs& args, hipStream_t s) {
   const int64_t x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(group, kCols);
   RPG_CHECK(static_cast<int64_t>(a.s.n_seqs) * a.n_heads <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs,
             a.n_heads);
-  const int groups = GroupsOf(a.s.n_seqs, args.groups.n_seqs, group);
   if (args.groups.n_seqs > 0) {
-    if (groups == 1)
+    const int rows = PrefixRows(a.s.n_seqs, args.groups.n_seqs, group);
+    if (rows == 128)
       LaunchPrefix<T, kDim, 1>(args, s);
-    else if (groups == 2)
+    else if (rows == 64)
       LaunchPrefix<T, kDim, 2>(args, s);
     else
       LaunchPrefix<T, kDim, 4>(args, s);
@@ -103,9 +96,14 @@ void LaunchJoin(const SharedArgs& a, hipStream_t s) {
 
 }  // namespace
 
+int PrefixRows(int64_t n_seqs, int64_t n_groups, int group) {
+  const int64_t rows = n_seqs * group / std::max<int64_t>(n_groups, 1);
+  return rows > 64 ? 128 : rows > 32 ? 64 : 32;
+}
+
 SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity) {
   const int group = n_heads / n_kv;
-  const int64_t tiles = TilesFor(n_seqs, n_groups, group, 128 / GroupsOf(n_seqs, n_groups, group));
+  const int64_t tiles = TilesFor(n_seqs, n_groups, group, PrefixRows(n_seqs, n_groups, group));
   const int64_t wgs = std::max<int64_t>(1, tiles * n_kv);
   const int64_t prefix = std::min({CeilDiv(512, wgs), CeilDiv(capacity, 256), int64_t{kMaxSplits / 2}});
   const int own = DecodeSplits(n_seqs, n_heads, n_kv, 2, capacity);

@@ -463,3 +463,57 @@ def test_more_new_tokens_than_positions(codes, dtype):
     cache = random_cache(b, codes)
     got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
     assert bool((got[:5] == 0).all()) and bool((got[5:] != 0).any(-1).all())
+
+
+def expect_head(b, cache, q, scale, i, h, heads):
+    """(out, bound) of all new tokens of sequence i for query head h, as `attention`
+    has them for one token."""
+    k, v, ks, vs = cache
+    n, m = b.lens[i], b.new[i]
+    kv = h // (heads // b.kv)
+    kk, there = rows_of(k, b, i, n)
+    kk, vv = kk[kv], rows_of(v, b, i, n)[0][kv]
+    ss, tt = scales_of(ks, b, i, n)[0][kv], scales_of(vs, b, i, n)[0][kv]
+    qq = q[int(b.starts[i]):int(b.starts[i]) + m, h].double()
+    seen = there[None, :] & (torch.arange(n)[None, :] <= torch.arange(n - m, n)[:, None])
+    s = (qq @ kk.t()) * ss * scale
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), 1) * tt
+    out, mass = p @ vv, p @ vv.abs()
+    size = (qq.abs() @ kk.abs().t()) * ss
+    ds = (size * seen).amax(1) * scale * (3 * q.shape[2] + 6) * 2.0 ** -24 + (s.abs() * seen).amax(1) * 2.0 ** -21
+    # many rows: weights in three parts of 8 bits (f32), two (f16), one (bf16)
+    weight_bits = {torch.float32: 24, torch.float16: 16, torch.bfloat16: 8}[b.dtype]
+    rel = torch.expm1(2 * ds) + (3 * seen.sum(1) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
+    bound = rel[:, None] * mass + 2.0 ** -140 * n * 448
+    return out, bound + plain.EPS[b.dtype] * (out.abs() + bound) + plain.TINY[b.dtype]
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,page", [(128, 128, 32, 16), (64, 96, 32, 64)])
+def test_prompts_of_many_rows(codes, dtype, dim, heads, kv, page):
+    """Enough rows for tiles of 128, in sequences that begin and end inside them, one
+    with a history, one with an unnamed page and one with a row that was not finite."""
+    lens, new = [150, 300, 64, 97], [150, 70, 64, 33]
+    b = Batch(lens, new, dtype, kv, dim, page, heads, seed=15)
+    b.table[1, 1] = -1
+    q = b.normal(b.tokens + 2, heads, dim, by=0.3)
+    _, table, lens_d, starts = b.gpu()
+    cache = random_cache(b, codes)
+    held_ = on_cpu(cache)
+    cache.v_scale[int(b.table[2, 40 // page]), 5, 40 % page] = math.nan
+    out = torch.full((b.tokens + 2, heads, dim), 5.0, dtype=dtype, device="cuda")
+    serving.prompt_attention(q.cuda(), cache, table, lens_d, starts, out=out)
+    group = heads // kv
+    for i in range(4):
+        at = slice(int(b.starts[i]), int(b.starts[i]) + new[i])
+        for h in (0, 5 * group, 5 * group + group - 1, heads - 1):
+            want, bound = expect_head(b, held_, q, dim ** -0.5, i, h, heads)
+            got = out[at, h]
+            if i == 2 and h // group == 5:
+                assert bool(got[40:].isnan().all())
+                got, want, bound = got[:40], want[:40], bound[:40]
+            close(got, want, bound)
+    assert bool((out[b.tokens:] == 5).all())
+    again = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts)[:b.tokens]
+    assert torch.equal(again.nan_to_num(7.0), out[:b.tokens].nan_to_num(7.0))

@@ -115,6 +115,13 @@ def test_groups_of_any_size(dtype, members):
     got = b.call(q, cache, table, l)
     for i in range(members):
         close(got[i], *want(b, q, i, 128 ** -0.5))
+    q = b.normal(members, 8, 128, by=0.3)
+    for codes in CODES:
+        cache = random_cache(b, codes)
+        held = on_cpu(cache)
+        got = b.call(q, cache, table, l)
+        for i in range(members):
+            close(got[i], *expect(b, held, q, 128 ** -0.5, i, lens[i] - 1, i))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
