@@ -336,8 +336,9 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
     }
   };
   const float c = a.scale * 1.44269504088896341f;
-  auto settle = [&](int step) {
-    char* kt = lds + (step & 1) * 2 * W::kTileBytes;
+  auto settle = [&](int step, auto buffer) {
+    constexpr int kAt = decltype(buffer)::value;
+    char* kt = lds + kAt * 2 * W::kTileBytes;
     char* vt = kt + W::kTileBytes;
 #pragma unroll
     for (int i = 0; i < W::kLoads; ++i) {
@@ -352,7 +353,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Operand8<C, BF16>(y[0], y[1]);
       *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Operand8<C, BF16>(y[2], y[3]);
     }
-    if (wave < 2) scales[step & 1][wave][lane] = wave == 0 ? scale * c : scale;
+    if (wave < 2) scales[kAt][wave][lane] = wave == 0 ? scale * c : scale;
   };
 
   const int k_at = (lane & 31) * W::kRowBytes + 16 * (h ^ KSwizzle<K, kDim>(lane & 31));
@@ -367,10 +368,11 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   if (steps > 0) {
     look_up(0);
     fetch(0);
-    settle(0);
+    settle(0, std::integral_constant<int, 0>{});
   }
   __syncthreads();
-  for (int step = 0; step < steps; ++step) {
+  auto work = [&](int step, auto buffer) {
+    constexpr int kAt = decltype(buffer)::value;
     const bool more = step + 1 < steps;
     bool named[4];
 #pragma unroll
@@ -381,10 +383,10 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
     }
     const int key0 = begin + step * W::kKeys;
     if (key0 <= wave_last && key0 < end) {
-      const char* kt = lds + (step & 1) * 2 * W::kTileBytes;
+      const char* kt = lds + kAt * 2 * W::kTileBytes;
       const char* vt = kt + W::kTileBytes;
       // lane e of each 16: of the key that the lanes' element e belongs to
-      const float* of_lane = scales[step & 1][0] + 8 * ((lane & 15) / 4) + 4 * h + lane % 4;
+      const float* of_lane = scales[kAt][0] + 8 * ((lane & 15) / 4) + 4 * h + lane % 4;
       const float ks[2] = {of_lane[0], of_lane[32]}, vs[2] = {of_lane[W::kKeys], of_lane[W::kKeys + 32]};
       F16v s[2];
 #pragma unroll
@@ -461,8 +463,12 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
         }
       }
     }
-    if (more) settle(step + 1);
+    if (more) settle(step + 1, std::integral_constant<int, 1 - kAt>{});
     __syncthreads();
+  };
+  for (int step = 0; step < steps; step += 2) {
+    work(step, std::integral_constant<int, 0>{});
+    if (step + 1 < steps) work(step + 1, std::integral_constant<int, 1>{});
   }
 
   l = lanes::AddXor32(l);

@@ -9,6 +9,8 @@
 namespace rpg {
 namespace rows {
 
+constexpr int kMaxHistory = 1 << 20, kMaxBiases = 1023;  // tokens of a row, entries of a row
+
 struct EditArgs {
   const char* logits = nullptr;
   char* out = nullptr;

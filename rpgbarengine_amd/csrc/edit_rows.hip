@@ -59,7 +59,11 @@ __device__ __forceinline__ uint32_t Pack2(float a, float b) {
 
 constexpr int kThreads = 256;
 constexpr int kSlice = 4096;                // tokens of a workgroup
-constexpr uint32_t kInPrompt = 0x80000000u;  // of a count: seen, whether made or not
+// A token's word in LDS: how often it was made (up to 2^20), whether the prompt has it,
+// and above that the last entry of the biases that names it, + 1.
+constexpr uint32_t kInPrompt = 1u << 21, kMade = kInPrompt - 1;
+constexpr int kBiasShift = 22;
+static_assert(kMaxBiases < 1 << (32 - kBiasShift) && kMaxHistory <= kMade, "fields of a word");
 
 // The parameters of a row.
 struct Row {
@@ -67,129 +71,162 @@ struct Row {
 };
 __device__ __forceinline__ float Edited(float x, uint32_t count, const Row& r) {
   x = x > 0.0f ? x / r.repetition : x * r.repetition;
-  const uint32_t made = count & ~kInPrompt;
+  const uint32_t made = count & kMade;
   return made != 0 ? x - r.frequency * static_cast<float>(made) - r.presence : x;
 }
 
+// -inf, in 16 bits twice
+template <typename T>
+constexpr uint32_t kLow = __is_same(T, BF16) ? 0xFF80FF80u : __is_same(T, F16) ? 0xFC00FC00u : 0xFF800000u;
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void EditKernel(EditArgs a) {
-  constexpr int kPer = 16 / kBytes<T>;                  // tokens of a load
-  constexpr int kLoads = kSlice / (kThreads * kPer);    // loads of a thread
-  __shared__ uint32_t count[kSlice];
-  __shared__ uint32_t biased[kSlice];  // the last entry of the list that names the token, + 1
+  constexpr int kPer = 16 / kBytes<T>;                // tokens of a load
+  constexpr int kLoads = kSlice / (kThreads * kPer);  // loads of a thread
+  __shared__ __align__(16) uint32_t count[kSlice];
+  __shared__ float bias_of[kMaxBiases];
+  __shared__ uint32_t touched[kSlice / 32];  // a bit for each token that history or biases name
   const int row = blockIdx.y, base = blockIdx.x * kSlice, tid = threadIdx.x;
   const int size = min(kSlice, a.vocab - base);
   const char* in = a.logits + row * a.row_bytes + static_cast<int64_t>(base) * kBytes<T>;
   char* out = a.out + row * a.out_bytes + static_cast<int64_t>(base) * kBytes<T>;
+  // Everything that the first round trip can bring is on its way before anything
+  // is waited for: logits, the history's first tokens (whatever its length), the
+  // list of biases, the row's parameters.
+  // Whole 16 bytes where both rows lie at such places, tokens one by one elsewhere.
+  const bool wide = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  auto place = [&](int j) { return (j * kThreads + tid) * kPer; };
+  U4 x[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const bool here = wide && (in != out || a.mask != nullptr) && place(j) + kPer <= size;
+    x[j] = here ? *reinterpret_cast<const U4*>(in + place(j) * kBytes<T>) : U4{};
+  }
+  constexpr int kIds = 4;  // tokens of a thread that are on their way together
+  const int32_t* ids = a.history + row * a.history_stride;
+  uint32_t at[kIds];
+  const bool history = a.history_size > 0;
+  auto bring = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) at[k] = static_cast<uint32_t>(ids[min(i0 + k * kThreads + tid, a.history_size - 1)]) - base;
+  };
+  if (history) bring(0);
+  uint32_t bias_at = ~0u;
+  float bias_value = 0.0f;
+  if (tid < a.n_biases) {
+    bias_at = static_cast<uint32_t>(a.bias_ids[row * a.bias_ids_stride + tid]) - base;
+    bias_value = a.bias[row * a.bias_stride + tid];
+  }
+  Row r = {1.0f, 0.0f, 0.0f};
+  if (a.repetition != nullptr) r.repetition = a.repetition[row];
+  if (a.presence != nullptr) r.presence = a.presence[row];
+  if (a.frequency != nullptr) r.frequency = a.frequency[row];
+  const int n = a.history_lens != nullptr ? max(0, min(a.history_lens[row], a.history_size)) : a.history_size;
+  const int prompt = a.prompts != nullptr ? a.prompts[row] : 0;
   const int mask_row = a.mask == nullptr ? -1 : a.mask_rows != nullptr ? a.mask_rows[row] : row;
+#pragma unroll
+  for (int i = 0; i < kSlice; i += 4 * kThreads) {
+    *reinterpret_cast<U4*>(&count[i + 4 * tid]) = U4{};
+  }
+  if (tid < kSlice / 32) touched[tid] = 0;
   const uint32_t* mask = mask_row >= 0 && mask_row < a.n_masks
                              ? reinterpret_cast<const uint32_t*>(a.mask) + mask_row * a.mask_stride + base / 32
                              : nullptr;
   // Where nothing but single tokens changes and the row stays where it is, only
   // those are touched.
   const bool sparse = in == out && mask == nullptr;
-  // Whole 16 bytes where both rows lie at such places, tokens one by one elsewhere.
-  const bool wide = ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  U4 x[kLoads];
-  if (wide && !sparse) {
+  uint32_t word[kLoads];  // of the mask (32 tokens hold whole loads)
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int at = (j * kThreads + tid) * kPer;
-      x[j] = at + kPer <= size ? *reinterpret_cast<const U4*>(in + at * kBytes<T>) : U4{};
+  for (int j = 0; j < kLoads; ++j)
+    word[j] = mask != nullptr && wide && place(j) + kPer <= size ? mask[place(j) / 32] : ~0u;
+  if (!(r.repetition > 0.0f)) r.repetition = 1.0f;
+  __syncthreads();
+  if (history) {
+    for (int i0 = 0;;) {
+#pragma unroll
+      for (int k = 0; k < kIds; ++k) {
+        const int i = i0 + k * kThreads + tid;
+        if (i >= n || at[k] >= static_cast<uint32_t>(size)) continue;
+        if (i < prompt)
+          atomicOr(&count[at[k]], kInPrompt);
+        else
+          atomicAdd(&count[at[k]], 1u);
+        atomicOr(&touched[at[k] / 32], 1u << (at[k] % 32));
+      }
+      i0 += kIds * kThreads;
+      if (i0 >= n) break;
+      bring(i0);
     }
   }
-  const bool lists = a.history != nullptr || a.bias_ids != nullptr;
-  Row r = {1.0f, 0.0f, 0.0f};
-  if (lists) {
-    for (int i = tid; i < kSlice; i += kThreads) count[i] = 0;
-    if (a.bias_ids != nullptr)
-      for (int i = tid; i < kSlice; i += kThreads) biased[i] = 0;
-    __syncthreads();
-    if (a.history != nullptr) {
-      if (a.repetition != nullptr) {
-        r.repetition = a.repetition[row];
-        if (!(r.repetition > 0.0f)) r.repetition = 1.0f;
+  __syncthreads();
+  if (a.n_biases > 0) {
+    for (int i = tid; i < a.n_biases; i += kThreads) {
+      if (i != tid) {
+        bias_at = static_cast<uint32_t>(a.bias_ids[row * a.bias_ids_stride + i]) - base;
+        bias_value = a.bias[row * a.bias_stride + i];
       }
-      if (a.presence != nullptr) r.presence = a.presence[row];
-      if (a.frequency != nullptr) r.frequency = a.frequency[row];
-      const int n = a.history_lens != nullptr ? max(0, min(a.history_lens[row], a.history_size)) : a.history_size;
-      const int prompt = a.prompts != nullptr ? a.prompts[row] : 0;
-      const int32_t* ids = a.history + row * a.history_stride;
-      constexpr int kIds = 4;  // on their way together
-      for (int i0 = tid; i0 < n; i0 += kIds * kThreads) {
-        uint32_t at[kIds];
-#pragma unroll
-        for (int k = 0; k < kIds; ++k) at[k] = static_cast<uint32_t>(ids[min(i0 + k * kThreads, n - 1)]) - base;
-#pragma unroll
-        for (int k = 0; k < kIds; ++k) {
-          const int i = i0 + k * kThreads;
-          if (i >= n || at[k] >= static_cast<uint32_t>(size)) continue;
-          if (i < prompt)
-            atomicOr(&count[at[k]], kInPrompt);
-          else
-            atomicAdd(&count[at[k]], 1u);
-        }
-      }
-    }
-    if (a.bias_ids != nullptr) {
-      const int32_t* ids = a.bias_ids + row * a.bias_ids_stride;
-      for (int i = tid; i < a.n_biases; i += kThreads) {
-        const uint32_t at = static_cast<uint32_t>(ids[i]) - base;
-        if (at < static_cast<uint32_t>(size)) atomicMax(&biased[at], static_cast<uint32_t>(i) + 1);
-      }
+      bias_of[i] = bias_value;
+      if (bias_at >= static_cast<uint32_t>(size)) continue;
+      // (entries of one token differ in the upper bits alone)
+      const uint32_t low = count[bias_at] & (kInPrompt | kMade);
+      atomicMax(&count[bias_at], static_cast<uint32_t>(i + 1) << kBiasShift | low);
+      atomicOr(&touched[bias_at / 32], 1u << (bias_at % 32));
     }
     __syncthreads();
   }
-  const float* bias = a.bias + row * a.bias_stride;
-  auto edit = [&](float v, int at, uint32_t word) {
-    if (lists) {
-      const uint32_t c = count[at];
-      if (c != 0) v = Edited(v, c, r);
-      if (a.bias_ids != nullptr) {
-        const uint32_t b = biased[at];
-        if (b != 0) v += bias[b - 1];
-      }
-    }
-    return (word >> (at % 32)) & 1 ? v : -__builtin_inff();
+  auto edit = [&](float v, int at) {
+    const uint32_t c = count[at];
+    if ((c & (kInPrompt | kMade)) != 0) v = Edited(v, c, r);
+    return c >> kBiasShift != 0 ? v + bias_of[(c >> kBiasShift) - 1] : v;
   };
-  auto untouched = [&](int at) {
-    return !lists || (count[at] == 0 && (a.bias_ids == nullptr || biased[at] == 0));
-  };
-  auto word_of = [&](int at) { return mask != nullptr ? mask[at / 32] : ~0u; };
   if (wide) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int at = (j * kThreads + tid) * kPer;  // (32 tokens of a mask's word hold whole loads)
+      const int at = place(j);
       if (at + kPer > size) continue;
+      const uint32_t here = touched[at / 32] >> (at % 32) & ((1u << kPer) - 1);
       if (sparse) {
-        bool same = true;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) same = same && untouched(at + e);
-        if (same) continue;
+        if (here == 0) continue;
         x[j] = *reinterpret_cast<const U4*>(in + at * kBytes<T>);
       }
-      const uint32_t word = word_of(at);
-      U4 y;
-      if constexpr (kBytes<T> == 4) {
+      U4 y = x[j];
+      if (here != 0) {
+        if constexpr (kBytes<T> == 4) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(edit(Get<T>(x[j], e), at + e, word));
-      } else {
+          for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(edit(Get<T>(y, e), at + e));
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          y[e / 2] = Pack2<T>(edit(Get<T>(x[j], e), at + e, word), edit(Get<T>(x[j], e + 1), at + e + 1, word));
+          for (int e = 0; e < 8; e += 2) y[e / 2] = Pack2<T>(edit(Get<T>(y, e), at + e), edit(Get<T>(y, e + 1), at + e + 1));
+        }
+      }
+      if (mask != nullptr) {
+        const uint32_t bits = word[j] >> (at % 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t keep;
+          if constexpr (kBytes<T> == 4)
+            keep = 0u - (bits >> e & 1);
+          else
+            keep = ((0u - (bits >> (2 * e) & 1)) & 0xFFFFu) | (0u - (bits >> (2 * e + 1) & 1)) << 16;
+          y[e] = (y[e] & keep) | (kLow<T> & ~keep);
+        }
       }
       *reinterpret_cast<U4*>(out + at * kBytes<T>) = y;
     }
   }
   // What is left of a row, or all of it.
   for (int at = (wide ? size / kPer * kPer : 0) + tid; at < size; at += kThreads) {
-    if (sparse && untouched(at)) continue;
-    const uint32_t word = word_of(at);
+    const bool here = touched[at / 32] >> (at % 32) & 1;
+    if (sparse && !here) continue;
+    const bool low = mask != nullptr && !(mask[at / 32] >> (at % 32) & 1);
     if constexpr (kBytes<T> == 4) {
-      reinterpret_cast<float*>(out)[at] = edit(reinterpret_cast<const float*>(in)[at], at, word);
+      float v = reinterpret_cast<const float*>(in)[at];
+      if (here) v = edit(v, at);
+      reinterpret_cast<float*>(out)[at] = low ? -__builtin_inff() : v;
     } else {
-      const U4 one = {reinterpret_cast<const uint16_t*>(in)[at], 0, 0, 0};
-      reinterpret_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(Pack2<T>(edit(Get<T>(one, 0), at, word), 0.0f));
+      uint32_t v = reinterpret_cast<const uint16_t*>(in)[at];
+      if (here) v = Pack2<T>(edit(Get<T>(U4{v, 0, 0, 0}, 0), at), 0.0f);
+      reinterpret_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(low ? kLow<T> : v);
     }
   }
 }

@@ -588,7 +588,7 @@ int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t n_rows, in
           if (p != nullptr) CheckPointer("a row parameter", p, 4);
         if (e.history != nullptr) {
           CheckList("history", e.history, n_rows == 1 ? 0 : e.history_stride);
-          RPG_CHECK(e.history_size >= 0 && e.history_size <= 1 << 24, "a history of %d tokens", e.history_size);
+          RPG_CHECK(e.history_size >= 0 && e.history_size <= rows::kMaxHistory, "a history of %d tokens", e.history_size);
           a.history = e.history;
           a.history_stride = n_rows == 1 ? 0 : e.history_stride;
           a.history_size = e.history_size;
@@ -606,7 +606,7 @@ int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t n_rows, in
         if (e.bias_ids != nullptr) {
           CheckList("bias_ids", e.bias_ids, n_rows == 1 ? 0 : e.bias_ids_stride);
           CheckList("bias", e.bias, n_rows == 1 ? 0 : e.bias_stride);
-          RPG_CHECK(e.n_biases >= 0 && e.n_biases <= 1 << 24, "%d biases", e.n_biases);
+          RPG_CHECK(e.n_biases >= 0 && e.n_biases <= rows::kMaxBiases, "%d biases", e.n_biases);
           a.bias_ids = e.bias_ids;
           a.bias = e.bias;
           a.bias_ids_stride = n_rows == 1 ? 0 : e.bias_ids_stride;
