@@ -173,6 +173,10 @@ struct CodesState {
   }
 };
 
+// Waves to a SIMD unit.
+template <typename T, int kDim>
+constexpr int kMinWaves = kBytes<T> == 4 ? 2 : kDim == 128 ? 3 : 4;
+
 // The workgroup's range over a cache of codes.
 template <typename C, typename T, int kDim>
 __device__ __forceinline__ void DecodeCodeRows(const CodesAttentionArgs& args, DecodePlace at, DecodeRange range) {
@@ -193,7 +197,7 @@ __device__ __forceinline__ void DecodeCodeRows(const CodesAttentionArgs& args, D
 
 // grid (sequence x key head x block of 16 query heads, key range)
 template <typename C, typename T, int kDim>
-__global__ __launch_bounds__(64 * kWaves, 2) void CodesDecodeKernel(CodesAttentionArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (kMinWaves<T, kDim>)) void CodesDecodeKernel(CodesAttentionArgs a) {
   const DecodePlace at = PlaceOf(a.a);
   DecodeRange range;
   if (!WholeRange(a.a, at.seq, &range)) return;
@@ -202,7 +206,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void CodesDecodeKernel(CodesAttenti
 
 // The positions of a sequence behind those that its group has in common.
 template <typename C, typename T, int kDim>
-__global__ __launch_bounds__(64 * kWaves, 2) void CodesOwnKernel(CodesSharedArgs a) {
+__global__ __launch_bounds__(64 * kWaves, (kMinWaves<T, kDim>)) void CodesOwnKernel(CodesSharedArgs a) {
   const DecodePlace at = PlaceOf(a.c.a);
   DecodeRange range;
   if (!OwnRange(a.c.a, a.groups, static_cast<int>(a.prefix_splits), at.seq, 0.0f, &range)) return;

@@ -203,6 +203,7 @@ __global__ __launch_bounds__(256) void AppendCodesKernel(CodesAppendArgs args) {
 
 // Rows of a thread, as in paged_append.hip.
 constexpr int kManyTokens = 1024;
+constexpr int kReadEach = 4;
 
 template <typename C, typename T, int kDim>
 void LaunchAppend(const CodesAppendArgs& args, hipStream_t s) {
@@ -218,47 +219,57 @@ void LaunchAppend(const CodesAppendArgs& args, hipStream_t s) {
   HIP_CHECK(hipGetLastError());
 }
 
-// grid (token, kEach x 256 / kLanes rows of it): the token's key heads, then its
-// value heads. Positions of unnamed pages give zeros.
+// grid (kEach tokens, 256 / kLanes rows of them): a token's rows are its key heads, then
+// its value heads. Positions of unnamed pages give zeros.
 template <typename C, typename T, int kDim, int kEach>
 __global__ __launch_bounds__(256) void ReadCodesKernel(CodesReadArgs a) {
   constexpr int kPer = 16 / kBytes<T>;
   constexpr int kLanes = kDim / kPer;
   constexpr int kRows = 256 / kLanes;
-  const int t = blockIdx.x;
+  const int t0 = blockIdx.x * kEach;
   const int c = threadIdx.x % kLanes;
-  const int rows = 2 * a.c.n_kv;
-  const int row0 = blockIdx.y * (kEach * kRows) + threadIdx.x / kLanes;
-  Sequence x;
-  if (!FindSequence(a.s, [&](int end, int) { return end <= t; }, &x)) return;
-  const int pos = x.len - x.n_new + (t - x.first);
-  if (t < x.first || pos < 0) return;
-  const int page = PageAt(a.c, a.s.table + x.seq * a.s.table_stride, pos);
-  const int r = pos & ((1 << a.c.page_log2) - 1);
-  const int64_t in_cache = max(page, 0) * a.c.page_bytes + r * static_cast<int64_t>(a.c.row_bytes) + kPer * c;
-  const int64_t in_scales = max(page, 0) * a.scales.page_bytes + 4 * r;
+  const int row = blockIdx.y * kRows + threadIdx.x / kLanes, at_row = min(row, 2 * a.c.n_kv - 1);
+  const bool is_v = at_row >= a.c.n_kv;
+  const int head = is_v ? at_row - a.c.n_kv : at_row;
+  // The tokens' places: mostly of one sequence.
+  int pos[kEach];
+  const int32_t* table[kEach];
+  Sequence x = {};
+  bool in = false;
+  int end = t0;  // of what is known
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int t = t0 + k;
+    if (t >= end && t < a.s.n_tokens) {
+      in = FindSequence(a.s, [&](int e, int) { return e <= t; }, &x);
+      end = in && t >= x.first ? x.first + x.n_new : t + 1;
+    }
+    pos[k] = in && t >= x.first && t < a.s.n_tokens ? x.len - x.n_new + (t - x.first) : -1;
+    table[k] = a.s.table + x.seq * a.s.table_stride;
+  }
+  int page[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) page[k] = pos[k] >= 0 ? PageAt(a.c, table[k], pos[k]) : -1;
   uint32_t codes[kEach][kPer / 4];
   float scale[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int row = min(row0 + k * kRows, rows - 1);
-    const bool is_v = row >= a.c.n_kv;
-    const int head = is_v ? row - a.c.n_kv : row;
-    const char* from = (is_v ? a.c.v : a.c.k) + head * a.c.head_bytes + in_cache;
+    const int r = max(pos[k], 0) & ((1 << a.c.page_log2) - 1);
+    const char* from = (is_v ? a.c.v : a.c.k) + head * a.c.head_bytes + max(page[k], 0) * a.c.page_bytes +
+                       r * static_cast<int64_t>(a.c.row_bytes) + kPer * c;
     if constexpr (kPer == 8) {
       const U2 u = *reinterpret_cast<const U2*>(from);
       codes[k][0] = u[0], codes[k][1] = u[1];
     } else {
       codes[k][0] = *reinterpret_cast<const uint32_t*>(from);
     }
-    scale[k] = *reinterpret_cast<const float*>((is_v ? a.scales.v : a.scales.k) + head * a.scales.head_bytes + in_scales);
+    scale[k] = *reinterpret_cast<const float*>((is_v ? a.scales.v : a.scales.k) + head * a.scales.head_bytes +
+                                               max(page[k], 0) * a.scales.page_bytes + 4 * r);
   }
+  const Rows& to = is_v ? a.v : a.k;
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int row = row0 + k * kRows;
-    if (row >= rows) continue;
-    const bool is_v = row >= a.c.n_kv;
-    const int head = is_v ? row - a.c.n_kv : row;
+    if (pos[k] < 0 || row >= 2 * a.c.n_kv) continue;
     float y[kPer];
 #pragma unroll
     for (int w = 0; w < kPer / 4; ++w) {
@@ -266,19 +277,26 @@ __global__ __launch_bounds__(256) void ReadCodesKernel(CodesReadArgs a) {
       y[4 * w] = lo[0], y[4 * w + 1] = lo[1], y[4 * w + 2] = hi[0], y[4 * w + 3] = hi[1];
     }
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) y[i] = page >= 0 ? y[i] * scale[k] : 0.0f;
-    const Rows& to = is_v ? a.v : a.k;
-    *reinterpret_cast<U4*>(to.p + t * to.token_bytes + head * to.head_bytes + 16 * c) = Narrow<T, kPer>(y);
+    for (int i = 0; i < kPer; ++i) y[i] = page[k] >= 0 ? y[i] * scale[k] : 0.0f;
+    *reinterpret_cast<U4*>(to.p + (t0 + k) * to.token_bytes + head * to.head_bytes + 16 * c) = Narrow<T, kPer>(y);
   }
+}
+
+template <typename C, typename T, int kDim, int kEach>
+void LaunchReadEach(const CodesReadArgs& a, hipStream_t s) {
+  constexpr int kPass = 256 * 16 / (kDim * kBytes<T>);
+  const uint32_t n = static_cast<uint32_t>(CeilDiv(a.s.n_tokens, kEach));
+  RPG_CHECK(n <= kMaxGroups, "%d tokens in one launch", a.s.n_tokens);
+  ReadCodesKernel<C, T, kDim, kEach><<<dim3(n, static_cast<uint32_t>(CeilDiv(2 * a.c.n_kv, kPass))), 256, 0, s>>>(a);
+  HIP_CHECK(hipGetLastError());
 }
 
 template <typename C, typename T, int kDim>
 void LaunchRead(const CodesReadArgs& a, hipStream_t s) {
-  constexpr int kPass = 256 * 16 / (kDim * kBytes<T>);
-  const uint32_t n = static_cast<uint32_t>(a.s.n_tokens);
-  RPG_CHECK(n <= kMaxGroups, "%u tokens in one launch", n);
-  ReadCodesKernel<C, T, kDim, 1><<<dim3(n, static_cast<uint32_t>(CeilDiv(2 * a.c.n_kv, kPass))), 256, 0, s>>>(a);
-  HIP_CHECK(hipGetLastError());
+  if (a.s.n_tokens >= kManyTokens * kReadEach)
+    LaunchReadEach<C, T, kDim, kReadEach>(a, s);
+  else
+    LaunchReadEach<C, T, kDim, 1>(a, s);
 }
 
 }  // namespace
