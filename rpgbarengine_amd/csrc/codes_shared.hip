@@ -1,0 +1,74 @@
+// Attention of one token per sequence over a cache of 8-bit codes where the first
+// positions of a group's sequences lie in the same pages (rpg_hip_quant_shared,
+// include/rpg_hip.h): as paged_shared.hip has it, with the products of
+// codes_prompt.hip and codes_decode.hip.
+
+#include <hip/hip_runtime.h>
+
+#include "codes_decode_body.h"
+#include "codes_dev.h"
+#include "codes_prompt_body.h"
+#include "common.h"
+#include "decode_body.h"
+#include "groups.h"
+#include "paged.h"
+#include "paged_dev.h"
+
+namespace rpg {
+namespace paged {
+namespace {
+
+// Grid: as SharedKernel's (paged_shared.hip). kWide: tiles of 128 rows, of 32 otherwise.
+template <typename C, typename T, int kDim, bool kWide>
+__global__ __launch_bounds__(256, kWide || kBytes<T> == 2 ? 2 : 1) void CodesSharedKernel(CodesSharedArgs args, SharedGrid g) {
+  const AttentionArgs& a = args.c.a;
+  __shared__ __align__(256) union {
+    std::conditional_t<kWide, WideLds<T, kDim>, SoloLds<kDim, 4>> prefix;
+    DecodeLds<kDim> own;
+  } shared;
+  const int prefix_splits = static_cast<int>(args.prefix_splits);
+  const int b = blockIdx.x;
+  if (b < g.prefix) {
+    const int bx = b % g.prefix_x, by = b / g.prefix_x;
+    if constexpr (kWide)
+      WideBody<C, T, kDim, true>(args.c, args.groups, prefix_splits, shared.prefix, bx, by, g.prefix_x);
+    else
+      SoloBody<C, T, kDim, 4, true>(args.c, args.groups, prefix_splits, shared.prefix, bx, by, g.prefix_x);
+  } else {
+    const DecodePlace at = PlaceOf(a, (b - g.prefix) % g.own_x);
+    const int y = a.splits - prefix_splits - 1 - (b - g.prefix) / g.own_x;
+    DecodeRange range;
+    if (!OwnRange(a, args.groups, prefix_splits, at.seq, y, 0.0f, &range)) return;
+    DecodeCodeRows<C, T, kDim>(args.c, shared.own, at, range);
+  }
+}
+
+template <typename C, typename T, int kDim>
+void Launch(const CodesSharedArgs& args, hipStream_t s) {
+  const AttentionArgs& a = args.c.a;
+  SharedArgs rows;
+  rows.a = a;
+  rows.groups = args.groups;
+  rows.prefix_splits = args.prefix_splits;
+  const bool wide = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv) == 128;
+  const SharedGrid g = GridOf(rows, wide ? 128 : kSoloRows);
+  const uint32_t n = static_cast<uint32_t>(g.prefix + g.own);
+  if (wide)
+    CodesSharedKernel<C, T, kDim, true><<<n, 256, 0, s>>>(args, g);
+  else
+    CodesSharedKernel<C, T, kDim, false><<<n, 256, 0, s>>>(args, g);
+  HIP_CHECK(hipGetLastError());
+  SharedJoin(rows, s);
+}
+
+}  // namespace
+
+void SharedCodes(const CodesSharedArgs& a, hipStream_t s) {
+  if (a.c.a.s.n_seqs == 0) return;
+  ByTypes(a.c.code, a.c.a.c, [&](auto code, auto type, auto dim) {
+    Launch<decltype(code), decltype(type), decltype(dim)::value>(a, s);
+  });
+}
+
+}  // namespace paged
+}  // namespace rpg

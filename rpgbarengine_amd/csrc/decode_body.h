@@ -181,13 +181,20 @@ struct State {
   }
 };
 
+template <int kDim>
+struct DecodeLds {
+  float so[kWaves][kCols][kDim + 4];
+  float sm[kWaves][kCols], sl[kWaves][kCols];
+};
+
 // Tiles of the range are brought by load(tile, pos), the queries by load_q(q, column),
 // and added up in a State; the waves' states are joined in LDS. T: of the rows.
 template <typename T, int kDim, typename Tl, typename St, typename Load, typename LoadQ>
-__device__ __forceinline__ void DecodeBody(const AttentionArgs& a, int seq, int h0, int n_cols, DecodeRange range,
-                                           Load&& load, LoadQ&& load_q) {
-  __shared__ float sm[kWaves][kCols], sl[kWaves][kCols];
-  __shared__ __align__(16) float so[kWaves][kCols][kDim + 4];
+__device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDim>& shared, int seq, int h0, int n_cols,
+                                           DecodeRange range, Load&& load, LoadQ&& load_q) {
+  auto& sm = shared.sm;
+  auto& sl = shared.sl;
+  auto& so = shared.so;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   St st;
   if (range.start < range.end) {
@@ -241,35 +248,36 @@ __device__ __forceinline__ void DecodeBody(const AttentionArgs& a, int seq, int 
   }
 }
 
-// The workgroup's sequence, key head and query heads: grid x is sequence x key head
-// x block of 16 query heads.
+// The workgroup's sequence, key head and query heads: bx counts sequence x key head x
+// block of 16 query heads.
 struct DecodePlace {
   int seq, kh, h0, n_cols;
 };
-__device__ __forceinline__ DecodePlace PlaceOf(const AttentionArgs& a) {
+__device__ __forceinline__ DecodePlace PlaceOf(const AttentionArgs& a, int bx) {
   const int group = a.n_heads / a.c.n_kv, blocks = (group + kCols - 1) / kCols;
-  const int hb = blockIdx.x % blocks, kh = blockIdx.x / blocks % a.c.n_kv, seq = blockIdx.x / blocks / a.c.n_kv;
+  const int hb = bx % blocks, kh = bx / blocks % a.c.n_kv, seq = bx / blocks / a.c.n_kv;
   return {seq, kh, kh * group + hb * kCols, min(kCols, group - hb * kCols)};
 }
 
-// Range blockIdx.y of all of a sequence's positions; false: there is no such range.
-__device__ __forceinline__ bool WholeRange(const AttentionArgs& a, int seq, DecodeRange* out) {
+// Range `y` of all of a sequence's positions; false: there is no such range.
+__device__ __forceinline__ bool WholeRange(const AttentionArgs& a, int seq, int y, DecodeRange* out) {
   const int len = Length(a.s, seq);
-  const int range = RangeOf(max(len, 1), a.splits), start = blockIdx.y * range;
-  *out = {start, min(len, start + range), range >= len, static_cast<int>(blockIdx.y), 0.0f};
-  return out->start < out->end || blockIdx.y == 0;
+  const int range = RangeOf(a, max(len, 1), a.splits), start = y * range;
+  *out = {start, min(len, start + range), range >= len, y, 0.0f};
+  return out->start < out->end || y == 0;
 }
 
 // The workgroup's range over a cache of rows.
 template <typename T, int kDim>
-__device__ __forceinline__ void DecodeRows(const AttentionArgs& a, DecodePlace at, DecodeRange range) {
+__device__ __forceinline__ void DecodeRows(const AttentionArgs& a, DecodeLds<kDim>& shared, DecodePlace at,
+                                           DecodeRange range) {
   using Tl = Tile<T, kDim>;
   using St = State<T, kDim>;
   const int lane = threadIdx.x & 63;
   const int32_t* table = a.s.table + at.seq * a.s.table_stride;
   const int64_t head_off = at.kh * a.c.head_bytes;
   DecodeBody<T, kDim, Tl, St>(
-      a, at.seq, at.h0, at.n_cols, range,
+      a, shared, at.seq, at.h0, at.n_cols, range,
       [&](Tl& t, int pos) { t.Load(a.c, table, head_off, pos, range.end - 1, lane); },
       [&](typename St::Query& q, int col) {
         const char* qp = a.q.p + at.seq * a.q.token_bytes + (at.h0 + col) * a.q.head_bytes + 16 * (lane >> 4);

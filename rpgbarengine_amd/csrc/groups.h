@@ -38,22 +38,18 @@ __device__ __forceinline__ int CommonKeys(const Seqs& s, const Seqs& groups, int
   return CommonOf(s, x.first, x.n_new, x.len).keys;
 }
 
-// The ranges that `len` positions are cut into, of `splits` at most.
-__device__ __forceinline__ int RangesOf(int len, int splits) {
-  if (len <= 0) return 0;
-  const int range = RangeOf(len, splits);
-  return (len + range - 1) / range;
-}
+// The ranges of `range` positions in `len`.
+__device__ __forceinline__ int RangesOf(int len, int range) { return len <= 0 ? 0 : (len + range - 1) / range; }
 
-// Range blockIdx.y of a sequence's own positions, behind the common ones; false:
+// Range `y` of a sequence's own positions, behind the common ones; false:
 // there is no such range. off: DecodeRange's.
-__device__ __forceinline__ bool OwnRange(const AttentionArgs& a, const Seqs& groups, int prefix_splits, int seq, float off,
-                                         DecodeRange* out) {
+__device__ __forceinline__ bool OwnRange(const AttentionArgs& a, const Seqs& groups, int prefix_splits, int seq, int y,
+                                         float off, DecodeRange* out) {
   const int len = Length(a.s, seq);
   if (len <= 0) return false;
   const int from = CommonKeys(a.s, groups, seq), own = len - from;
-  const int range = RangeOf(max(own, 1), a.splits - prefix_splits), start = from + blockIdx.y * range;
-  *out = {start, min(len, start + range), false, RangesOf(from, prefix_splits) + static_cast<int>(blockIdx.y), off};
+  const int range = RangeOf(a, max(own, 1), a.splits - prefix_splits), start = from + y * range;
+  *out = {start, min(len, start + range), false, RangesOf(from, RangeOf(max(from, 1), prefix_splits)) + y, off};
   return out->start < out->end;
 }
 

@@ -91,6 +91,7 @@ struct AttentionArgs {
   int32_t n_heads = 0;
   float scale = 0.0f;
   int32_t splits = 1;     // key ranges that a query's keys may be cut into
+  int32_t least = 0;      // positions of a range of a decode, where there are so many
   float* work = nullptr;  // partials of the ranges (WorkBytes)
 };
 
@@ -112,6 +113,7 @@ struct CodesAttentionArgs {
   int64_t code = kI8;
 };
 void DecodeCodes(const CodesAttentionArgs& a, hipStream_t s);
+int CodesDecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity, int* least);
 int CodesPromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity);
 void PromptCodes(const CodesAttentionArgs& a, hipStream_t s);
 
@@ -134,14 +136,19 @@ struct CodesSharedArgs {
   int64_t prefix_splits = 1;
 };
 struct SharedSplits {
-  int prefix, own;
+  int prefix, own, least;  // least: AttentionArgs'
 };
 // Rows of the tiles of the common positions: 32, 64 or 128, by what a group has.
 int PrefixRows(int64_t n_seqs, int64_t n_groups, int group);
-SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity);
+SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int bytes, int64_t capacity);
 void Shared(const SharedArgs& a, hipStream_t s);
 void SharedCodes(const CodesSharedArgs& a, hipStream_t s);
-void PrefixCodes(const CodesSharedArgs& a, hipStream_t s);  // its first part
+// Workgroups of a launch: prefix = prefix_x of each range of common positions, then
+// own = own_x of each range of own ones.
+struct SharedGrid {
+  int32_t prefix_x, prefix, own_x, own;
+};
+SharedGrid GridOf(const SharedArgs& a, int rows);
 // Joins what the ranges of either kind leave, of any cache.
 void SharedJoin(const SharedArgs& a, hipStream_t s);
 

@@ -41,17 +41,18 @@ namespace {
 // (64 x 4000 bf16 99 us, 96 so).
 template <typename T, int kDim>
 __global__ __launch_bounds__(64 * kWaves, kDim == 64 && kBytes<T> == 2 ? 4 : 2) void DecodeKernel(AttentionArgs a) {
-  const DecodePlace at = PlaceOf(a);
+  __shared__ __align__(16) DecodeLds<kDim> shared;
+  const DecodePlace at = PlaceOf(a, blockIdx.x);
   DecodeRange range;
-  if (!WholeRange(a, at.seq, &range)) return;
-  DecodeRows<T, kDim>(a, at, range);
+  if (!WholeRange(a, at.seq, blockIdx.y, &range)) return;
+  DecodeRows<T, kDim>(a, shared, at, range);
 }
 
 template <typename T, int kDim>
 __global__ __launch_bounds__(256) void DecodeJoinKernel(AttentionArgs a) {
   const int64_t row = blockIdx.x;
   const int seq = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
-  const int len = Length(a.s, seq), range = RangeOf(max(len, 1), a.splits);
+  const int len = Length(a.s, seq), range = RangeOf(a, max(len, 1), a.splits);
   if (range >= len) return;  // written by its one range
   JoinRow<T, kDim>(a, static_cast<int64_t>(a.s.n_seqs) * a.n_heads, row, (len + range - 1) / range,
                    a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes);

@@ -225,6 +225,11 @@ __device__ __forceinline__ int RangeOf(int len, int splits) {
   return ((len - 1) / splits / kRangeUnit + 1) * kRangeUnit;
 }
 
+// Of a decode with a.least.
+__device__ __forceinline__ int RangeOf(const AttentionArgs& a, int len, int splits) {
+  return max(RangeOf(len, splits), a.least);
+}
+
 // A workgroup's range of positions: [start, end) of a sequence, and where what comes
 // out goes: the output, or partials in a slot of the row's (then other ranges add
 // to it). off: what the range's weights are held above those of other kernels' ranges

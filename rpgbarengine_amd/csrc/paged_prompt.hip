@@ -47,7 +47,8 @@ namespace {
 
 template <typename T, int kDim, int kGroups, bool kShared>
 __global__ __launch_bounds__(kGroups == 8 ? 512 : 256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4 && !kShared) ? 1 : 2) void PromptKernel(AttentionArgs a) {
-  PromptBody<T, kDim, kGroups, kShared, false>(a, a.s, 1);
+  __shared__ __align__(256) PromptLds<T, kDim, kGroups, kShared> shared;
+  PromptBody<T, kDim, kGroups, kShared, false>(a, a.s, 1, shared, blockIdx.x, blockIdx.y, gridDim.x);
 }
 
 // Joins the key ranges of a tile's rows (four groups, 32 rows): workgroup = row.

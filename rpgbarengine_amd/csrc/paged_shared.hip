@@ -13,7 +13,11 @@
 // so nothing is masked but behind the last. The rest is a sequence's own.
 //
 // Bound: the common positions' products (a group of 32 sequences with four heads to a
-// key head multiplies each key 128 times), or the own positions' bytes.
+// key head multiplies each key 128 times) beside the own positions' bytes, and the
+// join. Measured, 32 heads on 8 of 128: 96 sequences in three groups behind 4000 to
+// 12000 positions with 100 to 2500 of their own, bf16, 376 MB, 100.7 us (a large copy's
+// rate: 74); 8 behind 2000, f32, 24.0 (launched one after another 31.8). Workgroups of
+// both kinds in turn instead of the common ones first: 129 and 28.6.
 
 #include <hip/hip_runtime.h>
 
@@ -31,18 +35,27 @@ namespace rpg {
 namespace paged {
 namespace {
 
+// One launch for both, so that the products of the common positions run beside the loads
+// of the others. A sequence's last ranges come first.
 template <typename T, int kDim, int kGroups>
-__global__ __launch_bounds__(256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4) ? 1 : 2) void PrefixKernel(SharedArgs a) {
-  PromptBody<T, kDim, kGroups, false, true>(a.a, a.groups, static_cast<int>(a.prefix_splits));
-}
-
-// grid (sequence x key head x block of 16 query heads, key range)
-template <typename T, int kDim>
-__global__ __launch_bounds__(64 * kWaves, kDim == 64 && kBytes<T> == 2 ? 4 : 2) void OwnKernel(SharedArgs a) {
-  const DecodePlace at = PlaceOf(a.a);
-  DecodeRange range;
-  if (!OwnRange(a.a, a.groups, static_cast<int>(a.prefix_splits), at.seq, kDecodeLift<T>, &range)) return;
-  DecodeRows<T, kDim>(a.a, at, range);
+__global__ __launch_bounds__(256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4) ? 1 : 2) void SharedKernel(SharedArgs args, SharedGrid g) {
+  const AttentionArgs& a = args.a;
+  __shared__ __align__(256) union {
+    PromptLds<T, kDim, kGroups, false> prefix;
+    DecodeLds<kDim> own;
+  } shared;
+  const int prefix_splits = static_cast<int>(args.prefix_splits);
+  const int b = blockIdx.x;
+  if (b < g.prefix) {
+    PromptBody<T, kDim, kGroups, false, true>(a, args.groups, prefix_splits, shared.prefix, b % g.prefix_x,
+                                              b / g.prefix_x, g.prefix_x);
+  } else {
+    const DecodePlace at = PlaceOf(a, (b - g.prefix) % g.own_x);
+    const int y = a.splits - prefix_splits - 1 - (b - g.prefix) / g.own_x;
+    DecodeRange range;
+    if (!OwnRange(a, args.groups, prefix_splits, at.seq, y, kDecodeLift<T>, &range)) return;
+    DecodeRows<T, kDim>(a, shared.own, at, range);
+  }
 }
 
 template <typename T, int kDim>
@@ -53,37 +66,23 @@ __global__ __launch_bounds__(256) void SharedJoinKernel(SharedArgs args) {
   const int seq = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
   const int len = Length(a.s, seq), from = len > 0 ? CommonKeys(a.s, args.groups, seq) : 0;
   JoinRow<T, kDim>(a, static_cast<int64_t>(a.s.n_seqs) * a.n_heads, row,
-                   RangesOf(from, splits) + RangesOf(len - from, a.splits - splits),
+                   RangesOf(from, RangeOf(max(from, 1), splits)) +
+                       RangesOf(len - from, RangeOf(a, max(len - from, 1), a.splits - splits)),
                    a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes);
-}
-
-template <typename T, int kDim, int kGroups>
-void LaunchPrefix(const SharedArgs& args, hipStream_t s) {
-  const AttentionArgs& a = args.a;
-  const int64_t tiles = TilesFor(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv, 128 / kGroups);
-  RPG_CHECK(tiles * a.c.n_kv <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs, a.n_heads);
-  PrefixKernel<T, kDim, kGroups>
-      <<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), static_cast<uint32_t>(args.prefix_splits)), 256, 0, s>>>(args);
-  HIP_CHECK(hipGetLastError());
 }
 
 template <typename T, int kDim>
 void Launch(const SharedArgs& args, hipStream_t s) {
   const AttentionArgs& a = args.a;
-  const int group = a.n_heads / a.c.n_kv;
-  const int64_t x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(group, kCols);
-  RPG_CHECK(static_cast<int64_t>(a.s.n_seqs) * a.n_heads <= kMaxGroups, "%d x %d query rows in one launch", a.s.n_seqs,
-            a.n_heads);
-  if (args.groups.n_seqs > 0) {
-    const int rows = PrefixRows(a.s.n_seqs, args.groups.n_seqs, group);
-    if (rows == 128)
-      LaunchPrefix<T, kDim, 1>(args, s);
-    else if (rows == 64)
-      LaunchPrefix<T, kDim, 2>(args, s);
-    else
-      LaunchPrefix<T, kDim, 4>(args, s);
-  }
-  OwnKernel<T, kDim><<<dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(a.splits - args.prefix_splits)), 64 * kWaves, 0, s>>>(args);
+  const int rows = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv);
+  const SharedGrid g = GridOf(args, rows);
+  const uint32_t n = static_cast<uint32_t>(g.prefix + g.own);
+  if (rows == 128)
+    SharedKernel<T, kDim, 1><<<n, 256, 0, s>>>(args, g);
+  else if (rows == 64)
+    SharedKernel<T, kDim, 2><<<n, 256, 0, s>>>(args, g);
+  else
+    SharedKernel<T, kDim, 4><<<n, 256, 0, s>>>(args, g);
   HIP_CHECK(hipGetLastError());
   SharedJoin(args, s);
 }
@@ -96,18 +95,40 @@ void LaunchJoin(const SharedArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Waves of a tile share its rows where a group has few: 32 rows are four waves' that
+// take the keys in turn.
 int PrefixRows(int64_t n_seqs, int64_t n_groups, int group) {
   const int64_t rows = n_seqs * group / std::max<int64_t>(n_groups, 1);
   return rows > 64 ? 128 : rows > 32 ? 64 : 32;
 }
 
-SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity) {
+SharedGrid GridOf(const SharedArgs& args, int rows) {
+  const AttentionArgs& a = args.a;
+  const int group = a.n_heads / a.c.n_kv;
+  const int64_t tiles = args.groups.n_seqs == 0 ? 0 : TilesFor(a.s.n_seqs, args.groups.n_seqs, group, rows);
+  const int64_t own_x = static_cast<int64_t>(a.s.n_seqs) * a.c.n_kv * CeilDiv(group, kCols);
+  const int64_t prefix = tiles * a.c.n_kv * args.prefix_splits, own = own_x * (a.splits - args.prefix_splits);
+  RPG_CHECK(prefix + own <= kMaxGroups && static_cast<int64_t>(a.s.n_seqs) * a.n_heads <= kMaxGroups,
+            "%d x %d query rows in one launch", a.s.n_seqs, a.n_heads);
+  return {static_cast<int32_t>(std::max<int64_t>(1, tiles * a.c.n_kv)), static_cast<int32_t>(prefix),
+          static_cast<int32_t>(own_x), static_cast<int32_t>(own)};
+}
+
+// Ranges of common positions for one workgroup per compute unit, so that own positions
+// run beside them (96 sequences in three groups behind 4000 to 12000, bf16: 103.4 us
+// aiming at 512 workgroups, 100.7 at 256, 99.5 at 192; 32 behind 30000 63.1, 57.1, 67.8),
+// two in f32, which the products alone keep busy (64 behind 4000: 88.8, 96.9), of 256
+// positions at least (8 behind 2000, f32: 24.0 us, with 512 30.2; 64 behind 64, bf16:
+// 29.2, with 128 31.5). Own ranges as a decode's, none below 512 where the batch fills
+// the card (the 96: 114.7 without a least, 110.8 with 512, 115.9 with 1024).
+SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int bytes, int64_t capacity) {
   const int group = n_heads / n_kv;
   const int64_t tiles = TilesFor(n_seqs, n_groups, group, PrefixRows(n_seqs, n_groups, group));
   const int64_t wgs = std::max<int64_t>(1, tiles * n_kv);
-  const int64_t prefix = std::min({CeilDiv(512, wgs), CeilDiv(capacity, 256), int64_t{kMaxSplits / 2}});
+  const int64_t prefix = std::min({CeilDiv(bytes == 4 ? 512 : 256, wgs), CeilDiv(capacity, 256), int64_t{kMaxSplits / 2}});
   const int own = DecodeSplits(n_seqs, n_heads, n_kv, 2, capacity);
-  return {static_cast<int>(std::max<int64_t>(1, prefix)), std::min(own, kMaxSplits / 2)};
+  const bool full = n_seqs * n_kv * CeilDiv(group, kCols) >= 256;
+  return {static_cast<int>(std::max<int64_t>(1, prefix)), std::min(own, kMaxSplits / 2), full ? 512 : 0};
 }
 
 void Shared(const SharedArgs& a, hipStream_t s) {

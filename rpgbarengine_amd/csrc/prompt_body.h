@@ -131,28 +131,43 @@ __device__ __forceinline__ void LdsDma(U4 src, char* to, int voff, int soff) {
 // with the most keys first. kPrefix: the tiles are of the groups of a.s's sequences
 // (`groups`), one token each; all rows see the positions that their group has in
 // common, and what comes out are partials, of prefix_splits ranges at most.
-template <typename T, int kDim, int kGroups, bool kShared, bool kPrefix>
-__device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& groups, int prefix_splits) {
+template <typename T, int kDim, int kGroups, bool kShared>
+struct PromptLds {
   using Sh = Shape<T, kDim, kGroups>;
   // A group of one wave needs no barriers: it takes the next K tile in as soon as
   // the scores are done and the next V tile after the second product, each in the
   // place of the last (half the LDS: two workgroups per compute unit). Groups of
   // several waves have two of each in turn.
-  constexpr bool kSolo = Sh::kGroupWaves == 1;
+  static constexpr bool kSolo = Sh::kGroupWaves == 1;
   // kShared: K and V take turns in one place, so that two workgroups fit a compute
   // unit even in f32: the other's products run while a tile is on its way.
   static_assert(kSolo || !kShared, "groups of one wave");
-  constexpr int kTiles = kShared ? 1 : kSolo ? 2 : 4;
-  __shared__ __align__(256) char lds[kGroups * kTiles * Sh::kTileBytes];  // per group [buffer][K tile, V tile]
-  __shared__ uint32_t page_ok[kGroups][2];     // per buffer: a byte for each unit of rows
-  __shared__ int any_odd, first_odd[kOddKinds][kDim];
+  static constexpr int kTiles = kShared ? 1 : kSolo ? 2 : 4;
+  char tiles[kGroups * kTiles * Sh::kTileBytes];  // per group [buffer][K tile, V tile]
+  uint32_t page_ok[kGroups][2];                   // per buffer: a byte for each unit of rows
+  int any_odd, first_odd[kOddKinds][kDim];
+  float sm[kGroups][Sh::kRows], sl[kGroups][Sh::kRows];  // of the groups' join
+};
+
+// bx, by, gx: the workgroup's place in the grid and its width.
+template <typename T, int kDim, int kGroups, bool kShared, bool kPrefix>
+__device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& groups, int prefix_splits,
+                                           PromptLds<T, kDim, kGroups, kShared>& shared, int bx, int by, int gx) {
+  using Sh = Shape<T, kDim, kGroups>;
+  using Lds = PromptLds<T, kDim, kGroups, kShared>;
+  constexpr bool kSolo = Lds::kSolo;
+  constexpr int kTiles = Lds::kTiles;
+  auto& lds = shared.tiles;
+  auto& page_ok = shared.page_ok;
+  auto& any_odd = shared.any_odd;
+  auto& first_odd = shared.first_odd;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int grp = wave / Sh::kGroupWaves, gw = wave % Sh::kGroupWaves;  // the wave's group, its place there
   const int group = a.n_heads / a.c.n_kv;
-  const int kh = blockIdx.x % a.c.n_kv;
+  const int kh = bx % a.c.n_kv;
   int seq;
   RowTile t;
-  if (!TileOf(kPrefix ? groups : a.s, group, Sh::kRows, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.c.n_kv), &seq, &t))
+  if (!TileOf(kPrefix ? groups : a.s, group, Sh::kRows, (gx - 1 - bx) / a.c.n_kv, &seq, &t))
     return;
   if constexpr (kPrefix) {
     const Common common = CommonOf(a.s, t.first, t.n_rows / group, t.len);
@@ -173,9 +188,9 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
   int key_begin = 0, key_end = max(keys, 0);
   if constexpr (kGroups >= 4 || kPrefix) {
     const int range = RangeOf(max(keys, 1), kPrefix ? prefix_splits : a.splits);
-    key_begin = blockIdx.y * range;
+    key_begin = by * range;
     key_end = min(key_end, key_begin + range);
-    if (key_begin >= key_end && (kPrefix || blockIdx.y > 0)) return;
+    if (key_begin >= key_end && (kPrefix || by > 0)) return;
   }
   // steps of the workgroup: a step of every group each
   const int steps = key_end <= key_begin ? 0 : (key_end - key_begin - 1) / (Sh::kKeys * kGroups) + 1;
@@ -536,8 +551,8 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
       if (row0 + 32 * gw + (lane & 31) < n_rows) {
         const int64_t rows = static_cast<int64_t>(a.s.n_seqs) * a.n_heads;
         const int64_t out_row = static_cast<int64_t>(first + token) * a.n_heads + head;
-        if (h == 0) PartStats(a, out_row)[blockIdx.y] = F2{m - kLift<T>, l};
-        float* to = PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(blockIdx.y) * kDim;
+        if (h == 0) PartStats(a, out_row)[by] = F2{m - kLift<T>, l};
+        float* to = PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(by) * kDim;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           if constexpr (kBytes<T> == 4 && kDim == 128)
@@ -574,7 +589,8 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
     }
   } else {
     // The groups' states, joined in LDS where the tiles were.
-    __shared__ float sm[kGroups][Sh::kRows], sl[kGroups][Sh::kRows];
+    auto& sm = shared.sm;
+    auto& sl = shared.sl;
     static_assert(kGroups == 1 || Sh::kRows * kDim * 4 <= kTiles * Sh::kTileBytes, "a group's state fits its tiles");
     // chunk c (four dimensions) of row r of group g
     auto at = [&](int g, int r, int c) {
@@ -627,8 +643,8 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
       } else {
         const int64_t rows = static_cast<int64_t>(kPrefix ? a.s.n_seqs : a.s.n_tokens) * a.n_heads;
         const int64_t out_row = static_cast<int64_t>(first + token_i) * a.n_heads + head_i;
-        if (d == 0) PartStats(a, out_row)[blockIdx.y] = F2{kPrefix ? mi - kLift<T> : mi, li};
-        *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(blockIdx.y) * kDim + d) = x;
+        if (d == 0) PartStats(a, out_row)[by] = F2{kPrefix ? mi - kLift<T> : mi, li};
+        *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, out_row) + static_cast<int64_t>(by) * kDim + d) = x;
       }
     }
   }

@@ -189,10 +189,11 @@ void CheckHeads(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads) {
             "%d x %d query rows", std::max(s.n_tokens, s.n_seqs), n_heads);
 }
 
-int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt, bool codes) {
+int Splits(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt, bool codes, int* least) {
+  *least = 0;
   const int bytes = ElementBytes(static_cast<int32_t>(c.type));
   if (codes && prompt) return paged::CodesPromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, s.capacity);
-  if (codes) return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, 2, s.capacity);
+  if (codes) return paged::CodesDecodeSplits(s.n_seqs, n_heads, c.n_kv, s.capacity, least);
   if (prompt) return paged::PromptSplits(s.n_tokens, s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
   return paged::DecodeSplits(s.n_seqs, n_heads, c.n_kv, bytes, s.capacity);
 }
@@ -203,7 +204,8 @@ bool Empty(const paged::Seqs& s, bool packed) { return s.n_seqs == 0 || (packed 
 int64_t AttentionWork(const paged::Cache& c, const paged::Seqs& s, int32_t n_heads, bool prompt, bool codes) {
   if (Empty(s, prompt)) return 0;
   const int64_t rows = static_cast<int64_t>(prompt ? s.n_tokens : s.n_seqs) * n_heads;
-  return paged::WorkBytes(rows, c.head_dim, Splits(c, s, n_heads, prompt, codes));
+  int least;
+  return paged::WorkBytes(rows, c.head_dim, Splits(c, s, n_heads, prompt, codes, &least));
 }
 
 void CheckWork(void* work, int64_t work_bytes, int64_t need) {
@@ -226,7 +228,7 @@ void AttentionRows(paged::AttentionArgs* to, const rpg_hip_rows* q, const rpg_hi
 }
 
 void AttentionParts(paged::AttentionArgs* a, bool prompt, bool codes, void* work, int64_t work_bytes) {
-  a->splits = Splits(a->c, a->s, a->n_heads, prompt, codes);
+  a->splits = Splits(a->c, a->s, a->n_heads, prompt, codes, &a->least);
   CheckWork(work, work_bytes, AttentionWork(a->c, a->s, a->n_heads, prompt, codes));
   a->work = static_cast<float*>(work);
 }
@@ -265,20 +267,21 @@ int32_t QuantAttention(const rpg_hip_quant_cache* cache, const rpg_hip_sequences
 }
 
 paged::SharedSplits SharedSizes(const paged::Cache& c, const paged::Seqs& s, int32_t n_groups, int32_t n_heads,
-                                int64_t* bytes) {
+                                bool codes, int64_t* bytes) {
   RPG_CHECK(n_groups >= 0, "%d groups", n_groups);
   CheckHeads(c, s, n_heads);
-  const paged::SharedSplits n = paged::SplitsOfShared(s.n_seqs, n_groups, n_heads, c.n_kv, s.capacity);
+  const paged::SharedSplits n = paged::SplitsOfShared(
+      s.n_seqs, n_groups, n_heads, c.n_kv, codes ? 2 : ElementBytes(static_cast<int32_t>(c.type)), s.capacity);
   *bytes = paged::WorkBytes(static_cast<int64_t>(s.n_seqs) * n_heads, c.head_dim, n.prefix + n.own);
   return n;
 }
 
 // The groups, splits and work memory of a call whose rows `a` has.
-paged::Seqs GroupsOf(const rpg_hip_groups* g, paged::AttentionArgs* a, int64_t* prefix_splits, void* work,
+paged::Seqs GroupsOf(const rpg_hip_groups* g, paged::AttentionArgs* a, bool codes, int64_t* prefix_splits, void* work,
                      int64_t work_bytes) {
   RPG_CHECK(g != nullptr, "the groups are null");
   int64_t need;
-  const paged::SharedSplits n = SharedSizes(a->c, a->s, g->n_groups, a->n_heads, &need);
+  const paged::SharedSplits n = SharedSizes(a->c, a->s, g->n_groups, a->n_heads, codes, &need);
   if (g->n_groups > 0) {
     CheckPointer("the groups' starts", g->starts, 4);
     CheckPointer("shared", g->shared, 4);
@@ -286,6 +289,7 @@ paged::Seqs GroupsOf(const rpg_hip_groups* g, paged::AttentionArgs* a, int64_t* 
   CheckWork(work, work_bytes, need);
   a->work = static_cast<float*>(work);
   a->splits = n.prefix + n.own;
+  a->least = n.least;
   *prefix_splits = n.prefix;
   paged::Seqs out;
   out.starts = g->starts;
@@ -504,7 +508,7 @@ int32_t rpg_hip_paged_shared(const rpg_hip_paged_cache* cache, const rpg_hip_seq
         a.a.s = SeqsOf(seqs, cache->page_size, false);
         if (Empty(a.a.s, false)) return 0;
         AttentionRows(&a.a, q, out, a.a.s.n_seqs, n_heads, scale);
-        a.groups = GroupsOf(groups, &a.a, &a.prefix_splits, work, work_bytes);
+        a.groups = GroupsOf(groups, &a.a, false, &a.prefix_splits, work, work_bytes);
         paged::Shared(a, static_cast<hipStream_t>(stream));
         return 0;
       },
@@ -518,7 +522,7 @@ int64_t rpg_hip_paged_shared_work(const rpg_hip_paged_cache* cache, const rpg_hi
         const paged::Cache c = CacheSizes(cache);
         const paged::Seqs s = SeqSizes(seqs, cache->page_size);
         int64_t bytes;
-        SharedSizes(c, s, n_groups, n_heads, &bytes);
+        SharedSizes(c, s, n_groups, n_heads, false, &bytes);
         return Empty(s, false) ? 0 : bytes;
       },
       -1);
@@ -536,7 +540,7 @@ int32_t rpg_hip_quant_shared(const rpg_hip_quant_cache* cache, const rpg_hip_seq
         a.c.a.s = SeqsOf(seqs, cache->page_size, false);
         if (Empty(a.c.a.s, false)) return 0;
         AttentionRows(&a.c.a, q, out, a.c.a.s.n_seqs, n_heads, scale);
-        a.groups = GroupsOf(groups, &a.c.a, &a.prefix_splits, work, work_bytes);
+        a.groups = GroupsOf(groups, &a.c.a, true, &a.prefix_splits, work, work_bytes);
         paged::SharedCodes(a, static_cast<hipStream_t>(stream));
         return 0;
       },
@@ -551,7 +555,7 @@ int64_t rpg_hip_quant_shared_work(const rpg_hip_quant_cache* cache, const rpg_hi
         const paged::Cache c = QuantSizes(cache, type, &scales);
         const paged::Seqs s = SeqSizes(seqs, cache->page_size);
         int64_t bytes;
-        SharedSizes(c, s, n_groups, n_heads, &bytes);
+        SharedSizes(c, s, n_groups, n_heads, true, &bytes);
         return Empty(s, false) ? 0 : bytes;
       },
       -1);
