@@ -7,8 +7,22 @@
 // transposed on 32 x 32 tiles, as in paged_prompt.hip.
 //
 // Few rows (CodesSoloKernel): workgroup (tile of 32 rows, key head, key range), whose
-// waves take blocks of 32 keys in turn, from memory to registers, and join their
-// states in LDS.
+// four or eight waves take blocks of 32 keys in turn, from memory to registers, and
+// join their states in LDS. Many (CodesWideKernel): tiles of 128 rows, a wave for 32;
+// a step's 64 keys go to LDS converted, once for the four waves.
+//
+// Weights times scales are rounded once for bf16 rows, as paged_prompt.hip's are (the
+// output is up to 1.35 times as far from exact as its own rounding leaves it; two
+// parts: four documents 638 us, one 535 at the time).
+//
+// Bound: the vector unit beside the matrix unit: per score a product with either scale
+// comes to the maximum, the exponential and the sum, and the codes' conversion.
+// Measured, 32 heads on 8 of 128: four documents of about 3000 tokens, 392 GFLOP, e4m3
+// in bf16, 477 us (821 TFLOP/s; a large product of a library reaches 1254, the same
+// over a cache of bf16 920); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16,
+// 18.2 us. Tried on documents: products of one 32-key block between the weighing of the
+// other 492 -> 492 (479 without), higher priority around products the same, pages
+// looked up another step ahead the same.
 
 #include <hip/hip_runtime.h>
 
@@ -37,9 +51,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttention
   SoloBody<C, T, kDim, kWaves, false>(a, a.a.s, 1, shared, blockIdx.x, blockIdx.y, gridDim.x);
 }
 
-// Tiles of 128 rows where those fill the compute units.
+// Tiles of 128 rows where those make three workgroups for every two compute units,
+// of 32 otherwise (1000 tokens 42.8 and 34.0 us, 4 x 300 24.2 and 27.6, 2000 82.6 and
+// 90.7).
 bool IsWide(int64_t n_tokens, int64_t n_seqs, int group, int n_kv) {
-  return TilesFor(n_tokens, n_seqs, group, 128) * n_kv >= 256;
+  return TilesFor(n_tokens, n_seqs, group, 128) * n_kv >= 384;
 }
 
 template <typename C, typename T, int kDim>
@@ -56,17 +72,29 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
     HIP_CHECK(hipGetLastError());
     return;
   }
-  CodesSoloKernel<C, T, kDim, 4><<<dim3(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits), 256, 0, s>>>(args);
+  // Eight waves where they find a compute unit to themselves and the keys are many (six
+  // turns 19.2 -> 18.2 us, 200 behind 1300 24.1 -> 22.6; 200 alone 10.0 and 10.9).
+  const int64_t wgs = tiles * a.c.n_kv * a.splits;
+  const dim3 grid(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits);
+  if (kBytes<T> == 2 && wgs <= 256 && a.s.capacity > 256)
+    CodesSoloKernel<C, T, kDim, 8><<<grid, 512, 0, s>>>(args);
+  else
+    CodesSoloKernel<C, T, kDim, 4><<<grid, 256, 0, s>>>(args);
   HIP_CHECK(hipGetLastError());
   if (a.splits > 1) PromptJoin(a, s);
 }
 
 }  // namespace
 
+// Key ranges where not even half the compute units have a workgroup, of 512 positions
+// at least, and as many as find one free; none for rows of up to 1536 positions where
+// a quarter of them have one (f16: 100 behind 1400, 104 workgroups, 25.6 us with two and
+// 22.2 with one, 30 behind 1000, 40 of them, 16.5 with three and 17.4 with one; 12
+// behind 30000 32).
 int CodesPromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
   const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, kSoloRows) * n_kv;
-  if (wgs >= 128) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min({CeilDiv(256, wgs), CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
+  if (wgs >= 128 || (wgs >= 64 && capacity <= 1536)) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min({256 / wgs, CeilDiv(capacity, 512), int64_t{kMaxSplits}})));
 }
 
 void PromptCodes(const CodesAttentionArgs& a, hipStream_t s) {

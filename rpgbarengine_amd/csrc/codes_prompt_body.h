@@ -74,13 +74,19 @@ struct SoloLds {
   float sm[kWaves][kSoloRows], sl[kWaves][kSoloRows];
 };
 
+// Parts of a weight: a prompt's of bf16 rows are rounded once.
+template <typename T, bool kPrefix>
+constexpr int PartsOf() {
+  return __is_same(T, BF16) && !kPrefix ? 1 : kWeightParts<T>;
+}
+
 // Few rows. kPrefix and the last three: as PromptBody's (prompt_body.h).
 template <typename C, typename T, int kDim, int kWaves, bool kPrefix>
 __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const Seqs& groups, int prefix_splits,
                                          SoloLds<kDim, kWaves>& shared, int bx, int by, int gx) {
   const AttentionArgs& a = args.a;
   using K = KeyType<T>;
-  constexpr int kQ = kDim / 16, kBlocks = kDim / 32;
+  constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = PartsOf<T, kPrefix>();
   auto& lds = shared.states;
   auto& sm = shared.sm;
   auto& sl = shared.sl;
@@ -169,7 +175,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      WeightParts<kWeightParts<T>> p;
+      WeightParts<kParts> p;
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -185,7 +191,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
         for (int i = 0; i < 4; ++i)
           x[i] = w % 2 ? Halves2<C, BF16, true>(w < 2 ? lo[i] : hi[i]) : Halves2<C, BF16, false>(w < 2 ? lo[i] : hi[i]);
 #pragma unroll
-        for (int i = kWeightParts<T> - 1; i >= 0; --i) o[w] = Mfma32<BF16>(x, p.x[i], o[w]);
+        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<BF16>(x, p.x[i], o[w]);
       }
     }
     now = next;
@@ -263,7 +269,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   const AttentionArgs& a = args.a;
   using W = Wide<T, kDim>;
   using K = KeyType<T>;
-  constexpr int kParts = __is_same(T, BF16) && !kPrefix ? 1 : kWeightParts<T>;
+  constexpr int kParts = PartsOf<T, kPrefix>();
   auto& lds = shared.tiles;
   auto& scales = shared.scales;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -284,14 +284,16 @@ def on_cpu(cache):
     return cache.k.cpu().float(), cache.v.cpu().float(), cache.k_scale.cpu(), cache.v_scale.cpu()
 
 
-def expect(b, cache, q, scale, i, pos, row):
-    """(out, bound) of the token at position pos of sequence i, row `row` of q."""
+def expect(b, cache, q, scale, i, pos, row, prompt=False):
+    """(out, bound) of the token at position pos of sequence i, row `row` of q. Weights
+    go to the second product in three parts of 8 bits (f32), two (16-bit rows), one
+    (prompts of bf16 rows)."""
     k, v, ks, vs = cache
     n = b.lens[i]
     kk, there = rows_of(k, b, i, n)
     seen = there & (torch.arange(n) <= pos)
     return attention(q[row], kk, rows_of(v, b, i, n)[0], scales_of(ks, b, i, n)[0], scales_of(vs, b, i, n)[0], seen, scale,
-                     b.dtype, 24 if b.dtype == torch.float32 else 16)
+                     b.dtype, 24 if b.dtype == torch.float32 else 8 if prompt and b.dtype == torch.bfloat16 else 16)
 
 
 LENS = [1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 300, 0]
@@ -369,7 +371,7 @@ def test_masked_places_hold_anything(codes, dtype, value, prompt):
     for i, n in enumerate(b.lens):
         for j in range(b.new[i]):
             row = int(b.starts[i]) + j
-            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row))
+            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row, prompt=bool(prompt)))
 
 
 @pytest.mark.parametrize("codes", CODES, ids=ident)
@@ -390,7 +392,7 @@ def test_a_row_that_was_not_finite(codes, dtype):
             for j in range(b.new[i]):
                 row, pos = int(b.starts[i]) + j, b.lens[i] - b.new[i] + j
                 hit = i == 0 and pos >= 70
-                want, bound = expect(b, held_, q, 64 ** -0.5, i, pos, row)
+                want, bound = expect(b, held_, q, 64 ** -0.5, i, pos, row, prompt=True)
                 heads = slice(0, 2) if hit else slice(0, 4)
                 close(got[row, heads], want[heads], bound[heads])
                 assert not hit or bool(got[row, 2:].isnan().all())
@@ -410,10 +412,10 @@ def test_scales_of_any_size(codes, dtype, power):
     cache = random_cache(b, codes)
     cache.v_scale.mul_(2.0 ** power)
     held_ = on_cpu(cache)
-    for got in (serving.decode_attention(q.cuda(), cache, table, lens),
-                serving.prompt_attention(q.cuda(), cache, table, lens, starts)):
+    for got, prompt in ((serving.decode_attention(q.cuda(), cache, table, lens), False),
+                        (serving.prompt_attention(q.cuda(), cache, table, lens, starts), True)):
         for i, n in enumerate(b.lens):
-            close(got[i], *expect(b, held_, q, 128 ** -0.5, i, n - 1, i))
+            close(got[i], *expect(b, held_, q, 128 ** -0.5, i, n - 1, i, prompt))
 
 
 @pytest.mark.parametrize("codes", CODES, ids=ident)
@@ -431,7 +433,7 @@ def test_prompt(codes, dtype, dim, heads, kv, page):
     for i, n in enumerate(b.lens):
         for j in range(b.new[i]):
             row = int(b.starts[i]) + j
-            close(out[row], *expect(b, held_, q, 0.1, i, n - b.new[i] + j, row))
+            close(out[row], *expect(b, held_, q, 0.1, i, n - b.new[i] + j, row, prompt=True))
     assert bool((out[b.tokens:] == 5).all())  # rows behind the last sequence
     again = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts, scale=0.1)
     assert torch.equal(again[:b.tokens], out[:b.tokens])
@@ -450,7 +452,7 @@ def test_prompt_behind_a_long_history(codes, dtype):
     for i, n in enumerate(b.lens):
         for j in range(b.new[i]):
             row = int(b.starts[i]) + j
-            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row))
+            close(got[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row, prompt=True))
 
 
 @pytest.mark.parametrize("codes", CODES, ids=ident)
@@ -481,7 +483,6 @@ def expect_head(b, cache, q, scale, i, h, heads):
     out, mass = p @ vv, p @ vv.abs()
     size = (qq.abs() @ kk.abs().t()) * ss
     ds = (size * seen).amax(1) * scale * (3 * q.shape[2] + 6) * 2.0 ** -24 + (s.abs() * seen).amax(1) * 2.0 ** -21
-    # many rows: weights in three parts of 8 bits (f32), two (f16), one (bf16)
     weight_bits = {torch.float32: 24, torch.float16: 16, torch.bfloat16: 8}[b.dtype]
     rel = torch.expm1(2 * ds) + (3 * seen.sum(1) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
     bound = rel[:, None] * mass + 2.0 ** -140 * n * 448
