@@ -104,8 +104,8 @@ __device__ __forceinline__ void LoadQuery(const char* p, int i, U4 (&q)[kParts][
   }
 }
 
-// Eight weights (times scales) as the parts of an operand.
-template <int kParts>
+// Eight weights (times scales) as the parts of an operand of type V.
+template <int kParts, typename V = BF16>
 struct WeightParts {
   U4 x[kParts];
   __device__ __forceinline__ void Set(int j, float a, float b) {
@@ -113,8 +113,8 @@ struct WeightParts {
       const Parts p = Split3(a, b);
       x[0][j] = p.hi, x[1][j] = p.mid, x[2][j] = p.lo;
     } else {
-      x[0][j] = Pack2<BF16>(a, b);
-      if constexpr (kParts == 2) x[1][j] = Rest2<BF16>(a, b, x[0][j]);
+      x[0][j] = Pack2<V>(a, b);
+      if constexpr (kParts == 2) x[1][j] = Rest2<V>(a, b, x[0][j]);
     }
   }
 };

@@ -11,9 +11,10 @@
 // join their states in LDS. Many (CodesWideKernel): tiles of 128 rows, a wave for 32;
 // a step's 64 keys go to LDS converted, once for the four waves.
 //
-// Weights times scales are rounded once for bf16 rows, as paged_prompt.hip's are (the
-// output is up to 1.35 times as far from exact as its own rounding leaves it; two
-// parts: four documents 638 us, one 535 at the time).
+// Weights times scales are rounded once for 16-bit rows, to their type, as
+// paged_prompt.hip's are (the output is up to 1.35 times as far from exact as its own
+// rounding leaves it; two parts: four documents bf16 638 us, one 535 at the time; 2000
+// tokens f16 84 us, one 73).
 //
 // Bound: the vector unit beside the matrix unit: per score a product with either scale
 // comes to the maximum, the exponential and the sum, and the codes' conversion.
@@ -76,10 +77,12 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
   // turns 19.2 -> 18.2 us, 200 behind 1300 24.1 -> 22.6; 200 alone 10.0 and 10.9).
   const int64_t wgs = tiles * a.c.n_kv * a.splits;
   const dim3 grid(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits);
-  if (kBytes<T> == 2 && wgs <= 256 && a.s.capacity > 256)
-    CodesSoloKernel<C, T, kDim, 8><<<grid, 512, 0, s>>>(args);
-  else
-    CodesSoloKernel<C, T, kDim, 4><<<grid, 256, 0, s>>>(args);
+  bool eight = false;
+  if constexpr (kBytes<T> == 2) {
+    eight = wgs <= 256 && a.s.capacity > 256;
+    if (eight) CodesSoloKernel<C, T, kDim, 8><<<grid, 512, 0, s>>>(args);
+  }
+  if (!eight) CodesSoloKernel<C, T, kDim, 4><<<grid, 256, 0, s>>>(args);
   HIP_CHECK(hipGetLastError());
   if (a.splits > 1) PromptJoin(a, s);
 }

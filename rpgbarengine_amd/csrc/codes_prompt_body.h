@@ -74,11 +74,34 @@ struct SoloLds {
   float sm[kWaves][kSoloRows], sl[kWaves][kSoloRows];
 };
 
-// Parts of a weight: a prompt's of bf16 rows are rounded once.
+// Prompts of 16-bit rows round a weight times its scale once, to the rows' type: what
+// the values' codes are multiplied as, and the parts of a weight.
 template <typename T, bool kPrefix>
-constexpr int PartsOf() {
-  return __is_same(T, BF16) && !kPrefix ? 1 : kWeightParts<T>;
-}
+constexpr bool kOnce = kBytes<T> == 2 && !kPrefix;
+template <typename T, bool kPrefix>
+using ValueType = std::conditional_t<kOnce<T, kPrefix> && __is_same(T, F16), F16, BF16>;
+template <typename T, bool kPrefix>
+constexpr int kPartsOf = kOnce<T, kPrefix> ? 1 : kWeightParts<T>;
+
+// f16 weights: the scales refer to a power of two that none of them passes so far (the
+// outputs are held divided by it), and the weights, of up to 2^kLazy, are held times
+// 2^kLift, their sums too, so that the largest product is 2^15 and what is below
+// 2^-32 of that is lost.
+template <typename V>
+constexpr float kLiftOf = __is_same(V, F16) ? 15.0f - kLazy : 0.0f;
+struct ScaleRef {
+  float ref = 0.0f, inverse = 0.0f;
+  // Takes in a wave's scales; what outputs have to be multiplied by.
+  __device__ __forceinline__ bool Raise(float scales, float* f) {
+    const float top = lanes::WaveMaxF(__builtin_fabsf(scales));
+    if (!(top > ref)) return false;
+    const float up = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 0x7F000000u));
+    *f = ref / up;
+    ref = up;
+    inverse = 1.0f / up;
+    return true;
+  }
+};
 
 // Few rows. kPrefix and the last three: as PromptBody's (prompt_body.h).
 template <typename C, typename T, int kDim, int kWaves, bool kPrefix>
@@ -86,7 +109,8 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
                                          SoloLds<kDim, kWaves>& shared, int bx, int by, int gx) {
   const AttentionArgs& a = args.a;
   using K = KeyType<T>;
-  constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = PartsOf<T, kPrefix>();
+  constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = kPartsOf<T, kPrefix>;
+  using V = ValueType<T, kPrefix>;
   auto& lds = shared.states;
   auto& sm = shared.sm;
   auto& sl = shared.sl;
@@ -123,6 +147,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
   const float c = a.scale * 1.44269504088896341f;
   float m = kNegInf, l = 0.0f;
   F16v o[kBlocks] = {};
+  ScaleRef scale_ref;
   Block<kDim> now, next;
   int pos = begin + wave * kSoloKeys;
   if (pos < end) now.Load(a.c, args.scales, table, kh, pos, t.len - 1, lane);
@@ -150,19 +175,29 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
         hidden |= in ? 0u : 1u << e;
         now.v[e] = now.ok[e / 8] && key < t.len ? now.v[e] : 0u;
       }
+      const int key = pos + 8 * (lane / 4 % 4) + 4 * h + lane % 4;
+      now.vs = (lane & 8 ? now.ok[1] : now.ok[0]) && key < t.len ? now.vs : 0.0f;
+    }
+    if constexpr (__is_same(V, F16)) {
+      float f;
+      if (scale_ref.Raise(now.vs, &f)) {
+#pragma unroll
+        for (int w = 0; w < kBlocks; ++w) o[w] *= f;
+      }
+      now.vs *= scale_ref.inverse;
     }
     float top = kNegInf;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
     top = lanes::MaxXor32(top);
-    if (__any(top > m)) {
+    if (__any(top > m + kLazy)) {  // as in paged_prompt.hip
       const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(MaxDiff(m, up));
       m = up;
       l *= f;
 #pragma unroll
       for (int w = 0; w < kBlocks; ++w) o[w] *= f;
     }
-    const float base = m == kNegInf ? 0.0f : m;
+    const float base = m == kNegInf ? 0.0f : m - kLiftOf<V>;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[e] = __builtin_amdgcn_exp2f(s[e] - base);
@@ -175,7 +210,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      WeightParts<kParts> p;
+      WeightParts<kParts, V> p;
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -189,9 +224,9 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
         U4 x;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x[i] = w % 2 ? Halves2<C, BF16, true>(w < 2 ? lo[i] : hi[i]) : Halves2<C, BF16, false>(w < 2 ? lo[i] : hi[i]);
+          x[i] = w % 2 ? Halves2<C, V, true>(w < 2 ? lo[i] : hi[i]) : Halves2<C, V, false>(w < 2 ? lo[i] : hi[i]);
 #pragma unroll
-        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<BF16>(x, p.x[i], o[w]);
+        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(x, p.x[i], o[w]);
       }
     }
     now = next;
@@ -209,7 +244,8 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
   float top = sm[0][r];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][r]);
-  const float f = __builtin_amdgcn_exp2f(MaxDiff(m, top));
+  float f = __builtin_amdgcn_exp2f(MaxDiff(m, top));
+  if constexpr (__is_same(V, F16)) f *= scale_ref.ref;
   if constexpr (kDim == 128) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) *at(wave, r, 8 * (e / 4) + 4 * h + e % 4) = F4{o[0][e], o[1][e], o[2][e], o[3][e]} * f;
@@ -269,7 +305,8 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   const AttentionArgs& a = args.a;
   using W = Wide<T, kDim>;
   using K = KeyType<T>;
-  constexpr int kParts = PartsOf<T, kPrefix>();
+  constexpr int kParts = kPartsOf<T, kPrefix>;
+  using V = ValueType<T, kPrefix>;
   auto& lds = shared.tiles;
   auto& scales = shared.scales;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -318,6 +355,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   constexpr int kWaveRows = 64 / kPer;
   U4 kc[W::kLoads], vc[W::kLoads];
   float scale = 0.0f;
+  bool scale_ok = false;
   bool ok[W::kLoads];
   int pages[4];  // of the step to come
   auto look_up = [&](int step) {
@@ -344,6 +382,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       scale = *(const __attribute__((address_space(1))) float*)((wave == 0 ? args.scales.k : args.scales.v) +
                                                                 max(page, 0) * args.scales.page_bytes +
                                                                 kh * args.scales.head_bytes + 4 * ((p0 & in_page) + lane % 16));
+      scale_ok = page >= 0 && key0 + lane < len;
     }
   };
   const float c = a.scale * 1.44269504088896341f;
@@ -361,10 +400,10 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const int ks = KSwizzle<K, kDim>(r), vs = VSwizzle<BF16, kDim>(r);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk) ^ ks)) = Operand8<C, K>(x[0], x[1]);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk + 1) ^ ks)) = Operand8<C, K>(x[2], x[3]);
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Operand8<C, BF16>(y[0], y[1]);
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Operand8<C, BF16>(y[2], y[3]);
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Operand8<C, V>(y[0], y[1]);
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Operand8<C, V>(y[2], y[3]);
     }
-    if (wave < 2) scales[kAt][wave][lane] = wave == 0 ? scale * c : scale;
+    if (wave < 2) scales[kAt][wave][lane] = wave == 0 ? scale * c : scale_ok ? scale : 0.0f;
   };
 
   const int k_at = (lane & 31) * W::kRowBytes + 16 * (h ^ KSwizzle<K, kDim>(lane & 31));
@@ -374,6 +413,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
     const int r = 8 * u + 4 * h + (lane & 15) / 4;
     v_at[u] = r * W::kRowBytes + 16 * ((2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^ VSwizzle<BF16, kDim>(r)) + 8 * (lane & 1);
   }
+  ScaleRef scale_ref;
   float m = kNegInf, l = 0.0f;
   F16v o[kDim / 32] = {};
   if (steps > 0) {
@@ -398,7 +438,17 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const char* vt = kt + W::kTileBytes;
       // lane e of each 16: of the key that the lanes' element e belongs to
       const float* of_lane = scales[kAt][0] + 8 * ((lane & 15) / 4) + 4 * h + lane % 4;
-      const float ks[2] = {of_lane[0], of_lane[32]}, vs[2] = {of_lane[W::kKeys], of_lane[W::kKeys + 32]};
+      const float ks[2] = {of_lane[0], of_lane[32]};
+      float vs[2] = {of_lane[W::kKeys], of_lane[W::kKeys + 32]};
+      if constexpr (__is_same(V, F16)) {
+        float f;
+        if (scale_ref.Raise(fmaxf(__builtin_fabsf(vs[0]), __builtin_fabsf(vs[1])), &f)) {
+#pragma unroll
+          for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
+        }
+        vs[0] *= scale_ref.inverse;
+        vs[1] *= scale_ref.inverse;
+      }
       F16v s[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -439,7 +489,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
 #pragma unroll
         for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
       }
-      const float base = m == kNegInf ? 0.0f : m;
+      const float base = m == kNegInf ? 0.0f : m - kLiftOf<V>;
       typedef short S4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -455,7 +505,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          WeightParts<kParts> p;
+          WeightParts<kParts, V> p;
 #pragma unroll
           for (int e = 0; e < 4; ++e) p.Set(e, s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
 #pragma unroll
@@ -469,7 +519,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
               v[2 * u] = x[0], v[2 * u + 1] = x[1];
             }
 #pragma unroll
-            for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<BF16>(v, p.x[i], o[w]);
+            for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(v, p.x[i], o[w]);
           }
         }
       }
@@ -496,7 +546,8 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<F4*>(to + 32 * w + 2 * e + 4 * h) = F4{o[w][e], o[w][e + 1], o[w][e + 2], o[w][e + 3]};
   } else {
-    const float inv = Inverse(m, l);
+    float inv = Inverse(m, l);
+    if constexpr (__is_same(V, F16)) inv *= scale_ref.ref;
     char* out = a.out.p + (t.first + token) * a.out.token_bytes + head * a.out.head_bytes;
 #pragma unroll
     for (int w = 0; w < kDim / 32; ++w)

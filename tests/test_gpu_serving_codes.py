@@ -243,7 +243,7 @@ def test_a_cache_whose_tensors_moved_is_refused():
 # ---- attention
 
 
-def attention(q, k, v, ks, vs, seen, scale, dtype, weight_bits):
+def attention(q, k, v, ks, vs, seen, scale, dtype, weight_bits, prompt=False):
     """q [heads, dim] over codes k, v [kv, n, dim] with scales ks, vs [kv, n], where
     seen [n]: (out, bound), float64. weight_bits: of a weight times its scale in the
     second product."""
@@ -267,7 +267,8 @@ def attention(q, k, v, ks, vs, seen, scale, dtype, weight_bits):
         # joins; the weight's rounding.
         ds = float(((kk.abs() @ qq.abs()) * ss).max()) * scale * (3 * dim + 6) * 2.0 ** -24 + float(s.abs().max()) * 2.0 ** -21
         rel = math.expm1(2 * ds) + (3 * len(s) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
-        bound[h] = rel * mass + 2.0 ** -140 * len(s) * 448
+        # (the scales of all of the sequence's keys count: later tokens' too)
+        bound[h] = rel * mass + 2.0 ** -140 * len(s) * 448 + least_weight(dtype, prompt, vs[kv].double(), vv) * float(p.max())
     return out, bound + plain.EPS[dtype] * (out.abs() + bound) + plain.TINY[dtype]
 
 
@@ -286,14 +287,24 @@ def on_cpu(cache):
 
 def expect(b, cache, q, scale, i, pos, row, prompt=False):
     """(out, bound) of the token at position pos of sequence i, row `row` of q. Weights
-    go to the second product in three parts of 8 bits (f32), two (16-bit rows), one
-    (prompts of bf16 rows)."""
+    go to the second product in three parts of 8 bits (f32), two (16-bit rows), in
+    prompts of 16-bit rows rounded once to their type."""
     k, v, ks, vs = cache
     n = b.lens[i]
     kk, there = rows_of(k, b, i, n)
     seen = there & (torch.arange(n) <= pos)
     return attention(q[row], kk, rows_of(v, b, i, n)[0], scales_of(ks, b, i, n)[0], scales_of(vs, b, i, n)[0], seen, scale,
-                     b.dtype, 24 if b.dtype == torch.float32 else 8 if prompt and b.dtype == torch.bfloat16 else 16)
+                     b.dtype, weight_bits(b.dtype, prompt), prompt)
+
+
+def weight_bits(dtype, prompt):
+    return {torch.float32: 24, torch.float16: 11 if prompt else 16, torch.bfloat16: 8 if prompt else 16}[dtype]
+
+
+def least_weight(dtype, prompt, ss, vv):
+    """What f16 weights of prompts lose below the type's range: held times 2^7, over a
+    power of two that the scales in ss reach half of at least, each off by 2^-25."""
+    return 2.0 ** -32 * 2 * float(ss.max()) * vv.abs().sum(-2) if prompt and dtype == torch.float16 and len(ss) else 0.0
 
 
 LENS = [1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 300, 0]
@@ -483,9 +494,8 @@ def expect_head(b, cache, q, scale, i, h, heads):
     out, mass = p @ vv, p @ vv.abs()
     size = (qq.abs() @ kk.abs().t()) * ss
     ds = (size * seen).amax(1) * scale * (3 * q.shape[2] + 6) * 2.0 ** -24 + (s.abs() * seen).amax(1) * 2.0 ** -21
-    weight_bits = {torch.float32: 24, torch.float16: 16, torch.bfloat16: 8}[b.dtype]
-    rel = torch.expm1(2 * ds) + (3 * seen.sum(1) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
-    bound = rel[:, None] * mass + 2.0 ** -140 * n * 448
+    rel = torch.expm1(2 * ds) + (3 * seen.sum(1) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits(b.dtype, True)
+    bound = rel[:, None] * mass + 2.0 ** -140 * n * 448 + least_weight(b.dtype, True, tt, vv)
     return out, bound + plain.EPS[b.dtype] * (out.abs() + bound) + plain.TINY[b.dtype]
 
 
