@@ -528,3 +528,102 @@ def test_prompts_of_many_rows(codes, dtype, dim, heads, kv, page):
     assert bool((out[b.tokens:] == 5).all())
     again = serving.prompt_attention(q.cuda(), cache, table, lens_d, starts)[:b.tokens]
     assert torch.equal(again.nan_to_num(7.0), out[:b.tokens].nan_to_num(7.0))
+
+
+# ---- refusals of the binding
+
+
+def test_refusals_on_tensors():
+    b = Batch([20, 5], [4, 1], torch.float32, 2, 64, 16, 4, seed=16)
+    rows, table, lens, starts = b.gpu()
+    cache = random_cache(b, torch.int8)
+    k, q, one = b.normal(5, 2, 64).cuda(), b.normal(5, 4, 64).cuda(), b.normal(2, 4, 64).cuda()
+    groups, shared = torch.tensor([0, 2], dtype=torch.int32).cuda(), torch.tensor([16], dtype=torch.int32).cuda()
+    E = eng.EngineError
+    for call in (lambda: serving.append(cache, table, lens, starts, k, k.half()),
+                 lambda: serving.append(cache, table, lens, starts, k.double(), k.double()),
+                 lambda: serving.append(cache, table, lens, starts, k[:, :1], k[:, :1]),
+                 lambda: serving.append(cache, table, lens, starts, k, k, q=q.half()),
+                 lambda: serving.append(cache, table, lens, starts, k.requires_grad_(), k.detach()),
+                 lambda: serving.read_rows(rows, table, lens, starts, k.detach(), k.detach()),
+                 lambda: serving.read_rows(cache, table, lens, None, k.detach(), k.detach()),
+                 lambda: serving.read_rows(cache, table, lens, starts, k.detach(), k.detach()[:4]),
+                 lambda: serving.read_rows(cache, table, lens, starts, q, q),
+                 lambda: serving.decode_attention(q, cache, table, lens),
+                 lambda: serving.decode_attention(one.double(), cache, table, lens),
+                 lambda: serving.decode_attention(one.cpu(), cache, table, lens),
+                 lambda: serving.decode_attention(one, cache, table.long(), lens),
+                 lambda: serving.decode_attention(one, cache, table, lens, out=one.half()),
+                 lambda: serving.prompt_attention(q, cache, table, lens, None),
+                 lambda: serving.prompt_attention(q, cache, table, lens, starts[:2]),
+                 lambda: serving.shared_attention(one, cache, table, lens, groups[:1], shared),
+                 lambda: serving.shared_attention(one, cache, table, lens, groups.long(), shared),
+                 lambda: serving.shared_attention(one, cache, table, lens, groups, shared.cpu()),
+                 lambda: serving.shared_attention(q, rows, table, lens, groups, shared),
+                 lambda: serving.shared_attention(one.half(), rows, table, lens, groups, shared),
+                 lambda: serving.shared_attention(one.clone().requires_grad_(), rows, table, lens, groups, shared)):
+        with pytest.raises(E):
+            call()
+    with torch.no_grad():  # nothing is recorded: parameters are fine
+        serving.decode_attention(one.clone().requires_grad_(), cache, table, lens)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(one, torch.ones_like(one))
+        for call in (lambda: serving.decode_attention(dual, cache, table, lens),
+                     lambda: serving.shared_attention(dual, cache, table, lens, groups, shared)):
+            with pytest.raises(E, match="tangent"):
+                call()
+
+
+def test_what_is_written_is_a_new_version():
+    b = Batch([20], [4], torch.float32, 2, 64, 16, 2, seed=17)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, torch.float8_e4m3fn)
+    k = b.normal(4, 2, 64).cuda()
+    held_ = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+    was = [x._version for x in held_]
+    serving.append(cache, table, lens, starts, k, k)
+    assert all(x._version > v for x, v in zip(held_, was))
+    ko, vo = torch.empty_like(k), torch.empty_like(k)
+    was = ko._version, vo._version
+    serving.read_rows(cache, table, lens, starts, ko, vo)
+    assert ko._version > was[0] and vo._version > was[1]
+
+
+@pytest.mark.parametrize("prompt", [0, 1], ids=["decode", "prompt"])
+def test_on_another_stream_and_replayed(prompt):
+    """A stream of the caller's; a captured call takes lengths and pages of its moment."""
+    b = Batch([700, 33], [2, 1] if prompt else [1, 1], torch.float16, 2, 128, 16, 8, seed=18)
+    q = b.normal(b.tokens, 8, 128, by=0.3)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, torch.int8)
+    held_, qd, out = on_cpu(cache), q.cuda(), torch.empty(b.tokens, 8, 128, dtype=torch.float16, device="cuda")
+
+    def call():
+        if prompt:
+            serving.prompt_attention(qd, cache, table, lens, starts, out=out)
+        else:
+            serving.decode_attention(qd, cache, table, lens, out=out)
+
+    def check():
+        for i, n in enumerate(b.lens):
+            for j in range(b.new[i]):
+                row = int(b.starts[i]) + j
+                close(out[row], *expect(b, held_, q, 128 ** -0.5, i, n - b.new[i] + j, row, prompt=bool(prompt)))
+
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for step in range(3):
+        b.lens = [700 - 200 * step, 33 - 16 * step]
+        b.table[0, 1] = b.table[0, 2 + step]
+        lens.copy_(torch.tensor(b.lens, dtype=torch.int32)), table.copy_(b.table)
+        out.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        check()

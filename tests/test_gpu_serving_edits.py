@@ -197,3 +197,38 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         same(out, *e.want(use))
+
+
+def test_refusals_on_tensors():
+    from rpgbarengine_amd import EngineError
+    x, ids = torch.randn(2, 64).cuda(), torch.zeros(2, 3, dtype=torch.int32).cuda()
+    two, bits = torch.ones(2).cuda(), torch.zeros(2, 2, dtype=torch.int32).cuda()
+    for kw in (dict(repetition=two), dict(history_lens=ids[:, 0]), dict(history=ids.long()), dict(history=ids[:1]),
+               dict(history=ids.t().contiguous().t()), dict(history=ids.cpu()), dict(history=ids, repetition=two.double()),
+               dict(history=ids, repetition=two[:1]), dict(history=ids, history_lens=two), dict(bias_ids=ids),
+               dict(bias=two[:, None]), dict(bias_ids=ids, bias=two[:, None]), dict(mask=bits[:, :1]), dict(mask=bits[:1]),
+               dict(mask_rows=ids[:, 0].contiguous()), dict(out=x.half()), dict(out=x[:1]), dict(out=x.t().contiguous().t()),
+               dict(bias_ids=ids, bias=torch.zeros(2, 3, device="cuda", requires_grad=True)),
+               dict(bias_ids=torch.zeros(2, 1024, dtype=torch.int32, device="cuda"), bias=torch.zeros(2, 1024, device="cuda"))):
+        with pytest.raises(EngineError):
+            serving.edit_logits(x, **kw)
+    for bad in (x[0], x.double(), x.cpu(), x.t().contiguous().t(), x.clone().requires_grad_()):
+        with pytest.raises(EngineError):
+            serving.edit_logits(bad)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(EngineError, match="tangent"):
+            serving.edit_logits(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+    version = x._version
+    serving.edit_logits(x, out=x)
+    assert x._version > version
+
+
+def test_as_many_biases_as_may_be():
+    g = torch.Generator().manual_seed(5)
+    ids = torch.randperm(6000, generator=g)[:1023].int()[None]
+    bias = torch.randn(1, 1023, generator=g)
+    x = torch.randn(1, 6000, generator=g)
+    got = serving.edit_logits(x.cuda(), ids.cuda(), bias_ids=ids.cuda(), bias=bias.cuda(), presence=torch.ones(1).cuda()).cpu()
+    want = x.double()
+    want[0, ids[0].long()] += bias[0].double() - 1.0
+    assert float((got.double() - want).abs().max()) <= 2 * 2.0 ** -24 * 12  # two roundings of values below 12
