@@ -381,9 +381,7 @@ typedef struct {
 } rpg_hip_groups;
 
 /* rpg_hip_paged_decode (rpg_hip_quant_decode) that reads what a group has in common
- * once. For 16-bit rows the weights are rounded over a group's common positions as
- * rpg_hip_paged_prompt has them. Group starts and shared positions are read on the
- * device. work: rpg_hip_paged_shared_work (rpg_hip_quant_shared_work) bytes. */
+ * once. Group starts and shared positions are read on the device. work: rpg_hip_paged_shared_work (rpg_hip_quant_shared_work) bytes. */
 RPG_HIP_API int32_t rpg_hip_paged_shared(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_groups* groups, const rpg_hip_rows* q, const rpg_hip_rows* out,
                                          int32_t n_heads, float scale, void* work, int64_t work_bytes, void* stream);

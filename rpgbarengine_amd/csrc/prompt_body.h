@@ -414,16 +414,20 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
       // output is up to 1.35 times as far from exact as its own rounding leaves it
       // (documents bf16: 2.2e-3 relative, 1.6e-3). Weights in two parts, as decode
       // has them, would make that 1.0, for another product: documents 410 -> 538 us,
-      // six turns f16 14.1 -> 15.2.
+      // six turns f16 14.1 -> 15.2. Positions that a group of sequences has in common
+      // (kPrefix) have two parts, as the decode that they stand for.
       typedef short S4 __attribute__((ext_vector_type(4)));
       // A operand: dimensions 32 w .., keys 32 b + 16 j + 4 h + {0 .. 3, 8 .. 11}
 #pragma unroll
       for (int b = 0; b < Sh::kBlocks; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          U4 p;
+          U4 p, rest;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[e] = Pack2<T>(s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) {
+            p[e] = Pack2<T>(s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
+            if constexpr (kPrefix) rest[e] = Rest2<T>(s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1], p[e]);
+          }
 #pragma unroll
           for (int w = 0; w < kDim / 32; ++w) {
             U4 v;
@@ -434,6 +438,7 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
                   U2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at));
               v[2 * u] = x[0], v[2 * u + 1] = x[1];
             }
+            if constexpr (kPrefix) o[w] = Mfma32<T>(v, rest, o[w]);
             o[w] = Mfma32<T>(v, p, o[w]);
           }
         }
@@ -523,9 +528,11 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
       }
     }
     // In f32 an infinite key, query or value that a row sees comes out as NaN,
-    // since the parts of an infinity are not one. A tile that ends with a NaN is
-    // gone through again, its values looked at and its scores in f32 products.
-    if (kBytes<T> == 2 || careful) break;
+    // since the parts of an infinity are not one, and where weights have two parts
+    // (kPrefix) an infinite value does, times a second part that is nothing. A tile
+    // that ends with a NaN is gone through again, its values looked at and its
+    // scores, in f32, in f32 products.
+    if ((kBytes<T> == 2 && !kPrefix) || careful) break;
     bool nan = false;
 #pragma unroll
     for (int w = 0; w < kDim / 32; ++w)

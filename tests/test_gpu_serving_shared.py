@@ -180,6 +180,51 @@ def test_masked_places_hold_anything(dtype, value):
             close(got[i], *expect(b, held, q, 128 ** -0.5, i, lens[i] - 1, i))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=ident)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("members", [2, 12, 30])
+def test_weights_keep_more_bits_than_the_type(dtype, dim, members):
+    """Values +-1, whose weighted sums cancel down to near nothing: what a weight's
+    rounding to 16 bits takes off would stand out. Two parts leave its square."""
+    lens = [400 + 3 * i for i in range(members)]
+    b = Shared([members], [400], lens, dtype, 2, dim, 16, 8, seed=33)
+    b.v = torch.where(b.v < 0, -1.0, 1.0).to(dtype)
+    q = b.normal(members, 8, dim, by=1.5)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    half = plain.EPS[dtype]
+    for i, n in enumerate(lens):
+        kk, there = plain.sequence_rows(b.k, b.table[i], n)
+        vv, _ = plain.sequence_rows(b.v, b.table[i], n)
+        w, bound = plain.attention(q[i], kk, vv, there, dim ** -0.5, torch.float32)
+        # The weights sum to 1 and the values are 1: a first part is within half of
+        # a step, relative, and the second part within half a step of what is left; an
+        # f16 second part, held times 2^7 at least, not closer than 2^-25.
+        bound += half * half + (n * 2.0 ** -32 if dtype == torch.float16 else 0.0)
+        close(got[i], w, bound + half * (w.abs() + bound) + plain.TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("members", [3, 30])
+def test_infinite_values_in_a_whole_step(dtype, members):
+    """An infinity among keys that all rows see, and more keys behind it."""
+    b = Shared([members], [640], [650 + i for i in range(members)], dtype, 2, 128, 16, 8, seed=34)
+    b.v[int(b.table[0, 3]), 0, 3, 5] = math.inf
+    b.v[int(b.table[0, 20]), 1, 2, 6] = -math.inf
+    b.v[int(b.table[0, 21]), 1, 2, 7], b.v[int(b.table[0, 30]), 1, 4, 7] = -math.inf, math.inf
+    q = b.normal(members, 8, 128)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l).double().cpu()
+    assert bool((got[:, :4, 5] == math.inf).all()) and bool((got[:, 4:, 6] == -math.inf).all())
+    assert bool(got[:, 4:, 7].isnan().all())
+    ok = torch.ones_like(got, dtype=torch.bool)
+    ok[:, :4, 5] = ok[:, 4:, 6:8] = False
+    assert bool(got[ok].isfinite().all())
+    for i in (0, members - 1):  # the other dimensions as without them
+        w, bound = want(b, q, i, 128 ** -0.5, v=b.v.masked_fill(~b.v.isfinite(), 0.0))
+        assert bool(((got[i] - w).abs() <= bound)[ok[i]].all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 def test_infinite_values_that_are_seen(dtype):
     """Among the common positions and in one sequence's own."""
