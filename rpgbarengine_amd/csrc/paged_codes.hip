@@ -113,27 +113,41 @@ __device__ __forceinline__ void StoreCodes(char* to, const uint32_t (&codes)[kPe
     *reinterpret_cast<uint32_t*>(to) = codes[0];
 }
 
-// grid (token, kEach x 256 / kLanes rows of it): the token's rows are its query
-// heads, then its key heads, then its value heads.
+// A wave's rows of one step: of one kind, so that what differs is decided by scalar
+// branches. Rows that there are not are the last one again, not stored.
+enum Kind { kQuery, kKey, kValue };
+struct Unit {
+  Kind kind;
+  int head, n;  // the first head, the kind's heads
+};
+template <int kSub>
+__device__ __forceinline__ Unit UnitOf(int u, int nq, int n_kv) {
+  const int uq = (nq + kSub - 1) / kSub, uk = (n_kv + kSub - 1) / kSub;
+  if (u < uq) return {kQuery, u * kSub, nq};
+  if (u < uq + uk) return {kKey, (u - uq) * kSub, n_kv};
+  return {kValue, (u - uq - uk) * kSub, n_kv};
+}
+
+// grid (token, kEach x 4 units of rows): a token's units are its query heads', then its
+// key heads', then its value heads'.
 template <typename C, typename T, int kDim, int kEach>
 __global__ __launch_bounds__(256) void AppendCodesKernel(CodesAppendArgs args) {
   const AppendArgs& a = args.a;
   constexpr int kPer = 16 / kBytes<T>;  // elements of a lane
   constexpr int kLanes = kDim / kPer;   // lanes of a row
-  constexpr int kRows = 256 / kLanes;   // rows of a pass
+  constexpr int kSub = 64 / kLanes;     // rows of a unit
   const int t = blockIdx.x;
-  const int c = threadIdx.x % kLanes;
-  const int nq = a.q.p != nullptr ? a.n_heads : 0, rows = nq + 2 * a.c.n_kv;
-  const int row0 = blockIdx.y * (kEach * kRows) + threadIdx.x / kLanes;
+  const int lane = threadIdx.x & 63, c = lane % kLanes, sub = lane / kLanes;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nq = a.q.p != nullptr ? a.n_heads : 0;
+  const int u0 = blockIdx.y * (kEach * 4) + wave;
   // The rows are on their way while the token's place is found.
   U4 raw[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int row = min(row0 + k * kRows, rows - 1);
-    const bool is_q = row < nq, is_v = row >= nq + a.c.n_kv;
-    const int head = is_q ? row : is_v ? row - nq - a.c.n_kv : row - nq;
-    const Rows& from = is_q ? a.q : is_v ? a.v : a.k;
-    raw[k] = Load16(from.p + t * from.token_bytes + head * from.head_bytes + 16 * c);
+    const Unit u = UnitOf<kSub>(u0 + 4 * k, nq, a.c.n_kv);
+    const Rows& from = u.kind == kQuery ? a.q : u.kind == kKey ? a.k : a.v;
+    raw[k] = Load16(from.p + t * from.token_bytes + min(u.head + sub, u.n - 1) * from.head_bytes + 16 * c);
   }
   Sequence x;
   if (!FindSequence(a.s, [&](int end, int) { return end <= t; }, &x)) return;  // behind the last sequence
@@ -157,13 +171,12 @@ __global__ __launch_bounds__(256) void AppendCodesKernel(CodesAppendArgs args) {
   }
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    const int row = row0 + k * kRows;
-    const bool is_q = row < nq, is_v = row >= nq + a.c.n_kv;
-    const int head = is_q ? row : is_v ? row - nq - a.c.n_kv : row - nq;
+    const Unit u = UnitOf<kSub>(u0 + 4 * k, nq, a.c.n_kv);
+    const int head = u.head + sub;
     float y[kPer];
     Widen<T, kPer>(raw[k], y);
-    if (!is_v) {
-      const float* gain = is_q ? a.q_norm : a.k_norm;
+    if (u.kind != kValue) {
+      const float* gain = u.kind == kQuery ? a.q_norm : a.k_norm;
       if (gain != nullptr) {
         float sum = 0.0f;
 #pragma unroll
@@ -185,19 +198,19 @@ __global__ __launch_bounds__(256) void AppendCodesKernel(CodesAppendArgs args) {
         }
       }
     }
-    if (is_q) {
-      if (row < rows)
+    if (u.kind == kQuery) {
+      if (head < u.n)
         *reinterpret_cast<U4*>(a.q_out.p + t * a.q_out.token_bytes + head * a.q_out.head_bytes + 16 * c) =
             Narrow<T, kPer>(y);
       continue;
     }
     uint32_t codes[kPer / 4];
     const float scale = Quantise<C, kPer, kLanes>(y, codes);
-    if (row >= rows || page < 0) continue;
-    StoreCodes<kPer>((is_v ? a.c.v : a.c.k) + head * a.c.head_bytes + in_cache, codes);
+    if (head >= u.n || page < 0) continue;
+    StoreCodes<kPer>((u.kind == kValue ? a.c.v : a.c.k) + head * a.c.head_bytes + in_cache, codes);
     if (c == 0)
-      *reinterpret_cast<float*>((is_v ? args.scales.v : args.scales.k) + head * args.scales.head_bytes + in_scales) =
-          scale;
+      *reinterpret_cast<float*>((u.kind == kValue ? args.scales.v : args.scales.k) + head * args.scales.head_bytes +
+                                in_scales) = scale;
   }
 }
 
@@ -205,18 +218,23 @@ __global__ __launch_bounds__(256) void AppendCodesKernel(CodesAppendArgs args) {
 constexpr int kManyTokens = 1024;
 constexpr int kReadEach = 4;
 
-template <typename C, typename T, int kDim>
-void LaunchAppend(const CodesAppendArgs& args, hipStream_t s) {
+template <typename C, typename T, int kDim, int kEach>
+void LaunchAppendEach(const CodesAppendArgs& args, hipStream_t s) {
   const AppendArgs& a = args.a;
-  const int rows = (a.q.p != nullptr ? a.n_heads : 0) + 2 * a.c.n_kv;
-  constexpr int kPass = 256 * 16 / (kDim * kBytes<T>);
+  constexpr int kSub = 64 * 16 / (kDim * kBytes<T>);
+  const int64_t units = CeilDiv(a.q.p != nullptr ? a.n_heads : 0, kSub) + 2 * CeilDiv(a.c.n_kv, kSub);
   const uint32_t n = static_cast<uint32_t>(a.s.n_tokens);
   RPG_CHECK(n <= kMaxGroups, "%u new tokens in one launch", n);
-  if (a.s.n_tokens >= kManyTokens)
-    AppendCodesKernel<C, T, kDim, 3><<<dim3(n, static_cast<uint32_t>(CeilDiv(rows, 3 * kPass))), 256, 0, s>>>(args);
-  else
-    AppendCodesKernel<C, T, kDim, 1><<<dim3(n, static_cast<uint32_t>(CeilDiv(rows, kPass))), 256, 0, s>>>(args);
+  AppendCodesKernel<C, T, kDim, kEach><<<dim3(n, static_cast<uint32_t>(CeilDiv(units, 4 * kEach))), 256, 0, s>>>(args);
   HIP_CHECK(hipGetLastError());
+}
+
+template <typename C, typename T, int kDim>
+void LaunchAppend(const CodesAppendArgs& a, hipStream_t s) {
+  if (a.a.s.n_tokens >= kManyTokens)
+    LaunchAppendEach<C, T, kDim, 3>(a, s);
+  else
+    LaunchAppendEach<C, T, kDim, 1>(a, s);
 }
 
 // grid (kEach tokens, 256 / kLanes rows of them): a token's rows are its key heads, then
