@@ -125,6 +125,25 @@ def test_groups_of_any_size(dtype, members):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_rows(dtype, dim):
+    """More than a thousand rows of few ranges, an odd number, empty sequences among them."""
+    lens = [0 if i % 9 == 4 else 60 + (7 * i) % 90 for i in range(67)]
+    b = Shared([40, 27], [48, 32], lens, dtype, 1, dim, 16, 17, seed=21, extra_pages=0)
+    q = b.normal(67, 17, dim, by=1.5)
+    cache, table, l, _ = b.gpu()
+    got = b.call(q, cache, table, l)
+    for i in (0, 4, 13, 39, 40, 58, 65, 66):
+        close(got[i], *want(b, q, i, dim ** -0.5))
+    q = b.normal(67, 17, dim, by=0.3)
+    quant = random_cache(b, CODES[1])
+    held = on_cpu(quant)
+    got = b.call(q, quant, table, l)
+    for i in (0, 4, 13, 39, 40, 58, 65, 66):
+        close(got[i], *expect(b, held, q, dim ** -0.5, i, lens[i] - 1, i))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 def test_sequences_of_no_group(dtype):
     """In front of the first group and behind the last; no groups at all; shared counts
     past what the table holds, and below 0."""
