@@ -36,7 +36,7 @@ __global__ __launch_bounds__(64 * kWaves, (kMinWaves<T, kDim>)) void CodesDecode
   const DecodePlace at = PlaceOf(a.a, blockIdx.x);
   DecodeRange range;
   if (!WholeRange(a.a, at.seq, static_cast<int>(gridDim.y - 1 - blockIdx.y), &range)) return;
-  DecodeCodeRows<C, T, kDim>(a, shared, at, range);
+  DecodeCodeRows<C, T, kDim>(a, shared, at.seq, at.kh, at.n_cols, range, at);
 }
 
 template <typename C, typename T, int kDim>

@@ -159,23 +159,24 @@ struct CodesState {
   }
 };
 
-// The workgroup's range over a cache of codes.
-template <typename C, typename T, int kDim>
-__device__ __forceinline__ void DecodeCodeRows(const CodesAttentionArgs& args, DecodeLds<kDim>& shared, DecodePlace at,
-                                               DecodeRange range) {
+// The workgroup's range over a cache of codes, pages by the table of sequence `seq`.
+template <typename C, typename T, int kDim, typename Place>
+__device__ __forceinline__ void DecodeCodeRows(const CodesAttentionArgs& args, DecodeLds<kDim>& shared, int seq, int kh,
+                                               int n_cols, DecodeRange range, Place&& place) {
   using Tl = CodesTile<kDim>;
   using St = CodesState<C, T, kDim>;
   const AttentionArgs& a = args.a;
   const int lane = threadIdx.x & 63;
-  const int32_t* table = a.s.table + at.seq * a.s.table_stride;
+  const int32_t* table = a.s.table + seq * a.s.table_stride;
   DecodeBody<T, kDim, Tl, St>(
-      a, shared, at.seq, at.h0, at.n_cols, range,
-      [&](Tl& t, int pos) { t.Load(a.c, args.scales, table, at.kh, pos, range.end - 1, lane); },
-      [&](typename St::Query& q, int col) {
-        const char* qp = a.q.p + at.seq * a.q.token_bytes + (at.h0 + col) * a.q.head_bytes + 16 * (lane >> 4) * kBytes<T>;
+      a, shared, n_cols, range,
+      [&](Tl& t, int pos) { t.Load(a.c, args.scales, table, kh, pos, range.end - 1, lane); },
+      [&](typename St::Query& q, ColumnPlace at) {
+        const char* qp = a.q.p + at.token * a.q.token_bytes + at.head * a.q.head_bytes + 16 * (lane >> 4) * kBytes<T>;
 #pragma unroll
         for (int i = 0; i < St::kQ; ++i) LoadQuery<T>(qp + (64 * (i / 2) + 8 * (i % 2)) * kBytes<T>, i, q.x);
-      });
+      },
+      place);
 }
 
 }  // namespace paged

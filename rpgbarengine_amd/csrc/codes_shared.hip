@@ -39,8 +39,17 @@ __global__ __launch_bounds__(256, kWide || kBytes<T> == 2 ? 2 : 1) void CodesSha
     const int y = a.splits - prefix_splits - 1 - (b - g.prefix) / g.own_x;
     DecodeRange range;
     if (!OwnRange(a, args.groups, prefix_splits, at.seq, y, 0.0f, &range)) return;
-    DecodeCodeRows<C, T, kDim>(args.c, shared.own, at, range);
+    DecodeCodeRows<C, T, kDim>(args.c, shared.own, at.seq, at.kh, at.n_cols, range, at);
   }
+}
+
+// As SharedSmallKernel (paged_shared.hip).
+template <typename C, typename T, int kDim>
+__global__ __launch_bounds__(64 * kWaves, 2) void CodesSharedSmallKernel(CodesSharedArgs args, SharedGrid g) {
+  __shared__ __align__(16) DecodeLds<kDim> shared;
+  SmallPlace at;
+  if (!SmallPlaceOf(args.c.a, args.groups, static_cast<int>(args.prefix_splits), g, blockIdx.x, 0.0f, &at)) return;
+  DecodeCodeRows<C, T, kDim>(args.c, shared, at.seq, at.kh, at.n_cols, at.range, at.columns);
 }
 
 template <typename C, typename T, int kDim>
@@ -50,11 +59,13 @@ void Launch(const CodesSharedArgs& args, hipStream_t s) {
   rows.a = a;
   rows.groups = args.groups;
   rows.prefix_splits = args.prefix_splits;
-  const bool wide = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv) == 128;
-  const SharedGrid g = GridOf(rows, wide ? 128 : kSoloRows);
+  const int tile = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads, a.c.n_kv, a.s.capacity);
+  const SharedGrid g = GridOf(rows, tile == 64 ? kSoloRows : tile);
   const uint32_t n = static_cast<uint32_t>(g.prefix + g.own);
-  if (wide)
+  if (tile == 128)
     CodesSharedKernel<C, T, kDim, true><<<n, 256, 0, s>>>(args, g);
+  else if (tile == kCols)
+    CodesSharedSmallKernel<C, T, kDim><<<n, 64 * kWaves, 0, s>>>(args, g);
   else
     CodesSharedKernel<C, T, kDim, false><<<n, 256, 0, s>>>(args, g);
   HIP_CHECK(hipGetLastError());

@@ -187,11 +187,15 @@ struct DecodeLds {
   float sm[kWaves][kCols], sl[kWaves][kCols];
 };
 
-// Tiles of the range are brought by load(tile, pos), the queries by load_q(q, column),
-// and added up in a State; the waves' states are joined in LDS. T: of the rows.
-template <typename T, int kDim, typename Tl, typename St, typename Load, typename LoadQ>
-__device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDim>& shared, int seq, int h0, int n_cols,
-                                           DecodeRange range, Load&& load, LoadQ&& load_q) {
+struct ColumnPlace {
+  int token, head;
+};
+// Tiles of the range are brought by load(tile, pos), the queries by load_q(q, place(column)),
+// and added up in a State; the waves' states are joined in LDS. place(column): the token
+// and query head of a column. T: of the rows.
+template <typename T, int kDim, typename Tl, typename St, typename Load, typename LoadQ, typename Place>
+__device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDim>& shared, int n_cols, DecodeRange range,
+                                           Load&& load, LoadQ&& load_q, Place&& place) {
   auto& sm = shared.sm;
   auto& sl = shared.sl;
   auto& so = shared.so;
@@ -199,7 +203,7 @@ __device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDi
   St st;
   if (range.start < range.end) {
     typename St::Query q;
-    load_q(q, min(lane & 15, n_cols - 1));
+    load_q(q, place(min(lane & 15, n_cols - 1)));
     const float c = a.scale * 1.44269504088896341f;
     int pos = range.start + wave * Tl::kKeys;
     Tl now, next;
@@ -237,11 +241,12 @@ __device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDi
       l += sl[w][h] * __builtin_amdgcn_exp2f(MaxDiff(sm[w][h], m));
       o += *reinterpret_cast<const F4*>(&so[w][h][d]);
     }
+    const ColumnPlace at = place(h);
     if (range.alone) {
       o *= Inverse(m, l);
-      Store4<T>(a.out.p + seq * a.out.token_bytes + (h0 + h) * a.out.head_bytes + d * kBytes<T>, o);
+      Store4<T>(a.out.p + at.token * a.out.token_bytes + at.head * a.out.head_bytes + d * kBytes<T>, o);
     } else {
-      const int64_t row = static_cast<int64_t>(seq) * a.n_heads + h0 + h;
+      const int64_t row = static_cast<int64_t>(at.token) * a.n_heads + at.head;
       if (d == 0) PartStats(a, row)[range.slot] = F2{m - range.off, l};
       *reinterpret_cast<F4*>(PartOut<kDim>(a, rows, row) + static_cast<int64_t>(range.slot) * kDim + d) = o;
     }
@@ -252,6 +257,7 @@ __device__ __forceinline__ void DecodeBody(const AttentionArgs& a, DecodeLds<kDi
 // block of 16 query heads.
 struct DecodePlace {
   int seq, kh, h0, n_cols;
+  __device__ __forceinline__ ColumnPlace operator()(int column) const { return {seq, h0 + column}; }
 };
 __device__ __forceinline__ DecodePlace PlaceOf(const AttentionArgs& a, int bx) {
   const int group = a.n_heads / a.c.n_kv, blocks = (group + kCols - 1) / kCols;
@@ -267,23 +273,23 @@ __device__ __forceinline__ bool WholeRange(const AttentionArgs& a, int seq, int 
   return out->start < out->end || y == 0;
 }
 
-// The workgroup's range over a cache of rows.
-template <typename T, int kDim>
-__device__ __forceinline__ void DecodeRows(const AttentionArgs& a, DecodeLds<kDim>& shared, DecodePlace at,
-                                           DecodeRange range) {
+// The workgroup's range over a cache of rows, pages by the table of sequence `seq`.
+template <typename T, int kDim, typename Place>
+__device__ __forceinline__ void DecodeRows(const AttentionArgs& a, DecodeLds<kDim>& shared, int seq, int kh, int n_cols,
+                                           DecodeRange range, Place&& place) {
   using Tl = Tile<T, kDim>;
   using St = State<T, kDim>;
   const int lane = threadIdx.x & 63;
-  const int32_t* table = a.s.table + at.seq * a.s.table_stride;
-  const int64_t head_off = at.kh * a.c.head_bytes;
+  const int32_t* table = a.s.table + seq * a.s.table_stride;
+  const int64_t head_off = kh * a.c.head_bytes;
   DecodeBody<T, kDim, Tl, St>(
-      a, shared, at.seq, at.h0, at.n_cols, range,
-      [&](Tl& t, int pos) { t.Load(a.c, table, head_off, pos, range.end - 1, lane); },
-      [&](typename St::Query& q, int col) {
-        const char* qp = a.q.p + at.seq * a.q.token_bytes + (at.h0 + col) * a.q.head_bytes + 16 * (lane >> 4);
+      a, shared, n_cols, range, [&](Tl& t, int pos) { t.Load(a.c, table, head_off, pos, range.end - 1, lane); },
+      [&](typename St::Query& q, ColumnPlace at) {
+        const char* qp = a.q.p + at.token * a.q.token_bytes + at.head * a.q.head_bytes + 16 * (lane >> 4);
 #pragma unroll
         for (int i = 0; i < Tl::kChunks; ++i) q.x[i] = Load16(qp + 64 * i);
-      });
+      },
+      place);
 }
 
 }  // namespace paged

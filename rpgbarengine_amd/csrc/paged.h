@@ -138,8 +138,8 @@ struct CodesSharedArgs {
 struct SharedSplits {
   int prefix, own, least;  // least: AttentionArgs'
 };
-// Rows of the tiles of the common positions: 32, 64 or 128, by what a group has.
-int PrefixRows(int64_t n_seqs, int64_t n_groups, int group);
+// Rows of the tiles of the common positions: 16, 32, 64 or 128.
+int PrefixRows(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity);
 SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int bytes, int64_t capacity);
 void Shared(const SharedArgs& a, hipStream_t s);
 void SharedCodes(const CodesSharedArgs& a, hipStream_t s);

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * kWaves, kDim == 64 && kBytes<T> == 2 ? 4 : 2) 
   const DecodePlace at = PlaceOf(a, blockIdx.x);
   DecodeRange range;
   if (!WholeRange(a, at.seq, blockIdx.y, &range)) return;
-  DecodeRows<T, kDim>(a, shared, at, range);
+  DecodeRows<T, kDim>(a, shared, at.seq, at.kh, at.n_cols, range, at);
 }
 
 template <typename T, int kDim>

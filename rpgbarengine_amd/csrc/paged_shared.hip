@@ -15,11 +15,12 @@
 // Bound: the common positions' products (a group of 32 sequences with four heads to a
 // key head multiplies each key 128 times) beside the own positions' bytes, and the
 // join. Measured, 32 heads on 8 of 128: 96 sequences in three groups behind 4000 to
-// 12000 positions with 100 to 2500 of their own, bf16, 376 MB, 108.8 us (a large copy's
-// rate: 74); 8 behind 2000, f32, 23.6 (launched one after another 31.8). Workgroups of
-// both kinds in turn instead of the common ones first: 129 and 28.6. Weights of common
-// positions in two parts, as decode has them, are 107 -> 108.8 us of the former, 50 ->
-// 61 where own positions are few; with one the output is 1.35 times as far from exact.
+// 12000 positions with 100 to 2500 of their own, bf16, 376 MB, 101.6 us (a large copy's
+// rate: 74); 8 behind 2000, f32, 21.5. Workgroups of
+// both kinds in turn instead of the common ones first: 129 us the former, 28.6 the latter
+// (then 23.6). Weights of common positions in two parts, as decode has them: 107 -> 108.8
+// us the former, 50 -> 61 where own positions are few (both then); with one part the
+// output is 1.35 times as far from exact.
 
 #include <hip/hip_runtime.h>
 
@@ -56,8 +57,19 @@ __global__ __launch_bounds__(256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 
     const int y = a.splits - prefix_splits - 1 - (b - g.prefix) / g.own_x;
     DecodeRange range;
     if (!OwnRange(a, args.groups, prefix_splits, at.seq, y, kDecodeLift<T>, &range)) return;
-    DecodeRows<T, kDim>(a, shared.own, at, range);
+    DecodeRows<T, kDim>(a, shared.own, at.seq, at.kh, at.n_cols, range, at);
   }
+}
+
+// Short work: tiles of 16 rows, whose common positions are attended as a sequence's own
+// are, with the rows of several sequences in the columns. The larger tiles' kernel starts
+// later (a workgroup of f32 has the unit to itself) and its tiles end in a longer joining.
+template <typename T, int kDim>
+__global__ __launch_bounds__(64 * kWaves, 2) void SharedSmallKernel(SharedArgs args, SharedGrid g) {
+  __shared__ __align__(16) DecodeLds<kDim> shared;
+  SmallPlace at;
+  if (!SmallPlaceOf(args.a, args.groups, static_cast<int>(args.prefix_splits), g, blockIdx.x, kDecodeLift<T>, &at)) return;
+  DecodeRows<T, kDim>(args.a, shared, at.seq, at.kh, at.n_cols, at.range, at.columns);
 }
 
 template <typename T, int kDim>
@@ -73,9 +85,9 @@ __global__ __launch_bounds__(256) void SharedJoinKernel(SharedArgs args) {
                    a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes);
 }
 
-// The same for many rows of few ranges, a wave each, without a barrier (3072 rows of up to
-// 13 ranges: 104.5 us a call with a workgroup for each, 102.9 so; 1024 of up to 31: 66.2
-// and 68.0).
+// The same for many rows of few ranges, a wave each, without a barrier (96 sequences of 32
+// heads, up to 13 ranges: 104.5 us a call with a workgroup for each, 101.6 so; 32 of up to
+// 31: 66.2 and 68.0).
 constexpr int kManyRows = 1024, kFewRanges = 24;
 template <typename T, int kDim>
 __global__ __launch_bounds__(256) void SharedJoinWaveKernel(SharedArgs args) {
@@ -96,11 +108,19 @@ __global__ __launch_bounds__(256) void SharedJoinWaveKernel(SharedArgs args) {
   const float l = lanes::WaveSumF(lane < n ? mine[1] * f : 0.0f);
   const float* po = PartOut<kDim>(a, rows, row) + kPer * lane;
   float o[kPer] = {};
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float w = lanes::ReadLaneF(f, s);
+  for (int s0 = 0; s0 < n; s0 += 4) {
+    float x[4][kPer];  // in flight together
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] += po[s * kDim + e] * w;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[j][e] = po[min(s0 + j, n - 1) * kDim + e];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (s0 + j >= n) break;
+      const float w = lanes::ReadLaneF(f, s0 + j);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += x[j][e] * w;
+    }
   }
   const float inv = Inverse(top, l);
   char* out = a.out.p + seq * a.out.token_bytes + head * a.out.head_bytes + kPer * kBytes<T> * lane;
@@ -117,15 +137,17 @@ __global__ __launch_bounds__(256) void SharedJoinWaveKernel(SharedArgs args) {
 template <typename T, int kDim>
 void Launch(const SharedArgs& args, hipStream_t s) {
   const AttentionArgs& a = args.a;
-  const int rows = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads / a.c.n_kv);
+  const int rows = PrefixRows(a.s.n_seqs, args.groups.n_seqs, a.n_heads, a.c.n_kv, a.s.capacity);
   const SharedGrid g = GridOf(args, rows);
   const uint32_t n = static_cast<uint32_t>(g.prefix + g.own);
   if (rows == 128)
     SharedKernel<T, kDim, 1><<<n, 256, 0, s>>>(args, g);
   else if (rows == 64)
     SharedKernel<T, kDim, 2><<<n, 256, 0, s>>>(args, g);
-  else
+  else if (rows == 32)
     SharedKernel<T, kDim, 4><<<n, 256, 0, s>>>(args, g);
+  else
+    SharedSmallKernel<T, kDim><<<n, 64 * kWaves, 0, s>>>(args, g);
   HIP_CHECK(hipGetLastError());
   SharedJoin(args, s);
 }
@@ -142,10 +164,15 @@ void LaunchJoin(const SharedArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Waves of a tile share its rows where a group has few: 32 rows are four waves' that
-// take the keys in turn.
-int PrefixRows(int64_t n_seqs, int64_t n_groups, int group) {
-  const int64_t rows = n_seqs * group / std::max<int64_t>(n_groups, 1);
+// By what a group has: of 64 and 32 rows two and all four waves take the keys of the same
+// rows in turn. Of 16 where the whole batch is little work: 8 sequences of 32 heads behind
+// 2000 positions f32 24.1 us with 32 rows, 21.5 with 16 (bf16 17.4 and 15.2, int8 codes of
+// f16 rows 15.6 and 13.5), 16 behind 4000 f32 42.9 and 36.4 (codes 20.8 and 18.8); but 8
+// behind 30000 91.3 and 99.4 (codes 34.1 and 38.9), 32 in four groups behind 4000, bf16,
+// 30.0 and 38.2.
+int PrefixRows(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int64_t capacity) {
+  const int64_t rows = n_seqs * (n_heads / n_kv) / std::max<int64_t>(n_groups, 1);
+  if (rows <= 64 && n_seqs * n_heads * capacity <= 3 << 20) return kCols;
   return rows > 64 ? 128 : rows > 32 ? 64 : 32;
 }
 
@@ -165,14 +192,14 @@ SharedGrid GridOf(const SharedArgs& args, int rows) {
 // run beside them (96 sequences in three groups behind 4000 to 12000, bf16: 103.4 us
 // aiming at 512 workgroups, 100.7 at 256, 99.5 at 192; 32 behind 30000 63.1, 57.1, 67.8),
 // two in f32, which the products alone keep busy (64 behind 4000: 88.8, 96.9), of 256
-// positions at least (8 behind 2000, f32: 24.0 us, with 512 30.2; 64 behind 64, bf16:
-// 29.2, with 128 31.5). Own ranges as a decode's, none below 512 where the batch fills
+// positions at least (64 behind 64, bf16: 29.2, with 128 31.5), 128 in tiles of 16 rows (8
+// behind 2000, f32: 24.7 us with 256, 21.6 with 128). Own ranges as a decode's, none below 512 where the batch fills
 // the card (the 96: 114.7 without a least, 110.8 with 512, 115.9 with 1024).
 SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int bytes, int64_t capacity) {
-  const int group = n_heads / n_kv;
-  const int64_t tiles = TilesFor(n_seqs, n_groups, group, PrefixRows(n_seqs, n_groups, group));
-  const int64_t wgs = std::max<int64_t>(1, tiles * n_kv);
-  const int64_t prefix = std::min({CeilDiv(bytes == 4 ? 512 : 256, wgs), CeilDiv(capacity, 256), int64_t{kMaxSplits / 2}});
+  const int group = n_heads / n_kv, rows = PrefixRows(n_seqs, n_groups, n_heads, n_kv, capacity);
+  const int64_t wgs = std::max<int64_t>(1, TilesFor(n_seqs, n_groups, group, rows) * n_kv);
+  const int64_t prefix = std::min(
+      {CeilDiv(bytes == 4 ? 512 : 256, wgs), CeilDiv(capacity, rows == kCols ? 128 : 256), int64_t{kMaxSplits / 2}});
   const int own = DecodeSplits(n_seqs, n_heads, n_kv, 2, capacity);
   const bool full = n_seqs * n_kv * CeilDiv(group, kCols) >= 256;
   return {static_cast<int>(std::max<int64_t>(1, prefix)), std::min(own, kMaxSplits / 2), full ? 512 : 0};

@@ -9,7 +9,7 @@ import pytest
 from test_cpu_serving_code import functions, overlaps  # noqa: F401 (a fixture)
 
 KERNELS = {"CodesDecodeKernel": 12, "CodesSoloKernel": 20, "CodesWideKernel": 12, "12SharedKernel": 18,
-           "CodesSharedKernel": 24}
+           "CodesSharedKernel": 24, "SharedSmallKernel": 18}
 
 
 @pytest.mark.parametrize("kernel", KERNELS)

@@ -33,8 +33,25 @@ class Shared(Batch):
                 self.table[i, :here] = self.table[src, :here]
             first += n
 
+    wide = 0  # columns that the table has at least
+
+    def gpu(self, *args, **kw):
+        cache, table, *rest = super().gpu(*args, **kw)
+        if table.shape[1] < self.wide:
+            table = torch.nn.functional.pad(table, (0, self.wide - table.shape[1]), value=-1)
+        return cache, table, *rest
+
     def call(self, q, cache, table, lens, **kw):
         return serving.shared_attention(q.cuda(), cache, table, lens, self.groups.cuda(), self.common.cuda(), **kw)
+
+
+@pytest.fixture(autouse=True, params=["narrow", "wide"])
+def width(request, monkeypatch):
+    """Tables of the sequences' own width and of room for a million positions and more:
+    what a batch may hold chooses the tiles that common positions are attended in."""
+    if request.param == "wide":
+        monkeypatch.setattr(Shared, "wide", 1 << 16)
+    return request.param
 
 
 def want(b, q, i, scale, k=None, v=None):
@@ -107,7 +124,7 @@ def test_long_common_positions(dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 @pytest.mark.parametrize("members", [1, 17, 40])
 def test_groups_of_any_size(dtype, members):
-    """Rows of one tile and of several, of 32 rows and of 128."""
+    """Rows of one tile and of several, of 16 and 32 rows and of 128."""
     lens = [130 + (5 * i) % 40 for i in range(members)]
     b = Shared([members], [128], lens, dtype, 1, 128, 16, 8, seed=members)
     q = b.normal(members, 8, 128, by=1.5)
