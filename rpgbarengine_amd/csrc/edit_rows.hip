@@ -12,7 +12,14 @@
 // launch does with no memory of its own; integer counts come out the same in
 // any order. The slice's logits are on their way meanwhile.
 //
-// Bound: the logits, read and written.
+// Bound: the logits, read and written; the slices' walks through the history beside it.
+// Measured: 192 rows of 151936 bf16, histories of up to 4096, 32 biases, masks on 0.3 of them,
+// 117 MB in 27.8 us (a plain copy 23.9; without histories 23.6; 24.2 in a captured graph);
+// 8 rows f32 9.6 us a call, 5.1 in a captured graph. Slices of 4096 by 256 threads, which
+// walk a history twice as often: 30.2 -> 32.1, of 16384 by 1024: 31.7. Edits one by one,
+// by the bits of what was touched: 27.8, 30.2 with all tokens of a load that holds one.
+// Biases in their own array in LDS instead of the upper bits of the counts: half the
+// workgroups to a compute unit, 44.7 (then 32).
 
 #include <hip/hip_runtime.h>
 
@@ -57,8 +64,8 @@ __device__ __forceinline__ uint32_t Pack2(float a, float b) {
   }
 }
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 4096;                // tokens of a workgroup
+constexpr int kThreads = 512;
+constexpr int kSlice = 8192;  // tokens of a workgroup
 // A token's word in LDS: how often it was made (up to 2^20), whether the prompt has it,
 // and above that the last entry of the biases that names it, + 1.
 constexpr uint32_t kInPrompt = 1u << 21, kMade = kInPrompt - 1;
@@ -190,14 +197,18 @@ __global__ __launch_bounds__(kThreads) void EditKernel(EditArgs a) {
         x[j] = *reinterpret_cast<const U4*>(in + at * kBytes<T>);
       }
       U4 y = x[j];
-      if (here != 0) {
+      for (uint32_t left = here; left != 0; left &= left - 1) {
+        const int e = __builtin_ctz(left), i = e * kBytes<T> / 4;
+        uint32_t w = i < 2 ? (i == 0 ? y[0] : y[1]) : i == 2 ? y[2] : y[3];
         if constexpr (kBytes<T> == 4) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = __float_as_uint(edit(Get<T>(y, e), at + e));
+          w = __float_as_uint(edit(__uint_as_float(w), at + e));
         } else {
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) y[e / 2] = Pack2<T>(edit(Get<T>(y, e), at + e), edit(Get<T>(y, e + 1), at + e + 1));
+          const int shift = e % 2 * 16;
+          const uint32_t v = Pack2<T>(edit(Get<T>(U4{w >> shift, 0, 0, 0}, 0), at + e), 0.0f) & 0xFFFFu;
+          w = (w & ~(0xFFFFu << shift)) | v << shift;
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = k == i ? w : y[k];
       }
       if (mask != nullptr) {
         const uint32_t bits = word[j] >> (at % 32);
