@@ -355,8 +355,9 @@ RPG_HIP_API int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const r
 /* rpg_hip_paged_decode and rpg_hip_paged_prompt over such a cache, q and out rows of
  * `type`. Scales are applied in f32 to scores and weights, codes are multiplied as
  * they are; weights times scales go to the product in two parts of 8 bits, for f32
- * rows in three, in prompts of bf16 rows in one. Queries are finite; a row whose scale is NaN makes NaN of what sees
- * it, and of nothing else. In places that no query sees codes and scales may be
+ * rows in three, in prompts of 16-bit rows rounded to their type once (f16: weights
+ * below 2^-31 of a row's largest are lost). Queries are finite; a row whose scale is
+ * NaN makes NaN of what sees it, and of nothing else. In places that no query sees codes and scales may be
  * anything, but for the NaN codes of e4m3 (which rpg_hip_quant_append never writes)
  * behind a prompt's token in its own sequence. work: rpg_hip_quant_work bytes. */
 RPG_HIP_API int32_t rpg_hip_quant_decode(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,
@@ -381,7 +382,8 @@ typedef struct {
 } rpg_hip_groups;
 
 /* rpg_hip_paged_decode (rpg_hip_quant_decode) that reads what a group has in common
- * once. Group starts and shared positions are read on the device. work: rpg_hip_paged_shared_work (rpg_hip_quant_shared_work) bytes. */
+ * once. Group starts and shared positions are read on the device. work:
+ * rpg_hip_paged_shared_work (rpg_hip_quant_shared_work) bytes. */
 RPG_HIP_API int32_t rpg_hip_paged_shared(const rpg_hip_paged_cache* cache, const rpg_hip_sequences* seqs,
                                          const rpg_hip_groups* groups, const rpg_hip_rows* q, const rpg_hip_rows* out,
                                          int32_t n_heads, float scale, void* work, int64_t work_bytes, void* stream);

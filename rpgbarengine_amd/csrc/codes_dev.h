@@ -29,6 +29,11 @@ __device__ __forceinline__ F2 Floats2(uint32_t u) {
   const int i = static_cast<int>(kHigh ? u >> 16 : u);
   return F2{static_cast<float>(static_cast<int8_t>(i)), static_cast<float>(static_cast<int8_t>(i >> 8))};
 }
+// codes of I8 plus 1152, as a pair of f16: 0x6400 + n is 1024 + n, the code is n - 128
+template <bool kHigh>
+__device__ __forceinline__ uint32_t Above1152(uint32_t u) {
+  return __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, kHigh ? 0x04030402u : 0x04010400u);
+}
 // the same as a pair of f16 or bf16
 template <typename C, typename T, bool kHigh>
 __device__ __forceinline__ uint32_t Halves2(uint32_t u) {
@@ -37,14 +42,37 @@ __device__ __forceinline__ uint32_t Halves2(uint32_t u) {
   } else if constexpr (__is_same(C, E4M3)) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 1.0f, kHigh));
   } else if constexpr (__is_same(T, F16)) {
-    // 0x6400 + n is 1024 + n in f16; the code is n - 128
-    const uint32_t n = __builtin_amdgcn_perm(0x64646464u, u ^ 0x80808080u, kHigh ? 0x04030402u : 0x04010400u);
-    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(H2, n) - H2{1152.0f, 1152.0f});
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(H2, Above1152<kHigh>(u)) - H2{1152.0f, 1152.0f});
   } else {
     // a whole number up to 128 has its bits in a float's upper half
     const F2 x = Floats2<I8, kHigh>(u);
     return __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u);
   }
+}
+
+// f16 values take the power of two of their scale with them, so that the weights, which
+// take what is left of it (from 1 up to 2), keep all of f16's range, however the rows'
+// scales differ. Within limits: no code is rounded or passes f16's largest value, nor does
+// 1152 of them.
+template <typename C>
+__device__ __forceinline__ float PowerOf(float scale) {
+  constexpr uint32_t kLow = __is_same(C, I8) ? 127 - 24 : 127 - 15, kHigh = __is_same(C, I8) ? 127 + 5 : 127 + 7;
+  return __uint_as_float(min(max(__float_as_uint(scale) & 0x7F800000u, kLow << 23), kHigh << 23));
+}
+// scale / power
+__device__ __forceinline__ float RestOf(float scale, float power) {
+  return scale * __uint_as_float(0x7F000000u - __float_as_uint(power));
+}
+// Halves2 of f16, times a power of two for either, in one instruction more than without
+template <bool kHigh>
+__device__ __forceinline__ uint32_t Halves2By(uint32_t u, H2 power) {
+  const H2 x = __builtin_bit_cast(H2, Above1152<kHigh>(u));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, power, power * H2{-1152.0f, -1152.0f}));
+}
+template <typename C, bool kHigh>
+__device__ __forceinline__ uint32_t Halves2By(uint32_t u, float power) {
+  if constexpr (__is_same(C, E4M3)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, power, kHigh));
+  return Halves2By<kHigh>(u, H2{static_cast<_Float16>(power), static_cast<_Float16>(power)});
 }
 
 // The value of lane i of each 16, to all of them: an operand modifier of the
@@ -63,10 +91,27 @@ __device__ __forceinline__ void ScaleBy(V& x, float v) {
   }
 }
 
+// x[e] = v of lane e of the 16
+template <int e, int n>
+__device__ __forceinline__ void FromLanes(float (&x)[n], float v) {
+  if constexpr (e < n) {
+    x[e] = OfLane<e>(v);
+    FromLanes<e + 1>(x, v);
+  }
+}
+
 // eight codes as a product's operand
 template <typename C, typename T>
 __device__ __forceinline__ U4 Operand8(uint32_t x, uint32_t y) {
   return U4{Halves2<C, T, false>(x), Halves2<C, T, true>(x), Halves2<C, T, false>(y), Halves2<C, T, true>(y)};
+}
+// of values, in f16 times a power of two
+template <typename C, typename V>
+__device__ __forceinline__ U4 Values8(uint32_t x, uint32_t y, float power) {
+  if constexpr (__is_same(V, F16))
+    return U4{Halves2By<C, false>(x, power), Halves2By<C, true>(x, power), Halves2By<C, false>(y, power),
+              Halves2By<C, true>(y, power)};
+  return Operand8<C, V>(x, y);
 }
 
 // For rows of type T: what the keys' codes are multiplied as, the parts that a query

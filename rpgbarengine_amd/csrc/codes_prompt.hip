@@ -14,14 +14,17 @@
 // Weights times scales are rounded once for 16-bit rows, to their type, as
 // paged_prompt.hip's are (the output is up to 1.35 times as far from exact as its own
 // rounding leaves it; two parts: four documents bf16 638 us, one 535 at the time; 2000
-// tokens f16 84 us, one 73).
+// tokens f16 84 us, one 73). f16 values take the powers of two of their scales with them
+// (codes_dev.h; six turns 17.0 -> 17.4 us, documents f16 523 -> 529): with all of a scale
+// on the weight, a row 2^15 times as large as the others took their weights' bits even
+// where it had none itself.
 //
 // Bound: the vector unit beside the matrix unit: per score a product with either scale
 // comes to the maximum, the exponential and the sum, and the codes' conversion.
 // Measured, 32 heads on 8 of 128: four documents of about 3000 tokens, 392 GFLOP, e4m3
-// in bf16, 477 us (821 TFLOP/s; a large product of a library reaches 1254, the same
-// over a cache of bf16 920); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16,
-// 18.2 us. Tried on documents: products of one 32-key block between the weighing of the
+// in bf16, 478 us (821 TFLOP/s; a large product of a library reaches 1254, the same
+// over a cache of bf16 960); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16,
+// 17 us. Tried on documents: products of one 32-key block between the weighing of the
 // other 492 -> 492 (479 without), higher priority around products the same, pages
 // looked up another step ahead the same.
 

@@ -83,10 +83,10 @@ using ValueType = std::conditional_t<kOnce<T, kPrefix> && __is_same(T, F16), F16
 template <typename T, bool kPrefix>
 constexpr int kPartsOf = kOnce<T, kPrefix> ? 1 : kWeightParts<T>;
 
-// f16 weights: the scales refer to a power of two that none of them passes so far (the
-// outputs are held divided by it), and the weights, of up to 2^kLazy, are held times
-// 2^kLift, their sums too, so that the largest product is 2^15 and what is below
-// 2^-32 of that is lost.
+// f16 weights: what the values leave of the scales (RestOf) refers to a power of two that
+// none of it passes so far (the outputs are held divided by it): 2 wherever scales lie in
+// f16's range. The weights, of up to 2^kLazy, are held times 2^kLift, their sums too, so
+// that the largest product is 2^15 and weights below 2^-31 are lost.
 template <typename V>
 constexpr float kLiftOf = __is_same(V, F16) ? 15.0f - kLazy : 0.0f;
 struct ScaleRef {
@@ -178,7 +178,11 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
       const int key = pos + 8 * (lane / 4 % 4) + 4 * h + lane % 4;
       now.vs = (lane & 8 ? now.ok[1] : now.ok[0]) && key < t.len ? now.vs : 0.0f;
     }
+    float power[16];  // of the values' scales
     if constexpr (__is_same(V, F16)) {
+      const float mine = PowerOf<C>(now.vs);
+      FromLanes<0>(power, mine);
+      now.vs = RestOf(now.vs, mine);
       float f;
       if (scale_ref.Raise(now.vs, &f)) {
 #pragma unroll
@@ -211,23 +215,39 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       WeightParts<kParts, V> p;
-      uint32_t lo[4], hi[4];
+      U4 x[kBlocks];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p.Set(i, s[8 * j + 2 * i], s[8 * j + 2 * i + 1]);
-        const uint32_t x = now.v[8 * j + 2 * i], y = now.v[8 * j + 2 * i + 1];
-        lo[i] = __builtin_amdgcn_perm(y, x, 0x05010400u);
-        if (kDim == 128) hi[i] = __builtin_amdgcn_perm(y, x, 0x07030602u);
+        const int e = 8 * j + 2 * i;  // two keys
+        p.Set(i, s[e], s[e + 1]);
+        const uint32_t u = now.v[e], v = now.v[e + 1];
+        if constexpr (__is_same(V, F16) && __is_same(C, E4M3)) {  // key by key
+          const uint32_t u01 = Halves2By<C, false>(u, power[e]), v01 = Halves2By<C, false>(v, power[e + 1]);
+          x[0][i] = __builtin_amdgcn_perm(v01, u01, 0x05040100u);
+          x[1][i] = __builtin_amdgcn_perm(v01, u01, 0x07060302u);
+          if constexpr (kDim == 128) {
+            const uint32_t u23 = Halves2By<C, true>(u, power[e]), v23 = Halves2By<C, true>(v, power[e + 1]);
+            x[2][i] = __builtin_amdgcn_perm(v23, u23, 0x05040100u);
+            x[3][i] = __builtin_amdgcn_perm(v23, u23, 0x07060302u);
+          }
+        } else {
+          const uint32_t lo = __builtin_amdgcn_perm(v, u, 0x05010400u), hi = __builtin_amdgcn_perm(v, u, 0x07030602u);
+          if constexpr (__is_same(V, F16)) {
+            const H2 by = {static_cast<_Float16>(power[e]), static_cast<_Float16>(power[e + 1])};
+            x[0][i] = Halves2By<false>(lo, by);
+            x[1][i] = Halves2By<true>(lo, by);
+            if constexpr (kDim == 128) x[2][i] = Halves2By<false>(hi, by), x[3][i] = Halves2By<true>(hi, by);
+          } else {
+            x[0][i] = Halves2<C, V, false>(lo);
+            x[1][i] = Halves2<C, V, true>(lo);
+            if constexpr (kDim == 128) x[2][i] = Halves2<C, V, false>(hi), x[3][i] = Halves2<C, V, true>(hi);
+          }
+        }
       }
 #pragma unroll
-      for (int w = 0; w < kBlocks; ++w) {
-        U4 x;
+      for (int w = 0; w < kBlocks; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = w % 2 ? Halves2<C, V, true>(w < 2 ? lo[i] : hi[i]) : Halves2<C, V, false>(w < 2 ? lo[i] : hi[i]);
-#pragma unroll
-        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(x, p.x[i], o[w]);
-      }
+        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(x[w], p.x[i], o[w]);
     }
     now = next;
   }
@@ -355,6 +375,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   constexpr int kWaveRows = 64 / kPer;
   U4 kc[W::kLoads], vc[W::kLoads];
   float scale = 0.0f;
+  float row_scale[W::kLoads];  // of the values whose codes the thread brings
   bool scale_ok = false;
   bool ok[W::kLoads];
   int pages[4];  // of the step to come
@@ -374,6 +395,10 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const uint32_t off = static_cast<uint32_t>(((r0 + i * W::kLoadRows) & 15) * a.c.row_bytes + 16 * chunk);
       kc[i] = Load16(a.c.k + at + off);
       vc[i] = Load16(a.c.v + at + off);
+      if constexpr (__is_same(V, F16))
+        row_scale[i] = *(const __attribute__((address_space(1))) float*)(args.scales.v + max(page, 0) * args.scales.page_bytes +
+                                                                         kh * args.scales.head_bytes +
+                                                                         4 * ((p0 & in_page) + ((r0 + i * W::kLoadRows) & 15)));
     }
     if (wave < 2) {
       const int u = lane / 16;
@@ -400,10 +425,14 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const int ks = KSwizzle<K, kDim>(r), vs = VSwizzle<BF16, kDim>(r);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk) ^ ks)) = Operand8<C, K>(x[0], x[1]);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk + 1) ^ ks)) = Operand8<C, K>(x[2], x[3]);
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Operand8<C, V>(y[0], y[1]);
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Operand8<C, V>(y[2], y[3]);
+      const float power = __is_same(V, F16) ? PowerOf<C>(row_scale[i]) : 1.0f;
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Values8<C, V>(y[0], y[1], power);
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Values8<C, V>(y[2], y[3], power);
     }
-    if (wave < 2) scales[kAt][wave][lane] = wave == 0 ? scale * c : scale_ok ? scale : 0.0f;
+    if (wave < 2) {
+      const float rest = __is_same(V, F16) ? RestOf(scale, PowerOf<C>(scale)) : scale;
+      scales[kAt][wave][lane] = wave == 0 ? scale * c : scale_ok ? rest : 0.0f;
+    }
   };
 
   const int k_at = (lane & 31) * W::kRowBytes + 16 * (h ^ KSwizzle<K, kDim>(lane & 31));

@@ -268,7 +268,7 @@ def attention(q, k, v, ks, vs, seen, scale, dtype, weight_bits, prompt=False):
         ds = float(((kk.abs() @ qq.abs()) * ss).max()) * scale * (3 * dim + 6) * 2.0 ** -24 + float(s.abs().max()) * 2.0 ** -21
         rel = math.expm1(2 * ds) + (3 * len(s) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits
         # (the scales of all of the sequence's keys count: later tokens' too)
-        bound[h] = rel * mass + 2.0 ** -140 * len(s) * 448 + least_weight(dtype, prompt, vs[kv].double(), vv) * float(p.max())
+        bound[h] = rel * mass + 2.0 ** -140 * len(s) * 448 + least_weight(dtype, prompt, vs[kv].double(), tt, vv) * float(p.max())
     return out, bound + plain.EPS[dtype] * (out.abs() + bound) + plain.TINY[dtype]
 
 
@@ -301,10 +301,22 @@ def weight_bits(dtype, prompt):
     return {torch.float32: 24, torch.float16: 11 if prompt else 16, torch.bfloat16: 8 if prompt else 16}[dtype]
 
 
-def least_weight(dtype, prompt, ss, vv):
-    """What f16 weights of prompts lose below the type's range: held times 2^7, over a
-    power of two that the scales in ss reach half of at least, each off by 2^-25."""
-    return 2.0 ** -32 * 2 * float(ss.max()) * vv.abs().sum(-2) if prompt and dtype == torch.float16 and len(ss) else 0.0
+def least_weight(dtype, prompt, every, ss, vv):
+    """What f16 weights of prompts lose below the type's range. A code is multiplied times
+    the power of two in its scale, within 2^-24 .. 2^5 (e4m3 2^-15 .. 2^7), and its weight
+    takes the rest of the scale: held times 2^7, over a power of two that the rests (of
+    `every` scale) reach half of at least, each off by 2^-25. (The larger of the two
+    types' bounds.) ss, vv: of the keys that are seen."""
+    if not prompt or dtype != torch.float16 or not len(ss):
+        return 0.0
+
+    def power(x):
+        return 2.0 ** x.clamp(min=2.0 ** -149).log2().floor().clamp(lo, hi)
+
+    least = []
+    for lo, hi in ((-24, 5), (-15, 7)):
+        least.append(2.0 ** -32 * 2 * float((every / power(every)).max()) * (power(ss)[..., None] * vv.abs()).sum(-2))
+    return torch.maximum(*least)
 
 
 LENS = [1, 2, 15, 16, 17, 31, 32, 33, 64, 127, 128, 129, 300, 0]
@@ -431,6 +443,27 @@ def test_scales_of_any_size(codes, dtype, power):
 
 @pytest.mark.parametrize("codes", CODES, ids=ident)
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
+@pytest.mark.parametrize("dim,heads,kv,new", [(128, 4, 2, 9), (64, 96, 32, 300)], ids=["few", "many"])
+def test_a_large_row_that_weighs_nothing(codes, dtype, dim, heads, kv, new):
+    """One row of values 2^22 times as large as the others, with next to no weight: the
+    output is the others'."""
+    b = Batch([330], [new], dtype, kv, dim, 16, heads, seed=16)
+    q = b.normal(b.tokens, heads, dim, by=0.3).abs().add(0.5).to(dtype)
+    _, table, lens, starts = b.gpu()
+    cache = random_cache(b, codes)
+    cache.v_scale.copy_(torch.exp(torch.randn(cache.v_scale.shape, generator=b.gen)).mul(2.0 ** -15))
+    page, at = int(b.table[0, 1]), 5
+    cache.v_scale[page, :, at] = 100.0
+    cache.k[page, :, at] = torch.full((kv, dim), -96.0, device="cuda").to(codes)
+    cache.k_scale[page, :, at] = 0.1
+    held_ = on_cpu(cache)
+    got = serving.prompt_attention(q.cuda(), cache, table, lens, starts)
+    for h in (0, heads // 2, heads - 1):
+        close(got[:, h], *expect_head(b, held_, q, dim ** -0.5, 0, h, heads))
+
+
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+@pytest.mark.parametrize("dtype", DTYPES, ids=ident)
 @pytest.mark.parametrize("dim,heads,kv,page", [(128, 8, 2, 16), (64, 5, 1, 32), (128, 3, 3, 64), (64, 34, 2, 16)])
 def test_prompt(codes, dtype, dim, heads, kv, page):
     lens, new = [70, 33, 1, 5, 130, 64, 0, 100], [70, 3, 1, 0, 40, 64, 0, 1]
@@ -495,7 +528,7 @@ def expect_head(b, cache, q, scale, i, h, heads):
     size = (qq.abs() @ kk.abs().t()) * ss
     ds = (size * seen).amax(1) * scale * (3 * q.shape[2] + 6) * 2.0 ** -24 + (s.abs() * seen).amax(1) * 2.0 ** -21
     rel = torch.expm1(2 * ds) + (3 * seen.sum(1) + 18) * 2.0 ** -23 + 2.0 ** -weight_bits(b.dtype, True)
-    bound = rel[:, None] * mass + 2.0 ** -140 * n * 448 + least_weight(b.dtype, True, tt, vv)
+    bound = rel[:, None] * mass + 2.0 ** -140 * n * 448 + least_weight(b.dtype, True, tt, tt, vv)
     return out, bound + plain.EPS[b.dtype] * (out.abs() + bound) + plain.TINY[b.dtype]
 
 
