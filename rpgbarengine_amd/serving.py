@@ -523,6 +523,8 @@ def edit_logits(logits, history=None, history_lens=None, prompts=None, repetitio
         h, row[:5] = (0, 0, 0), [0] * 5
     if not b[2]:
         b = w = (0, 0, 0)
+    if not masks:  # no mask that a row could go by
+        m, row[5] = (0, 0, 0), 0
     edits = _EDITS.pack(h[0], h[1], *row[:5], b[0], b[1], w[0], w[1], m[0] or 0, m[1], row[5], h[2], b[2], masks)
     _enqueue(dev, _lib().rpg_hip_edit_logits, _TYPES[logits.dtype], logits.data_ptr(), rows, vocab, logits.stride(0), edits,
              out.data_ptr(), out.stride(0))

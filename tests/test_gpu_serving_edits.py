@@ -176,6 +176,13 @@ def test_empty_lists_and_rows():
     assert serving.edit_logits(x[:0]).shape == (0, 50)
 
 
+def test_no_masks_for_rows_that_go_by_none():
+    x = torch.randn(3, 70, device="cuda")
+    none = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
+    rows = torch.full((3,), -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(serving.edit_logits(x, mask=none, mask_rows=rows), x)
+
+
 def test_captured_and_replayed():
     """A replay takes the history, its length and the masks of its moment."""
     e = Edits(3, 5000, torch.bfloat16, 100, seed=11)
