@@ -225,7 +225,7 @@ def _vector(x, name, n, dtype, device):
 
 def _enqueue(device, f, *args):
     """f(*args, stream) on the current stream of the tensors' GPU, that GPU current."""
-    if torch.cuda.current_device() == device.index:
+    if _current() == device.index:
         rc = f(*args, _stream(device.index))
     else:
         with torch.cuda.device(device):
@@ -252,6 +252,7 @@ def _stream(index):
 
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same without a Stream object for each call
     _stream = torch._C._cuda_getCurrentRawStream
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def append(cache, table, lens, starts, k, v, q=None, q_out=None, q_norm=None, k_norm=None,

@@ -230,6 +230,40 @@ def test_views_of_larger_pools():
     assert torch.equal(ko, -vo)
 
 
+@pytest.mark.parametrize("codes", CODES, ids=ident)
+def test_pages_past_32_bits(codes):
+    """Pages two GiB apart, scales as far: what each operator gives is that of the same
+    pages side by side, to the bit."""
+    b = Batch([33, 16], [33, 16], torch.bfloat16, 2, 64, 16, 4, seed=17, spare=1)
+    assert b.n_pages == 5
+    apart = (1 << 31) - (1 << 20)
+    pool = torch.empty(5 * apart, dtype=torch.int8, device="cuda")
+
+    def view(at, dtype, shape, stride):
+        return torch.as_strided(pool.view(dtype), shape, stride, at // dtype.itemsize)
+
+    k, v = (view(at << 16, codes, (5, 2, 16, 64), (apart, 1024, 64, 1)) for at in (0, 1))
+    ks, vs = (view(at << 16, torch.float32, (5, 2, 16), (apart // 4, 16, 1)) for at in (2, 3))
+    far, near = serving.QuantCache(k, v, ks, vs), serving.QuantCache.zeros(5, 16, 2, 64, codes)
+    for x in (k, v):
+        x.view(torch.int8).zero_()
+    ks.zero_(), vs.zero_()
+    _, table, lens, starts = b.gpu()
+    rows, q = b.normal(49, 2, 64).cuda(), b.normal(49, 4, 64, by=0.5).cuda()
+    groups, shared = torch.tensor([0, 2], dtype=torch.int32).cuda(), torch.tensor([16], dtype=torch.int32).cuda()
+    table[1, 0] = table[0, 0]
+    got = []
+    for cache in (far, near):
+        serving.append(cache, table[:1], lens[:1], starts[:2], rows, -rows)
+        ko, vo = torch.zeros_like(rows), torch.zeros_like(rows)
+        serving.read_rows(cache, table, lens, starts, ko, vo)
+        got.append((ko, vo, serving.prompt_attention(q, cache, table, lens, starts),
+                    serving.decode_attention(q[:2], cache, table, lens),
+                    serving.shared_attention(q[:2], cache, table, lens, groups, shared)))
+    for x, y in zip(*got):
+        assert torch.equal(x, y) and bool(x.isfinite().all()) and bool((x != 0).any())
+
+
 def test_a_cache_whose_tensors_moved_is_refused():
     cache = serving.QuantCache.zeros(4, 16, 2, 64)
     b = Batch([5], [5], torch.float32, 2, 64, 16, 2)
@@ -443,7 +477,7 @@ def test_scales_of_any_size(codes, dtype, power):
 
 @pytest.mark.parametrize("codes", CODES, ids=ident)
 @pytest.mark.parametrize("dtype", DTYPES, ids=ident)
-@pytest.mark.parametrize("dim,heads,kv,new", [(128, 4, 2, 9), (64, 96, 32, 300)], ids=["few", "many"])
+@pytest.mark.parametrize("dim,heads,kv,new", [(128, 4, 2, 9), (64, 192, 32, 300)], ids=["few", "many"])
 def test_a_large_row_that_weighs_nothing(codes, dtype, dim, heads, kv, new):
     """One row of values 2^22 times as large as the others, with next to no weight: the
     output is the others'."""
