@@ -11,7 +11,7 @@
 //
 // Bound: the codes' and scales' bytes, each read once. Measured, 32 heads on 8 of 128: 64
 // sequences of 201 to 11167 positions, e4m3 in bf16, 382 MB in 86.3 us (a large copy's
-// rate: 75; 64 of 2826 each, as many bytes: 76.5; the ragged batch's ends are the rest); 8
+// rate: 75; 64 of 2826 each, as many bytes: 83; the join is 4.6 of either); 8
 // of about 1090, 16 heads, int8 in f16, 11.5 us, 9.4 of them the kernel's and 3.5 the
 // join's. A row's scale is a lane's, and comes to the scores as an operand modifier
 // (each lane loading its own keys' scales: 98 us the former, 94.5 so, both then).
@@ -61,12 +61,16 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
 // As DecodeSplits. Where the batch alone fills the card, no range is below 1024
 // positions: a table for the longest sequence of a ragged batch would cut all of them
 // into as many (64 of 201 to 11167, e4m3: 96.0 us so, 91.8 with 512, 87.9 with 1024, 93.5
-// with 2048), and the last ranges, which few sequences have, come first (86.4).
+// with 2048), and the last ranges, which few sequences have, come first (86.4). Ranges of
+// 1024 also for the longest where one workgroup to a sequence and key head is one to two
+// for each compute unit, or half of one: 32 of the same lengths 49.8 -> 47.0 us, 16 32.6
+// -> 30.7 (f32 34.9 -> 25.5), 16 of 100 to 40000 56.4 -> 49.3; but 8 of them 19.5 -> 20.6,
+// 32 of 2826 each 43.5 -> 44.2.
 int CodesDecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity, int* least) {
   *least = 0;
   if (capacity <= 640) return 1;
   const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));
-  const int64_t fill = 256 / base, cap = CeilDiv(capacity, 2048);
+  const int64_t fill = 256 / base, cap = CeilDiv(capacity, base >= 128 && base < 512 ? 1024 : 2048);
   if (fill <= cap) *least = 1024;
   const int64_t want = std::max(fill, cap);
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, kRangeUnit), int64_t{kMaxSplits}})));
