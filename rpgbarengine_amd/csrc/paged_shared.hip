@@ -191,15 +191,18 @@ SharedGrid GridOf(const SharedArgs& args, int rows) {
 // Ranges of common positions for one workgroup per compute unit, so that own positions
 // run beside them (96 sequences in three groups behind 4000 to 12000, bf16: 103.4 us
 // aiming at 512 workgroups, 100.7 at 256, 99.5 at 192; 32 behind 30000 63.1, 57.1, 67.8),
-// two in f32, which the products alone keep busy (64 behind 4000: 88.8, 96.9), of 256
-// positions at least (64 behind 64, bf16: 29.2, with 128 31.5), 128 in tiles of 16 rows (8
-// behind 2000, f32: 24.7 us with 256, 21.6 with 128). Own ranges as a decode's, none below 512 where the batch fills
-// the card (the 96: 114.7 without a least, 110.8 with 512, 115.9 with 1024).
+// two in f32, which the products alone keep busy (64 behind 4000: 88.8, 96.9), and none
+// above 2560 positions, so that the longest group does not end alone (128 in eight groups
+// behind 500 to 8000 91.8 us without, 84.9 so; 64 in 16 behind 100 to 10000 84.8, 76.2; on
+// int8 codes of f16 rows the former 72.1, 75.2). Of 256 positions at least (64 behind 64,
+// bf16: 29.2, with 128 31.5), 128 in tiles of 16 rows (8 behind 2000, f32: 24.7 us with
+// 256, 21.6 with 128). Own ranges as a decode's, none below 512 where the batch fills the
+// card (the 96: 114.7 without a least, 110.8 with 512, 115.9 with 1024).
 SharedSplits SplitsOfShared(int64_t n_seqs, int64_t n_groups, int n_heads, int n_kv, int bytes, int64_t capacity) {
   const int group = n_heads / n_kv, rows = PrefixRows(n_seqs, n_groups, n_heads, n_kv, capacity);
   const int64_t wgs = std::max<int64_t>(1, TilesFor(n_seqs, n_groups, group, rows) * n_kv);
-  const int64_t prefix = std::min(
-      {CeilDiv(bytes == 4 ? 512 : 256, wgs), CeilDiv(capacity, rows == kCols ? 128 : 256), int64_t{kMaxSplits / 2}});
+  const int64_t want = std::max(CeilDiv(bytes == 4 ? 512 : 256, wgs), CeilDiv(capacity, 2560));
+  const int64_t prefix = std::min({want, CeilDiv(capacity, rows == kCols ? 128 : 256), int64_t{kMaxSplits / 2}});
   const int own = DecodeSplits(n_seqs, n_heads, n_kv, 2, capacity);
   const bool full = n_seqs * n_kv * CeilDiv(group, kCols) >= 256;
   return {static_cast<int>(std::max<int64_t>(1, prefix)), std::min(own, kMaxSplits / 2), full ? 512 : 0};
