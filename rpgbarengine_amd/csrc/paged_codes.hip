@@ -3,14 +3,14 @@
 // rotated as in paged_append.hip, in fp32; values as they are) is stored as
 //   a = max |y|,  scale = a / M,  code = y M / a to the nearest, even at ties
 // with M the largest code (127, 448), and read as code x scale. The quotient is
-// the correctly rounded one: 16-bit rows have many that lie midway between two
-// codes, and there y (M / a) would fall to either side.
+// the correctly rounded one, of the whole product y M: 16-bit rows have many that lie
+// midway between two codes, and there y (M / a) would fall to either side.
 //
 // Bound: bytes, or for few tokens the launch and its dependent round trips. A row
 // is one 16-byte load of 8, 16 or 32 adjacent lanes; the sum of squares, the
 // rotation's partner and the maximum cross lanes by DPP. A wave's rows are of one kind
 // (query, key or value), so that none goes through another's steps. Measured, 32 heads on
-// 8 of 128, e4m3: 4060 tokens of 12 sequences bf16, 93 MB in 23.6 us (a large copy's rate:
+// 8 of 128, e4m3: 4060 tokens of 12 sequences bf16, 93 MB in 23.1 us (a large copy's rate:
 // 18.3; the norm, the rotation and the codes' quotients are the rest: rows of any kind in
 // a wave 26.2); 8 tokens f32 3.9 us in the kernel, 11 in the call. Read, 24 sessions, bf16:
 // 37.3 us (33); one session of 1100 positions, int8 in f32, 7.4 (4.7 in a captured graph).
@@ -68,8 +68,9 @@ __device__ __forceinline__ float Quantise(const float (&y)[kPer], uint32_t (&cod
   float q[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const float n = some ? y[i] * f * kLargest<C> : 0.0f, q0 = n * inv;
-    q[i] = __builtin_fmaf(__builtin_fmaf(-q0, a, n), inv, q0);
+    // (y M in two parts: all of it counts)
+    const float x = some ? y[i] * f : 0.0f, n = x * kLargest<C>, q0 = n * inv;
+    q[i] = __builtin_fmaf(__builtin_fmaf(-q0, a, n) + __builtin_fmaf(x, kLargest<C>, -n), inv, q0);
   }
 #pragma unroll
   for (int w = 0; w < kPer / 4; ++w) {
