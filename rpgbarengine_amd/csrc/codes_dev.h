@@ -20,7 +20,6 @@ template <typename C>
 constexpr float kLargest = __is_same(C, I8) ? 127.0f : 448.0f;
 
 typedef _Float16 H2 __attribute__((ext_vector_type(2)));
-typedef __bf16 B2 __attribute__((ext_vector_type(2)));
 
 // codes 2 kHigh and 2 kHigh + 1 of four
 template <typename C, bool kHigh>
@@ -50,31 +49,6 @@ __device__ __forceinline__ uint32_t Halves2(uint32_t u) {
   }
 }
 
-// f16 values take the power of two of their scale with them, so that the weights, which
-// take what is left of it (from 1 up to 2), keep all of f16's range, however the rows'
-// scales differ. Within limits: no code is rounded or passes f16's largest value, nor does
-// 1152 of them.
-template <typename C>
-__device__ __forceinline__ float PowerOf(float scale) {
-  constexpr uint32_t kLow = __is_same(C, I8) ? 127 - 24 : 127 - 15, kHigh = __is_same(C, I8) ? 127 + 5 : 127 + 7;
-  return __uint_as_float(min(max(__float_as_uint(scale) & 0x7F800000u, kLow << 23), kHigh << 23));
-}
-// scale / power
-__device__ __forceinline__ float RestOf(float scale, float power) {
-  return scale * __uint_as_float(0x7F000000u - __float_as_uint(power));
-}
-// Halves2 of f16, times a power of two for either, in one instruction more than without
-template <bool kHigh>
-__device__ __forceinline__ uint32_t Halves2By(uint32_t u, H2 power) {
-  const H2 x = __builtin_bit_cast(H2, Above1152<kHigh>(u));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, power, power * H2{-1152.0f, -1152.0f}));
-}
-template <typename C, bool kHigh>
-__device__ __forceinline__ uint32_t Halves2By(uint32_t u, float power) {
-  if constexpr (__is_same(C, E4M3)) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, power, kHigh));
-  return Halves2By<kHigh>(u, H2{static_cast<_Float16>(power), static_cast<_Float16>(power)});
-}
-
 // The value of lane i of each 16, to all of them: an operand modifier of the
 // instruction that takes it. Scales of the rows that a lane's scores belong to come
 // that way, a register for 16 of them.
@@ -91,29 +65,11 @@ __device__ __forceinline__ void ScaleBy(V& x, float v) {
   }
 }
 
-// x[e] = v of lane e of the 16
-template <int e, int n>
-__device__ __forceinline__ void FromLanes(float (&x)[n], float v) {
-  if constexpr (e < n) {
-    x[e] = OfLane<e>(v);
-    FromLanes<e + 1>(x, v);
-  }
-}
-
 // eight codes as a product's operand
 template <typename C, typename T>
 __device__ __forceinline__ U4 Operand8(uint32_t x, uint32_t y) {
   return U4{Halves2<C, T, false>(x), Halves2<C, T, true>(x), Halves2<C, T, false>(y), Halves2<C, T, true>(y)};
 }
-// of values, in f16 times a power of two
-template <typename C, typename V>
-__device__ __forceinline__ U4 Values8(uint32_t x, uint32_t y, float power) {
-  if constexpr (__is_same(V, F16))
-    return U4{Halves2By<C, false>(x, power), Halves2By<C, true>(x, power), Halves2By<C, false>(y, power),
-              Halves2By<C, true>(y, power)};
-  return Operand8<C, V>(x, y);
-}
-
 // For rows of type T: what the keys' codes are multiplied as, the parts that a query
 // takes (f32: three exact bf16 parts, Split3), and those of a weight times a
 // value's scale, in bf16: of 8 bits each, so two are as fine as an f16 output's
@@ -149,8 +105,8 @@ __device__ __forceinline__ void LoadQuery(const char* p, int i, U4 (&q)[kParts][
   }
 }
 
-// Eight weights (times scales) as the parts of an operand of type V.
-template <int kParts, typename V = BF16>
+// Eight weights (times scales) as the parts of an operand.
+template <int kParts>
 struct WeightParts {
   U4 x[kParts];
   __device__ __forceinline__ void Set(int j, float a, float b) {
@@ -158,8 +114,8 @@ struct WeightParts {
       const Parts p = Split3(a, b);
       x[0][j] = p.hi, x[1][j] = p.mid, x[2][j] = p.lo;
     } else {
-      x[0][j] = Pack2<V>(a, b);
-      if constexpr (kParts == 2) x[1][j] = Rest2<V>(a, b, x[0][j]);
+      x[0][j] = Pack2<BF16>(a, b);
+      if constexpr (kParts == 2) x[1][j] = Rest2<BF16>(a, b, x[0][j]);
     }
   }
 };

@@ -11,13 +11,12 @@
 // join their states in LDS. Many (CodesWideKernel): tiles of 128 rows, a wave for 32;
 // a step's 64 keys go to LDS converted, once for the four waves.
 //
-// Weights times scales are rounded once for 16-bit rows, to their type, as
-// paged_prompt.hip's are (the output is up to 1.35 times as far from exact as its own
-// rounding leaves it; two parts: four documents bf16 638 us, one 535 at the time; 2000
-// tokens f16 84 us, one 73). f16 values take the powers of two of their scales with them
-// (codes_dev.h; six turns 17.0 -> 17.4 us, documents f16 523 -> 529): with all of a scale
-// on the weight, a row 2^15 times as large as the others took their weights' bits even
-// where it had none itself.
+// Weights times scales go to the product in parts of bf16, whose range is that of fp32, as
+// in codes_decode.hip: f16 ones would have to be held over the largest scale, which may be
+// a later token's, and the tokens before it would lose their weights' bits to it. For bf16
+// rows they are rounded once, as paged_prompt.hip's are (the output is 1.40 times as far
+// from exact as its own rounding leaves it; two parts: four documents bf16 638 us, one 535
+// at the time).
 //
 // Bound: the vector unit beside the matrix unit: per score a product with either scale
 // comes to the maximum, the exponential and the sum, and the codes' conversion.

@@ -74,34 +74,9 @@ struct SoloLds {
   float sm[kWaves][kSoloRows], sl[kWaves][kSoloRows];
 };
 
-// Prompts of 16-bit rows round a weight times its scale once, to the rows' type: what
-// the values' codes are multiplied as, and the parts of a weight.
+// The parts of a weight times its scale. Prompts of bf16 rows round it once.
 template <typename T, bool kPrefix>
-constexpr bool kOnce = kBytes<T> == 2 && !kPrefix;
-template <typename T, bool kPrefix>
-using ValueType = std::conditional_t<kOnce<T, kPrefix> && __is_same(T, F16), F16, BF16>;
-template <typename T, bool kPrefix>
-constexpr int kPartsOf = kOnce<T, kPrefix> ? 1 : kWeightParts<T>;
-
-// f16 weights: what the values leave of the scales (RestOf) refers to a power of two that
-// none of it passes so far (the outputs are held divided by it): 2 wherever scales lie in
-// f16's range. The weights, of up to 2^kLazy, are held times 2^kLift, their sums too, so
-// that the largest product is 2^15 and weights below 2^-31 are lost.
-template <typename V>
-constexpr float kLiftOf = __is_same(V, F16) ? 15.0f - kLazy : 0.0f;
-struct ScaleRef {
-  float ref = 0.0f, inverse = 0.0f;
-  // Takes in a wave's scales; what outputs have to be multiplied by.
-  __device__ __forceinline__ bool Raise(float scales, float* f) {
-    const float top = lanes::WaveMaxF(__builtin_fabsf(scales));
-    if (!(top > ref)) return false;
-    const float up = __uint_as_float(min((__float_as_uint(top) + 0x7FFFFFu) & 0x7F800000u, 0x7F000000u));
-    *f = ref / up;
-    ref = up;
-    inverse = 1.0f / up;
-    return true;
-  }
-};
+constexpr int kPartsOf = __is_same(T, BF16) && !kPrefix ? 1 : kWeightParts<T>;
 
 // Few rows. kPrefix and the last three: as PromptBody's (prompt_body.h).
 template <typename C, typename T, int kDim, int kWaves, bool kPrefix>
@@ -110,7 +85,6 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
   const AttentionArgs& a = args.a;
   using K = KeyType<T>;
   constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = kPartsOf<T, kPrefix>;
-  using V = ValueType<T, kPrefix>;
   auto& lds = shared.states;
   auto& sm = shared.sm;
   auto& sl = shared.sl;
@@ -147,7 +121,6 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
   const float c = a.scale * 1.44269504088896341f;
   float m = kNegInf, l = 0.0f;
   F16v o[kBlocks] = {};
-  ScaleRef scale_ref;
   Block<kDim> now, next;
   int pos = begin + wave * kSoloKeys;
   if (pos < end) now.Load(a.c, args.scales, table, kh, pos, t.len - 1, lane);
@@ -178,18 +151,6 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
       const int key = pos + 8 * (lane / 4 % 4) + 4 * h + lane % 4;
       now.vs = (lane & 8 ? now.ok[1] : now.ok[0]) && key < t.len ? now.vs : 0.0f;
     }
-    float power[16];  // of the values' scales
-    if constexpr (__is_same(V, F16)) {
-      const float mine = PowerOf<C>(now.vs);
-      FromLanes<0>(power, mine);
-      now.vs = RestOf(now.vs, mine);
-      float f;
-      if (scale_ref.Raise(now.vs, &f)) {
-#pragma unroll
-        for (int w = 0; w < kBlocks; ++w) o[w] *= f;
-      }
-      now.vs *= scale_ref.inverse;
-    }
     float top = kNegInf;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
@@ -201,7 +162,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
 #pragma unroll
       for (int w = 0; w < kBlocks; ++w) o[w] *= f;
     }
-    const float base = m == kNegInf ? 0.0f : m - kLiftOf<V>;
+    const float base = m == kNegInf ? 0.0f : m;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       s[e] = __builtin_amdgcn_exp2f(s[e] - base);
@@ -214,40 +175,22 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      WeightParts<kParts, V> p;
+      WeightParts<kParts> p;
       U4 x[kBlocks];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int e = 8 * j + 2 * i;  // two keys
         p.Set(i, s[e], s[e + 1]);
         const uint32_t u = now.v[e], v = now.v[e + 1];
-        if constexpr (__is_same(V, F16) && __is_same(C, E4M3)) {  // key by key
-          const uint32_t u01 = Halves2By<C, false>(u, power[e]), v01 = Halves2By<C, false>(v, power[e + 1]);
-          x[0][i] = __builtin_amdgcn_perm(v01, u01, 0x05040100u);
-          x[1][i] = __builtin_amdgcn_perm(v01, u01, 0x07060302u);
-          if constexpr (kDim == 128) {
-            const uint32_t u23 = Halves2By<C, true>(u, power[e]), v23 = Halves2By<C, true>(v, power[e + 1]);
-            x[2][i] = __builtin_amdgcn_perm(v23, u23, 0x05040100u);
-            x[3][i] = __builtin_amdgcn_perm(v23, u23, 0x07060302u);
-          }
-        } else {
-          const uint32_t lo = __builtin_amdgcn_perm(v, u, 0x05010400u), hi = __builtin_amdgcn_perm(v, u, 0x07030602u);
-          if constexpr (__is_same(V, F16)) {
-            const H2 by = {static_cast<_Float16>(power[e]), static_cast<_Float16>(power[e + 1])};
-            x[0][i] = Halves2By<false>(lo, by);
-            x[1][i] = Halves2By<true>(lo, by);
-            if constexpr (kDim == 128) x[2][i] = Halves2By<false>(hi, by), x[3][i] = Halves2By<true>(hi, by);
-          } else {
-            x[0][i] = Halves2<C, V, false>(lo);
-            x[1][i] = Halves2<C, V, true>(lo);
-            if constexpr (kDim == 128) x[2][i] = Halves2<C, V, false>(hi), x[3][i] = Halves2<C, V, true>(hi);
-          }
-        }
+        const uint32_t lo = __builtin_amdgcn_perm(v, u, 0x05010400u), hi = __builtin_amdgcn_perm(v, u, 0x07030602u);
+        x[0][i] = Halves2<C, BF16, false>(lo);
+        x[1][i] = Halves2<C, BF16, true>(lo);
+        if constexpr (kDim == 128) x[2][i] = Halves2<C, BF16, false>(hi), x[3][i] = Halves2<C, BF16, true>(hi);
       }
 #pragma unroll
       for (int w = 0; w < kBlocks; ++w)
 #pragma unroll
-        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(x[w], p.x[i], o[w]);
+        for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<BF16>(x[w], p.x[i], o[w]);
     }
     now = next;
   }
@@ -264,8 +207,7 @@ __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const S
   float top = sm[0][r];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][r]);
-  float f = __builtin_amdgcn_exp2f(MaxDiff(m, top));
-  if constexpr (__is_same(V, F16)) f *= scale_ref.ref;
+  const float f = __builtin_amdgcn_exp2f(MaxDiff(m, top));
   if constexpr (kDim == 128) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) *at(wave, r, 8 * (e / 4) + 4 * h + e % 4) = F4{o[0][e], o[1][e], o[2][e], o[3][e]} * f;
@@ -326,7 +268,6 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   using W = Wide<T, kDim>;
   using K = KeyType<T>;
   constexpr int kParts = kPartsOf<T, kPrefix>;
-  using V = ValueType<T, kPrefix>;
   auto& lds = shared.tiles;
   auto& scales = shared.scales;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -375,7 +316,6 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   constexpr int kWaveRows = 64 / kPer;
   U4 kc[W::kLoads], vc[W::kLoads];
   float scale = 0.0f;
-  float row_scale[W::kLoads];  // of the values whose codes the thread brings
   bool scale_ok = false;
   bool ok[W::kLoads];
   int pages[4];  // of the step to come
@@ -395,10 +335,6 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const uint32_t off = static_cast<uint32_t>(((r0 + i * W::kLoadRows) & 15) * a.c.row_bytes + 16 * chunk);
       kc[i] = Load16(a.c.k + at + off);
       vc[i] = Load16(a.c.v + at + off);
-      if constexpr (__is_same(V, F16))
-        row_scale[i] = *(const __attribute__((address_space(1))) float*)(args.scales.v + max(page, 0) * args.scales.page_bytes +
-                                                                         kh * args.scales.head_bytes +
-                                                                         4 * ((p0 & in_page) + ((r0 + i * W::kLoadRows) & 15)));
     }
     if (wave < 2) {
       const int u = lane / 16;
@@ -425,14 +361,10 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       const int ks = KSwizzle<K, kDim>(r), vs = VSwizzle<BF16, kDim>(r);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk) ^ ks)) = Operand8<C, K>(x[0], x[1]);
       *reinterpret_cast<U4*>(kr + 16 * ((2 * chunk + 1) ^ ks)) = Operand8<C, K>(x[2], x[3]);
-      const float power = __is_same(V, F16) ? PowerOf<C>(row_scale[i]) : 1.0f;
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Values8<C, V>(y[0], y[1], power);
-      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Values8<C, V>(y[2], y[3], power);
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk) ^ vs)) = Operand8<C, BF16>(y[0], y[1]);
+      *reinterpret_cast<U4*>(vr + 16 * ((2 * chunk + 1) ^ vs)) = Operand8<C, BF16>(y[2], y[3]);
     }
-    if (wave < 2) {
-      const float rest = __is_same(V, F16) ? RestOf(scale, PowerOf<C>(scale)) : scale;
-      scales[kAt][wave][lane] = wave == 0 ? scale * c : scale_ok ? rest : 0.0f;
-    }
+    if (wave < 2) scales[kAt][wave][lane] = wave == 0 ? scale * c : scale_ok ? scale : 0.0f;
   };
 
   const int k_at = (lane & 31) * W::kRowBytes + 16 * (h ^ KSwizzle<K, kDim>(lane & 31));
@@ -442,7 +374,6 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
     const int r = 8 * u + 4 * h + (lane & 15) / 4;
     v_at[u] = r * W::kRowBytes + 16 * ((2 * ((lane >> 4) & 1) + (lane & 3) / 2) ^ VSwizzle<BF16, kDim>(r)) + 8 * (lane & 1);
   }
-  ScaleRef scale_ref;
   float m = kNegInf, l = 0.0f;
   F16v o[kDim / 32] = {};
   if (steps > 0) {
@@ -468,16 +399,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       // lane e of each 16: of the key that the lanes' element e belongs to
       const float* of_lane = scales[kAt][0] + 8 * ((lane & 15) / 4) + 4 * h + lane % 4;
       const float ks[2] = {of_lane[0], of_lane[32]};
-      float vs[2] = {of_lane[W::kKeys], of_lane[W::kKeys + 32]};
-      if constexpr (__is_same(V, F16)) {
-        float f;
-        if (scale_ref.Raise(fmaxf(__builtin_fabsf(vs[0]), __builtin_fabsf(vs[1])), &f)) {
-#pragma unroll
-          for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
-        }
-        vs[0] *= scale_ref.inverse;
-        vs[1] *= scale_ref.inverse;
-      }
+      const float vs[2] = {of_lane[W::kKeys], of_lane[W::kKeys + 32]};
       F16v s[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -518,7 +440,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
 #pragma unroll
         for (int w = 0; w < kDim / 32; ++w) o[w] *= f;
       }
-      const float base = m == kNegInf ? 0.0f : m - kLiftOf<V>;
+      const float base = m == kNegInf ? 0.0f : m;
       typedef short S4 __attribute__((ext_vector_type(4)));
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -534,7 +456,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          WeightParts<kParts, V> p;
+          WeightParts<kParts> p;
 #pragma unroll
           for (int e = 0; e < 4; ++e) p.Set(e, s[b][8 * j + 2 * e], s[b][8 * j + 2 * e + 1]);
 #pragma unroll
@@ -548,7 +470,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
               v[2 * u] = x[0], v[2 * u + 1] = x[1];
             }
 #pragma unroll
-            for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<V>(v, p.x[i], o[w]);
+            for (int i = kParts - 1; i >= 0; --i) o[w] = Mfma32<BF16>(v, p.x[i], o[w]);
           }
         }
       }
@@ -575,8 +497,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
       for (int e = 0; e < 16; e += 4)
         *reinterpret_cast<F4*>(to + 32 * w + 2 * e + 4 * h) = F4{o[w][e], o[w][e + 1], o[w][e + 2], o[w][e + 3]};
   } else {
-    float inv = Inverse(m, l);
-    if constexpr (__is_same(V, F16)) inv *= scale_ref.ref;
+    const float inv = Inverse(m, l);
     char* out = a.out.p + (t.first + token) * a.out.token_bytes + head * a.out.head_bytes;
 #pragma unroll
     for (int w = 0; w < kDim / 32; ++w)
