@@ -355,7 +355,7 @@ RPG_HIP_API int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const r
 /* rpg_hip_paged_decode and rpg_hip_paged_prompt over such a cache, q and out rows of
  * `type`. Scales are applied in f32 to scores and weights, codes are multiplied as
  * they are; weights times scales go to the product in two parts of 8 bits, for f32
- * rows in three, in prompts of bf16 rows in one. Queries are finite; a row whose scale is
+ * rows in three. Queries are finite; a row whose scale is
  * NaN makes NaN of what sees it, and of nothing else. In places that no query sees codes and scales may be
  * anything, but for the NaN codes of e4m3 (which rpg_hip_quant_append never writes)
  * behind a prompt's token in its own sequence. work: rpg_hip_quant_work bytes. */

@@ -13,19 +13,20 @@
 //
 // Weights times scales go to the product in parts of bf16, whose range is that of fp32, as
 // in codes_decode.hip: f16 ones would have to be held over the largest scale, which may be
-// a later token's, and the tokens before it would lose their weights' bits to it. For bf16
-// rows they are rounded once, as paged_prompt.hip's are (the output is 1.40 times as far
-// from exact as its own rounding leaves it; two parts: four documents bf16 638 us, one 535
-// at the time).
+// a later token's, and the tokens before it would lose their weights' bits to it. Two parts
+// (f32 rows: three) leave the output as exact as its own rounding does; rounded to the
+// rows' type once, it is 1.40 (bf16) and 1.41 (f16) times as far from exact, and four
+// documents e4m3 bf16 take 501 us instead of 645, 2000 tokens 66 instead of 81.5.
 //
-// Bound: the vector unit beside the matrix unit: per score a product with either scale
-// comes to the maximum, the exponential and the sum, and the codes' conversion.
-// Measured, 32 heads on 8 of 128: four documents of about 3000 tokens, 392 GFLOP, e4m3
-// in bf16, 478 us (821 TFLOP/s; a large product of a library reaches 1254, the same
-// over a cache of bf16 960); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16,
-// 17 us. Tried on documents: products of one 32-key block between the weighing of the
-// other 492 -> 492 (479 without), higher priority around products the same, pages
-// looked up another step ahead the same.
+// Bound: the matrix unit, which the second parts take half as long again, and the vector
+// unit, hardly at once (documents: busy for 44 and 54 % of the cycles): per score a product
+// with either scale comes to the maximum, the exponential, the sum and the second part,
+// and the codes' conversion. Measured, 32 heads on 8 of 128: four documents of about 3000 tokens, 392 GFLOP, e4m3 in bf16, 637 to 645 us
+// (612 TFLOP/s of the definition's, 918 of the products'; a large product of a library
+// reaches 1254); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16, 17 us. Tried on
+// documents with one part: products of one 32-key block between the weighing of the other
+// 492 -> 492 (479 without), higher priority around products the same, pages looked up
+// another step ahead the same.
 
 #include <hip/hip_runtime.h>
 
@@ -55,8 +56,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void CodesSoloKernel(CodesAttention
 }
 
 // Tiles of 128 rows where those make three workgroups for every two compute units,
-// of 32 otherwise (1000 tokens 42.8 and 34.0 us, 4 x 300 24.2 and 27.6, 2000 82.6 and
-// 90.7).
+// of 32 otherwise (1000 tokens 43.2 and 34.3 us, 4 x 300 25.1 and 27.6, 2000 84.4 and
+// 91.8).
 bool IsWide(int64_t n_tokens, int64_t n_seqs, int group, int n_kv) {
   return TilesFor(n_tokens, n_seqs, group, 128) * n_kv >= 384;
 }
@@ -76,7 +77,7 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
     return;
   }
   // Eight waves where they find a compute unit to themselves and the keys are many (six
-  // turns 19.2 -> 18.2 us, 200 behind 1300 24.1 -> 22.6; 200 alone 10.0 and 10.9).
+  // turns 18.7 -> 18.0 us, 200 behind 1300 24.2 -> 22.3; 200 alone 9.9 and 10.2).
   const int64_t wgs = tiles * a.c.n_kv * a.splits;
   const dim3 grid(static_cast<uint32_t>(tiles * a.c.n_kv), a.splits);
   bool eight = false;
@@ -93,9 +94,9 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
 
 // Key ranges where not even half the compute units have a workgroup, of 512 positions
 // at least, and as many as find one free; none for rows of up to 1536 positions where
-// a quarter of them have one (f16: 100 behind 1400, 104 workgroups, 25.6 us with two and
-// 22.2 with one, 30 behind 1000, 40 of them, 16.5 with three and 17.4 with one; 12
-// behind 30000 32).
+// a quarter of them have one (f16: 100 behind 1400, 104 workgroups, 25.4 us with two and
+// 21.9 with one, 30 behind 1000, 40 of them, 16.4 with three and 17.1 with one; 12
+// behind 30000 32 and 266).
 int CodesPromptSplits(int64_t n_tokens, int64_t n_seqs, int n_heads, int n_kv, int64_t capacity) {
   const int64_t wgs = TilesFor(n_tokens, n_seqs, n_heads / n_kv, kSoloRows) * n_kv;
   if (wgs >= 128 || (wgs >= 64 && capacity <= 1536)) return 1;

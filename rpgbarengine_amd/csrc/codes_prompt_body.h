@@ -74,17 +74,13 @@ struct SoloLds {
   float sm[kWaves][kSoloRows], sl[kWaves][kSoloRows];
 };
 
-// The parts of a weight times its scale. Prompts of bf16 rows round it once.
-template <typename T, bool kPrefix>
-constexpr int kPartsOf = __is_same(T, BF16) && !kPrefix ? 1 : kWeightParts<T>;
-
 // Few rows. kPrefix and the last three: as PromptBody's (prompt_body.h).
 template <typename C, typename T, int kDim, int kWaves, bool kPrefix>
 __device__ __forceinline__ void SoloBody(const CodesAttentionArgs& args, const Seqs& groups, int prefix_splits,
                                          SoloLds<kDim, kWaves>& shared, int bx, int by, int gx) {
   const AttentionArgs& a = args.a;
   using K = KeyType<T>;
-  constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = kPartsOf<T, kPrefix>;
+  constexpr int kQ = kDim / 16, kBlocks = kDim / 32, kParts = kWeightParts<T>;
   auto& lds = shared.states;
   auto& sm = shared.sm;
   auto& sl = shared.sl;
@@ -267,7 +263,7 @@ __device__ __forceinline__ void WideBody(const CodesAttentionArgs& args, const S
   const AttentionArgs& a = args.a;
   using W = Wide<T, kDim>;
   using K = KeyType<T>;
-  constexpr int kParts = kPartsOf<T, kPrefix>;
+  constexpr int kParts = kWeightParts<T>;
   auto& lds = shared.tiles;
   auto& scales = shared.scales;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -10,7 +10,7 @@ from test_gpu_serving_codes import CODES, expect, ident, on_cpu, random_cache, r
 
 pytestmark = pytest.mark.gpu
 
-HALVES = [torch.float16]
+HALVES = [torch.float16, torch.bfloat16]
 # tiles of 32 rows by eight waves, by four, in several ranges, and tiles of 128 rows
 SIZES = {"few": ([70, 290, 33], [9, 20, 33], 128, 8, 2), "short": ([64, 30], [64, 30], 64, 6, 3),
          "long": ([1500], [12], 128, 4, 1), "many": ([150, 330], [150, 200], 64, 192, 32)}
