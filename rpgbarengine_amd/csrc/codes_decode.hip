@@ -65,13 +65,20 @@ void Launch(const CodesAttentionArgs& args, hipStream_t s) {
 // 1024 also for the longest where one workgroup to a sequence and key head is one to two
 // for each compute unit, or half of one: 32 of the same lengths 49.8 -> 47.0 us, 16 32.6
 // -> 30.7 (f32 34.9 -> 25.5), 16 of 100 to 40000 56.4 -> 49.3; but 8 of them 19.5 -> 20.6,
-// 32 of 2826 each 43.5 -> 44.2.
+// 32 of 2826 each 43.5 -> 44.2. Batches below that are cut into one workgroup per compute
+// unit, and a table that asks for more ranges than that (one wider than its sequences, as
+// a captured graph keeps) cuts none below 384 positions: 8 of 1090, 16 heads, f16, 12.7 us in
+// a table of their own width, in one for 8192 and one for 131072 18.7 and 21.7 with ranges of
+// 1024, 13.0 and 15.8 with 384, 12.9 and 16.1 with 128 (f32, 32 heads, 13.6; 20.1 and 23.5,
+// 13.8 and 17.0, 13.8 and 19.1); 12 ragged in one for 16384 28.4, 24.1 and 24.3; of one or
+// two sequences, whose workgroups are few, as the table has it: one of 1000 in one for 131072
+// 14.1, 10.7 and 8.8.
 int CodesDecodeSplits(int64_t n_seqs, int n_heads, int n_kv, int64_t capacity, int* least) {
   *least = 0;
   if (capacity <= 640) return 1;
   const int64_t base = std::max<int64_t>(1, n_seqs * n_kv * CeilDiv(n_heads / n_kv, kCols));
   const int64_t fill = 256 / base, cap = CeilDiv(capacity, base >= 128 && base < 512 ? 1024 : 2048);
-  if (fill <= cap) *least = 1024;
+  if (fill <= cap) *least = base >= 128 ? 1024 : base >= 32 ? 384 : 0;
   const int64_t want = std::max(fill, cap);
   return static_cast<int>(std::max<int64_t>(1, std::min({want, CeilDiv(capacity, kRangeUnit), int64_t{kMaxSplits}})));
 }
