@@ -432,7 +432,7 @@ typedef struct {
 
 /* logits [rows][vocab], row_stride elements apart, edited into out (which may be
  * logits, with its stride: then rows without a mask are touched only where tokens
- * change). Any alignment of the type; vocab <= 2^24, rows <= 65535, history_size
+ * change; and else lies apart from them). Any alignment of the type; vocab <= 2^24, rows <= 65535, history_size
  * <= 2^20, n_biases <= 1023. No work memory. */
 RPG_HIP_API int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t rows, int64_t vocab,
                                         int64_t row_stride, const rpg_hip_edits* edits, void* out,

@@ -328,6 +328,17 @@ void AppendRows(paged::AppendArgs* to, const rpg_hip_rows* k, const rpg_hip_rows
   a.rope_rows = rope_rows;
 }
 
+// Rows that are written while others are read, `bytes` each: those of one number lie in
+// one place, or none of them touches another (two parts of the rows of one matrix may).
+void CheckApart(const char* out_overlaps_in, const void* out, int64_t out_stride, const void* in, int64_t in_stride,
+                int64_t n_rows, int64_t bytes) {
+  const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(in));
+  if (d == 0 || d >= (n_rows - 1) * in_stride + bytes || -d >= (n_rows - 1) * out_stride + bytes) return;
+  const bool matrix = n_rows > 1 && out_stride == in_stride;
+  const int64_t off = matrix ? (d % out_stride + out_stride) % out_stride : 0;
+  RPG_CHECK(matrix && off >= bytes && out_stride - off >= bytes, "%s", out_overlaps_in);
+}
+
 // Rows of 4-byte elements that may be given more than once (stride 0).
 void CheckList(const char* what, const void* p, int64_t stride) {
   CheckPointer(what, p, 4);
@@ -586,6 +597,7 @@ int32_t rpg_hip_edit_logits(int32_t type, const void* logits, int64_t n_rows, in
         a.type = static_cast<uint32_t>(type);
         a.rows = static_cast<int32_t>(n_rows);
         a.vocab = static_cast<int32_t>(vocab);
+        CheckApart("out overlaps logits", out, a.out_bytes, logits, a.row_bytes, n_rows, vocab * bytes);
         for (const void* p : {static_cast<const void*>(e.history_lens), static_cast<const void*>(e.prompts),
                               static_cast<const void*>(e.repetition), static_cast<const void*>(e.presence),
                               static_cast<const void*>(e.frequency), static_cast<const void*>(e.mask_rows)})

@@ -468,7 +468,7 @@ def _list(x, name, rows, dtype, device):
 def edit_logits(logits, history=None, history_lens=None, prompts=None, repetition=None, presence=None, frequency=None,
                 bias_ids=None, bias=None, mask=None, mask_rows=None, out=None):
     """logits [rows, vocab] with penalties, biases and masks, into out (made when not
-    given; may be logits). In this order, where c counts how often a row's history
+    given; may be logits, and else lies apart from them). In this order, where c counts how often a row's history
     holds a token behind the row's prompt:
 
         x = x / repetition if x > 0 else x * repetition   tokens of the history
