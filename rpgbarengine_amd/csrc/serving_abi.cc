@@ -476,6 +476,7 @@ int32_t rpg_hip_quant_read(const rpg_hip_quant_cache* cache, const rpg_hip_seque
         RPG_CHECK(a.c.n_kv <= 65536, "%d key heads", a.c.n_kv);
         a.k = RowsOf("k", k, a.c, a.s.n_tokens, a.c.n_kv, true);
         a.v = RowsOf("v", v, a.c, a.s.n_tokens, a.c.n_kv, true);
+        RPG_CHECK(a.k.p != a.v.p, "k and v are the same rows");
         paged::ReadCodes(a, static_cast<hipStream_t>(stream));
         return 0;
       },

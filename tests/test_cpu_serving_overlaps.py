@@ -4,8 +4,8 @@ anything touches a GPU."""
 import pytest
 
 from rpgbarengine_amd import serving
-from test_cpu_serving import A, ref, refused
-from test_cpu_serving_more import edits
+from test_cpu_serving import A, ref, refused, rows, seqs
+from test_cpu_serving_more import edits, quant
 
 
 @pytest.mark.parametrize("kind,size", [(0, 4), (1, 2), (30, 2)])
@@ -25,3 +25,8 @@ def test_logits_apart_are_no_overlap(n, stride, out_stride, off):
     """What is refused here is the next argument in order."""
     refused(serving._lib().rpg_hip_edit_logits(1, A, n, 300, stride, ref(edits(repetition=A + 1)), A + off * 2, out_stride, None),
             "row parameter")
+
+
+@pytest.mark.parametrize("kind", [0, 1, 30])
+def test_keys_and_values_read_into_the_same_rows(kind):
+    refused(serving._lib().rpg_hip_quant_read(ref(quant()), ref(seqs()), kind, ref(rows()), ref(rows()), None), "the same rows")
