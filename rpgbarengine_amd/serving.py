@@ -263,7 +263,7 @@ def append(cache, table, lens, starts, k, v, q=None, q_out=None, q_norm=None, k_
     k_norm and q_norm (float32 [dim]) and rotated by rope (float32 [positions,
     dim]: cos | sin) where those are given. A QuantCache holds each row as codes and
     a scale; k, v and q are of one type. Returns q_out."""
-    quant = type(cache) is QuantCache
+    quant = isinstance(cache, QuantCache)
     kind = _row_type(k, "k") if quant else None
     kr, vr = _rows(k, "k", cache, kind), _rows(v, "v", cache, kind)
     n = k.shape[0]
@@ -304,7 +304,7 @@ def read_rows(cache: QuantCache, table, lens, starts, k_out, v_out):
     go to rows starts[s] .. starts[s + 1] of k_out and v_out [tokens, key heads, dim],
     both of one type. Rows of no sequence are left as they are; positions whose pages
     the table does not name read as zeros. Returns (k_out, v_out)."""
-    if type(cache) is not QuantCache:
+    if not isinstance(cache, QuantCache):
         raise EngineError("cache is a QuantCache")
     kind = _row_type(k_out, "k_out")
     kr, vr = _rows(k_out, "k_out", cache, kind), _rows(v_out, "v_out", cache, kind)
@@ -335,7 +335,7 @@ def _quant_work_bytes(n_kv, page_size, head_dim, kind, pages, n_seqs, n_tokens, 
 
 
 def _attention(q, cache, table, lens, starts, scale, out, prompt):
-    quant = type(cache) is QuantCache
+    quant = isinstance(cache, QuantCache)
     kind = _row_type(q, "q") if quant else None
     qr = _rows(q, "q", cache, kind)
     n_tokens = q.shape[0] if prompt else 0
@@ -397,7 +397,7 @@ def shared_attention(q, cache, table, lens, groups, shared, scale=None, out=None
     groups[g + 1] (int32 [groups + 1]), and the tables of those that have positions
     name the same pages for the first shared[g] (int32 [groups]) positions. out (may
     be q) is made when not given."""
-    quant = type(cache) is QuantCache
+    quant = isinstance(cache, QuantCache)
     kind = _row_type(q, "q") if quant else None
     qr = _rows(q, "q", cache, kind)
     seqs, n_seqs, pages = _seqs(cache, table, lens, None, 0)
