@@ -336,7 +336,7 @@ typedef struct {
 
 /* rpg_hip_paged_append into such a cache. A row y (keys: as normed and rotated in
  * f32; values: as they are) with the largest magnitude a is held as scale a / M, M
- * the largest code, and codes y M / a, to the nearest, even at ties. Where a is below
+ * the largest code, and codes y M / a in f32, to the nearest, even at ties. Where a is below
  * 2^-112 scale and codes are 0; where y is not finite the scale is NaN, the codes 0:
  * the whole row reads as NaN. */
 RPG_HIP_API int32_t rpg_hip_quant_append(const rpg_hip_quant_cache* cache, const rpg_hip_sequences* seqs, int32_t type,

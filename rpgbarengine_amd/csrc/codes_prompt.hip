@@ -21,12 +21,12 @@
 // Bound: the matrix unit, which the second parts take half as long again, and the vector
 // unit, hardly at once (documents: busy for 44 and 54 % of the cycles): per score a product
 // with either scale comes to the maximum, the exponential, the sum and the second part,
-// and the codes' conversion. Measured, 32 heads on 8 of 128: four documents of about 3000 tokens, 392 GFLOP, e4m3 in bf16, 637 to 645 us
-// (612 TFLOP/s of the definition's, 918 of the products'; a large product of a library
-// reaches 1254); six turns of 13 to 50 tokens behind 400 to 1000, i8 in f16, 17 us. Tried on
-// documents with one part: products of one 32-key block between the weighing of the other
-// 492 -> 492 (479 without), higher priority around products the same, pages looked up
-// another step ahead the same.
+// and the codes' conversion. Measured, 32 heads on 8 of 128: four documents of about 3000
+// tokens, 392 GFLOP, e4m3 in bf16, 622 to 645 us (620 TFLOP/s of the definition's, 930 of the
+// products'; a large product of a library reaches 1254); six turns of 13 to 50 tokens behind
+// 400 to 1000, i8 in f16, 17 us. Tried on documents with one part: products of one 32-key
+// block between the weighing of the other 492 -> 492 (479 without), higher priority around
+// products the same, pages looked up another step ahead the same.
 
 #include <hip/hip_runtime.h>
 
@@ -43,6 +43,9 @@ namespace rpg {
 namespace paged {
 namespace {
 
+// Two workgroups to a compute unit: f32 rows of 128 keep 45 (i8) and 60 (e4m3) registers in
+// memory for it (documents 1254 and 1315 us; with all in registers and one workgroup 1394
+// and 1350; 2000 tokens i8, which have one to a unit anyway, 177 and 131).
 template <typename C, typename T, int kDim>
 __global__ __launch_bounds__(256, 2) void CodesWideKernel(CodesAttentionArgs a) {
   __shared__ __align__(256) WideLds<T, kDim> shared;

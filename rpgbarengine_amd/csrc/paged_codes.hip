@@ -3,8 +3,9 @@
 // rotated as in paged_append.hip, in fp32; values as they are) is stored as
 //   a = max |y|,  scale = a / M,  code = y M / a to the nearest, even at ties
 // with M the largest code (127, 448), and read as code x scale. The quotient is
-// the correctly rounded one, of the whole product y M: 16-bit rows have many that lie
-// midway between two codes, and there y (M / a) would fall to either side.
+// fp32's, of the whole product y M: 16-bit rows have many that lie midway between two
+// codes, and there y (M / a) would fall to either side. (Where fp32 rounds a quotient onto
+// the middle the code is the even one: 16 of 12 million of f32 rows are not the nearest.)
 //
 // Bound: bytes, or for few tokens the launch and its dependent round trips. A row
 // is one 16-byte load of 8, 16 or 32 adjacent lanes; the sum of squares, the

@@ -15,12 +15,14 @@
 // Bound: the common positions' products (a group of 32 sequences with four heads to a
 // key head multiplies each key 128 times) beside the own positions' bytes, and the
 // join. Measured, 32 heads on 8 of 128: 96 sequences in three groups behind 4000 to
-// 12000 positions with 100 to 2500 of their own, bf16, 376 MB, 101.6 us (a large copy's
-// rate: 74); 8 behind 2000, f32, 21.5. Workgroups of
-// both kinds in turn instead of the common ones first: 129 us the former, 28.6 the latter
-// (then 23.6). Weights of common positions in two parts, as decode has them: 107 -> 108.8
-// us the former, 50 -> 61 where own positions are few (both then); with one part the
-// output is 1.35 times as far from exact.
+// 12000 positions with 100 to 2500 of their own, bf16, 376 MB, 102 to 107 us (a large copy's
+// rate: 74); 8 behind 2000, f32, 21, of which the products take 2 to 4 (4096 cycles of a wave,
+// two of which may share a unit) and the second launch 4: what is left, not measured apart, are
+// the round trips in front of the first product (starts and counts, lengths, the table, rows)
+// and the waves' join. Workgroups of both kinds in turn instead of the common ones first:
+// 129 us the former, 28.6 the latter (then 23.6). Weights of common positions in two parts,
+// as decode has them: 107 -> 108.8 us the former, 50 -> 61 where own positions are few (both
+// then); with one part the output is about 1.4 times as far from exact.
 
 #include <hip/hip_runtime.h>
 
@@ -39,7 +41,9 @@ namespace paged {
 namespace {
 
 // One launch for both, so that the products of the common positions run beside the loads
-// of the others. A sequence's last ranges come first.
+// of the others. A sequence's last ranges come first. Two workgroups of 128 rows to a compute
+// unit, for which f32 rows of 128 keep 34 registers in memory (96 sessions f32 288 us, with all
+// in registers and one workgroup 326; 64 behind 4000 89 and 103).
 template <typename T, int kDim, int kGroups>
 __global__ __launch_bounds__(256, kGroups == 2 || (kGroups == 4 && kBytes<T> == 4) ? 1 : 2) void SharedKernel(SharedArgs args, SharedGrid g) {
   const AttentionArgs& a = args.a;
@@ -192,7 +196,8 @@ SharedGrid GridOf(const SharedArgs& args, int rows) {
 // run beside them (96 sequences in three groups behind 4000 to 12000, bf16: 103.4 us
 // aiming at 512 workgroups, 100.7 at 256, 99.5 at 192; 32 behind 30000 63.1, 57.1, 67.8),
 // two in f32, which the products alone keep busy (64 behind 4000: 88.8, 96.9), and none
-// above 2560 positions, so that the longest group does not end alone (128 in eight groups
+// above 2560 positions (where the table has up to 655360), so that the longest group does not
+// end alone (128 in eight groups
 // behind 500 to 8000 91.8 us without, 84.9 so; 64 in 16 behind 100 to 10000 84.8, 76.2; on
 // int8 codes of f16 rows the former 72.1, 75.2). Of 256 positions at least (64 behind 64,
 // bf16: 29.2, with 128 31.5), 128 in tiles of 16 rows (8 behind 2000, f32: 24.7 us with

@@ -411,8 +411,8 @@ __device__ __forceinline__ void PromptBody(const AttentionArgs& a, const Seqs& g
     } else {
       // The weights are rounded to the cache's 16 bits for the product (each
       // by at most half a step, as V itself was); the sum has them unrounded. The
-      // output is up to 1.35 times as far from exact as its own rounding leaves it
-      // (documents bf16: 2.2e-3 relative, 1.6e-3). Weights in two parts, as decode
+      // output is 1.1 to 1.6 times as far from exact as its own rounding leaves it, the
+      // more the flatter the weights (documents bf16: 2.2e-3 relative, 1.6e-3). Weights in two parts, as decode
       // has them, would make that 1.0, for another product: documents 410 -> 538 us,
       // six turns f16 14.1 -> 15.2. Positions that a group of sequences has in common
       // (kPrefix) have two parts, as the decode that they stand for.

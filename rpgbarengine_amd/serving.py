@@ -395,8 +395,9 @@ def shared_attention(q, cache, table, lens, groups, shared, scale=None, out=None
     """decode_attention where the first positions of a group's sequences lie in the
     same pages, which are read once for the group: group g is sequences groups[g] ..
     groups[g + 1] (int32 [groups + 1]), and the tables of those that have positions
-    name the same pages for the first shared[g] (int32 [groups]) positions. out (may
-    be q) is made when not given."""
+    name the same pages for the first shared[g] (int32 [groups]) positions (a larger
+    count gives some of them another's keys and values). out (may be q) is made when not
+    given."""
     quant = isinstance(cache, QuantCache)
     kind = _row_type(q, "q") if quant else None
     qr = _rows(q, "q", cache, kind)
