@@ -22,7 +22,7 @@
 // unit, hardly at once (documents: busy for 44 and 54 % of the cycles): per score a product
 // with either scale comes to the maximum, the exponential, the sum and the second part,
 // and the codes' conversion. Measured, 32 heads on 8 of 128: four documents of about 3000
-// tokens, 392 GFLOP, e4m3 in bf16, 622 to 645 us (620 TFLOP/s of the definition's, 930 of the
+// tokens, 392 GFLOP, e4m3 in bf16, 613 to 645 us (610 to 640 TFLOP/s, 910 to 960 of the
 // products'; a large product of a library reaches 1254); six turns of 13 to 50 tokens behind
 // 400 to 1000, i8 in f16, 17 us. Tried on documents with one part: products of one 32-key
 // block between the weighing of the other 492 -> 492 (479 without), higher priority around
